@@ -1,0 +1,240 @@
+// Host plan of one step's attention over the paged cache: which rows read
+// which keys, in pieces that fill the GPU.  Plain C++ with no device code.
+//
+// A row is one query head of one token; the G query heads that share a kv
+// head make G consecutive rows of a token, and everything below is per kv
+// head (the kernel's grid has the kv heads as its second factor).
+//
+// Sequences are sorted by their page lists, so that those with a common start
+// lie side by side, and walked as a tree: a run of whole pages that several
+// sequences share, all of it before each one's first new token, becomes one
+// segment with the rows of all of them, when the bytes this saves outweigh
+// the partial results it adds; what is left of a sequence is a segment of its
+// own with the causal limit.  A segment's rows are cut into tiles and its keys
+// into pieces of about equal length.  Rows whose keys lie in several pieces
+// get a partial result from each and are joined by a second kernel.
+#pragma once
+
+#include <algorithm>
+#include <cstdint>
+#include <vector>
+
+#include "kv_tables.h"
+
+namespace exq {
+
+// One workgroup's work for one kv head: rows [row0, row0 + n_rows) of the
+// plan's row order against the keys at positions [key0, key1), the page of
+// position p being pages[page_at + p / page_tokens] (an index into the plan's
+// words).  causal: a row sees positions up to its token's own only.  part: the
+// partial result of row row0 (rows follow), -1 when the rows have no other
+// piece and the result is final.
+struct AttnItem {
+    int32_t row0, n_rows, key0, key1, page_at, causal, part, pad;
+};
+// One token: its place in the sequence and its slot in the pool (page *
+// page_tokens + offset), and, for plan order: the token that stands there and
+// that one's position.
+struct PlanToken {
+    int32_t pos, slot, order, order_pos;
+};
+struct PlanHeader {
+    int32_t n_tokens, n_items, n_joined;  // n_joined: rows with more than one piece
+    int32_t join_rows;                    // word index of the joined rows' numbers
+    int32_t join_at;                      // n_joined + 1 word indices into the partial numbers
+    int32_t parts;                        // partial results of one kv head
+    int32_t pad[10];
+};
+static_assert(sizeof(AttnItem) == 32 && sizeof(PlanToken) == 16 && sizeof(PlanHeader) == 64, "words of the device plan");
+
+struct PlanShape {
+    int group;       // query heads of one kv head
+    int n_kv;
+    int token_bytes; // K and V of one token and kv head
+    int part_bytes;  // one row's partial result
+    int workgroups;  // that run at once
+};
+
+struct AttnPlan {
+    static constexpr int kTileRows = 128;   // rows of one workgroup at most
+    static constexpr int kMinKeys = 256;    // no piece is cut shorter
+    static constexpr int kKeyStep = 64;     // pieces are multiples of it
+
+    std::vector<PlanToken> tokens;  // by token; order fields by plan order
+    std::vector<AttnItem> items;    // page_at, relative to `pages`
+    std::vector<int32_t> pages;
+    std::vector<int32_t> join_rows, join_at, join_parts;
+    int parts = 0;
+    bool writable = true;  // no new token's page has another holder
+
+    void build(const KvTables &kv, int n, const int *seqs, const int *n_new, const PlanShape &shape) {
+        kv_ = &kv;
+        shape_ = shape;
+        pt_ = kv.page_tokens();
+        tokens.clear();
+        items.clear();
+        pages.clear();
+        join_rows.clear();
+        join_at.clear();
+        join_parts.clear();
+        segs_.clear();
+        parts = 0;
+        writable = true;
+        nodes_.clear();
+        for (int i = 0; i < n; ++i) {
+            const KvTables::Seq &s = kv.seq(seqs[i]);
+            const int first = (int)tokens.size(), q0 = s.len - n_new[i];
+            for (int p = q0; p < s.len; ++p) {
+                const int page = s.pages[(size_t)p / pt_];
+                if (kv.holders(page) > 1) writable = false;
+                tokens.push_back({p, page * pt_ + p % pt_, 0, 0});
+            }
+            if (n_new[i] > 0) nodes_.push_back({&s, first, n_new[i], q0 / pt_, 0});
+        }
+        if (tokens.empty()) return;
+        std::stable_sort(nodes_.begin(), nodes_.end(), [](const Node &a, const Node &b) {
+            const int most = std::min(a.shareable, b.shareable), d = agree(a, b, 0, most);
+            return d < most ? a.seq->pages[d] < b.seq->pages[d] : a.shareable < b.shareable;
+        });
+        int at = 0;
+        for (Node &nd : nodes_) {
+            nd.row0 = at * shape_.group;
+            for (int t = 0; t < nd.n_new; ++t, ++at) {
+                tokens[at].order = nd.first + t;
+                tokens[at].order_pos = tokens[nd.first + t].pos;
+            }
+        }
+        walk();
+        cut((int)tokens.size() * shape_.group);
+    }
+
+  private:
+    struct Node {
+        const KvTables::Seq *seq;
+        int first, n_new, shareable, row0;  // shareable: whole pages before the first new token
+    };
+    struct Segment {
+        int row0, n_rows, key0, key1, page_at, causal;
+    };
+    struct Span {
+        int lo, hi, start, depth;  // nodes [lo, hi) share their first `depth` pages; pages from `start` on are unread
+    };
+
+    // How many leading pages two sequences have in common, at least `from` and at
+    // most `most`.  Pages are only shared by forks, which share a whole start: a
+    // page in common means that all before it are, so a binary search finds the end.
+    static int agree(const Node &a, const Node &b, int from, int most) {
+        while (from < most) {
+            const int mid = from + (most - from) / 2;
+            if (a.seq->pages[mid] == b.seq->pages[mid]) from = mid + 1;
+            else most = mid;
+        }
+        return from;
+    }
+
+    int list_pages(const KvTables::Seq &s, int from, int to) {
+        // positions keep their own page index: pages[at + p / page_tokens]
+        const int at = (int)pages.size() - from;
+        pages.insert(pages.end(), s.pages.begin() + from, s.pages.begin() + to);
+        return at;
+    }
+
+    void walk() {
+        std::vector<Span> todo;
+        todo.push_back({0, (int)nodes_.size(), 0, 0});
+        while (!todo.empty()) {
+            Span sp = todo.back();
+            todo.pop_back();
+            const Node &a = nodes_[sp.lo];
+            if (sp.hi - sp.lo == 1) {
+                const int len = a.seq->len, all = (len + pt_ - 1) / pt_;
+                const int page_at = list_pages(*a.seq, sp.start, all);
+                segs_.push_back({a.row0, a.n_new * shape_.group, sp.start * pt_, len, page_at, 1});
+                continue;
+            }
+            // how far all of them agree: the sorted range's ends decide
+            const Node &z = nodes_[sp.hi - 1];
+            int most = z.shareable;
+            for (int i = sp.lo; i < sp.hi; ++i) most = std::min(most, nodes_[i].shareable);
+            const int d = agree(a, z, sp.depth, most);
+            const int rows = z.row0 + z.n_new * shape_.group - a.row0;
+            const long long run = (long long)(d - sp.start) * pt_;
+            // saved: the run's keys and values for all but one; added: every row's partial result, written and read
+            if (run > 0 && (sp.hi - sp.lo - 1) * run * shape_.token_bytes > 2LL * rows * shape_.part_bytes) {
+                const int page_at = list_pages(*a.seq, sp.start, d);
+                segs_.push_back({a.row0, rows, sp.start * pt_, d * pt_, page_at, 0});
+                sp.start = d;
+            }
+            // children: neighbours that agree on the next page
+            for (int lo = sp.lo; lo < sp.hi;) {
+                int hi = lo + 1;
+                if (nodes_[lo].shareable > d)
+                    while (hi < sp.hi && nodes_[hi].shareable > d && nodes_[hi].seq->pages[d] == nodes_[lo].seq->pages[d])
+                        ++hi;
+                todo.push_back({lo, hi, sp.start, hi - lo > 1 ? d + 1 : d});
+                lo = hi;
+            }
+        }
+    }
+
+    void cut(int rows) {
+        long long total = 0;
+        for (const Segment &s : segs_)
+            total += (long long)((s.n_rows + kTileRows - 1) / kTileRows) * (s.key1 - s.key0);
+        const long long target = std::max(1, shape_.workgroups / shape_.n_kv);
+        const long long piece = std::max<long long>(kMinKeys, (total + target - 1) / target);
+        std::vector<int> count(rows, 0);
+        for (const Segment &s : segs_) {
+            for (int r = 0; r < s.n_rows; r += kTileRows) {
+                const int nr = std::min(kTileRows, s.n_rows - r);
+                int key1 = s.key1;
+                if (s.causal)  // the tile's last token sees no further than itself
+                    key1 = std::min(key1, tokens[(s.row0 + r + nr - 1) / shape_.group].order_pos + 1);
+                const int keys = key1 - s.key0;
+                const int n = (int)((keys + piece / 2) / piece) > 1 ? (int)((keys + piece - 1) / piece) : 1;
+                const int step = ((keys + n - 1) / n + kKeyStep - 1) / kKeyStep * kKeyStep;
+                for (int k = 0; k < keys; k += step) {
+                    items.push_back({s.row0 + r, nr, s.key0 + k, std::min(s.key0 + k + step, key1), s.page_at,
+                                     s.causal, -1, 0});
+                    for (int j = 0; j < nr; ++j) count[s.row0 + r + j]++;
+                }
+            }
+        }
+        // long pieces first: the short ones fill the end
+        std::stable_sort(items.begin(), items.end(), [](const AttnItem &a, const AttnItem &b) {
+            const auto tiles = [](const AttnItem &i) { return i.n_rows > 32 ? 2 : 1; };
+            return (long long)tiles(a) * (a.key1 - a.key0) > (long long)tiles(b) * (b.key1 - b.key0);
+        });
+        std::vector<int> start(rows + 1, 0);
+        for (int r = 0; r < rows; ++r) {
+            start[r + 1] = start[r] + (count[r] > 1 ? count[r] : 0);
+            if (count[r] > 1) {
+                join_rows.push_back(r);
+                join_at.push_back(start[r]);
+            }
+        }
+        join_at.push_back(start[rows]);
+        join_parts.resize(start[rows]);
+        // (a tile's rows all have the same pieces or more: any of them joined makes the item partial)
+        std::vector<int> filled(rows, 0);
+        for (AttnItem &it : items) {
+            bool joined = false;
+            for (int j = 0; j < it.n_rows; ++j) joined |= count[it.row0 + j] > 1;
+            if (!joined) continue;
+            it.part = parts;
+            for (int j = 0; j < it.n_rows; ++j) {
+                const int r = it.row0 + j;
+                if (count[r] > 1) join_parts[start[r] + filled[r]++] = parts + j;
+            }
+            parts += it.n_rows;
+        }
+    }
+
+    const KvTables *kv_ = nullptr;
+    PlanShape shape_{};
+    int pt_ = 0;
+    std::vector<Node> nodes_;
+    std::vector<Segment> segs_;
+};
+
+}  // namespace exq

@@ -12,6 +12,7 @@
 
 #include "common.h"
 #include "edgexpu_hip.h"
+#include "lib.h"
 
 using namespace exq;
 
@@ -731,6 +732,30 @@ struct edgexpu_hip_weight {
     int n_in;
     bool owned;
 };
+
+namespace exq {
+
+bool lib_ready(const char *what) {
+    if (!ensure_init()) return false;
+    int dev = -1;
+    if (!hip_ok(hipGetDevice(&dev), "hipGetDevice")) return false;
+    if (dev == g.device) return true;
+    set_error(-4, "%s: the current device is %d, the library's %d", what, dev, g.device);
+    return false;
+}
+
+void lib_error(int code, const char *fmt, ...) {
+    char msg[sizeof(g.msg)];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(msg, sizeof(msg), fmt, ap);
+    va_end(ap);
+    set_error(code, "%s", msg);
+}
+
+bool lib_hip(hipError_t e, const char *what) { return hip_ok(e, what); }
+
+}  // namespace exq
 
 extern "C" {
 

@@ -1,4 +1,4 @@
-"""Python front end of the MI355X quantized-weight path.
+"""Python front end of the MI355X quantized-weight path and of the ops between its projections.
 
 Thin ctypes bindings over the C-ABI of ``lib/libedgexpu_hip.so`` (declared in
 ``include/edgexpu_hip.h``) and ``lib/libedgexpu_kernels.so`` (the reference-named
@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import sys
 
 PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_DIR = os.path.join(PKG_DIR, "lib")
@@ -121,6 +122,35 @@ class HipLib:
         self.layer_linear_dev = _sig(L, "edgexpu_hip_layer_linear_dev", C.c_int,
                                      [C.c_int, _vp, _vp, _vp, _vp, C.c_float, _vp, C.c_uint32, _vp, _vp, _vp,
                                       C.c_int, C.c_int, _vp])
+
+        ip = C.POINTER(C.c_int)
+        self.kv_pool_bytes = _sig(L, "edgexpu_hip_kv_pool_bytes", C.c_size_t, [C.c_uint32] + [C.c_int] * 5)
+        self.kv_create = _sig(L, "edgexpu_hip_kv_create", _vp, [_vp, C.c_uint32] + [C.c_int] * 6)
+        self.kv_destroy = _sig(L, "edgexpu_hip_kv_destroy", C.c_int, [_vp])
+        self.kv_pool = _sig(L, "edgexpu_hip_kv_pool", _vp, [_vp])
+        self.kv_free_pages = _sig(L, "edgexpu_hip_kv_free_pages", C.c_int, [_vp])
+        self.kv_new = _sig(L, "edgexpu_hip_kv_new", C.c_int, [_vp])
+        self.kv_fork = _sig(L, "edgexpu_hip_kv_fork", C.c_int, [_vp, C.c_int, ip, C.c_int, ip, _vp])
+        self.kv_extend = _sig(L, "edgexpu_hip_kv_extend", C.c_int, [_vp, C.c_int, ip, ip, _vp])
+        self.kv_truncate = _sig(L, "edgexpu_hip_kv_truncate", C.c_int, [_vp, C.c_int, C.c_int])
+        self.kv_release = _sig(L, "edgexpu_hip_kv_release", C.c_int, [_vp, C.c_int, ip])
+        self.kv_compact = _sig(L, "edgexpu_hip_kv_compact", C.c_int, [_vp, ip, _vp])
+        self.kv_length = _sig(L, "edgexpu_hip_kv_length", C.c_int, [_vp, C.c_int])
+        self.kv_tables = _sig(L, "edgexpu_hip_kv_tables", C.c_int, [_vp, C.c_int, ip, ip, C.c_int])
+        self.batch_create = _sig(L, "edgexpu_hip_batch_create", _vp, [_vp, C.c_int, C.c_int, C.c_int])
+        self.batch_destroy = _sig(L, "edgexpu_hip_batch_destroy", None, [_vp])
+        self.batch_set = _sig(L, "edgexpu_hip_batch_set", C.c_int, [_vp, C.c_int, ip, ip, _vp])
+        self.batch_tokens = _sig(L, "edgexpu_hip_batch_tokens", C.c_int, [_vp])
+        self.rope_create = _sig(L, "edgexpu_hip_rope_create", _vp, [C.c_int, C.c_double, C.c_double, _vp, C.c_int])
+        self.rope_destroy = _sig(L, "edgexpu_hip_rope_destroy", None, [_vp])
+        self.qk_norm_rope_dev = _sig(L, "edgexpu_hip_qk_norm_rope_dev", C.c_int,
+                                     [_vp, _vp, _vp, C.c_longlong, _vp, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_int,
+                                      _vp, _vp, C.c_float, _vp, _vp, _vp])
+        self.kv_append_dev = _sig(L, "edgexpu_hip_kv_append_dev", C.c_int,
+                                  [_vp, _vp, C.c_longlong, _vp, C.c_longlong, _vp, C.c_longlong, _vp, C.c_int, _vp, _vp,
+                                   C.c_float, _vp, _vp])
+        self.attention_dev = _sig(L, "edgexpu_hip_attention_dev", C.c_int,
+                                  [_vp, _vp, _vp, C.c_int, C.c_float, _vp])
 
     def last_error(self) -> tuple[int, str]:
         buf = C.create_string_buffer(512)
@@ -375,6 +405,205 @@ def gate_up_silu(w_gate, w_up, qtype: int, x, n_ff: int, n_in: int, norm_weight=
     L.check(L.gate_up_silu_dev(out.data_ptr(), x.data_ptr(), _ptr(norm_weight), eps, w_gate.data_ptr(),
                                w_up.data_ptr(), qtype, _ptr(b_gate), _ptr(b_up), m, n_ff, n_in, _stream()),
             "gate_up_silu")
+    return out
+
+
+# ------------------------------------- rotation, paged cache, attention
+
+
+def _ints(v):
+    return (C.c_int * len(v))(*v)
+
+
+class KvCache:
+    """A paged cache of keys and values (edgexpu_hip_kv_*): ``n_pages`` pages of
+    ``page_tokens`` tokens in each of ``n_layers`` layers, values of type F32, F16
+    or Q8_0.  ``pool`` is its memory, a flat uint8 device tensor (allocated here
+    unless given); sequences are numbers."""
+
+    def __init__(self, qtype: int, n_layers: int, n_kv_heads: int, head_dim: int, page_tokens: int, n_pages: int,
+                 max_seqs: int, pool=None):
+        import torch
+
+        L = hip()
+        self._h = None
+        size = L.kv_pool_bytes(qtype, n_layers, n_kv_heads, head_dim, page_tokens, n_pages)
+        if pool is None:
+            pool = torch.empty(size, dtype=torch.uint8, device="cuda")
+        elif pool.dtype != torch.uint8 or pool.dim() != 1 or not pool.is_contiguous() or pool.numel() != size:
+            raise ValueError(f"pool must be a flat uint8 tensor of {size} bytes")
+        self.pool, self.n_kv_heads, self.head_dim = pool, n_kv_heads, head_dim
+        h = L.kv_create(_ptr(pool) if size else None, qtype, n_layers, n_kv_heads, head_dim, page_tokens, n_pages,
+                        max_seqs)
+        L.check(bool(h), "kv_create")
+        self._h = h
+
+    def __del__(self):
+        if getattr(self, "_h", None) and not sys.is_finalizing():
+            _HIP.kv_destroy(self._h)
+
+    def new(self) -> int:
+        """A new empty sequence."""
+        s = _HIP.kv_new(self._h)
+        _HIP.check(s >= 0, "kv_new")
+        return s
+
+    def fork(self, parents, copy: bool = False) -> list:
+        """A child of each of ``parents``, sharing its pages, or with ``copy`` with copies of them."""
+        n = len(parents)
+        out = (C.c_int * n)()
+        _HIP.check(_HIP.kv_fork(self._h, n, _ints(parents), int(copy), out, _stream()), "kv_fork")
+        return list(out)
+
+    def extend(self, seqs, n_new):
+        """Adds n_new[i] token slots to seqs[i]."""
+        if len(seqs) != len(n_new):
+            raise ValueError("seqs and n_new differ in length")
+        _HIP.check(_HIP.kv_extend(self._h, len(seqs), _ints(seqs), _ints(n_new), _stream()), "kv_extend")
+
+    def truncate(self, seq: int, n_tokens: int):
+        _HIP.check(_HIP.kv_truncate(self._h, seq, n_tokens), "kv_truncate")
+
+    def release(self, seqs):
+        _HIP.check(_HIP.kv_release(self._h, len(seqs), _ints(seqs)), "kv_release")
+
+    def compact(self) -> int:
+        """Moves the pages in use to the front of the pool; returns how many there are."""
+        n = C.c_int()
+        _HIP.check(_HIP.kv_compact(self._h, C.byref(n), _stream()), "kv_compact")
+        return n.value
+
+    def length(self, seq: int) -> int:
+        n = _HIP.kv_length(self._h, seq)
+        if n < 0:
+            raise ValueError(f"sequence {seq} is not in use")
+        return n
+
+    def tables(self, seqs):
+        """The sequences' page numbers, an int32 array [len(seqs), most pages] with -1 behind each."""
+        import numpy as np
+
+        ids, n = _ints(seqs), len(seqs)
+        w = _HIP.kv_tables(self._h, n, ids, None, 0)
+        _HIP.check(w >= 0, "kv_tables")
+        out = np.empty((n, w), dtype=np.int32)
+        if out.size:
+            _HIP.check(_HIP.kv_tables(self._h, n, ids, out.ctypes.data_as(C.POINTER(C.c_int)), w) >= 0, "kv_tables")
+        return out
+
+    def free_pages(self) -> int:
+        return _HIP.kv_free_pages(self._h)
+
+
+class KvBatch:
+    """What one step computes, shared by its layers (edgexpu_hip_batch_*)."""
+
+    def __init__(self, cache: KvCache, n_heads: int, max_seqs: int, max_tokens: int):
+        self._h = None
+        self.cache, self.n_heads = cache, n_heads
+        h = _HIP.batch_create(cache._h, n_heads, max_seqs, max_tokens)
+        _HIP.check(bool(h), "batch_create")
+        self._h = h
+
+    def __del__(self):
+        if getattr(self, "_h", None) and not sys.is_finalizing():
+            _HIP.batch_destroy(self._h)
+
+    def set(self, seqs, n_new):
+        """The last n_new[i] tokens of seqs[i] are the step's."""
+        if len(seqs) != len(n_new):
+            raise ValueError("seqs and n_new differ in length")
+        _HIP.check(_HIP.batch_set(self._h, len(seqs), _ints(seqs), _ints(n_new), _stream()), "batch_set")
+
+    def tokens(self) -> int:
+        return _HIP.batch_tokens(self._h)
+
+
+class Rope:
+    """A model's position rotation (edgexpu_hip_rope_create); ``factors`` n_rot/2 numbers."""
+
+    def __init__(self, n_rot: int, base: float = 10000.0, scale: float = 1.0, factors=None, interleaved: bool = False):
+        L = hip()
+        self._h = None
+        if factors is not None:
+            if len(factors) != n_rot // 2:
+                raise ValueError(f"{len(factors)} factors for {n_rot // 2} pairs")
+            factors = (C.c_float * len(factors))(*factors)
+        h = L.rope_create(n_rot, base, scale, factors, int(interleaved))
+        L.check(bool(h), "rope_create")
+        self._h = h
+
+    def __del__(self):
+        if getattr(self, "_h", None) and not sys.is_finalizing():
+            _HIP.rope_destroy(self._h)
+
+
+def _rows(x, n: int, what: str):
+    """Rows of n float32 values, which may lie apart (a slice of a wider buffer)."""
+    import torch
+
+    if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != n or x.stride(1) != 1:
+        raise ValueError(f"{what} must be float32 [tokens, {n}] with dense rows")
+    return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), n)
+
+
+def qk_norm_rope(q, k, n_heads: int, n_kv_heads: int, pos, rope: Rope | None = None, q_weight=None, k_weight=None,
+                 eps: float = 1e-6, q_out=None, k_out=None):
+    """Per-head RMSNorm and rotation of q [tokens, n_heads * head_dim] and k
+    [tokens, n_kv_heads * head_dim] at the int32 positions ``pos``
+    (edgexpu_hip_qk_norm_rope_dev); rows may be slices of a wider buffer."""
+    import torch
+
+    m, dim = q.shape[0], q.shape[1] // n_heads
+    ldq, ldk = _rows(q, n_heads * dim, "q"), _rows(k, n_kv_heads * dim, "k")
+    if k.shape[0] != m or (pos is not None and (pos.numel() != m or pos.dtype != torch.int32)):
+        raise ValueError("q, k and the int32 pos must have the same tokens")
+    if q_out is None:
+        q_out = torch.empty((m, n_heads * dim), dtype=torch.float32, device=q.device)
+    if k_out is None:
+        k_out = torch.empty((m, n_kv_heads * dim), dtype=torch.float32, device=q.device)
+    L = hip()
+    L.check(L.qk_norm_rope_dev(_ptr(q_out), _ptr(k_out), _ptr(q), ldq, _ptr(k), ldk, m, n_heads, n_kv_heads, dim,
+                               _ptr(q_weight), _ptr(k_weight), eps, rope._h if rope else None, _ptr(pos), _stream()),
+            "qk_norm_rope")
+    return q_out, k_out
+
+
+def kv_append(batch: KvBatch, layer: int, q, k, v, rope: Rope | None = None, q_weight=None, k_weight=None,
+              eps: float = 1e-6, q_out=None):
+    """Norms and rotates the batch's q and k, stores k and v in the cache's
+    ``layer``, returns q (edgexpu_hip_kv_append_dev)."""
+    import torch
+
+    c, m = batch.cache, batch.tokens()
+    dim = c.head_dim
+    ldq = _rows(q, batch.n_heads * dim, "q")
+    ldk, ldv = _rows(k, c.n_kv_heads * dim, "k"), _rows(v, c.n_kv_heads * dim, "v")
+    if min(q.shape[0], k.shape[0], v.shape[0]) < m:
+        raise ValueError(f"q, k and v need the batch's {m} tokens")
+    if q_out is None:
+        q_out = torch.empty((m, batch.n_heads * dim), dtype=torch.float32, device=q.device)
+    L = _HIP
+    L.check(L.kv_append_dev(_ptr(q_out), _ptr(q), ldq, _ptr(k), ldk, _ptr(v), ldv, batch._h, layer, _ptr(q_weight),
+                            _ptr(k_weight), eps, rope._h if rope else None, _stream()), "kv_append")
+    return q_out
+
+
+def attention(batch: KvBatch, layer: int, q, scale: float | None = None, out=None):
+    """Causal attention of the batch's tokens over the cache's ``layer``
+    (edgexpu_hip_attention_dev): q [tokens, n_heads * head_dim] float32; scale
+    1/sqrt(head_dim) unless given."""
+    import torch
+
+    n = batch.n_heads * batch.cache.head_dim
+    if q.dtype != torch.float32 or not q.is_contiguous() or q.numel() < batch.tokens() * n:
+        raise ValueError(f"q must be dense float32 [tokens, {n}] with the batch's {batch.tokens()} tokens")
+    if out is None:
+        out = torch.empty((batch.tokens(), n), dtype=torch.float32, device=q.device)
+    if scale is None:
+        scale = batch.cache.head_dim ** -0.5
+    L = _HIP
+    L.check(L.attention_dev(_ptr(out), _ptr(q), batch._h, layer, scale, _stream()), "attention")
     return out
 
 

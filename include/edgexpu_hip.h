@@ -322,6 +322,141 @@ int edgexpu_hip_gate_up_silu_dev(float *act, const float *x, const float *norm_w
                                  const void *w_up, uint32_t type, const float *b_gate, const float *b_up, int m,
                                  int n_ff, int n_in, void *stream);
 
+/* ---- between the projections: rotation, paged cache, attention ----
+ * What a decoder layer does between its q/k/v and output projections
+ * (per-head norms, RoPE, the key/value cache and attention over it:
+ * src/native.c:2536-2571, src/cpu_kernel.c:659-760, src/kv_cache.c:22-127 of
+ * the reference, where the cache is one sequence's f32 window), for a batch of
+ * sequences on device-resident activations.  A step is
+ *   edgexpu_hip_kv_extend (slots for the new tokens), edgexpu_hip_batch_set
+ *   (what the step computes), then for each layer edgexpu_hip_kv_append_dev
+ *   and edgexpu_hip_attention_dev.
+ * All of these run on the device of edgexpu_hip_init and refuse (error -4) a
+ * caller whose current device is another.  Work on one cache goes to one
+ * stream, or to streams that the caller orders: the host tables change when a
+ * call returns, the device work it queued runs later. */
+
+/* A paged cache of keys and values: n_layers x n_pages pages of page_tokens
+ * tokens.  A layer's page holds K, then V; each holds, for every kv head, the
+ * page's tokens one after the other:
+ *   F32, F16: page_tokens rows of head_dim values;
+ *   Q8_0: page_tokens rows of head_dim int8 codes, then page_tokens rows of
+ *     head_dim/32 f16 scales (the Q8_0 blocks of edgexpu_hip_quantize_q8_0_dev
+ *     with codes and scales apart, so that codes start at 16-byte addresses).
+ * The whole is [layer][page][K, V][kv head], edgexpu_hip_kv_pool_bytes bytes.
+ * head_dim is 64, 96, 128 or 256; page_tokens 16, 32, 64, 128 or 256;
+ * n_pages * page_tokens < 2^31.
+ *
+ * A sequence is a number below max_seqs with a length and a list of pages.
+ * Sequences made by edgexpu_hip_kv_fork share pages; a page that others hold
+ * too is copied before a sequence grows in it.  New pages are the free ones
+ * with the lowest numbers, new sequences the lowest free numbers.  A call that
+ * does not have the pages or sequences it needs is refused (error -6) and
+ * changes nothing. */
+typedef struct edgexpu_hip_kv edgexpu_hip_kv;
+
+/* Bytes of such a pool; 0 (no error) for a shape that is not supported. */
+size_t edgexpu_hip_kv_pool_bytes(uint32_t type, int n_layers, int n_kv_heads, int head_dim, int page_tokens,
+                                 int n_pages);
+/* dev_pool: device memory of that many bytes, 16-byte aligned, not owned and
+ * kept alive by the caller; NULL: allocated here.  NULL on error. */
+edgexpu_hip_kv *edgexpu_hip_kv_create(void *dev_pool, uint32_t type, int n_layers, int n_kv_heads, int head_dim,
+                                      int page_tokens, int n_pages, int max_seqs);
+/* Waits for the device, then frees.  Refused (error -2) while batches of it live. */
+int edgexpu_hip_kv_destroy(edgexpu_hip_kv *kv);
+void *edgexpu_hip_kv_pool(const edgexpu_hip_kv *kv);
+int edgexpu_hip_kv_free_pages(const edgexpu_hip_kv *kv);
+
+/* A new empty sequence; -1 (error -6) when max_seqs are in use. */
+int edgexpu_hip_kv_new(edgexpu_hip_kv *kv);
+/* children[i] = a new sequence with the contents of parents[i] (which may
+ * repeat).  copy == 0: it shares the parent's pages; no device work.  copy != 0:
+ * it gets pages of its own, copied on `stream`. */
+int edgexpu_hip_kv_fork(edgexpu_hip_kv *kv, int n, const int *parents, int copy, int *children, void *stream);
+/* Adds n_new[i] >= 0 token slots to seqs[i] (no sequence twice).  The slots'
+ * contents are whatever the pages held.  Where a sequence grows in a page that
+ * others hold too, the page's tokens are copied to a page of its own on
+ * `stream`, in every layer. */
+int edgexpu_hip_kv_extend(edgexpu_hip_kv *kv, int n, const int *seqs, const int *n_new, void *stream);
+/* Cuts a sequence to its first n_tokens tokens; pages beyond them are let go. */
+int edgexpu_hip_kv_truncate(edgexpu_hip_kv *kv, int seq, int n_tokens);
+/* Ends sequences (no sequence twice): their numbers are free, and their pages
+ * that no other sequence holds. */
+int edgexpu_hip_kv_release(edgexpu_hip_kv *kv, int n, const int *seqs);
+/* Closes the pool up: with L pages in use, those numbered L and above move (in
+ * every layer, on `stream`) to the free ones below L, both in ascending order.
+ * *n_used (may be NULL) receives L: pages from L on are then unused. */
+int edgexpu_hip_kv_compact(edgexpu_hip_kv *kv, int *n_used, void *stream);
+/* Length in tokens of a sequence; -1 for a number that is not in use. */
+int edgexpu_hip_kv_length(const edgexpu_hip_kv *kv, int seq);
+/* Writes the page numbers of seqs[i] to out[i * ld ...], -1 behind them.
+ * Returns the largest page count (out may be NULL to ask for it), -1 on error
+ * (a number not in use, ld below the largest count). */
+int edgexpu_hip_kv_tables(const edgexpu_hip_kv *kv, int n, const int *seqs, int *out, int ld);
+
+/* What one step computes, shared by the layers of the step: the last
+ * n_new[i] >= 0 tokens of seqs[i] (no sequence twice) are the step's tokens, in
+ * that order; the tables are read here, and attention is planned: runs of pages
+ * that several of the sequences share (edgexpu_hip_kv_fork) are read once for
+ * all of them where that saves more than it costs.  Any later change to the
+ * cache's sequences makes the batch stale: calls with it are refused (error
+ * -2) until it is set again.
+ * n_heads: query heads, a multiple of the cache's kv heads (query head h reads
+ * kv head h / (n_heads / n_kv_heads)).
+ * edgexpu_hip_batch_set copies the plan to the device on `stream`; it is
+ * refused (error -7) while a stream of this thread is captured.  Its device
+ * buffers grow as plans need; a batch that a captured call has used keeps its
+ * buffers, and a plan that outgrows them is refused (error -7): set the largest
+ * one before the capture.  A captured step replays with whatever plan the last
+ * set has put there.  Calls of one batch share its workspace: on one stream, or
+ * ordered by the caller. */
+typedef struct edgexpu_hip_batch edgexpu_hip_batch;
+edgexpu_hip_batch *edgexpu_hip_batch_create(edgexpu_hip_kv *kv, int n_heads, int max_seqs, int max_tokens);
+/* Waits for the device, then frees. */
+void edgexpu_hip_batch_destroy(edgexpu_hip_batch *b);
+int edgexpu_hip_batch_set(edgexpu_hip_batch *b, int n, const int *seqs, const int *n_new, void *stream);
+/* Tokens of the last set; 0 before one. */
+int edgexpu_hip_batch_tokens(const edgexpu_hip_batch *b);
+
+/* The rotation of a model: the first n_rot values of a head (even, at most
+ * 256) turn in pairs by position * scale * base^(-2i / n_rot) / factors[i] (host
+ * array of n_rot/2, NULL: ones), pair i being the values i and i + n_rot/2, or
+ * with `interleaved` 2i and 2i + 1 (the reference's two RoPE forms,
+ * src/cpu_kernel.c:659-760).  Angles are kept in 64 bits and reduced there, so
+ * far positions lose nothing.  NULL on error. */
+typedef struct edgexpu_hip_rope edgexpu_hip_rope;
+edgexpu_hip_rope *edgexpu_hip_rope_create(int n_rot, double base, double scale, const float *factors,
+                                          int interleaved);
+void edgexpu_hip_rope_destroy(edgexpu_hip_rope *r);
+
+/* Per-head RMSNorm (q_weight, k_weight: head_dim values each, NULL: none) and
+ * rotation (rope NULL: none) of q [m][n_heads][head_dim] and k
+ * [m][n_kv_heads][head_dim] in one pass; token t stands at pos[t] >= 0 (device
+ * int32).  Rows start ldq, ldk values apart (q, k and v may be slices of one
+ * buffer); q_out and k_out are dense and may be q and k where those are dense
+ * too.  head_dim even, at most 256.  k and k_out may be NULL with n_kv_heads 0. */
+int edgexpu_hip_qk_norm_rope_dev(float *q_out, float *k_out, const float *q, long long ldq, const float *k,
+                                 long long ldk, int m, int n_heads, int n_kv_heads, int head_dim,
+                                 const float *q_weight, const float *k_weight, float eps,
+                                 const edgexpu_hip_rope *rope, const int32_t *pos, void *stream);
+/* The same for the batch's tokens at their positions, with k (normed and
+ * rotated) and v written to their slots of the cache in `layer` instead of
+ * k_out.  Values are rounded once, to nearest, to the cache's type (f16: beyond
+ * 65504 infinity; Q8_0 as edgexpu_hip_quantize_q8_0_dev).  Refused (error -2)
+ * where a slot's page is held by another sequence too. */
+int edgexpu_hip_kv_append_dev(float *q_out, const float *q, long long ldq, const float *k, long long ldk,
+                              const float *v, long long ldv, edgexpu_hip_batch *b, int layer, const float *q_weight,
+                              const float *k_weight, float eps, const edgexpu_hip_rope *rope, void *stream);
+/* out[t][h] = sum_j softmax_j(scale * q[t][h] . K_j) V_j over the positions j
+ * up to token t's own of its sequence, for the batch's tokens: q and out
+ * [tokens][n_heads][head_dim] f32, dense, 16-byte aligned, out may be q.
+ * Products of f16 and Q8_0 caches run on the matrix cores with q and the
+ * weights as two f16 parts each (22 bits), sums in f32: results as those of 32
+ * bits.  Contents of slots that a token does not see (behind the sequence's
+ * end, or of later tokens of the step) have no influence, NaN and infinities
+ * included. */
+int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip_batch *b, int layer, float scale, void *stream);
+
 /* ---- host-pointer entry points (synchronous: inputs copied in, outputs
  * copied out before return; the PCIe copies are part of the call) ---- */
 
