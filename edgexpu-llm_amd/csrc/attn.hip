@@ -1,11 +1,40 @@
 // Attention of a step's tokens over the paged cache, by the plan of
-// attn_plan.h: out = sum_j p_j V_j / sum_j p_j, p_j = exp(scale q.K_j - m).
+// attn_plan.h: out = sum_j p_j V_j / sum_j p_j, p_j = exp(scale q.K_j - m), one
+// pass over the keys with the running maximum m and sum.
+//
+// Both products run on the matrix cores with the keys as the rows of the
+// first operand, so that a query row is one column, held by the four lanes
+// l, l + 16, l + 32, l + 48 through everything:
+//   S^T = K Q^T   (16 keys x 16 query rows a tile): lane l gets, for query row
+//                 l % 16, the keys 4 (l / 16) + r, r = 0..3;
+//   O^T = V^T P^T (16 values x 16 query rows): the weights a lane has are the
+//                 weights it must supply, in an order of keys that the V
+//                 operand follows; no exchange between lanes.
+// K and V come into LDS by DMA (16-byte pieces of a row permuted so that the
+// reads below meet no bank twice); V is read transposed (ds_read_..._tr).
+//
+// Arithmetic.  F16 and Q8_0: q (after an exact power-of-two scaling of its row
+// that keeps both parts in range) and the weights as two f16 parts, high and
+// rest, 22 bits together, against f16 values or the integer codes (exact in
+// f16); two products each, f32 sums: the error of f32 arithmetic, at twice the
+// matrix work, which stays under the time of the loads wherever few rows share
+// them.  A single f16 part would lose 2^-12 of every weight.  Q8_0 scales are
+// applied to the partial sums of a block (K) and to the weights (V).  F32:
+// the f32 matrix instructions.  Weights are 2^(s - m + 7) with m at most 8
+// behind the true maximum: it is raised, and the sums rescaled, only when a
+// tile exceeds it by 2^8 (an exponent range the f16 parts have to spare).
 #include <hip/hip_runtime.h>
 
+#include "gemm_common.h"
 #include "kv.h"
 #include "lib.h"
 
 namespace exq {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef int v2i __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -20,72 +49,662 @@ struct AttnArgs {
     size_t part_cap;
 };
 
-// One value of a cached row.
-template <int TYPE>
-__device__ __forceinline__ float kv_value(const uint8_t *head, int off, int e, int dim, int page_tokens) {
-    if (TYPE == kTypeF32) return reinterpret_cast<const float *>(head)[(size_t)off * dim + e];
-    if (TYPE == kTypeF16) return (float)reinterpret_cast<const _Float16 *>(head)[(size_t)off * dim + e];
-    const float d = (float)reinterpret_cast<const _Float16 *>(head + (size_t)page_tokens * dim)[off * (dim / 32) + e / 32];
-    return (float)reinterpret_cast<const int8_t *>(head)[(size_t)off * dim + e] * d;
+// Sizes of a tile of TT keys: a unit is its K or its V rows in LDS.
+template <int TYPE, int DIM>
+struct Geo {
+    static constexpr int TT = TYPE == kTypeF32 ? 16 : 32;
+    static constexpr int HALVES = TT / 16;
+    static constexpr int RB = TYPE == kTypeF32 ? DIM * 4 : TYPE == kTypeF16 ? DIM * 2 : DIM;  // row bytes
+    static constexpr int CPR = RB / 16;                                                      // 16-byte pieces
+    static constexpr int NB = DIM / 32;
+    static constexpr int SB = TYPE == kTypeQ8_0 ? 2 * NB : 0;  // scale bytes of a row
+    static constexpr int UNIT = TT * (RB + SB);
+    static constexpr int CODE_OPS = (16 * RB + 1023) / 1024;  // DMA instructions for 16 rows
+    static constexpr int HALF_OPS = CODE_OPS + (SB ? 1 : 0);
+    static constexpr int OPS = HALVES * HALF_OPS;
+    static constexpr int ND = DIM / 16;
+    // few rows: each wave has its own ring of units; many rows: tiles shared by the workgroup
+    static constexpr int RING = UNIT * 16 <= 80 * 1024 ? 4 : 2;
+    static constexpr int SHARED = 3;
+    static constexpr int RT = DIM == 256 ? 1 : 2;  // 16-row tiles of a wave, many rows
+    static constexpr int LDS = 4 * RING * UNIT > SHARED * 2 * UNIT ? 4 * RING * UNIT : SHARED * 2 * UNIT;
+    static constexpr int MERGE = 4 * 16 * (DIM + 2) * 4;
+    static constexpr int LDS_BYTES = LDS > MERGE ? LDS : MERGE;
+};
+
+// Piece permutation of row `row` of a tile: piece c lies at c ^ swz.  Chosen so
+// that 16 rows read at one piece (K), or 8 rows at two neighbouring pieces and
+// 16 rows at one (V, transposed reads of 16 and 8 bits), or 4 rows 4 apart at
+// 4 pieces (V, F32), fall on different banks of 64.
+template <int TYPE, int DIM, bool V>
+__device__ __forceinline__ int swz(int row) {
+    if (TYPE == kTypeF32) {
+        if (DIM == 96) return (row >> 1) & 7;
+        return ((row >> 2) & 3) << 2 | (row & 3);
+    }
+    if (TYPE == kTypeF16) {
+        if (DIM == 64) return ((row >> 1) & 3) << 1 | ((row >> 3) & 1);
+        if (DIM == 96) return ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
+        return (row & 7) << 1 | ((row >> 3) & 1);
+    }
+    if (V) {
+        const int b4 = (row >> 4) & 1;
+        if (DIM == 64) return ((row >> 2) & 1) | b4 << 1;
+        if (DIM == 96) return b4;
+        if (DIM == 128) return ((row >> 1) & 3) | b4 << 2;
+        return (row & 7) | b4 << 3;
+    }
+    if (DIM == 64) return (row >> 2) & 3;
+    if (DIM == 96) return (row >> 3) & 1;
+    if (DIM == 128) return (row >> 1) & 7;
+    return row & 15;
 }
 
-// One wave a row, its keys one after the other.
+__device__ __forceinline__ float xor16(float v) {
+    return __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(v), 0x401f));
+}
+// Maximum and sum over the four lanes of a query row.
+__device__ __forceinline__ float col_max(float v) {
+    v = fmaxf(v, xor16(v));
+    return fmaxf(v, shfl_xor_f(v, 32));
+}
+__device__ __forceinline__ float col_sum(float v) {
+    v += xor16(v);
+    return v + shfl_xor_f(v, 32);
+}
+
+// High part and rest of eight values.
+__device__ __forceinline__ void split8(const float (&x)[8], v8h &hi, v8h &lo) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        hi[j] = (_Float16)x[j];
+        lo[j] = (_Float16)(x[j] - (float)hi[j]);
+    }
+}
+
+// Four signed bytes as f16 (exact): 1024 + (byte + 128) built by v_perm, minus 1152.
+__device__ __forceinline__ void bytes_h4(uint32_t w, _Float16 *o) {
+    const uint32_t u = w ^ 0x80808080u;
+    h2 p[2];
+    bytes_to_h2(u, 0x64646464u, p);
+    const h2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+    p[0] = p[0] - off;
+    p[1] = p[1] - off;
+    o[0] = p[0][0];
+    o[1] = p[0][1];
+    o[2] = p[1][0];
+    o[3] = p[1][1];
+}
+__device__ __forceinline__ v8h bytes_h8(uint32_t a, uint32_t b) {
+    _Float16 o[8];
+    bytes_h4(a, o);
+    bytes_h4(b, o + 4);
+    return v8h{o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7]};
+}
+
+__device__ __forceinline__ v4f mfma16(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ v4f mfma4(float a, float b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+typedef __attribute__((address_space(3))) v2i lds_v2i;
+
+__device__ __forceinline__ void lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// Where a piece of work reads: the pages of one kv head of one layer.
+struct Source {
+    const __attribute__((address_space(4))) int32_t *pages;  // page of position p: pages[p >> shift]
+    const uint8_t *base;                                      // the layer's, at this head's K
+    size_t page_bytes;
+    uint32_t head_bytes, v_off;
+    int shift, last;  // last: the highest page index there is
+};
+
 template <int TYPE, int DIM>
-__global__ __launch_bounds__(256) void attn_kernel(const AttnArgs a) {
-    const PlanHeader *hd = reinterpret_cast<const PlanHeader *>(a.head);
-    const AttnItem *items = reinterpret_cast<const AttnItem *>(hd + 1);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n_kv = a.kv.n_kv;
-    constexpr int E = (DIM + 63) / 64;
-    for (long long w = blockIdx.x; w < (long long)hd->n_items * n_kv; w += gridDim.x) {
-        const AttnItem it = items[w / n_kv];
-        const int h = (int)(w % n_kv);
-        for (int r = wave; r < it.n_rows; r += 4) {
-            const int row = it.row0 + r, g = row % a.group;
+struct Loader {
+    using G = Geo<TYPE, DIM>;
+    // One DMA of 16 rows' unit `which`: sub-operation `sub`, from the tile at position p0, half hf, to LDS byte `to`.
+    static __device__ __forceinline__ void op(const Source &s, int which, int hf, int sub, int p0, uint32_t to, int lane) {
+        const int p = p0 + 16 * hf;
+        const int page = __builtin_amdgcn_readfirstlane(s.pages[min(p >> s.shift, s.last)]);
+        const uint8_t *b = s.base + (size_t)page * s.page_bytes + (which ? s.v_off : 0u);
+        const v4u rs = rsrc_words(b, s.head_bytes);
+        const uint32_t off = (uint32_t)(p & ((1 << s.shift) - 1));
+        if (G::SB != 0 && sub == G::CODE_OPS) {
+            const uint32_t so = ((uint32_t)DIM << s.shift) + off * G::SB;
+            if (lane < G::SB) dma16(to + G::TT * G::RB + hf * 16 * G::SB, lane * 16, rs, so);
+            return;
+        }
+        const int at = sub * 1024 + lane * 16, row = at / G::RB, piece = at % G::RB / 16;
+        const int sw = which ? swz<TYPE, DIM, true>(hf * 16 + row) : swz<TYPE, DIM, false>(hf * 16 + row);
+        const uint32_t vo = (uint32_t)(row * G::RB + ((piece ^ sw) * 16)), so = off * G::RB;
+        const uint32_t dst = to + hf * 16 * G::RB + sub * 1024;
+        if (16 * G::RB % 1024 != 0 && sub == G::CODE_OPS - 1) {
+            if (lane < 16 * G::RB % 1024 / 16) dma16(dst, vo, rs, so);
+        } else {
+            dma16(dst, vo, rs, so);
+        }
+    }
+    // A whole unit by one wave.
+    static __device__ __forceinline__ void unit(const Source &s, int which, int p0, uint32_t to, int lane) {
+#pragma unroll
+        for (int hf = 0; hf < G::HALVES; ++hf)
+#pragma unroll
+            for (int k = 0; k < G::HALF_OPS; ++k) op(s, which, hf, k, p0, to, lane);
+    }
+    // This wave's part of a tile's two units (every wave issues the same number).
+    static constexpr int TILE_OPS = 2 * G::OPS, SHARE = (TILE_OPS + 3) / 4;
+    static __device__ __forceinline__ void share(const Source &s, int p0, uint32_t to, int wave, int lane) {
+#pragma unroll
+        for (int k = 0; k < SHARE; ++k) {
+            int j = wave + 4 * k;
+            if (j >= TILE_OPS) j -= 4;  // once more what it has just loaded
+            const int which = j >= G::OPS ? 1 : 0, i = j - which * G::OPS;
+            op(s, which, i / G::HALF_OPS, i % G::HALF_OPS, p0, to + which * G::UNIT, lane);
+        }
+    }
+};
+
+// A wave's query rows: RT tiles of 16, row l % 16 of a tile on lane l.
+template <int TYPE, int DIM, int RT>
+struct Rows {
+    using G = Geo<TYPE, DIM>;
+    static constexpr int NQ = TYPE == kTypeF32 ? G::ND : G::NB;
+    v8h qh[TYPE == kTypeF32 ? 1 : RT][TYPE == kTypeF32 ? 1 : G::NB], ql[TYPE == kTypeF32 ? 1 : RT][TYPE == kTypeF32 ? 1 : G::NB];
+    v4f qf[TYPE == kTypeF32 ? RT : 1][TYPE == kTypeF32 ? G::ND : 1];
+    float rs[RT], m[RT], l[RT];  // score factor; running maximum (of base-2 exponents), this lane's part of the sum
+    int lim[RT];                 // positions below are seen
+    v4f acc[RT][G::ND];
+    int ve;                      // Q8_0: acc is in units of 2^ve
+    float s[RT][G::HALVES][4];
+
+    __device__ __forceinline__ void load(const AttnArgs &a, const AttnItem &it, int h, int row_from, int lane) {
+        const int g = lane >> 4;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const int r = min(row_from + 16 * t + (lane & 15), it.n_rows - 1), row = it.row0 + r;
             const PlanToken *pt = reinterpret_cast<const PlanToken *>(a.head) - (row / a.group + 1);
-            const int token = pt->order, key1 = it.causal ? min(it.key1, pt->order_pos + 1) : it.key1;
-            const size_t at = (((size_t)token * n_kv + h) * a.group + g) * DIM;
-            float qv[E], acc[E], m = -INFINITY, l = 0.0f;
+            lim[t] = it.causal ? min(it.key1, pt->order_pos + 1) : it.key1;
+            const float *q = a.q + (((size_t)pt->order * a.kv.n_kv + h) * a.group + row % a.group) * DIM;
+            if constexpr (TYPE == kTypeF32) {
 #pragma unroll
-            for (int j = 0; j < E; ++j) {
-                qv[j] = lane + 64 * j < DIM ? a.q[at + lane + 64 * j] : 0.0f;
-                acc[j] = 0.0f;
+                for (int c = 0; c < G::ND; ++c) qf[t][c] = *reinterpret_cast<const v4f *>(q + c * 16 + g * 4);
+                rs[t] = a.scale * kLog2e;
+            } else {
+                float x[G::NB][8], top = 0.0f;
+#pragma unroll
+                for (int c = 0; c < G::NB; ++c) {
+                    const v4f u = *reinterpret_cast<const v4f *>(q + c * 32 + g * 8);
+                    const v4f v = *reinterpret_cast<const v4f *>(q + c * 32 + g * 8 + 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        x[c][j] = u[j];
+                        x[c][4 + j] = v[j];
+                        top = fmaxf(top, fmaxf(fabsf(u[j]), fabsf(v[j])));
+                    }
+                }
+                top = col_max(top);
+                // the row's largest value in [2^14, 2^15)
+                const int e = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
+#pragma unroll
+                for (int c = 0; c < G::NB; ++c) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[c][j] = ldexpf(x[c][j], -e);
+                    split8(x[c], qh[t][c], ql[t][c]);
+                }
+                rs[t] = ldexpf(a.scale * kLog2e, e);
             }
-            for (int p = it.key0; p < key1; ++p) {
-                const int page = a.head[it.page_at + (p >> a.kv.page_shift)], off = p & (a.page_tokens - 1);
-                const uint8_t *k = a.kv.base + (size_t)page * a.kv.page_bytes + (size_t)h * a.kv.head_bytes;
-                const uint8_t *v = k + (size_t)n_kv * a.kv.head_bytes;
-                float s = 0.0f;
+            m[t] = -INFINITY;
+            l[t] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < E; ++j)
-                    if (lane + 64 * j < DIM) s = fmaf(qv[j], kv_value<TYPE>(k, off, lane + 64 * j, DIM, a.page_tokens), s);
+            for (int d = 0; d < G::ND; ++d) acc[t][d] = v4f{0, 0, 0, 0};
+        }
+        ve = -24;
+    }
+
+    // Scores of the K unit at ku.
+    __device__ __forceinline__ void scores(const uint8_t *ku, int lane) {
+        const int g = lane >> 4, c16 = lane & 15;
 #pragma unroll
-                for (int o = 32; o > 0; o >>= 1) s += shfl_xor_f(s, o);
-                s *= a.scale * kLog2e;
-                const float mn = fmaxf(m, s);
-                const float c = m == -INFINITY ? 0.0f : exp2f(m - mn), e = exp2f(s - mn);
-                l = l * c + e;
+        for (int hf = 0; hf < G::HALVES; ++hf) {
+            const int row = hf * 16 + c16, sw = swz<TYPE, DIM, false>(row);
+            const uint8_t *kr = ku + row * G::RB;
+            v4f o[RT];
 #pragma unroll
-                for (int j = 0; j < E; ++j)
-                    if (lane + 64 * j < DIM)
-                        acc[j] = fmaf(e, kv_value<TYPE>(v, off, lane + 64 * j, DIM, a.page_tokens), acc[j] * c);
-                m = mn;
+            for (int t = 0; t < RT; ++t) o[t] = v4f{0, 0, 0, 0};
+            if constexpr (TYPE == kTypeF32) {
+#pragma unroll
+                for (int c = 0; c < G::ND; ++c) {
+                    const v4f k = *reinterpret_cast<const v4f *>(kr + (((c * 4 + g) ^ sw) * 16));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int t = 0; t < RT; ++t) o[t] = mfma4(k[j], qf[t][c][j], o[t]);
+                }
+            } else if constexpr (TYPE == kTypeF16) {
+#pragma unroll
+                for (int c = 0; c < G::NB; ++c) {
+                    const v8h k = *reinterpret_cast<const v8h *>(kr + (((c * 4 + g) ^ sw) * 16));
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) o[t] = mfma16(k, ql[t][c], o[t]);
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) o[t] = mfma16(k, qh[t][c], o[t]);
+                }
+            } else {
+                const _Float16 *ds = reinterpret_cast<const _Float16 *>(ku + G::TT * G::RB) + (hf * 16 + g * 4) * G::NB;
+#pragma unroll
+                for (int c = 0; c < G::NB; ++c) {
+                    const v2u w = *reinterpret_cast<const v2u *>(kr + (((c * 2 + (g >> 1)) ^ sw) * 16) + (g & 1) * 8);
+                    const v8h k = bytes_h8(w[0], w[1]);
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) {
+                        v4f b = mfma16(k, ql[t][c], v4f{0, 0, 0, 0});
+                        b = mfma16(k, qh[t][c], b);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[t][r] = fmaf((float)ds[r * G::NB + c], b[r], o[t][r]);
+                    }
+                }
             }
-            if (it.part < 0) {
 #pragma unroll
-                for (int j = 0; j < E; ++j)
-                    if (lane + 64 * j < DIM) a.out[at + lane + 64 * j] = acc[j] / l;
-                continue;
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[t][hf][r] = o[t][r] * rs[t];
+        }
+    }
+
+    // Positions at or past a row's limit get no weight.
+    __device__ __forceinline__ void mask(int p0, int lane) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int hf = 0; hf < G::HALVES; ++hf)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (p0 + hf * 16 + (lane >> 4) * 4 + r >= lim[t]) s[t][hf][r] = -INFINITY;
+    }
+
+    __device__ __forceinline__ void rescale(float c, int t) {
+#pragma unroll
+        for (int d = 0; d < G::ND; ++d) acc[t][d] *= c;
+    }
+
+    // Scores become weights; the maximum is raised where they exceed it by 8.
+    __device__ __forceinline__ void weights() {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int hf = 0; hf < G::HALVES; ++hf)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][hf][r]);
+            if (__builtin_amdgcn_ballot_w64(top > m[t] + 8.0f) != 0) {
+                const float mn = fmaxf(m[t], col_max(top));
+                const float c = m[t] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[t] - mn);
+                m[t] = mn;
+                l[t] *= c;
+                rescale(c, t);
             }
-            const size_t ps = (size_t)(it.part + r) * n_kv + h;
+            const float off = m[t] == -INFINITY ? 0.0f : m[t] - 7.0f;
 #pragma unroll
-            for (int j = 0; j < E; ++j)
-                if (lane + 64 * j < DIM) a.part[ps * DIM + lane + 64 * j] = acc[j];
-            if (lane == 0) {
-                float *ml = a.part + a.part_cap * DIM + 2 * ps;
-                ml[0] = m;
-                ml[1] = l;
+            for (int hf = 0; hf < G::HALVES; ++hf)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[t][hf][r] = __builtin_amdgcn_exp2f(s[t][hf][r] - off);
+                    l[t] += s[t][hf][r];
+                }
+        }
+    }
+
+    // acc += V^T P^T for the V unit at vu.
+    __device__ __forceinline__ void values(const uint8_t *vu, int lane) {
+        const int g = lane >> 4, c16 = lane & 15;
+        if constexpr (TYPE == kTypeF32) {
+#pragma unroll
+            for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = g * 4 + r, sw = swz<TYPE, DIM, true>(row);
+                    const float v = *reinterpret_cast<const float *>(vu + row * G::RB + (((d * 4 + (c16 >> 2)) ^ sw) * 16) + (c16 & 3) * 4);
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) acc[t][d] = mfma4(v, s[t][0][r], acc[t][d]);
+                }
+        } else if constexpr (TYPE == kTypeF16) {
+            v8h ph[RT], pl[RT];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const float p[8] = {s[t][0][0], s[t][0][1], s[t][0][2], s[t][0][3], s[t][1][0], s[t][1][1], s[t][1][2], s[t][1][3]};
+                split8(p, ph[t], pl[t]);
+            }
+            const int row = g * 4 + (c16 >> 2), sw = swz<TYPE, DIM, true>(row);  // the same for row + 16
+#pragma unroll
+            for (int d = 0; d < G::ND; ++d) {
+                const uint8_t *at = vu + row * G::RB + (((d * 2 + ((c16 >> 1) & 1)) ^ sw) * 16) + (c16 & 1) * 8;
+                const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)at);
+                const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(at + 16 * G::RB));
+                const v8h v = __builtin_bit_cast(v8h, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, pl[t], acc[t][d]);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, ph[t], acc[t][d]);
+            }
+        } else {
+            // this lane's keys: 4 g + r of both halves; their blocks' scales
+            const _Float16 *ds = reinterpret_cast<const _Float16 *>(vu + G::TT * G::RB) + g * 4 * G::NB;
+            float sc[2][4][G::NB], top = 0.0f;
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int b = 0; b < G::NB; ++b) {
+                        sc[hf][r][b] = (float)ds[(hf * 16 + r) * G::NB + b];
+                        top = fmaxf(top, fabsf(sc[hf][r][b]));
+                    }
+            // scales at most 1 in the units of acc: weights times scale stay in f16's range
+            if (__builtin_amdgcn_ballot_w64(top > ldexpf(1.0f, ve)) != 0) {
+                top = col_max(top);
+                const int e = top < INFINITY ? __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top)) : 16;
+                if (e > ve) {
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) rescale(ldexpf(1.0f, ve - e), t);
+                    ve = e;
+                }
+            }
+            const float f = ldexpf(1.0f, -ve);
+            const int k = c16 >> 1, row = (k < 4 ? g * 4 + k : 16 + g * 4 + k - 4), sw = swz<TYPE, DIM, true>(row);
+#pragma unroll
+            for (int b = 0; b < G::NB; ++b) {
+                v8h ph[RT], pl[RT];
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    float p[8];
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) p[hf * 4 + r] = s[t][hf][r] * (sc[hf][r][b] * f);
+                    split8(p, ph[t], pl[t]);
+                }
+#pragma unroll
+                for (int d = 2 * b; d < 2 * b + 2; ++d) {
+                    const uint8_t *at = vu + row * G::RB + ((d ^ sw) * 16) + (c16 & 1) * 8;
+                    const v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)at);
+                    const v8h v = bytes_h8((uint32_t)w[0], (uint32_t)w[1]);
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, pl[t], acc[t][d]);
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, ph[t], acc[t][d]);
+                }
             }
         }
+    }
+
+    // Whether any value that this tile's rows may read is not finite.
+    __device__ __forceinline__ bool odd_values(const uint8_t *vu, int lane) {
+        bool bad = false;
+        if (TYPE == kTypeF32) {
+            for (int i = lane * 4; i < G::TT * G::RB; i += 256)
+                bad |= (*reinterpret_cast<const uint32_t *>(vu + i) & 0x7f800000u) == 0x7f800000u;
+        } else {
+            const uint8_t *at = TYPE == kTypeF16 ? vu : vu + G::TT * G::RB;
+            for (int i = lane * 4; i < (TYPE == kTypeF16 ? G::TT * G::RB : G::TT * G::SB); i += 256) {
+                const uint32_t w = *reinterpret_cast<const uint32_t *>(at + i);
+                bad |= (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
+            }
+        }
+        return __builtin_amdgcn_ballot_w64(bad) != 0;
+    }
+
+    // values() for a tile with infinities or NaN in it, at the causal limit: 0 *
+    // infinity must not reach the rows that do not see them.  Key by key.
+    __device__ __forceinline__ void values_one_by_one(const uint8_t *vu, int p0, int lane) {
+        const int g = lane >> 4;
+        const float unit = TYPE == kTypeQ8_0 ? ldexpf(1.0f, -ve) : 1.0f;
+#pragma unroll 1
+        for (int row = 0; row < G::TT; ++row) {
+            const int sw = swz<TYPE, DIM, true>(row);
+            float p[RT];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                float mine = 0.0f;  // this lane's weight of key 16 hf + 4 g + r
+#pragma unroll
+                for (int i = 0; i < 4 * G::HALVES; ++i)
+                    if (i == (row >> 4) * 4 + (row & 3)) mine = s[t][i >> 2][i & 3];
+                p[t] = __shfl(mine, ((row >> 2) & 3) * 16 + (lane & 15), 64);
+            }
+#pragma unroll
+            for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = d * 16 + g * 4 + j;
+                    constexpr int es = TYPE == kTypeF32 ? 4 : TYPE == kTypeF16 ? 2 : 1;
+                    const uint8_t *at = vu + row * G::RB + (((e * es / 16) ^ sw) * 16) + e * es % 16;
+                    float v;
+                    if (TYPE == kTypeF32) v = *reinterpret_cast<const float *>(at);
+                    else if (TYPE == kTypeF16) v = (float)*reinterpret_cast<const _Float16 *>(at);
+                    else
+                        v = (float)*reinterpret_cast<const int8_t *>(at) * unit *
+                            (float)reinterpret_cast<const _Float16 *>(vu + G::TT * G::RB)[row * G::NB + e / 32];
+#pragma unroll
+                    for (int t = 0; t < RT; ++t)
+                        if (p0 + row < lim[t]) acc[t][d][j] = fmaf(p[t], v, acc[t][d][j]);
+                }
+        }
+    }
+
+    // No row of the wave sees this position or any behind it.
+    __device__ __forceinline__ int last_limit() const {
+        int v = lim[RT - 1];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) v = max(v, lim[t]);
+        return __builtin_amdgcn_readlane(v, 15);
+    }
+
+    // acc in units of one, l the row's whole sum.
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            l[t] = col_sum(l[t]);
+            if (TYPE == kTypeQ8_0) rescale(ldexpf(1.0f, ve), t);
+        }
+    }
+};
+
+// Slots past the last key may hold anything: their V rows (their scales) become zero in LDS.
+template <int TYPE, int DIM>
+__device__ __forceinline__ void clear_tail(uint8_t *vu, int valid, int tid, int n) {
+    using G = Geo<TYPE, DIM>;
+    if (TYPE == kTypeQ8_0) {
+        for (int i = valid * G::SB / 2 + tid; i < G::TT * G::SB / 2; i += n)
+            reinterpret_cast<uint16_t *>(vu + G::TT * G::RB)[i] = 0;
+    } else {
+        for (int i = valid * G::CPR + tid; i < G::TT * G::CPR; i += n) reinterpret_cast<v4u *>(vu)[i] = v4u{0, 0, 0, 0};
+    }
+}
+
+// The rows of one column tile: token and head of row r of the item.
+__device__ __forceinline__ float *out_row(const AttnArgs &a, const AttnItem &it, int h, int r, int dim) {
+    const int row = it.row0 + r;
+    const PlanToken *pt = reinterpret_cast<const PlanToken *>(a.head) - (row / a.group + 1);
+    return a.out + (((size_t)pt->order * a.kv.n_kv + h) * a.group + row % a.group) * dim;
+}
+
+// Few rows (at most 16): the four waves take every fourth tile of keys each, on
+// their own (no barrier), and join their sums at the end.
+template <int TYPE, int DIM>
+__device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it, const Source &src, int h, uint8_t *lds,
+                                           int wave, int lane) {
+    using G = Geo<TYPE, DIM>;
+    using L = Loader<TYPE, DIM>;
+    Rows<TYPE, DIM, 1> w;
+    const int tiles = (it.key1 - it.key0 + G::TT - 1) / G::TT;
+    const int mine = (tiles - wave + 3) / 4, units = 2 * mine;
+    const uint32_t ring = lds_addr(lds) + wave * G::RING * G::UNIT;
+    uint8_t *ringp = lds + wave * G::RING * G::UNIT;
+    const auto pos = [&](int u) { return it.key0 + (wave + 4 * (u >> 1)) * G::TT; };
+    const auto issue = [&](int u) {
+        if (u < units) L::unit(src, u & 1, pos(u), ring + (u % G::RING) * G::UNIT, lane);
+    };
+    const auto arrive = [&](int u) {  // unit u is there; what was read before it may be overwritten
+        if (u + G::RING - 2 < units) wait_dma<(G::RING - 2) * G::OPS>();
+        else wait_dma<0>();
+        lds_done();
+        issue(u + G::RING - 1);
+    };
+    w.load(a, it, h, 0, lane);
+    wait_dma<0>();
+    for (int u = 0; u < G::RING - 1; ++u) issue(u);
+    // the first row's limit: a tile below it needs no mask
+    const int first = it.causal ? __builtin_amdgcn_readfirstlane(w.lim[0]) : it.key1;
+    for (int i = 0; i < mine; ++i) {
+        const int p0 = pos(2 * i);
+        const bool edge = p0 + G::TT > first;
+        arrive(2 * i);
+        w.scores(ringp + (2 * i % G::RING) * G::UNIT, lane);
+        if (edge) w.mask(p0, lane);
+        w.weights();
+        arrive(2 * i + 1);
+        uint8_t *vu = ringp + ((2 * i + 1) % G::RING) * G::UNIT;
+        if (edge) {
+            if (p0 + G::TT > it.key1) {
+                clear_tail<TYPE, DIM>(vu, it.key1 - p0, lane, 64);
+                lds_done();
+            }
+            if (w.odd_values(vu, lane)) {
+                w.values_one_by_one(vu, p0, lane);
+                continue;
+            }
+        }
+        w.values(vu, lane);
+    }
+    w.finish();
+    // join the waves: [wave][row][DIM], then maxima and sums
+    __syncthreads();
+    float *mo = reinterpret_cast<float *>(lds), *ml = mo + 4 * 16 * DIM;
+    const int c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int d = 0; d < G::ND; ++d) *reinterpret_cast<v4f *>(mo + (wave * 16 + c) * DIM + d * 16 + g * 4) = w.acc[0][d];
+    if (g == 0) {
+        ml[2 * (wave * 16 + c)] = w.m[0];
+        ml[2 * (wave * 16 + c) + 1] = w.l[0];
+    }
+    __syncthreads();
+    const int tid = wave * 64 + lane;
+    for (int i = tid; i < it.n_rows * (DIM / 4); i += 256) {
+        const int r = i / (DIM / 4), e = i % (DIM / 4) * 4;
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) m = fmaxf(m, ml[2 * (v * 16 + r)]);
+        v4f o = {0, 0, 0, 0};
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const float mv = ml[2 * (v * 16 + r)];
+            if (mv == -INFINITY && ml[2 * (v * 16 + r) + 1] == 0.0f) continue;  // no key of this wave's is seen
+            const float f = __builtin_amdgcn_exp2f(mv - m);
+            l += f * ml[2 * (v * 16 + r) + 1];
+            o += f * *reinterpret_cast<const v4f *>(mo + (v * 16 + r) * DIM + e);
+        }
+        if (it.part < 0) {
+            *reinterpret_cast<v4f *>(out_row(a, it, h, r, DIM) + e) = o / l;
+        } else {
+            const size_t ps = (size_t)(it.part + r) * a.kv.n_kv + h;
+            *reinterpret_cast<v4f *>(a.part + ps * DIM + e) = o;
+            if (e == 0) {
+                float *d = a.part + a.part_cap * DIM + 2 * ps;
+                d[0] = m;
+                d[1] = l;
+            }
+        }
+    }
+    __syncthreads();
+}
+
+// Many rows: every wave has its own, and all read the same tiles of keys.
+template <int TYPE, int DIM>
+__device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &it, const Source &src, int h, uint8_t *lds,
+                                            int row_from, int wave, int lane) {
+    using G = Geo<TYPE, DIM>;
+    using L = Loader<TYPE, DIM>;
+    constexpr int RT = G::RT;
+    Rows<TYPE, DIM, RT> w;
+    const int mine = row_from + wave * 16 * RT;  // (past the last row: computed from that row, not stored)
+    const int tiles = (it.key1 - it.key0 + G::TT - 1) / G::TT;
+    const uint32_t base = lds_addr(lds);
+    const auto issue = [&](int i) {
+        if (i < tiles) L::share(src, it.key0 + i * G::TT, base + (i % G::SHARED) * 2 * G::UNIT, wave, lane);
+    };
+    w.load(a, it, h, mine, lane);
+    wait_dma<0>();
+    for (int i = 0; i < G::SHARED - 1; ++i) issue(i);
+    const int first = it.causal ? __builtin_amdgcn_readfirstlane(w.lim[0]) : it.key1;
+    const int wave_last = it.causal ? w.last_limit() : it.key1;
+    for (int i = 0; i < tiles; ++i) {
+        const int p0 = it.key0 + i * G::TT;
+        if (i + G::SHARED - 2 < tiles) wait_dma<(G::SHARED - 2) * L::SHARE>();
+        else wait_dma<0>();
+        lds_done();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        issue(i + G::SHARED - 1);
+        uint8_t *ku = lds + (i % G::SHARED) * 2 * G::UNIT, *vu = ku + G::UNIT;
+        if (p0 + G::TT > it.key1) {  // (the last tile, for all waves)
+            clear_tail<TYPE, DIM>(vu, it.key1 - p0, wave * 64 + lane, 256);
+            lds_done();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        }
+        if (p0 >= wave_last) continue;  // behind all of this wave's rows
+        const bool edge = p0 + G::TT > first;
+        w.scores(ku, lane);
+        if (edge) w.mask(p0, lane);
+        w.weights();
+        if (edge && w.odd_values(vu, lane)) w.values_one_by_one(vu, p0, lane);
+        else w.values(vu, lane);
+    }
+    w.finish();
+    const int c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int r = mine + 16 * t + c;
+        if (r >= it.n_rows) continue;
+        if (it.part < 0) {
+            float *o = out_row(a, it, h, r, DIM);
+#pragma unroll
+            for (int d = 0; d < G::ND; ++d) *reinterpret_cast<v4f *>(o + d * 16 + g * 4) = w.acc[t][d] / w.l[t];
+        } else {
+            const size_t ps = (size_t)(it.part + r) * a.kv.n_kv + h;
+#pragma unroll
+            for (int d = 0; d < G::ND; ++d) *reinterpret_cast<v4f *>(a.part + ps * DIM + d * 16 + g * 4) = w.acc[t][d];
+            if (g == 0) {
+                float *d = a.part + a.part_cap * DIM + 2 * ps;
+                d[0] = w.m[t];
+                d[1] = w.l[t];
+            }
+        }
+    }
+    __syncthreads();
+}
+
+template <int TYPE, int DIM>
+__global__ __launch_bounds__(256, 2) void attn_kernel(const AttnArgs a) {
+    using G = Geo<TYPE, DIM>;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const PlanHeader *hd = reinterpret_cast<const PlanHeader *>(a.head);
+    const AttnItem *items = reinterpret_cast<const AttnItem *>(hd + 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n_kv = a.kv.n_kv;
+    const long long all = (long long)hd->n_items * n_kv;
+    for (long long i = blockIdx.x; i < all; i += gridDim.x) {
+        const AttnItem it = items[i / n_kv];
+        const int h = (int)(i % n_kv);
+        Source s;
+        s.pages = (const __attribute__((address_space(4))) int32_t *)(uintptr_t)(a.head + it.page_at);
+        s.base = a.kv.base + (size_t)h * a.kv.head_bytes;
+        s.page_bytes = a.kv.page_bytes;
+        s.head_bytes = a.kv.head_bytes;
+        s.v_off = (uint32_t)n_kv * a.kv.head_bytes;
+        s.shift = a.kv.page_shift;
+        s.last = (it.key1 - 1) >> a.kv.page_shift;
+        if (it.n_rows <= 16) attend_few<TYPE, DIM>(a, it, s, h, lds, wave, lane);
+        else
+            for (int r = 0; r < it.n_rows; r += 64 * G::RT) attend_many<TYPE, DIM>(a, it, s, h, lds, r, wave, lane);
     }
 }
 
@@ -124,11 +743,24 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 
 namespace {
 
+template <int TYPE, int DIM>
+hipError_t launch_typed(const AttnArgs &a, unsigned grid, hipStream_t st) {
+    constexpr int bytes = Geo<TYPE, DIM>::LDS_BYTES;
+    static_assert(bytes <= 160 * 1024, "the rings fit the gfx950 LDS");
+    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(attn_kernel<TYPE, DIM>),
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (set != hipSuccess) return set;
+    hipLaunchKernelGGL((attn_kernel<TYPE, DIM>), dim3(grid), dim3(256), bytes, st, a);
+    return hipGetLastError();
+}
+
 template <int DIM>
 hipError_t launch_attention(const AttnArgs &a, int type, unsigned grid, unsigned join_grid, hipStream_t st) {
-    if (type == kTypeF32) hipLaunchKernelGGL((attn_kernel<kTypeF32, DIM>), dim3(grid), dim3(256), 0, st, a);
-    else if (type == kTypeF16) hipLaunchKernelGGL((attn_kernel<kTypeF16, DIM>), dim3(grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((attn_kernel<kTypeQ8_0, DIM>), dim3(grid), dim3(256), 0, st, a);
+    hipError_t e;
+    if (type == kTypeF32) e = launch_typed<kTypeF32, DIM>(a, grid, st);
+    else if (type == kTypeF16) e = launch_typed<kTypeF16, DIM>(a, grid, st);
+    else e = launch_typed<kTypeQ8_0, DIM>(a, grid, st);
+    if (e != hipSuccess) return e;
     if (join_grid != 0) hipLaunchKernelGGL((attn_join_kernel<DIM>), dim3(join_grid), dim3(256), 0, st, a);
     return hipGetLastError();
 }

@@ -39,14 +39,19 @@ def values(pool_values, layer, pages, n):
             np.zeros((p.shape[2], 0, p.shape[4])) for j in (0, 1)]
 
 
-def attend(q, k, v, first, scale):
+def attend(q, k, v, first, scale, qtype):
     """(out, tolerance) [new, heads, dim] of q [new, heads, dim] at the positions from `first` on.
 
     The tolerance: with S the largest sum of |scale q_i k_i| and n keys, a score is off by at most
     (dim + 8) eps32 S (sums of dim products, q in parts that miss 2^-22 = 4 eps32 of it, two scalings), its
     exponent's argument by 2 eps32 S more, so a weight by twice that relatively (its own and the
     maximum's); exp2 and the weight's parts add 8 eps32, the two sums (n + 8) eps32 each.  Numerator and
-    denominator both carry these, hence the factor 2."""
+    denominator both carry these, hence the factor 2.
+
+    F16 and Q8_0 weights are two f16 parts of p = 2^(s - m + 7), the largest of a row between 2^7 and 2^15; the second
+    part rounds to steps of 2^-24 at the finest, so a weight is off by up to 2^-25, 2^-32 of the row's largest, whatever
+    its own size.  With Q8_0 the parts are of p d / D, D at most twice the largest scale d, which makes it 2^-31 of the
+    largest weight times the largest value, and n such terms add up."""
     m, H, dim = q.shape
     kv = k.shape[0]
     q = torch.from_numpy(q).double()
@@ -61,7 +66,8 @@ def attend(q, k, v, first, scale):
             out[t, h] = (w @ vh[:n]).numpy()
             big = float((kh[:n].abs() @ q[t, h].abs()).max()) * abs(scale)
             rel = 2 * ((dim + 12) * 2 * EPS32 * big + (8 + 2 * (n + 8)) * EPS32)
-            tol[t, h] = ((w @ vh[:n].abs()) * rel).numpy() + 1e-30
+            floor = 0.0 if qtype == E.F32 else n * 2.0 ** -31 * float(w.max() * vh[:n].abs().max())
+            tol[t, h] = ((w @ vh[:n].abs()) * rel).numpy() + floor + 1e-30
     return out, tol
 
 

@@ -60,7 +60,7 @@ def check_attention(cache, qtype, layers, n_pages, page, seqs, n_new, heads, rng
     for s, m in zip(seqs, n_new):
         n = cache.length(s)
         k, v = P.values(vals, layer, [p for p in cache.tables([s])[0] if p >= 0], n)
-        want, tol = P.attend(q[at: at + m].reshape(m, heads, dim), k, v, n - m, scale or dim ** -0.5)
+        want, tol = P.attend(q[at: at + m].reshape(m, heads, dim), k, v, n - m, scale or dim ** -0.5, qtype)
         err = np.abs(got[at: at + m].reshape(m, heads, dim) - want)
         assert np.all(err <= tol), f"sequence of {n}, {m} new: {np.max(err / tol):.3g} times the tolerance"
         if m:
@@ -160,20 +160,21 @@ def test_values_of_later_tokens_have_no_influence(hipdev, qtype):
     q = dev(rng.standard_normal((new, 2 * dim)).astype(np.float32))
     batch = E.KvBatch(c, 2, 1, new)
     batch.set([s], [new])
-    before = E.attention(batch, 0, q).clone()
     t = torch.float16 if qtype == E.F16 else torch.float32
     view = c.pool.view(t).view(4, 2, 1, page, dim)
+    k, v = P.values(pool_values(c, qtype, 1, 4, page), 0, [p for p in c.tables([s])[0] if p >= 0], n)
+    want, tol = P.attend(q.cpu().numpy().reshape(new, 2, dim), k, v, n - new, dim ** -0.5, qtype)
     for bad, which in ((float("inf"), 1), (float("nan"), 1), (float("nan"), 0), (float("-inf"), 0)):
         keep = view.clone()
         at = n - 7
         view[at // page, which, 0, at % page, 5] = bad
-        got = E.attention(batch, 0, q)
+        err = np.abs(E.attention(batch, 0, q).cpu().numpy().reshape(new, 2, dim) - want)
         rows = new - 7
-        assert torch.equal(got[:rows], before[:rows]), (bad, which)
+        assert np.all(err[:rows] <= tol[:rows]), (bad, which)
         if which == 1:
-            later = got[rows:].view(-1, 2, dim)
-            assert not torch.isfinite(later[..., 5]).any()
-            assert torch.isfinite(later[..., 6:]).all() and torch.equal(later[..., :5], before[rows:].view(-1, 2, dim)[..., :5])
+            assert not np.isfinite(err[rows:, :, 5]).any()
+            others = [e for e in range(dim) if e != 5]
+            assert np.all(err[rows:][..., others] <= tol[rows:][..., others]), bad
         view.copy_(keep)
 
 
@@ -199,7 +200,7 @@ def test_long_cache_offsets_beyond_32_bits(hipdev):
         got = E.attention(b, layer, dev(q)).cpu().numpy().reshape(1, 8, dim)
         x = v[layer, at: at + 3].double().cpu().numpy()
         k, w = (np.concatenate(list(x[:, j].transpose(0, 2, 1, 3)), 0)[:600].transpose(1, 0, 2) for j in (0, 1))
-        want, tol = P.attend(q.reshape(1, 8, dim), k, w, 599, dim ** -0.5)
+        want, tol = P.attend(q.reshape(1, 8, dim), k, w, 599, dim ** -0.5, E.F16)
         assert np.all(np.abs(got - want) <= tol)
     # a copy there too
     want = v[:, at:].clone()
@@ -408,7 +409,7 @@ def test_a_prompt_then_forked_answers(hipdev, qtype):
                     err = np.abs(g[:, n - m:].transpose(1, 0, 2) - w)
                     assert np.all(err <= np.abs(w).max() * (step_of + 30 * P.EPS32) * 1.01)
                 qs = qr[at: at + m].cpu().numpy().reshape(m, heads, dim)
-                want, tol = P.attend(qs, k64, v64, n - m, dim ** -0.5)
+                want, tol = P.attend(qs, k64, v64, n - m, dim ** -0.5, qtype)
                 assert np.all(np.abs(got[at: at + m].reshape(m, heads, dim) - want) <= tol)
                 at += m
 
