@@ -69,7 +69,10 @@ struct Geo {
     static constexpr int RT = DIM == 256 ? 1 : 2;  // 16-row tiles of a wave, many rows
     static constexpr int LDS = 4 * RING * UNIT > SHARED * 2 * UNIT ? 4 * RING * UNIT : SHARED * 2 * UNIT;
     static constexpr int MERGE = 4 * 16 * (DIM + 2) * 4;
-    static constexpr int LDS_BYTES = LDS > MERGE ? LDS : MERGE;
+    static constexpr int ODD = LDS > MERGE ? LDS : MERGE;  // marks of values that are not finite, a wave each
+    static constexpr int ODD_WORDS = TT * NB;
+    static constexpr int LDS_BYTES = ODD + 4 * ODD_WORDS * 4;
+    static constexpr int PER_CU = LDS_BYTES <= 80 * 1024 ? 2 : 1;  // workgroups that LDS leaves room for
 };
 
 // Piece permutation of row `row` of a tile: piece c lies at c ^ swz.  Chosen so
@@ -113,12 +116,21 @@ __device__ __forceinline__ float col_sum(float v) {
     return v + shfl_xor_f(v, 32);
 }
 
+__device__ __forceinline__ float wave_max(float v) {
+    return col_max(row16_max(v));
+}
+
 // High part and rest of eight values.
 __device__ __forceinline__ void split8(const float (&x)[8], v8h &hi, v8h &lo) {
+    typedef float v2f __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        hi[j] = (_Float16)x[j];
-        lo[j] = (_Float16)(x[j] - (float)hi[j]);
+    for (int j = 0; j < 8; j += 2) {
+        const h2 h = __builtin_convertvector((v2f{x[j], x[j + 1]}), h2);
+        const h2 l = __builtin_convertvector((v2f{fmaf((float)h[0], -1.0f, x[j]), fmaf((float)h[1], -1.0f, x[j + 1])}), h2);
+        hi[j] = h[0];
+        hi[j + 1] = h[1];
+        lo[j] = l[0];
+        lo[j + 1] = l[1];
     }
 }
 
@@ -148,7 +160,30 @@ __device__ __forceinline__ v4f mfma4(float a, float b, v4f c) { return __builtin
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 typedef __attribute__((address_space(3))) v2i lds_v2i;
 
+// The lane number as a value the compiler knows nothing of: addresses made from
+// it are not computed in front of the loops around, where they would hold
+// registers all along.
+__device__ __forceinline__ int here(int lane) {
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
+// A barrier without the waits on memory of __syncthreads (the DMAs of later tiles stay in flight).
+__device__ __forceinline__ void workgroup_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 __device__ __forceinline__ void lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// The token of row r of an item, and where its output goes.
+__device__ __forceinline__ const PlanToken *token_of(const AttnArgs &a, const AttnItem &it, int r) {
+    return reinterpret_cast<const PlanToken *>(a.head) - ((it.row0 + r) / a.group + 1);
+}
+__device__ __forceinline__ size_t row_at(const AttnArgs &a, const AttnItem &it, int h, int r, int dim) {
+    return (((size_t)token_of(a, it, r)->order * a.kv.n_kv + h) * a.group + (it.row0 + r) % a.group) * dim;
+}
 
 // Where a piece of work reads: the pages of one kv head of one layer.
 struct Source {
@@ -211,7 +246,7 @@ struct Rows {
     static constexpr int NQ = TYPE == kTypeF32 ? G::ND : G::NB;
     v8h qh[TYPE == kTypeF32 ? 1 : RT][TYPE == kTypeF32 ? 1 : G::NB], ql[TYPE == kTypeF32 ? 1 : RT][TYPE == kTypeF32 ? 1 : G::NB];
     v4f qf[TYPE == kTypeF32 ? RT : 1][TYPE == kTypeF32 ? G::ND : 1];
-    float rs[RT], m[RT], l[RT];  // score factor; running maximum (of base-2 exponents), this lane's part of the sum
+    float rs[RT], m[RT], l[RT];  // score factor (positive); running maximum (of base-2 exponents), this lane's part of the sum
     int lim[RT];                 // positions below are seen
     v4f acc[RT][G::ND];
     int ve;                      // Q8_0: acc is in units of 2^ve
@@ -219,16 +254,18 @@ struct Rows {
 
     __device__ __forceinline__ void load(const AttnArgs &a, const AttnItem &it, int h, int row_from, int lane) {
         const int g = lane >> 4;
+        // a negative scale turns q around; zero makes q zero
+        const float sign = a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f;
+        const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            const int r = min(row_from + 16 * t + (lane & 15), it.n_rows - 1), row = it.row0 + r;
-            const PlanToken *pt = reinterpret_cast<const PlanToken *>(a.head) - (row / a.group + 1);
-            lim[t] = it.causal ? min(it.key1, pt->order_pos + 1) : it.key1;
-            const float *q = a.q + (((size_t)pt->order * a.kv.n_kv + h) * a.group + row % a.group) * DIM;
+            const int r = min(row_from + 16 * t + (lane & 15), it.n_rows - 1);
+            lim[t] = it.causal ? min(it.key1, token_of(a, it, r)->order_pos + 1) : it.key1;
+            const float *q = a.q + row_at(a, it, h, r, DIM);
             if constexpr (TYPE == kTypeF32) {
 #pragma unroll
-                for (int c = 0; c < G::ND; ++c) qf[t][c] = *reinterpret_cast<const v4f *>(q + c * 16 + g * 4);
-                rs[t] = a.scale * kLog2e;
+                for (int c = 0; c < G::ND; ++c) qf[t][c] = sign * *reinterpret_cast<const v4f *>(q + c * 16 + g * 4);
+                rs[t] = scale;
             } else {
                 float x[G::NB][8], top = 0.0f;
 #pragma unroll
@@ -237,8 +274,8 @@ struct Rows {
                     const v4f v = *reinterpret_cast<const v4f *>(q + c * 32 + g * 8 + 4);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        x[c][j] = u[j];
-                        x[c][4 + j] = v[j];
+                        x[c][j] = sign * u[j];
+                        x[c][4 + j] = sign * v[j];
                         top = fmaxf(top, fmaxf(fabsf(u[j]), fabsf(v[j])));
                     }
                 }
@@ -251,7 +288,8 @@ struct Rows {
                     for (int j = 0; j < 8; ++j) x[c][j] = ldexpf(x[c][j], -e);
                     split8(x[c], qh[t][c], ql[t][c]);
                 }
-                rs[t] = ldexpf(a.scale * kLog2e, e);
+                // (not zero: a masked score is -infinity times this)
+                rs[t] = fmaxf(ldexpf(scale, e), 1.17549435e-38f);
             }
             m[t] = -INFINITY;
             l[t] = 0.0f;
@@ -307,7 +345,7 @@ struct Rows {
 #pragma unroll
             for (int t = 0; t < RT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[t][hf][r] = o[t][r] * rs[t];
+                for (int r = 0; r < 4; ++r) s[t][hf][r] = o[t][r];
         }
     }
 
@@ -336,6 +374,7 @@ struct Rows {
             for (int hf = 0; hf < G::HALVES; ++hf)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][hf][r]);
+            top *= rs[t];
             if (__builtin_amdgcn_ballot_w64(top > m[t] + 8.0f) != 0) {
                 const float mn = fmaxf(m[t], col_max(top));
                 const float c = m[t] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[t] - mn);
@@ -348,7 +387,7 @@ struct Rows {
             for (int hf = 0; hf < G::HALVES; ++hf)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[t][hf][r] = __builtin_amdgcn_exp2f(s[t][hf][r] - off);
+                    s[t][hf][r] = __builtin_amdgcn_exp2f(fmaf(s[t][hf][r], rs[t], -off));
                     l[t] += s[t][hf][r];
                 }
         }
@@ -401,7 +440,7 @@ struct Rows {
                     }
             // scales at most 1 in the units of acc: weights times scale stay in f16's range
             if (__builtin_amdgcn_ballot_w64(top > ldexpf(1.0f, ve)) != 0) {
-                top = col_max(top);
+                top = wave_max(top);
                 const int e = top < INFINITY ? __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top)) : 16;
                 if (e > ve) {
 #pragma unroll
@@ -437,56 +476,21 @@ struct Rows {
         }
     }
 
-    // Whether any value that this tile's rows may read is not finite.
-    __device__ __forceinline__ bool odd_values(const uint8_t *vu, int lane) {
-        bool bad = false;
-        if (TYPE == kTypeF32) {
-            for (int i = lane * 4; i < G::TT * G::RB; i += 256)
-                bad |= (*reinterpret_cast<const uint32_t *>(vu + i) & 0x7f800000u) == 0x7f800000u;
-        } else {
-            const uint8_t *at = TYPE == kTypeF16 ? vu : vu + G::TT * G::RB;
-            for (int i = lane * 4; i < (TYPE == kTypeF16 ? G::TT * G::RB : G::TT * G::SB); i += 256) {
-                const uint32_t w = *reinterpret_cast<const uint32_t *>(at + i);
-                bad |= (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
-            }
-        }
-        return __builtin_amdgcn_ballot_w64(bad) != 0;
-    }
-
-    // values() for a tile with infinities or NaN in it, at the causal limit: 0 *
-    // infinity must not reach the rows that do not see them.  Key by key.
-    __device__ __forceinline__ void values_one_by_one(const uint8_t *vu, int p0, int lane) {
+    // The sums that a key's values marked in `odd` (NB words a key) belong to become NaN for the rows that see it.
+    __device__ __forceinline__ void spoil(const uint32_t *odd, int p0, int lane) {
         const int g = lane >> 4;
-        const float unit = TYPE == kTypeQ8_0 ? ldexpf(1.0f, -ve) : 1.0f;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            uint32_t w[G::NB] = {};
 #pragma unroll 1
-        for (int row = 0; row < G::TT; ++row) {
-            const int sw = swz<TYPE, DIM, true>(row);
-            float p[RT];
+            for (int k = 0; k < G::TT && p0 + k < lim[t]; ++k)
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                float mine = 0.0f;  // this lane's weight of key 16 hf + 4 g + r
-#pragma unroll
-                for (int i = 0; i < 4 * G::HALVES; ++i)
-                    if (i == (row >> 4) * 4 + (row & 3)) mine = s[t][i >> 2][i & 3];
-                p[t] = __shfl(mine, ((row >> 2) & 3) * 16 + (lane & 15), 64);
-            }
+                for (int b = 0; b < G::NB; ++b) w[b] |= odd[k * G::NB + b];
 #pragma unroll
             for (int d = 0; d < G::ND; ++d)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int e = d * 16 + g * 4 + j;
-                    constexpr int es = TYPE == kTypeF32 ? 4 : TYPE == kTypeF16 ? 2 : 1;
-                    const uint8_t *at = vu + row * G::RB + (((e * es / 16) ^ sw) * 16) + e * es % 16;
-                    float v;
-                    if (TYPE == kTypeF32) v = *reinterpret_cast<const float *>(at);
-                    else if (TYPE == kTypeF16) v = (float)*reinterpret_cast<const _Float16 *>(at);
-                    else
-                        v = (float)*reinterpret_cast<const int8_t *>(at) * unit *
-                            (float)reinterpret_cast<const _Float16 *>(vu + G::TT * G::RB)[row * G::NB + e / 32];
-#pragma unroll
-                    for (int t = 0; t < RT; ++t)
-                        if (p0 + row < lim[t]) acc[t][d][j] = fmaf(p[t], v, acc[t][d][j]);
-                }
+                for (int j = 0; j < 4; ++j)
+                    if (w[d / 2] >> ((d & 1) * 16 + g * 4 + j) & 1) acc[t][d][j] = __builtin_nanf("");
         }
     }
 
@@ -520,11 +524,57 @@ __device__ __forceinline__ void clear_tail(uint8_t *vu, int valid, int tid, int 
     }
 }
 
-// The rows of one column tile: token and head of row r of the item.
-__device__ __forceinline__ float *out_row(const AttnArgs &a, const AttnItem &it, int h, int r, int dim) {
-    const int row = it.row0 + r;
-    const PlanToken *pt = reinterpret_cast<const PlanToken *>(a.head) - (row / a.group + 1);
-    return a.out + (((size_t)pt->order * a.kv.n_kv + h) * a.group + row % a.group) * dim;
+// Whether the V unit at vu holds a value (a scale) that is not finite.
+template <int TYPE, int DIM>
+__device__ __forceinline__ bool odd_values(const uint8_t *vu, int lane) {
+    using G = Geo<TYPE, DIM>;
+    const uint8_t *at = TYPE == kTypeQ8_0 ? vu + G::TT * G::RB : vu;
+    constexpr int n = TYPE == kTypeQ8_0 ? G::TT * G::SB : G::TT * G::RB;
+    constexpr uint32_t lo = TYPE == kTypeF32 ? 0x7f800000u : 0x7c00u, hi = TYPE == kTypeF32 ? lo : lo << 16;
+    bool bad = false;
+#pragma unroll 2
+    for (int i = lane * 4; i < n; i += 256) {
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(at + i);
+        bad |= (w & lo) == lo || (w & hi) == hi;
+    }
+    return __builtin_amdgcn_ballot_w64(bad) != 0;
+}
+
+// In a tile at the causal limit 0 * infinity must not reach the rows that do
+// not see the key.  One wave marks the values that are not finite in `odd`
+// (NB words a key, bit e % 32 of word e / 32 for value e; a Q8_0 scale marks its
+// block) and makes them zero; spoil() then does to the rows that see them what
+// the product would have done.
+template <int TYPE, int DIM>
+__device__ __forceinline__ void mark_odd(uint8_t *vu, uint32_t *odd, int lane) {
+    using G = Geo<TYPE, DIM>;
+    if (lane >= G::TT) return;
+    const int sw = swz<TYPE, DIM, true>(lane);
+#pragma unroll 1
+    for (int b = 0; b < G::NB; ++b) {
+        uint32_t w = 0;
+        if (TYPE == kTypeQ8_0) {
+            uint16_t *d = reinterpret_cast<uint16_t *>(vu + G::TT * G::RB) + lane * G::NB + b;
+            if ((*d & 0x7c00u) == 0x7c00u) {
+                w = ~0u;
+                *d = 0;
+            }
+        } else {
+            constexpr int es = TYPE == kTypeF32 ? 4 : 2;
+#pragma unroll 1
+            for (int j = 0; j < 32; ++j) {
+                const int e = b * 32 + j;
+                uint8_t *at = vu + lane * G::RB + (((e * es / 16) ^ sw) * 16) + e * es % 16;
+                const bool bad = TYPE == kTypeF32 ? (*reinterpret_cast<uint32_t *>(at) & 0x7f800000u) == 0x7f800000u
+                                                  : (*reinterpret_cast<uint16_t *>(at) & 0x7c00u) == 0x7c00u;
+                if (!bad) continue;
+                w |= 1u << j;
+                if (TYPE == kTypeF32) *reinterpret_cast<uint32_t *>(at) = 0;
+                else *reinterpret_cast<uint16_t *>(at) = 0;
+            }
+        }
+        odd[lane * G::NB + b] = w;
+    }
 }
 
 // Few rows (at most 16): the four waves take every fourth tile of keys each, on
@@ -568,9 +618,11 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
                 clear_tail<TYPE, DIM>(vu, it.key1 - p0, lane, 64);
                 lds_done();
             }
-            if (w.odd_values(vu, lane)) {
-                w.values_one_by_one(vu, p0, lane);
-                continue;
+            if (odd_values<TYPE, DIM>(vu, here(lane))) {
+                uint32_t *odd = reinterpret_cast<uint32_t *>(lds + G::ODD) + wave * G::ODD_WORDS;
+                mark_odd<TYPE, DIM>(vu, odd, here(lane));
+                lds_done();
+                w.spoil(odd, p0, here(lane));
             }
         }
         w.values(vu, lane);
@@ -603,7 +655,7 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
             o += f * *reinterpret_cast<const v4f *>(mo + (v * 16 + r) * DIM + e);
         }
         if (it.part < 0) {
-            *reinterpret_cast<v4f *>(out_row(a, it, h, r, DIM) + e) = o / l;
+            *reinterpret_cast<v4f *>(a.out + row_at(a, it, h, r, DIM) + e) = o / l;
         } else {
             const size_t ps = (size_t)(it.part + r) * a.kv.n_kv + h;
             *reinterpret_cast<v4f *>(a.part + ps * DIM + e) = o;
@@ -636,28 +688,35 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
     for (int i = 0; i < G::SHARED - 1; ++i) issue(i);
     const int first = it.causal ? __builtin_amdgcn_readfirstlane(w.lim[0]) : it.key1;
     const int wave_last = it.causal ? w.last_limit() : it.key1;
+    // (the workgroup's first row: the least limit of all waves)
+    const int all_first = it.causal ? min(it.key1, token_of(a, it, row_from)->order_pos + 1) : it.key1;
     for (int i = 0; i < tiles; ++i) {
         const int p0 = it.key0 + i * G::TT;
         if (i + G::SHARED - 2 < tiles) wait_dma<(G::SHARED - 2) * L::SHARE>();
         else wait_dma<0>();
         lds_done();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
+        workgroup_barrier();
         issue(i + G::SHARED - 1);
         uint8_t *ku = lds + (i % G::SHARED) * 2 * G::UNIT, *vu = ku + G::UNIT;
         if (p0 + G::TT > it.key1) {  // (the last tile, for all waves)
             clear_tail<TYPE, DIM>(vu, it.key1 - p0, wave * 64 + lane, 256);
             lds_done();
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
+            workgroup_barrier();
+        }
+        if (p0 + G::TT > all_first && odd_values<TYPE, DIM>(vu, here(lane))) {  // the same for all waves
+            uint32_t *odd = reinterpret_cast<uint32_t *>(lds + G::ODD);
+            workgroup_barrier();
+            if (wave == 0) mark_odd<TYPE, DIM>(vu, odd, here(lane));
+            lds_done();
+            workgroup_barrier();
+            w.spoil(odd, p0, here(lane));
+            workgroup_barrier();
         }
         if (p0 >= wave_last) continue;  // behind all of this wave's rows
-        const bool edge = p0 + G::TT > first;
         w.scores(ku, lane);
-        if (edge) w.mask(p0, lane);
+        if (p0 + G::TT > first) w.mask(p0, lane);
         w.weights();
-        if (edge && w.odd_values(vu, lane)) w.values_one_by_one(vu, p0, lane);
-        else w.values(vu, lane);
+        w.values(vu, lane);
     }
     w.finish();
     const int c = lane & 15, g = lane >> 4;
@@ -666,7 +725,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
         const int r = mine + 16 * t + c;
         if (r >= it.n_rows) continue;
         if (it.part < 0) {
-            float *o = out_row(a, it, h, r, DIM);
+            float *o = a.out + row_at(a, it, h, r, DIM);
 #pragma unroll
             for (int d = 0; d < G::ND; ++d) *reinterpret_cast<v4f *>(o + d * 16 + g * 4) = w.acc[t][d] / w.l[t];
         } else {
@@ -684,16 +743,16 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
 }
 
 template <int TYPE, int DIM>
-__global__ __launch_bounds__(256, 2) void attn_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(256, (Geo<TYPE, DIM>::PER_CU)) void attn_kernel(const AttnArgs a) {
     using G = Geo<TYPE, DIM>;
     extern __shared__ __align__(16) uint8_t lds[];
     const PlanHeader *hd = reinterpret_cast<const PlanHeader *>(a.head);
     const AttnItem *items = reinterpret_cast<const AttnItem *>(hd + 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n_kv = a.kv.n_kv;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n_kv = a.kv.n_kv;
     const long long all = (long long)hd->n_items * n_kv;
     for (long long i = blockIdx.x; i < all; i += gridDim.x) {
         const AttnItem it = items[i / n_kv];
-        const int h = (int)(i % n_kv);
+        const int h = (int)(i % n_kv), lane = here(threadIdx.x & 63);
         Source s;
         s.pages = (const __attribute__((address_space(4))) int32_t *)(uintptr_t)(a.head + it.page_at);
         s.base = a.kv.base + (size_t)h * a.kv.head_bytes;
