@@ -120,6 +120,12 @@ __device__ __forceinline__ float wave_max(float v) {
     return col_max(row16_max(v));
 }
 
+__device__ __forceinline__ float wave_sum_f32(float v) {
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) v += reduce_partner(v, off);
+    return col_sum(v);
+}
+
 // High part and rest of eight values.
 __device__ __forceinline__ void split8(const float (&x)[8], v8h &hi, v8h &lo) {
     typedef float v2f __attribute__((ext_vector_type(2)));
@@ -197,13 +203,21 @@ struct Source {
 template <int TYPE, int DIM>
 struct Loader {
     using G = Geo<TYPE, DIM>;
+    // The pages of a tile's two halves, asked for one tile ahead of their use.
+    struct Pages {
+        int at[G::HALVES];
+    };
+    static __device__ __forceinline__ Pages pages(const Source &s, int p0) {
+        Pages pg;
+#pragma unroll
+        for (int hf = 0; hf < G::HALVES; ++hf) pg.at[hf] = s.pages[min((p0 + 16 * hf) >> s.shift, s.last)];
+        return pg;
+    }
     // One DMA of 16 rows' unit `which`: sub-operation `sub`, from the tile at position p0, half hf, to LDS byte `to`.
-    static __device__ __forceinline__ void op(const Source &s, int which, int hf, int sub, int p0, uint32_t to, int lane) {
-        const int p = p0 + 16 * hf;
-        const int page = __builtin_amdgcn_readfirstlane(s.pages[min(p >> s.shift, s.last)]);
-        const uint8_t *b = s.base + (size_t)page * s.page_bytes + (which ? s.v_off : 0u);
+    static __device__ __forceinline__ void op(const Source &s, int page, int which, int hf, int sub, int p0, uint32_t to, int lane) {
+        const uint8_t *b = s.base + (size_t)(uint32_t)page * s.page_bytes + (which ? s.v_off : 0u);
         const v4u rs = rsrc_words(b, s.head_bytes);
-        const uint32_t off = (uint32_t)(p & ((1 << s.shift) - 1));
+        const uint32_t off = (uint32_t)((p0 + 16 * hf) & ((1 << s.shift) - 1));
         if (G::SB != 0 && sub == G::CODE_OPS) {
             const uint32_t so = ((uint32_t)DIM << s.shift) + off * G::SB;
             if (lane < G::SB) dma16(to + G::TT * G::RB + hf * 16 * G::SB, lane * 16, rs, so);
@@ -220,21 +234,20 @@ struct Loader {
         }
     }
     // A whole unit by one wave.
-    static __device__ __forceinline__ void unit(const Source &s, int which, int p0, uint32_t to, int lane) {
+    static __device__ __forceinline__ void unit(const Source &s, const Pages &pg, int which, int p0, uint32_t to, int lane) {
 #pragma unroll
         for (int hf = 0; hf < G::HALVES; ++hf)
 #pragma unroll
-            for (int k = 0; k < G::HALF_OPS; ++k) op(s, which, hf, k, p0, to, lane);
+            for (int k = 0; k < G::HALF_OPS; ++k) op(s, pg.at[hf], which, hf, k, p0, to, lane);
     }
     // This wave's part of a tile's two units (every wave issues the same number).
-    static constexpr int TILE_OPS = 2 * G::OPS, SHARE = (TILE_OPS + 3) / 4;
-    static __device__ __forceinline__ void share(const Source &s, int p0, uint32_t to, int wave, int lane) {
+    static constexpr int TILE_OPS = 2 * G::OPS, SHARE = TILE_OPS / 4;
+    static_assert(TILE_OPS % 4 == 0, "whole shares");
+    static __device__ __forceinline__ void share(const Source &s, const Pages &pg, int p0, uint32_t to, int wave, int lane) {
 #pragma unroll
         for (int k = 0; k < SHARE; ++k) {
-            int j = wave + 4 * k;
-            if (j >= TILE_OPS) j -= 4;  // once more what it has just loaded
-            const int which = j >= G::OPS ? 1 : 0, i = j - which * G::OPS;
-            op(s, which, i / G::HALF_OPS, i % G::HALF_OPS, p0, to + which * G::UNIT, lane);
+            const int j = wave * SHARE + k, which = j >= G::OPS ? 1 : 0, i = j - which * G::OPS, hf = i / G::HALF_OPS;
+            op(s, G::HALVES == 1 || hf == 0 ? pg.at[0] : pg.at[G::HALVES - 1], which, hf, i % G::HALF_OPS, p0, to + which * G::UNIT, lane);
         }
     }
 };
@@ -590,28 +603,38 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
     const uint32_t ring = lds_addr(lds) + wave * G::RING * G::UNIT;
     uint8_t *ringp = lds + wave * G::RING * G::UNIT;
     const auto pos = [&](int u) { return it.key0 + (wave + 4 * (u >> 1)) * G::TT; };
-    const auto issue = [&](int u) {
-        if (u < units) L::unit(src, u & 1, pos(u), ring + (u % G::RING) * G::UNIT, lane);
+    const auto issue = [&](int u, const typename L::Pages &pg) {
+        if (u < units) L::unit(src, pg, u & 1, pos(u), ring + (u % G::RING) * G::UNIT, lane);
     };
     const auto arrive = [&](int u) {  // unit u is there; what was read before it may be overwritten
         if (u + G::RING - 2 < units) wait_dma<(G::RING - 2) * G::OPS>();
         else wait_dma<0>();
         lds_done();
-        issue(u + G::RING - 1);
     };
+    static_assert(G::RING % 2 == 0, "the units asked for while tile i is computed are V of tile i + RING/2 - 1, K of the next");
+    constexpr int ahead = G::RING / 2 - 1;
+    typename L::Pages now = L::pages(src, pos(0)), then = now;
     w.load(a, it, h, 0, lane);
     wait_dma<0>();
-    for (int u = 0; u < G::RING - 1; ++u) issue(u);
+    for (int u = 0; u < G::RING - 1; ++u) {
+        if (u > 0 && u % 2 == 0) now = L::pages(src, pos(u));
+        issue(u, now);
+    }
+    then = L::pages(src, pos(2 * ahead + 2));
     // the first row's limit: a tile below it needs no mask
     const int first = it.causal ? __builtin_amdgcn_readfirstlane(w.lim[0]) : it.key1;
     for (int i = 0; i < mine; ++i) {
         const int p0 = pos(2 * i);
         const bool edge = p0 + G::TT > first;
         arrive(2 * i);
+        issue(2 * (i + ahead) + 1, now);
         w.scores(ringp + (2 * i % G::RING) * G::UNIT, lane);
         if (edge) w.mask(p0, lane);
         w.weights();
         arrive(2 * i + 1);
+        issue(2 * (i + ahead) + 2, then);
+        now = then;
+        then = L::pages(src, pos(2 * (i + ahead) + 4));
         uint8_t *vu = ringp + ((2 * i + 1) % G::RING) * G::UNIT;
         if (edge) {
             if (p0 + G::TT > it.key1) {
@@ -680,12 +703,13 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
     const int mine = row_from + wave * 16 * RT;  // (past the last row: computed from that row, not stored)
     const int tiles = (it.key1 - it.key0 + G::TT - 1) / G::TT;
     const uint32_t base = lds_addr(lds);
-    const auto issue = [&](int i) {
-        if (i < tiles) L::share(src, it.key0 + i * G::TT, base + (i % G::SHARED) * 2 * G::UNIT, wave, lane);
+    const auto issue = [&](int i, const typename L::Pages &pg) {
+        if (i < tiles) L::share(src, pg, it.key0 + i * G::TT, base + (i % G::SHARED) * 2 * G::UNIT, wave, lane);
     };
     w.load(a, it, h, mine, lane);
     wait_dma<0>();
-    for (int i = 0; i < G::SHARED - 1; ++i) issue(i);
+    for (int i = 0; i < G::SHARED - 1; ++i) issue(i, L::pages(src, it.key0 + i * G::TT));
+    typename L::Pages next = L::pages(src, it.key0 + (G::SHARED - 1) * G::TT);
     const int first = it.causal ? __builtin_amdgcn_readfirstlane(w.lim[0]) : it.key1;
     const int wave_last = it.causal ? w.last_limit() : it.key1;
     // (the workgroup's first row: the least limit of all waves)
@@ -696,7 +720,8 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
         else wait_dma<0>();
         lds_done();
         workgroup_barrier();
-        issue(i + G::SHARED - 1);
+        issue(i + G::SHARED - 1, next);
+        next = L::pages(src, p0 + G::SHARED * G::TT);
         uint8_t *ku = lds + (i % G::SHARED) * 2 * G::UNIT, *vu = ku + G::UNIT;
         if (p0 + G::TT > it.key1) {  // (the last tile, for all waves)
             clear_tail<TYPE, DIM>(vu, it.key1 - p0, wave * 64 + lane, 256);
@@ -767,36 +792,77 @@ __global__ __launch_bounds__(256, (Geo<TYPE, DIM>::PER_CU)) void attn_kernel(con
     }
 }
 
-// Rows with several pieces: one wave a row and kv head joins its partial
-// results, out = sum_i 2^(m_i - m) acc_i / sum_i 2^(m_i - m) l_i.
+// Rows with several pieces: a workgroup joins a row's partial results of one
+// kv head, out = sum_i 2^(m_i - m) acc_i / sum_i 2^(m_i - m) l_i.  Its groups of
+// DIM / 4 lanes take every GROUPS-th piece, in order, and are added up in order:
+// the result does not depend on timing.  Bound by the latency of three dependent
+// loads (the list, the maxima, the sums), so every piece's loads go out at once.
 template <int DIM>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
+    constexpr int W = DIM / 4, GROUPS = 256 / W, kMost = 256;
+    __shared__ float weight[kMost];
+    __shared__ int piece[kMost];
+    __shared__ float red[4];
+    __shared__ v4f sums[GROUPS * W];
     const PlanHeader *hd = reinterpret_cast<const PlanHeader *>(a.head);
-    const int lane = threadIdx.x & 63, n_kv = a.kv.n_kv;
-    constexpr int E = (DIM + 63) / 64;
-    for (long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); w < (long long)hd->n_joined * n_kv;
-         w += 4LL * gridDim.x) {
+    const int tid = threadIdx.x, n_kv = a.kv.n_kv, grp = tid / W, e = tid % W * 4;
+    const float *mls = a.part + a.part_cap * DIM;
+    const long long all = (long long)hd->n_joined * n_kv;
+    for (long long w = blockIdx.x; w < all; w += gridDim.x) {
         const int i = (int)(w / n_kv), h = (int)(w % n_kv);
         const int row = a.head[hd->join_rows + i];
         const int p0 = a.head[hd->join_at + i], p1 = a.head[hd->join_at + i + 1];
-        const float *mls = a.part + a.part_cap * DIM;
-        float m = -INFINITY, l = 0.0f, acc[E] = {};
-        for (int p = p0; p < p1; ++p) m = fmaxf(m, mls[2 * ((size_t)a.head[p] * n_kv + h)]);
-        for (int p = p0; p < p1; ++p) {
-            const size_t ps = (size_t)a.head[p] * n_kv + h;
-            const float mi = mls[2 * ps];
-            if (mi == -INFINITY) continue;  // a piece behind the row's last position
-            const float c = exp2f(mi - m);
-            l += c * mls[2 * ps + 1];
-#pragma unroll
-            for (int j = 0; j < E; ++j)
-                if (lane + 64 * j < DIM) acc[j] = fmaf(c, a.part[ps * DIM + lane + 64 * j], acc[j]);
+        float m = -INFINITY, l = 0.0f;
+        v4f acc = {0, 0, 0, 0};
+        for (int from = p0; from < p1; from += kMost) {  // (one round up to 256 pieces)
+            const int n = min(kMost, p1 - from);
+            float mi = -INFINITY, li = 0.0f;
+            int ps = 0;
+            if (tid < n) {
+                ps = a.head[from + tid];
+                const float2 ml = *reinterpret_cast<const float2 *>(mls + 2 * ((size_t)ps * n_kv + h));
+                mi = ml.x;
+                li = ml.y;
+            }
+            const float wm = wave_max(mi);
+            __syncthreads();
+            if ((tid & 63) == 0) red[tid >> 6] = wm;
+            __syncthreads();
+            const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+            const float c = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            // a piece behind the row's last position has no weight (a NaN sum has)
+            const float f = mi == -INFINITY && li == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mi - mn);
+            weight[tid] = f;
+            piece[tid] = ps;
+            m = mn;
+            l *= c;
+            acc *= c;
+            __syncthreads();
+            li = f == 0.0f ? 0.0f : f * li;
+            li = wave_sum_f32(li);
+            __syncthreads();
+            if ((tid & 63) == 0) red[tid >> 6] = li;
+            if (grp < GROUPS) {
+#pragma unroll 4
+                for (int p = grp; p < n; p += GROUPS) {
+                    const float wp = weight[p];
+                    const v4f v = *reinterpret_cast<const v4f *>(a.part + ((size_t)piece[p] * n_kv + h) * DIM + e);
+                    if (wp != 0.0f) acc += wp * v;
+                }
+            }
+            __syncthreads();
+            l += (red[0] + red[1]) + (red[2] + red[3]);
         }
-        const PlanToken *pt = reinterpret_cast<const PlanToken *>(a.head) - (row / a.group + 1);
-        float *out = a.out + (((size_t)pt->order * n_kv + h) * a.group + row % a.group) * DIM;
+        if (grp < GROUPS) sums[grp * W + tid % W] = acc;
+        __syncthreads();
+        if (tid < W) {
+            v4f o = sums[tid];
 #pragma unroll
-        for (int j = 0; j < E; ++j)
-            if (lane + 64 * j < DIM) out[lane + 64 * j] = acc[j] / l;
+            for (int k = 1; k < GROUPS; ++k) o += sums[k * W + tid];
+            const PlanToken *pt = reinterpret_cast<const PlanToken *>(a.head) - (row / a.group + 1);
+            *reinterpret_cast<v4f *>(a.out + (((size_t)pt->order * n_kv + h) * a.group + row % a.group) * DIM + e) = o / l;
+        }
+        __syncthreads();
     }
 }
 
@@ -853,9 +919,9 @@ extern "C" int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip
     // One workgroup an item and kv head; a captured call, whose plan may be
     // replaced before a replay, takes a fixed grid that walks whatever is there.
     const long long items = (long long)b->plan.items.size() * kv->n_kv;
-    const long long joins = ((long long)b->plan.join_rows.size() * kv->n_kv + 3) / 4;
+    const long long joins = (long long)b->plan.join_rows.size() * kv->n_kv;
     const unsigned grid = capturing ? 1024u : (unsigned)std::min<long long>(items, 1 << 20);
-    const unsigned join_grid = capturing ? 256u : (unsigned)std::min<long long>(joins, 4096);
+    const unsigned join_grid = capturing ? 1024u : (unsigned)std::min<long long>(joins, 1 << 20);
     if (grid == 0) return 1;
     hipError_t e;
     switch (kv->dim) {

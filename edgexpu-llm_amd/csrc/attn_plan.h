@@ -132,6 +132,8 @@ struct AttnPlan {
         return from;
     }
 
+    static long long tiles(int rows) { return (rows + kTileRows - 1) / kTileRows; }
+
     int list_pages(const KvTables::Seq &s, int from, int to) {
         // positions keep their own page index: pages[at + p / page_tokens]
         const int at = (int)pages.size() - from;
@@ -159,8 +161,12 @@ struct AttnPlan {
             const int d = agree(a, z, sp.depth, most);
             const int rows = z.row0 + z.n_new * shape_.group - a.row0;
             const long long run = (long long)(d - sp.start) * pt_;
-            // saved: the run's keys and values for all but one; added: every row's partial result, written and read
-            if (run > 0 && (sp.hi - sp.lo - 1) * run * shape_.token_bytes > 2LL * rows * shape_.part_bytes) {
+            // Saved: the run for as many workgroups as fewer have to walk it (a chunk of many tokens has its
+            // own, which are bound by the products and save nothing); added: every row's partial result, written
+            // and read.
+            long long apart = 0;
+            for (int i = sp.lo; i < sp.hi; ++i) apart += tiles(nodes_[i].n_new * shape_.group);
+            if ((apart - tiles(rows)) * run * shape_.token_bytes > 2LL * rows * shape_.part_bytes) {
                 const int page_at = list_pages(*a.seq, sp.start, d);
                 segs_.push_back({a.row0, rows, sp.start * pt_, d * pt_, page_at, 0});
                 sp.start = d;
@@ -180,7 +186,7 @@ struct AttnPlan {
     void cut(int rows) {
         long long total = 0;
         for (const Segment &s : segs_)
-            total += (long long)((s.n_rows + kTileRows - 1) / kTileRows) * (s.key1 - s.key0);
+            total += tiles(s.n_rows) * (s.key1 - s.key0);
         const long long target = std::max(1, shape_.workgroups / shape_.n_kv);
         const long long piece = std::max<long long>(kMinKeys, (total + target - 1) / target);
         std::vector<int> count(rows, 0);
@@ -202,8 +208,7 @@ struct AttnPlan {
         }
         // long pieces first: the short ones fill the end
         std::stable_sort(items.begin(), items.end(), [](const AttnItem &a, const AttnItem &b) {
-            const auto tiles = [](const AttnItem &i) { return i.n_rows > 32 ? 2 : 1; };
-            return (long long)tiles(a) * (a.key1 - a.key0) > (long long)tiles(b) * (b.key1 - b.key0);
+            return a.key1 - a.key0 > b.key1 - b.key0;
         });
         std::vector<int> start(rows + 1, 0);
         for (int r = 0; r < rows; ++r) {
