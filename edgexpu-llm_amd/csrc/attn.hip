@@ -65,7 +65,7 @@ struct Geo {
     static constexpr int ND = DIM / 16;
     // few rows: each wave has its own ring of units; many rows: tiles shared by the workgroup
     static constexpr int RING = UNIT * 16 <= 80 * 1024 ? 4 : 2;
-    static constexpr int SHARED = 3;
+    static constexpr int SHARED = 4;  // (the few-row rings take as much LDS or more)
     static constexpr int RT = DIM == 256 ? 1 : 2;  // 16-row tiles of a wave, many rows
     static constexpr int LDS = 4 * RING * UNIT > SHARED * 2 * UNIT ? 4 * RING * UNIT : SHARED * 2 * UNIT;
     static constexpr int MERGE = 4 * 16 * (DIM + 2) * 4;
@@ -124,6 +124,12 @@ __device__ __forceinline__ float wave_sum_f32(float v) {
 #pragma unroll
     for (int off = 1; off < 16; off <<= 1) v += reduce_partner(v, off);
     return col_sum(v);
+}
+
+// The larger of two pairs of unsigned 16-bit numbers (v_pk_max_u16).
+__device__ __forceinline__ uint32_t max_u16(uint32_t a, uint32_t b) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
 
 // High part and rest of eight values.
@@ -263,7 +269,7 @@ struct Rows {
     int lim[RT];                 // positions below are seen
     v4f acc[RT][G::ND];
     int ve;                      // Q8_0: acc is in units of 2^ve
-    float s[RT][G::HALVES][4];
+    float s[RT][G::HALVES][4], p[RT][G::HALVES][4];  // a tile's scores, its weights
 
     __device__ __forceinline__ void load(const AttnArgs &a, const AttnItem &it, int h, int row_from, int lane) {
         const int g = lane >> 4;
@@ -378,8 +384,8 @@ struct Rows {
         for (int d = 0; d < G::ND; ++d) acc[t][d] *= c;
     }
 
-    // Scores become weights; the maximum is raised where they exceed it by 8.
-    __device__ __forceinline__ void weights() {
+    // The maximum is raised where scores exceed it by 8.
+    __device__ __forceinline__ void raise() {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             float top = -INFINITY;
@@ -395,13 +401,20 @@ struct Rows {
                 l[t] *= c;
                 rescale(c, t);
             }
+        }
+    }
+
+    // Scores become weights.
+    __device__ __forceinline__ void weights() {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
             const float off = m[t] == -INFINITY ? 0.0f : m[t] - 7.0f;
 #pragma unroll
             for (int hf = 0; hf < G::HALVES; ++hf)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[t][hf][r] = __builtin_amdgcn_exp2f(fmaf(s[t][hf][r], rs[t], -off));
-                    l[t] += s[t][hf][r];
+                    p[t][hf][r] = __builtin_amdgcn_exp2f(fmaf(s[t][hf][r], rs[t], -off));
+                    l[t] += p[t][hf][r];
                 }
         }
     }
@@ -417,14 +430,14 @@ struct Rows {
                     const int row = g * 4 + r, sw = swz<TYPE, DIM, true>(row);
                     const float v = *reinterpret_cast<const float *>(vu + row * G::RB + (((d * 4 + (c16 >> 2)) ^ sw) * 16) + (c16 & 3) * 4);
 #pragma unroll
-                    for (int t = 0; t < RT; ++t) acc[t][d] = mfma4(v, s[t][0][r], acc[t][d]);
+                    for (int t = 0; t < RT; ++t) acc[t][d] = mfma4(v, p[t][0][r], acc[t][d]);
                 }
         } else if constexpr (TYPE == kTypeF16) {
             v8h ph[RT], pl[RT];
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                const float p[8] = {s[t][0][0], s[t][0][1], s[t][0][2], s[t][0][3], s[t][1][0], s[t][1][1], s[t][1][2], s[t][1][3]};
-                split8(p, ph[t], pl[t]);
+                const float x[8] = {p[t][0][0], p[t][0][1], p[t][0][2], p[t][0][3], p[t][1][0], p[t][1][1], p[t][1][2], p[t][1][3]};
+                split8(x, ph[t], pl[t]);
             }
             const int row = g * 4 + (c16 >> 2), sw = swz<TYPE, DIM, true>(row);  // the same for row + 16
 #pragma unroll
@@ -439,18 +452,17 @@ struct Rows {
                 for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, ph[t], acc[t][d]);
             }
         } else {
-            // this lane's keys: 4 g + r of both halves; their blocks' scales
-            const _Float16 *ds = reinterpret_cast<const _Float16 *>(vu + G::TT * G::RB) + g * 4 * G::NB;
-            float sc[2][4][G::NB], top = 0.0f;
+            // this lane's keys: 4 g + r of both halves; their blocks' scales, two to a word
+            const uint32_t *ds = reinterpret_cast<const uint32_t *>(vu + G::TT * G::RB) + g * 2 * G::NB;
+            uint32_t sc[2][2 * G::NB], most = 0;
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int b = 0; b < G::NB; ++b) {
-                        sc[hf][r][b] = (float)ds[(hf * 16 + r) * G::NB + b];
-                        top = fmaxf(top, fabsf(sc[hf][r][b]));
-                    }
+                for (int i = 0; i < 2 * G::NB; ++i) {
+                    sc[hf][i] = ds[hf * 8 * G::NB + i];
+                    most = max_u16(most, sc[hf][i] & 0x7fff7fffu);
+                }
+            float top = f16_bits_to_f32(max(most & 0xffffu, most >> 16));
             // scales at most 1 in the units of acc: weights times scale stay in f16's range
             if (__builtin_amdgcn_ballot_w64(top > ldexpf(1.0f, ve)) != 0) {
                 top = wave_max(top);
@@ -468,12 +480,15 @@ struct Rows {
                 v8h ph[RT], pl[RT];
 #pragma unroll
                 for (int t = 0; t < RT; ++t) {
-                    float p[8];
+                    float x[8];
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) p[hf * 4 + r] = s[t][hf][r] * (sc[hf][r][b] * f);
-                    split8(p, ph[t], pl[t]);
+                        for (int r = 0; r < 4; ++r) {
+                            const int i = r * G::NB + b;
+                            x[hf * 4 + r] = p[t][hf][r] * (f16_bits_to_f32(sc[hf][i / 2] >> (i % 2 * 16)) * f);
+                        }
+                    split8(x, ph[t], pl[t]);
                 }
 #pragma unroll
                 for (int d = 2 * b; d < 2 * b + 2; ++d) {
@@ -630,6 +645,7 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
         issue(2 * (i + ahead) + 1, now);
         w.scores(ringp + (2 * i % G::RING) * G::UNIT, lane);
         if (edge) w.mask(p0, lane);
+        w.raise();
         w.weights();
         arrive(2 * i + 1);
         issue(2 * (i + ahead) + 2, then);
@@ -692,17 +708,20 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
     __syncthreads();
 }
 
-// Many rows: every wave has its own, and all read the same tiles of keys.
-template <int TYPE, int DIM>
+// Many rows: every wave has its own (RT tiles of 16), and all read the same
+// tiles of keys.  The scores of tile i + 1 are computed in front of the values
+// of tile i, so that matrix instructions and the exponentials of tile i can run
+// side by side.
+template <int TYPE, int DIM, int RT>
 __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &it, const Source &src, int h, uint8_t *lds,
                                             int row_from, int wave, int lane) {
     using G = Geo<TYPE, DIM>;
     using L = Loader<TYPE, DIM>;
-    constexpr int RT = G::RT;
     Rows<TYPE, DIM, RT> w;
     const int mine = row_from + wave * 16 * RT;  // (past the last row: computed from that row, not stored)
     const int tiles = (it.key1 - it.key0 + G::TT - 1) / G::TT;
     const uint32_t base = lds_addr(lds);
+    const auto unit_at = [&](int i) { return lds + (i % G::SHARED) * 2 * G::UNIT; };
     const auto issue = [&](int i, const typename L::Pages &pg) {
         if (i < tiles) L::share(src, pg, it.key0 + i * G::TT, base + (i % G::SHARED) * 2 * G::UNIT, wave, lane);
     };
@@ -714,15 +733,19 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
     const int wave_last = it.causal ? w.last_limit() : it.key1;
     // (the workgroup's first row: the least limit of all waves)
     const int all_first = it.causal ? min(it.key1, token_of(a, it, row_from)->order_pos + 1) : it.key1;
+    if (tiles > G::SHARED - 2) wait_dma<(G::SHARED - 2) * L::SHARE>();
+    else wait_dma<0>();
+    workgroup_barrier();
+    w.scores(unit_at(0), lane);
     for (int i = 0; i < tiles; ++i) {
         const int p0 = it.key0 + i * G::TT;
-        if (i + G::SHARED - 2 < tiles) wait_dma<(G::SHARED - 2) * L::SHARE>();
+        uint8_t *vu = unit_at(i) + G::UNIT;
+        if (i + G::SHARED - 2 < tiles) wait_dma<(G::SHARED - 3) * L::SHARE>();  // tile i + 1 is there
         else wait_dma<0>();
         lds_done();
         workgroup_barrier();
         issue(i + G::SHARED - 1, next);
         next = L::pages(src, p0 + G::SHARED * G::TT);
-        uint8_t *ku = lds + (i % G::SHARED) * 2 * G::UNIT, *vu = ku + G::UNIT;
         if (p0 + G::TT > it.key1) {  // (the last tile, for all waves)
             clear_tail<TYPE, DIM>(vu, it.key1 - p0, wave * 64 + lane, 256);
             lds_done();
@@ -738,9 +761,10 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
             workgroup_barrier();
         }
         if (p0 >= wave_last) continue;  // behind all of this wave's rows
-        w.scores(ku, lane);
         if (p0 + G::TT > first) w.mask(p0, lane);
+        w.raise();
         w.weights();
+        w.scores(unit_at(i + 1), lane);  // (behind the last tile: of whatever lies there, and not used)
         w.values(vu, lane);
     }
     w.finish();
@@ -787,8 +811,9 @@ __global__ __launch_bounds__(256, (Geo<TYPE, DIM>::PER_CU)) void attn_kernel(con
         s.shift = a.kv.page_shift;
         s.last = (it.key1 - 1) >> a.kv.page_shift;
         if (it.n_rows <= 16) attend_few<TYPE, DIM>(a, it, s, h, lds, wave, lane);
-        else
-            for (int r = 0; r < it.n_rows; r += 64 * G::RT) attend_many<TYPE, DIM>(a, it, s, h, lds, r, wave, lane);
+        else if (G::RT == 1 || it.n_rows <= 64)
+            for (int r = 0; r < it.n_rows; r += 64) attend_many<TYPE, DIM, 1>(a, it, s, h, lds, r, wave, lane);
+        else attend_many<TYPE, DIM, G::RT>(a, it, s, h, lds, 0, wave, lane);
     }
 }
 
