@@ -65,9 +65,11 @@ struct Geo {
     static constexpr int ND = DIM / 16;
     // few rows: each wave has its own ring of units; many rows: tiles shared by the workgroup
     static constexpr int RING = UNIT * 16 <= 80 * 1024 ? 4 : 2;
-    static constexpr int SHARED = 4;  // (the few-row rings take as much LDS or more)
+    static constexpr int SHARED = 4;
+    static constexpr int TILE16 = 32 * DIM * 2;  // a unit's values as f16
+    static constexpr int MANY = SHARED * 2 * UNIT + (SB ? 3 * TILE16 : 0);  // (Q8_0: codes of K, both parts of V)
     static constexpr int RT = DIM == 256 ? 1 : 2;  // 16-row tiles of a wave, many rows
-    static constexpr int LDS = 4 * RING * UNIT > SHARED * 2 * UNIT ? 4 * RING * UNIT : SHARED * 2 * UNIT;
+    static constexpr int LDS = 4 * RING * UNIT > MANY ? 4 * RING * UNIT : MANY;
     static constexpr int MERGE = 4 * 16 * (DIM + 2) * 4;
     static constexpr int ODD = LDS > MERGE ? LDS : MERGE;  // marks of values that are not finite, a wave each
     static constexpr int ODD_WORDS = TT * NB;
@@ -318,8 +320,8 @@ struct Rows {
         ve = -24;
     }
 
-    // Scores of the K unit at ku.
-    __device__ __forceinline__ void scores(const uint8_t *ku, int lane) {
+    // Scores of the K unit at ku; k16: its codes as f16 (Q8_0, many rows).
+    __device__ __forceinline__ void scores(const uint8_t *ku, const uint8_t *k16, int lane) {
         const int g = lane >> 4, c16 = lane & 15;
 #pragma unroll
         for (int hf = 0; hf < G::HALVES; ++hf) {
@@ -350,8 +352,13 @@ struct Rows {
                 const _Float16 *ds = reinterpret_cast<const _Float16 *>(ku + G::TT * G::RB) + (hf * 16 + g * 4) * G::NB;
 #pragma unroll
                 for (int c = 0; c < G::NB; ++c) {
-                    const v2u w = *reinterpret_cast<const v2u *>(kr + (((c * 2 + (g >> 1)) ^ sw) * 16) + (g & 1) * 8);
-                    const v8h k = bytes_h8(w[0], w[1]);
+                    v8h k;
+                    if (k16 != nullptr) {
+                        k = *reinterpret_cast<const v8h *>(k16 + row * DIM * 2 + (((c * 4 + g) ^ swz<kTypeF16, DIM, false>(row)) * 16));
+                    } else {
+                        const v2u w = *reinterpret_cast<const v2u *>(kr + (((c * 2 + (g >> 1)) ^ sw) * 16) + (g & 1) * 8);
+                        k = bytes_h8(w[0], w[1]);
+                    }
 #pragma unroll
                     for (int t = 0; t < RT; ++t) {
                         v4f b = mfma16(k, ql[t][c], v4f{0, 0, 0, 0});
@@ -419,6 +426,49 @@ struct Rows {
         }
     }
 
+    // acc += V^T P^T for f16 values in rows of DIM, or (PARTS) for their high parts at vu and the rests at vl.
+    template <bool PARTS>
+    __device__ __forceinline__ void values16(const uint8_t *vu, const uint8_t *vl, int lane) {
+        const int g = lane >> 4, c16 = lane & 15;
+        v8h ph[RT], pl[RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const float x[8] = {p[t][0][0], p[t][0][1], p[t][0][2], p[t][0][3], p[t][1][0], p[t][1][1], p[t][1][2], p[t][1][3]};
+            split8(x, ph[t], pl[t]);
+        }
+        const int row = g * 4 + (c16 >> 2), sw = swz<kTypeF16, DIM, true>(row);  // the same for row + 16
+        const auto read = [&](const uint8_t *from, int d) {
+            const uint8_t *at = from + row * DIM * 2 + (((d * 2 + ((c16 >> 1) & 1)) ^ sw) * 16) + (c16 & 1) * 8;
+            const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)at);
+            const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(at + 16 * DIM * 2));
+            return __builtin_bit_cast(v8h, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+#pragma unroll
+        for (int d = 0; d < G::ND; ++d) {
+            const v8h v = read(vu, d);
+            if (PARTS) {
+                const v8h rest = read(vl, d);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(rest, ph[t], acc[t][d]);
+            }
+#pragma unroll
+            for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, pl[t], acc[t][d]);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, ph[t], acc[t][d]);
+        }
+    }
+
+    // Q8_0: the unit of acc is raised to 2^e where the largest scale `top` (of the wave's lanes together) exceeds it.
+    __device__ __forceinline__ void raise_unit(float top) {
+        if (__builtin_amdgcn_ballot_w64(top > ldexpf(1.0f, ve)) == 0) return;
+        top = wave_max(top);
+        const int e = top < INFINITY ? __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top)) : 16;
+        if (e <= ve) return;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) rescale(ldexpf(1.0f, ve - e), t);
+        ve = e;
+    }
+
     // acc += V^T P^T for the V unit at vu.
     __device__ __forceinline__ void values(const uint8_t *vu, int lane) {
         const int g = lane >> 4, c16 = lane & 15;
@@ -433,24 +483,7 @@ struct Rows {
                     for (int t = 0; t < RT; ++t) acc[t][d] = mfma4(v, p[t][0][r], acc[t][d]);
                 }
         } else if constexpr (TYPE == kTypeF16) {
-            v8h ph[RT], pl[RT];
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                const float x[8] = {p[t][0][0], p[t][0][1], p[t][0][2], p[t][0][3], p[t][1][0], p[t][1][1], p[t][1][2], p[t][1][3]};
-                split8(x, ph[t], pl[t]);
-            }
-            const int row = g * 4 + (c16 >> 2), sw = swz<TYPE, DIM, true>(row);  // the same for row + 16
-#pragma unroll
-            for (int d = 0; d < G::ND; ++d) {
-                const uint8_t *at = vu + row * G::RB + (((d * 2 + ((c16 >> 1) & 1)) ^ sw) * 16) + (c16 & 1) * 8;
-                const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)at);
-                const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(at + 16 * G::RB));
-                const v8h v = __builtin_bit_cast(v8h, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, pl[t], acc[t][d]);
-#pragma unroll
-                for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, ph[t], acc[t][d]);
-            }
+            values16<false>(vu, nullptr, lane);
         } else {
             // this lane's keys: 4 g + r of both halves; their blocks' scales, two to a word
             const uint32_t *ds = reinterpret_cast<const uint32_t *>(vu + G::TT * G::RB) + g * 2 * G::NB;
@@ -462,17 +495,9 @@ struct Rows {
                     sc[hf][i] = ds[hf * 8 * G::NB + i];
                     most = max_u16(most, sc[hf][i] & 0x7fff7fffu);
                 }
-            float top = f16_bits_to_f32(max(most & 0xffffu, most >> 16));
+            const float top = f16_bits_to_f32(max(most & 0xffffu, most >> 16));
             // scales at most 1 in the units of acc: weights times scale stay in f16's range
-            if (__builtin_amdgcn_ballot_w64(top > ldexpf(1.0f, ve)) != 0) {
-                top = wave_max(top);
-                const int e = top < INFINITY ? __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top)) : 16;
-                if (e > ve) {
-#pragma unroll
-                    for (int t = 0; t < RT; ++t) rescale(ldexpf(1.0f, ve - e), t);
-                    ve = e;
-                }
-            }
+            raise_unit(top);
             const float f = ldexpf(1.0f, -ve);
             const int k = c16 >> 1, row = (k < 4 ? g * 4 + k : 16 + g * 4 + k - 4), sw = swz<TYPE, DIM, true>(row);
 #pragma unroll
@@ -605,6 +630,39 @@ __device__ __forceinline__ void mark_odd(uint8_t *vu, uint32_t *odd, int lane) {
     }
 }
 
+// Q8_0, many rows: a tile's K codes and V values become f16 in LDS once for all
+// waves.  V: code * scale / unit (18 bits) as high part and rest.  Each wave
+// multiplying its own operands out took twice the vector instructions.
+template <int DIM>
+__device__ __forceinline__ void expand(const uint8_t *ku, const uint8_t *vu, uint8_t *to, float unit, int tid) {
+    using G = Geo<kTypeQ8_0, DIM>;
+    constexpr int PIECES = 32 * DIM / 16;
+#pragma unroll
+    for (int k = 0; k < (PIECES + 255) / 256; ++k) {
+        const int i = tid + 256 * k, row = i / G::CPR, c = i % G::CPR;
+        if (PIECES % 256 != 0 && i >= PIECES) break;
+        const int s16 = swz<kTypeF16, DIM, false>(row);
+        uint8_t *o = to + row * DIM * 2;
+        const int o0 = ((2 * c) ^ s16) * 16, o1 = ((2 * c + 1) ^ s16) * 16;
+        const v4u kw = *reinterpret_cast<const v4u *>(ku + row * G::RB + ((c ^ swz<kTypeQ8_0, DIM, false>(row)) * 16));
+        const v4u vw = *reinterpret_cast<const v4u *>(vu + row * G::RB + ((c ^ swz<kTypeQ8_0, DIM, true>(row)) * 16));
+        *reinterpret_cast<v8h *>(o + o0) = bytes_h8(kw[0], kw[1]);
+        *reinterpret_cast<v8h *>(o + o1) = bytes_h8(kw[2], kw[3]);
+        const float f = (float)reinterpret_cast<const _Float16 *>(vu + G::TT * G::RB)[row * G::NB + c / 2] * unit;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const v8h q = bytes_h8(vw[2 * j], vw[2 * j + 1]);
+            float x[8];
+            v8h hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (float)q[e] * f;
+            split8(x, hi, lo);
+            *reinterpret_cast<v8h *>(o + G::TILE16 + (j ? o1 : o0)) = hi;
+            *reinterpret_cast<v8h *>(o + 2 * G::TILE16 + (j ? o1 : o0)) = lo;
+        }
+    }
+}
+
 // Few rows (at most 16): the four waves take every fourth tile of keys each, on
 // their own (no barrier), and join their sums at the end.
 template <int TYPE, int DIM>
@@ -643,7 +701,7 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
         const bool edge = p0 + G::TT > first;
         arrive(2 * i);
         issue(2 * (i + ahead) + 1, now);
-        w.scores(ringp + (2 * i % G::RING) * G::UNIT, lane);
+        w.scores(ringp + (2 * i % G::RING) * G::UNIT, nullptr, lane);
         if (edge) w.mask(p0, lane);
         w.raise();
         w.weights();
@@ -736,7 +794,8 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
     if (tiles > G::SHARED - 2) wait_dma<(G::SHARED - 2) * L::SHARE>();
     else wait_dma<0>();
     workgroup_barrier();
-    w.scores(unit_at(0), lane);
+    uint8_t *wide = lds + G::SHARED * 2 * G::UNIT;  // Q8_0: f16 codes of the next tile's K, parts of this tile's V
+    w.scores(unit_at(0), nullptr, lane);
     for (int i = 0; i < tiles; ++i) {
         const int p0 = it.key0 + i * G::TT;
         uint8_t *vu = unit_at(i) + G::UNIT;
@@ -760,12 +819,23 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
             w.spoil(odd, p0, here(lane));
             workgroup_barrier();
         }
+        if constexpr (TYPE == kTypeQ8_0) {
+            float top = 0.0f;  // (every wave comes to the same unit)
+            for (int k = lane; k < G::TT * G::NB; k += 64)
+                top = fmaxf(top, fabsf((float)reinterpret_cast<const _Float16 *>(vu + G::TT * G::RB)[k]));
+            w.raise_unit(top);
+            expand<DIM>(unit_at(i + 1), vu, wide, ldexpf(1.0f, -w.ve), wave * 64 + lane);
+            lds_done();
+            workgroup_barrier();
+        }
         if (p0 >= wave_last) continue;  // behind all of this wave's rows
         if (p0 + G::TT > first) w.mask(p0, lane);
         w.raise();
         w.weights();
-        w.scores(unit_at(i + 1), lane);  // (behind the last tile: of whatever lies there, and not used)
-        w.values(vu, lane);
+        // (behind the last tile: scores of whatever lies there, and not used)
+        w.scores(unit_at(i + 1), TYPE == kTypeQ8_0 ? wide : nullptr, lane);
+        if constexpr (TYPE == kTypeQ8_0) w.template values16<true>(wide + G::TILE16, wide + 2 * G::TILE16, lane);
+        else w.values(vu, lane);
     }
     w.finish();
     const int c = lane & 15, g = lane >> 4;
