@@ -961,7 +961,22 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
     }
 }
 
+// Measured: 8 kv heads, 512 workgroups at once; keys of 4096 tokens a sequence
+// for few rows (bound by the loads, 5 to 6 TB/s), of one run of 131072 for more.
+RowCost attn_cost(int type, int dim) {
+    const int d = dim == 64 ? 0 : dim == 96 ? 1 : dim == 128 ? 2 : 3;  // (96: between its neighbours)
+    static const RowCost f32[4] = {{460, 970, 1540}, {660, 1350, 2180}, {860, 1740, 2820}, {1760, 4850, 9520}};
+    static const RowCost f16[4] = {{260, 320, 530}, {370, 450, 680}, {470, 590, 830}, {860, 1520, 2860}};
+    static const RowCost q80[4] = {{150, 590, 780}, {220, 740, 950}, {280, 880, 1130}, {660, 2680, 5240}};
+    return type == kTypeF32 ? f32[d] : type == kTypeF16 ? f16[d] : q80[d];
+}
+
 namespace {
+
+template <int DIM>
+int per_cu(int type) {
+    return type == kTypeF32 ? Geo<kTypeF32, DIM>::PER_CU : type == kTypeF16 ? Geo<kTypeF16, DIM>::PER_CU : Geo<kTypeQ8_0, DIM>::PER_CU;
+}
 
 template <int TYPE, int DIM>
 hipError_t launch_typed(const AttnArgs &a, unsigned grid, hipStream_t st) {
@@ -986,6 +1001,10 @@ hipError_t launch_attention(const AttnArgs &a, int type, unsigned grid, unsigned
 }
 
 }  // namespace
+
+int attn_workgroups(int type, int dim) {
+    return 256 * (dim == 64 ? per_cu<64>(type) : dim == 96 ? per_cu<96>(type) : dim == 128 ? per_cu<128>(type) : per_cu<256>(type));
+}
 
 }  // namespace exq
 

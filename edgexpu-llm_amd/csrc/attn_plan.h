@@ -47,11 +47,16 @@ struct PlanHeader {
 };
 static_assert(sizeof(AttnItem) == 32 && sizeof(PlanToken) == 16 && sizeof(PlanHeader) == 64, "words of the device plan");
 
+// What a workgroup takes for one key, in tenths of a nanosecond with all others
+// at work, for at most 16, 64 and 128 rows.
+struct RowCost {
+    int few, some, many;
+};
 struct PlanShape {
     int group;       // query heads of one kv head
     int n_kv;
-    int token_bytes; // K and V of one token and kv head
-    int part_bytes;  // one row's partial result
+    RowCost cost;
+    int part_cost;   // a row's partial result, written and read, in the same unit
     int workgroups;  // that run at once
 };
 
@@ -132,7 +137,12 @@ struct AttnPlan {
         return from;
     }
 
-    static long long tiles(int rows) { return (rows + kTileRows - 1) / kTileRows; }
+    // Of one key for these rows.
+    long long cost(int rows) const {
+        const int rest = rows % kTileRows;
+        return (long long)(rows / kTileRows) * shape_.cost.many +
+               (rest == 0 ? 0 : rest <= 16 ? shape_.cost.few : rest <= 64 ? shape_.cost.some : shape_.cost.many);
+    }
 
     int list_pages(const KvTables::Seq &s, int from, int to) {
         // positions keep their own page index: pages[at + p / page_tokens]
@@ -161,12 +171,11 @@ struct AttnPlan {
             const int d = agree(a, z, sp.depth, most);
             const int rows = z.row0 + z.n_new * shape_.group - a.row0;
             const long long run = (long long)(d - sp.start) * pt_;
-            // Saved: the run for as many workgroups as fewer have to walk it (a chunk of many tokens has its
-            // own, which are bound by the products and save nothing); added: every row's partial result, written
-            // and read.
+            // Saved: the run's time for each sequence alone less that for all (chunks of many tokens, which are
+            // bound by the products, save nothing); added: every row's partial result, written and read.
             long long apart = 0;
-            for (int i = sp.lo; i < sp.hi; ++i) apart += tiles(nodes_[i].n_new * shape_.group);
-            if ((apart - tiles(rows)) * run * shape_.token_bytes > 2LL * rows * shape_.part_bytes) {
+            for (int i = sp.lo; i < sp.hi; ++i) apart += cost(nodes_[i].n_new * shape_.group);
+            if ((apart - cost(rows)) * run > (long long)rows * shape_.part_cost) {
                 const int page_at = list_pages(*a.seq, sp.start, d);
                 segs_.push_back({a.row0, rows, sp.start * pt_, d * pt_, page_at, 0});
                 sp.start = d;
@@ -185,10 +194,9 @@ struct AttnPlan {
 
     void cut(int rows) {
         long long total = 0;
-        for (const Segment &s : segs_)
-            total += tiles(s.n_rows) * (s.key1 - s.key0);
+        for (const Segment &s : segs_) total += cost(s.n_rows) * (s.key1 - s.key0);
         const long long target = std::max(1, shape_.workgroups / shape_.n_kv);
-        const long long piece = std::max<long long>(kMinKeys, (total + target - 1) / target);
+        const long long share = (total + target - 1) / target;  // of one workgroup
         std::vector<int> count(rows, 0);
         for (const Segment &s : segs_) {
             for (int r = 0; r < s.n_rows; r += kTileRows) {
@@ -197,6 +205,7 @@ struct AttnPlan {
                 if (s.causal)  // the tile's last token sees no further than itself
                     key1 = std::min(key1, tokens[(s.row0 + r + nr - 1) / shape_.group].order_pos + 1);
                 const int keys = key1 - s.key0;
+                const long long piece = std::max<long long>(kMinKeys, share / cost(nr));
                 const int n = (int)((keys + piece / 2) / piece) > 1 ? (int)((keys + piece - 1) / piece) : 1;
                 const int step = ((keys + n - 1) / n + kKeyStep - 1) / kKeyStep * kKeyStep;
                 for (int k = 0; k < keys; k += step) {
@@ -207,8 +216,8 @@ struct AttnPlan {
             }
         }
         // long pieces first: the short ones fill the end
-        std::stable_sort(items.begin(), items.end(), [](const AttnItem &a, const AttnItem &b) {
-            return a.key1 - a.key0 > b.key1 - b.key0;
+        std::stable_sort(items.begin(), items.end(), [this](const AttnItem &a, const AttnItem &b) {
+            return cost(a.n_rows) * (a.key1 - a.key0) > cost(b.n_rows) * (b.key1 - b.key0);
         });
         std::vector<int> start(rows + 1, 0);
         for (int r = 0; r < rows; ++r) {

@@ -69,4 +69,8 @@ inline KvView kv_view(const edgexpu_hip_kv *kv, int layer) {
 // false (sticky error) unless the batch is set, fresh and `layer` exists; *capturing: the call is being recorded.
 bool batch_ready(edgexpu_hip_batch *b, int layer, hipStream_t st, const char *what, bool *capturing);
 
+// attn.hip: what its kernel takes for a key, and how many of its workgroups run at once.
+RowCost attn_cost(int type, int dim);
+int attn_workgroups(int type, int dim);
+
 }  // namespace exq

@@ -435,8 +435,10 @@ int edgexpu_hip_batch_set(edgexpu_hip_batch *b, int n, const int *seqs, const in
     }
     return guarded("batch_set", 0, [&] {
         b->set = false;
-        const int token_bytes = (int)(2 * b->kv->head_bytes / kt.page_tokens());
-        b->plan.build(kt, n, seqs, n_new, {b->n_heads / b->kv->n_kv, b->kv->n_kv, token_bytes, (b->kv->dim + 2) * 4, 512});
+        const edgexpu_hip_kv *kv = b->kv;
+        b->plan.build(kt, n, seqs, n_new,
+                      {b->n_heads / kv->n_kv, kv->n_kv, attn_cost(kv->type, kv->dim), (kv->dim + 2) * 4 * 2,
+                       attn_workgroups(kv->type, kv->dim)});
         if (!upload(b, (hipStream_t)stream)) return 0;
         b->epoch = kt.epoch();
         b->set = true;

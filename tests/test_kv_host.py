@@ -35,7 +35,7 @@ def lib(tmp_path_factory):
 
 
 _POINTERS = {("host_fork", 1), ("host_fork", 3), ("host_extend", 1), ("host_extend", 2), ("host_release", 1),
-             ("host_moves", 0), ("host_pages", 1), ("host_plan", 1), ("host_plan", 2), ("host_plan_get", 1)}
+             ("host_moves", 0), ("host_pages", 1), ("host_plan", 1), ("host_plan", 2), ("host_plan", 5), ("host_plan_get", 1)}
 
 
 def ints(v):
@@ -223,8 +223,8 @@ def test_refusals_change_nothing(lib):
 # ------------------------------------------------------------------ the plan
 
 
-def plan(h, seqs, n_new, group, n_kv=2, token_bytes=512, part_bytes=520, wgs=512):
-    h.L.host_plan(h.h, len(seqs), ints(seqs), ints(n_new), group, n_kv, token_bytes, part_bytes, wgs)
+def plan(h, seqs, n_new, group, n_kv=2, cost=(47, 59, 83), part_cost=104, wgs=512):
+    h.L.host_plan(h.h, len(seqs), ints(seqs), ints(n_new), group, n_kv, ints(cost), part_cost, wgs)
     out = []
     for what, w in enumerate((4, 8, 1, 1, 1, 1, 2)):
         n = h.L.host_plan_get(h.h, what, None)
