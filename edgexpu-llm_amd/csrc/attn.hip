@@ -47,6 +47,7 @@ struct AttnArgs {
     float scale;
     int group, page_tokens;
     size_t part_cap;
+    long long work, joins;  // items and joined rows, times kv heads; -1 (a captured call): as the plan says
 };
 
 // Sizes of a tile of TT keys: a unit is its K or its V rows in LDS.
@@ -687,13 +688,13 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
     static_assert(G::RING % 2 == 0, "the units asked for while tile i is computed are V of tile i + RING/2 - 1, K of the next");
     constexpr int ahead = G::RING / 2 - 1;
     typename L::Pages now = L::pages(src, pos(0)), then = now;
-    w.load(a, it, h, 0, lane);
-    wait_dma<0>();
     for (int u = 0; u < G::RING - 1; ++u) {
         if (u > 0 && u % 2 == 0) now = L::pages(src, pos(u));
         issue(u, now);
     }
     then = L::pages(src, pos(2 * ahead + 2));
+    w.load(a, it, h, 0, lane);  // (behind the first DMAs: one latency less; its loads wait for theirs)
+    wait_dma<0>();
     // the first row's limit: a tile below it needs no mask
     const int first = it.causal ? __builtin_amdgcn_readfirstlane(w.lim[0]) : it.key1;
     for (int i = 0; i < mine; ++i) {
@@ -783,16 +784,14 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
     const auto issue = [&](int i, const typename L::Pages &pg) {
         if (i < tiles) L::share(src, pg, it.key0 + i * G::TT, base + (i % G::SHARED) * 2 * G::UNIT, wave, lane);
     };
-    w.load(a, it, h, mine, lane);
-    wait_dma<0>();
     for (int i = 0; i < G::SHARED - 1; ++i) issue(i, L::pages(src, it.key0 + i * G::TT));
     typename L::Pages next = L::pages(src, it.key0 + (G::SHARED - 1) * G::TT);
+    w.load(a, it, h, mine, lane);  // (behind the first DMAs: one latency less; its loads wait for theirs)
     const int first = it.causal ? __builtin_amdgcn_readfirstlane(w.lim[0]) : it.key1;
     const int wave_last = it.causal ? w.last_limit() : it.key1;
     // (the workgroup's first row: the least limit of all waves)
     const int all_first = it.causal ? min(it.key1, token_of(a, it, row_from)->order_pos + 1) : it.key1;
-    if (tiles > G::SHARED - 2) wait_dma<(G::SHARED - 2) * L::SHARE>();
-    else wait_dma<0>();
+    wait_dma<0>();
     workgroup_barrier();
     uint8_t *wide = lds + G::SHARED * 2 * G::UNIT;  // Q8_0: f16 codes of the next tile's K, parts of this tile's V
     w.scores(unit_at(0), nullptr, lane);
@@ -866,12 +865,21 @@ __global__ __launch_bounds__(256, (Geo<TYPE, DIM>::PER_CU)) void attn_kernel(con
     using G = Geo<TYPE, DIM>;
     extern __shared__ __align__(16) uint8_t lds[];
     const PlanHeader *hd = reinterpret_cast<const PlanHeader *>(a.head);
-    const AttnItem *items = reinterpret_cast<const AttnItem *>(hd + 1);
+    // (constant memory: scalar loads)
+    const auto *items = (const __attribute__((address_space(4))) AttnItem *)(uintptr_t)(hd + 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n_kv = a.kv.n_kv;
-    const long long all = (long long)hd->n_items * n_kv;
+    const long long all = a.work >= 0 ? a.work : (long long)hd->n_items * n_kv;
     for (long long i = blockIdx.x; i < all; i += gridDim.x) {
-        const AttnItem it = items[i / n_kv];
-        const int h = (int)(i % n_kv), lane = here(threadIdx.x & 63);
+        const auto &from = items[(int)i / n_kv];
+        AttnItem it;
+        it.row0 = from.row0;
+        it.n_rows = from.n_rows;
+        it.key0 = from.key0;
+        it.key1 = from.key1;
+        it.page_at = from.page_at;
+        it.causal = from.causal;
+        it.part = from.part;
+        const int h = (int)i % n_kv, lane = here(threadIdx.x & 63);
         Source s;
         s.pages = (const __attribute__((address_space(4))) int32_t *)(uintptr_t)(a.head + it.page_at);
         s.base = a.kv.base + (size_t)h * a.kv.head_bytes;
@@ -902,7 +910,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
     const PlanHeader *hd = reinterpret_cast<const PlanHeader *>(a.head);
     const int tid = threadIdx.x, n_kv = a.kv.n_kv, grp = tid / W, e = tid % W * 4;
     const float *mls = a.part + a.part_cap * DIM;
-    const long long all = (long long)hd->n_joined * n_kv;
+    const long long all = a.joins >= 0 ? a.joins : (long long)hd->n_joined * n_kv;
     for (long long w = blockIdx.x; w < all; w += gridDim.x) {
         const int i = (int)(w / n_kv), h = (int)(w % n_kv);
         const int row = a.head[hd->join_rows + i];
@@ -1034,6 +1042,8 @@ extern "C" int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip
     // replaced before a replay, takes a fixed grid that walks whatever is there.
     const long long items = (long long)b->plan.items.size() * kv->n_kv;
     const long long joins = (long long)b->plan.join_rows.size() * kv->n_kv;
+    a.work = capturing ? -1 : items;
+    a.joins = capturing ? -1 : joins;
     const unsigned grid = capturing ? 1024u : (unsigned)std::min<long long>(items, 1 << 20);
     const unsigned join_grid = capturing ? 1024u : (unsigned)std::min<long long>(joins, 1 << 20);
     if (grid == 0) return 1;

@@ -58,11 +58,11 @@ struct PlanShape {
     RowCost cost;
     int part_cost;   // a row's partial result, written and read, in the same unit
     int workgroups;  // that run at once
+    int min_keys;    // no piece is cut shorter
 };
 
 struct AttnPlan {
     static constexpr int kTileRows = 128;   // rows of one workgroup at most
-    static constexpr int kMinKeys = 256;    // no piece is cut shorter
     static constexpr int kKeyStep = 64;     // pieces are multiples of it
 
     std::vector<PlanToken> tokens;  // by token; order fields by plan order
@@ -205,7 +205,7 @@ struct AttnPlan {
                 if (s.causal)  // the tile's last token sees no further than itself
                     key1 = std::min(key1, tokens[(s.row0 + r + nr - 1) / shape_.group].order_pos + 1);
                 const int keys = key1 - s.key0;
-                const long long piece = std::max<long long>(kMinKeys, share / cost(nr));
+                const long long piece = std::max<long long>(shape_.min_keys, share / cost(nr));
                 const int n = (int)((keys + piece / 2) / piece) > 1 ? (int)((keys + piece - 1) / piece) : 1;
                 const int step = ((keys + n - 1) / n + kKeyStep - 1) / kKeyStep * kKeyStep;
                 for (int k = 0; k < keys; k += step) {

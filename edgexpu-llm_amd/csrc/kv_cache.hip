@@ -436,9 +436,10 @@ int edgexpu_hip_batch_set(edgexpu_hip_batch *b, int n, const int *seqs, const in
     return guarded("batch_set", 0, [&] {
         b->set = false;
         const edgexpu_hip_kv *kv = b->kv;
+        static const int wgs = tuning_knob("EXQ_ATTN_WGS", 4), min_keys = tuning_knob("EXQ_ATTN_KEYS", 256);
         b->plan.build(kt, n, seqs, n_new,
                       {b->n_heads / kv->n_kv, kv->n_kv, attn_cost(kv->type, kv->dim), (kv->dim + 2) * 4 * 2,
-                       attn_workgroups(kv->type, kv->dim)});
+                       attn_workgroups(kv->type, kv->dim) * wgs / 4, min_keys});
         if (!upload(b, (hipStream_t)stream)) return 0;
         b->epoch = kt.epoch();
         b->set = true;

@@ -438,8 +438,8 @@ class KvCache:
         L.check(bool(h), "kv_create")
         self._h = h
 
-    def __del__(self):
-        if getattr(self, "_h", None) and not sys.is_finalizing():
+    def __del__(self, gone=sys.is_finalizing):
+        if getattr(self, "_h", None) and not gone():
             _HIP.kv_destroy(self._h)
 
     def new(self) -> int:
@@ -505,8 +505,8 @@ class KvBatch:
         _HIP.check(bool(h), "batch_create")
         self._h = h
 
-    def __del__(self):
-        if getattr(self, "_h", None) and not sys.is_finalizing():
+    def __del__(self, gone=sys.is_finalizing):
+        if getattr(self, "_h", None) and not gone():
             _HIP.batch_destroy(self._h)
 
     def set(self, seqs, n_new):
@@ -533,18 +533,17 @@ class Rope:
         L.check(bool(h), "rope_create")
         self._h = h
 
-    def __del__(self):
-        if getattr(self, "_h", None) and not sys.is_finalizing():
+    def __del__(self, gone=sys.is_finalizing):
+        if getattr(self, "_h", None) and not gone():
             _HIP.rope_destroy(self._h)
 
 
-def _rows(x, n: int, what: str):
-    """Rows of n float32 values, which may lie apart (a slice of a wider buffer)."""
-    import torch
-
-    if x.dtype != torch.float32 or x.dim() != 2 or x.shape[1] != n or x.stride(1) != 1:
+def _rows(x, n: int, what: str) -> int:
+    """The distance of rows of n float32 values, which may be a slice of a wider buffer."""
+    ld, one = x.stride() if x.dim() == 2 else (0, 0)
+    if one != 1 or x.shape[1] != n or x.element_size() != 4 or not x.is_floating_point():
         raise ValueError(f"{what} must be float32 [tokens, {n}] with dense rows")
-    return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), n)
+    return ld if ld >= n else n if x.shape[0] < 2 else ld
 
 
 def qk_norm_rope(q, k, n_heads: int, n_kv_heads: int, pos, rope: Rope | None = None, q_weight=None, k_weight=None,
@@ -573,19 +572,16 @@ def kv_append(batch: KvBatch, layer: int, q, k, v, rope: Rope | None = None, q_w
               eps: float = 1e-6, q_out=None):
     """Norms and rotates the batch's q and k, stores k and v in the cache's
     ``layer``, returns q (edgexpu_hip_kv_append_dev)."""
-    import torch
-
     c, m = batch.cache, batch.tokens()
-    dim = c.head_dim
-    ldq = _rows(q, batch.n_heads * dim, "q")
-    ldk, ldv = _rows(k, c.n_kv_heads * dim, "k"), _rows(v, c.n_kv_heads * dim, "v")
-    if min(q.shape[0], k.shape[0], v.shape[0]) < m:
+    n, nk = batch.n_heads * c.head_dim, c.n_kv_heads * c.head_dim
+    ldq, ldk, ldv = _rows(q, n, "q"), _rows(k, nk, "k"), _rows(v, nk, "v")
+    if q.shape[0] < m or k.shape[0] < m or v.shape[0] < m:
         raise ValueError(f"q, k and v need the batch's {m} tokens")
     if q_out is None:
-        q_out = torch.empty((m, batch.n_heads * dim), dtype=torch.float32, device=q.device)
-    L = _HIP
-    L.check(L.kv_append_dev(_ptr(q_out), _ptr(q), ldq, _ptr(k), ldk, _ptr(v), ldv, batch._h, layer, _ptr(q_weight),
-                            _ptr(k_weight), eps, rope._h if rope else None, _stream()), "kv_append")
+        q_out = q.new_empty((m, n))
+    if not _HIP.kv_append_dev(q_out.data_ptr(), q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, batch._h, layer,
+                              _ptr(q_weight), _ptr(k_weight), eps, None if rope is None else rope._h, _stream()):
+        _HIP.check(0, "kv_append")
     return q_out
 
 
@@ -593,17 +589,15 @@ def attention(batch: KvBatch, layer: int, q, scale: float | None = None, out=Non
     """Causal attention of the batch's tokens over the cache's ``layer``
     (edgexpu_hip_attention_dev): q [tokens, n_heads * head_dim] float32; scale
     1/sqrt(head_dim) unless given."""
-    import torch
-
-    n = batch.n_heads * batch.cache.head_dim
-    if q.dtype != torch.float32 or not q.is_contiguous() or q.numel() < batch.tokens() * n:
-        raise ValueError(f"q must be dense float32 [tokens, {n}] with the batch's {batch.tokens()} tokens")
+    m, n = batch.tokens(), batch.n_heads * batch.cache.head_dim
+    if q.element_size() != 4 or not q.is_floating_point() or not q.is_contiguous() or q.numel() < m * n:
+        raise ValueError(f"q must be dense float32 [tokens, {n}] with the batch's {m} tokens")
     if out is None:
-        out = torch.empty((batch.tokens(), n), dtype=torch.float32, device=q.device)
+        out = q.new_empty((m, n))
     if scale is None:
         scale = batch.cache.head_dim ** -0.5
-    L = _HIP
-    L.check(L.attention_dev(_ptr(out), _ptr(q), batch._h, layer, scale, _stream()), "attention")
+    if not _HIP.attention_dev(out.data_ptr(), q.data_ptr(), batch._h, layer, scale, _stream()):
+        _HIP.check(0, "attention")
     return out
 
 

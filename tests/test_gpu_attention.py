@@ -217,6 +217,8 @@ def test_long_cache_offsets_beyond_32_bits(hipdev):
 @pytest.mark.parametrize("dim,n_rot,inter,norm,heads,kv,m", [
     (64, 64, True, False, 9, 3, 1), (128, 128, False, True, 32, 8, 5), (256, 64, False, True, 4, 2, 3), (96, 32, True, True, 6, 2, 7),
     (10, 10, False, True, 3, 1, 4), (2, 2, True, False, 1, 1, 2), (128, 0, False, True, 4, 4, 3), (254, 100, True, True, 2, 1, 9),
+    (128, 128, False, True, 32, 8, 700), (64, 48, False, False, 7, 3, 1), (256, 256, True, True, 5, 0, 2), (128, 12, False, True, 3, 2, 5),
+    (96, 96, False, True, 5, 3, 40), (128, 68, True, False, 1, 1, 3),
 ])
 def test_qk_norm_rope(hipdev, dim, n_rot, inter, norm, heads, kv, m):
     rng = np.random.default_rng(dim * 7 + n_rot)
