@@ -45,7 +45,7 @@ struct AttnArgs {
     float *part;
     KvView kv;
     float scale;
-    int group, page_tokens;
+    int group;
     size_t part_cap;
     long long work, joins;  // items and joined rows, times kv heads; -1 (a captured call): as the plan says
 };
@@ -70,6 +70,9 @@ struct Geo {
     static constexpr int TILE16 = 32 * DIM * 2;  // a unit's values as f16
     static constexpr int MANY = SHARED * 2 * UNIT + (SB ? 3 * TILE16 : 0);  // (Q8_0: codes of K, both parts of V)
     static constexpr int RT = DIM == 256 ? 1 : 2;  // 16-row tiles of a wave, many rows
+    // 17 to 32 rows as few: with f16 no faster than the shared tiles (128: 56 and 57 ns a key), else near twice
+    // (Q8_0 47 and 86, f32 101 and 169).
+    static constexpr bool PAIR = RT == 2 && TYPE != kTypeF16;
     static constexpr int LDS = 4 * RING * UNIT > MANY ? 4 * RING * UNIT : MANY;
     static constexpr int MERGE = 4 * 16 * (DIM + 2) * 4;
     static constexpr int ODD = LDS > MERGE ? LDS : MERGE;  // marks of values that are not finite, a wave each
@@ -212,52 +215,49 @@ struct Source {
 template <int TYPE, int DIM>
 struct Loader {
     using G = Geo<TYPE, DIM>;
-    // The pages of a tile's two halves, asked for one tile ahead of their use.
+    // The page of position p.  Asked for one tile ahead of its use.
+    static __device__ __forceinline__ int page(const Source &s, int p) { return s.pages[min(p >> s.shift, s.last)]; }
+    // 16 rows of K (which = 0) or V at position p, half hf of the unit at LDS byte `to`: their sub-operations sub0 to
+    // sub0 + N - 1 of HALF_OPS, a DMA instruction each (with Q8_0 the last one is the scales).
+    template <int N>
+    static __device__ __forceinline__ void rows(const Source &s, int page, int which, int hf, int sub0, int p, uint32_t to, int lane) {
+        const v4u rs = rsrc_words(s.base + (size_t)(uint32_t)page * s.page_bytes + (which ? s.v_off : 0u), s.head_bytes);
+        const uint32_t off = (uint32_t)(p & ((1 << s.shift) - 1));
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (G::SB != 0 && k == G::CODE_OPS) {
+                const uint32_t so = ((uint32_t)DIM << s.shift) + off * G::SB;
+                if (lane < G::SB) dma16(to + G::TT * G::RB + hf * 16 * G::SB, lane * 16, rs, so);
+                continue;
+            }
+            const int at = (sub0 + k) * 1024 + lane * 16, row = at / G::RB, piece = at % G::RB / 16;
+            const int sw = which ? swz<TYPE, DIM, true>(hf * 16 + row) : swz<TYPE, DIM, false>(hf * 16 + row);
+            const uint32_t vo = (uint32_t)(row * G::RB + ((piece ^ sw) * 16)), dst = to + hf * 16 * G::RB + (sub0 + k) * 1024;
+            if (16 * G::RB % 1024 == 0 || k < G::CODE_OPS - 1) dma16(dst, vo, rs, off * G::RB);
+            else if (lane < 16 * G::RB % 1024 / 16) dma16(dst, vo, rs, off * G::RB);
+        }
+    }
+    // A whole unit by one wave.
     struct Pages {
         int at[G::HALVES];
     };
     static __device__ __forceinline__ Pages pages(const Source &s, int p0) {
         Pages pg;
 #pragma unroll
-        for (int hf = 0; hf < G::HALVES; ++hf) pg.at[hf] = s.pages[min((p0 + 16 * hf) >> s.shift, s.last)];
+        for (int hf = 0; hf < G::HALVES; ++hf) pg.at[hf] = page(s, p0 + 16 * hf);
         return pg;
     }
-    // One DMA of 16 rows' unit `which`: sub-operation `sub`, from the tile at position p0, half hf, to LDS byte `to`.
-    static __device__ __forceinline__ void op(const Source &s, int page, int which, int hf, int sub, int p0, uint32_t to, int lane) {
-        const uint8_t *b = s.base + (size_t)(uint32_t)page * s.page_bytes + (which ? s.v_off : 0u);
-        const v4u rs = rsrc_words(b, s.head_bytes);
-        const uint32_t off = (uint32_t)((p0 + 16 * hf) & ((1 << s.shift) - 1));
-        if (G::SB != 0 && sub == G::CODE_OPS) {
-            const uint32_t so = ((uint32_t)DIM << s.shift) + off * G::SB;
-            if (lane < G::SB) dma16(to + G::TT * G::RB + hf * 16 * G::SB, lane * 16, rs, so);
-            return;
-        }
-        const int at = sub * 1024 + lane * 16, row = at / G::RB, piece = at % G::RB / 16;
-        const int sw = which ? swz<TYPE, DIM, true>(hf * 16 + row) : swz<TYPE, DIM, false>(hf * 16 + row);
-        const uint32_t vo = (uint32_t)(row * G::RB + ((piece ^ sw) * 16)), so = off * G::RB;
-        const uint32_t dst = to + hf * 16 * G::RB + sub * 1024;
-        if (16 * G::RB % 1024 != 0 && sub == G::CODE_OPS - 1) {
-            if (lane < 16 * G::RB % 1024 / 16) dma16(dst, vo, rs, so);
-        } else {
-            dma16(dst, vo, rs, so);
-        }
-    }
-    // A whole unit by one wave.
     static __device__ __forceinline__ void unit(const Source &s, const Pages &pg, int which, int p0, uint32_t to, int lane) {
 #pragma unroll
-        for (int hf = 0; hf < G::HALVES; ++hf)
-#pragma unroll
-            for (int k = 0; k < G::HALF_OPS; ++k) op(s, pg.at[hf], which, hf, k, p0, to, lane);
+        for (int hf = 0; hf < G::HALVES; ++hf) rows<G::HALF_OPS>(s, pg.at[hf], which, hf, 0, p0 + 16 * hf, to, lane);
     }
-    // This wave's part of a tile's two units (every wave issues the same number).
-    static constexpr int TILE_OPS = 2 * G::OPS, SHARE = TILE_OPS / 4;
-    static_assert(TILE_OPS % 4 == 0, "whole shares");
-    static __device__ __forceinline__ void share(const Source &s, const Pages &pg, int p0, uint32_t to, int wave, int lane) {
-#pragma unroll
-        for (int k = 0; k < SHARE; ++k) {
-            const int j = wave * SHARE + k, which = j >= G::OPS ? 1 : 0, i = j - which * G::OPS, hf = i / G::HALF_OPS;
-            op(s, G::HALVES == 1 || hf == 0 ? pg.at[0] : pg.at[G::HALVES - 1], which, hf, i % G::HALF_OPS, p0, to + which * G::UNIT, lane);
-        }
+    // A wave's part of a tile's two units: 16 rows of one of them, or half of those (every wave the same number).
+    static constexpr int SHARE = G::HALVES == 2 ? G::HALF_OPS : G::CODE_OPS / 2;
+    static_assert(G::HALVES == 2 || (G::SB == 0 && G::CODE_OPS % 2 == 0), "equal shares");
+    static __device__ __forceinline__ int share_at(int p0, int wave) { return G::HALVES == 2 ? p0 + 16 * (wave & 1) : p0; }
+    static __device__ __forceinline__ void share(const Source &s, int page, int p0, uint32_t to, int wave, int lane) {
+        rows<SHARE>(s, page, wave >> 1, G::HALVES == 2 ? wave & 1 : 0, G::HALVES == 2 ? 0 : (wave & 1) * SHARE, share_at(p0, wave),
+                    to + (wave >> 1) * G::UNIT, lane);
     }
 };
 
@@ -664,14 +664,14 @@ __device__ __forceinline__ void expand(const uint8_t *ku, const uint8_t *vu, uin
     }
 }
 
-// Few rows (at most 16): the four waves take every fourth tile of keys each, on
-// their own (no barrier), and join their sums at the end.
-template <int TYPE, int DIM>
+// Few rows (at most 16 RT): the four waves take every fourth tile of keys each,
+// on their own (no barrier), and join their sums at the end.
+template <int TYPE, int DIM, int RT>
 __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it, const Source &src, int h, uint8_t *lds,
                                            int wave, int lane) {
     using G = Geo<TYPE, DIM>;
     using L = Loader<TYPE, DIM>;
-    Rows<TYPE, DIM, 1> w;
+    Rows<TYPE, DIM, RT> w;
     const int tiles = (it.key1 - it.key0 + G::TT - 1) / G::TT;
     const int mine = (tiles - wave + 3) / 4, units = 2 * mine;
     const uint32_t ring = lds_addr(lds) + wave * G::RING * G::UNIT;
@@ -726,19 +726,21 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
         w.values(vu, lane);
     }
     w.finish();
-    // join the waves: [wave][row][DIM], then maxima and sums
-    __syncthreads();
+    // join the waves, 16 rows at a time: [wave][row][DIM], then maxima and sums
     float *mo = reinterpret_cast<float *>(lds), *ml = mo + 4 * 16 * DIM;
     const int c = lane & 15, g = lane >> 4;
+    const int tid = wave * 64 + lane;
 #pragma unroll
-    for (int d = 0; d < G::ND; ++d) *reinterpret_cast<v4f *>(mo + (wave * 16 + c) * DIM + d * 16 + g * 4) = w.acc[0][d];
+    for (int t = 0; t < RT; ++t) {
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < G::ND; ++d) *reinterpret_cast<v4f *>(mo + (wave * 16 + c) * DIM + d * 16 + g * 4) = w.acc[t][d];
     if (g == 0) {
-        ml[2 * (wave * 16 + c)] = w.m[0];
-        ml[2 * (wave * 16 + c) + 1] = w.l[0];
+        ml[2 * (wave * 16 + c)] = w.m[t];
+        ml[2 * (wave * 16 + c) + 1] = w.l[t];
     }
     __syncthreads();
-    const int tid = wave * 64 + lane;
-    for (int i = tid; i < it.n_rows * (DIM / 4); i += 256) {
+    for (int i = tid; i < min(16, it.n_rows - 16 * t) * (DIM / 4); i += 256) {
         const int r = i / (DIM / 4), e = i % (DIM / 4) * 4;
         float m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -753,9 +755,9 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
             o += f * *reinterpret_cast<const v4f *>(mo + (v * 16 + r) * DIM + e);
         }
         if (it.part < 0) {
-            *reinterpret_cast<v4f *>(a.out + row_at(a, it, h, r, DIM) + e) = o / l;
+            *reinterpret_cast<v4f *>(a.out + row_at(a, it, h, 16 * t + r, DIM) + e) = o / l;
         } else {
-            const size_t ps = (size_t)(it.part + r) * a.kv.n_kv + h;
+            const size_t ps = (size_t)(it.part + 16 * t + r) * a.kv.n_kv + h;
             *reinterpret_cast<v4f *>(a.part + ps * DIM + e) = o;
             if (e == 0) {
                 float *d = a.part + a.part_cap * DIM + 2 * ps;
@@ -763,6 +765,7 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
                 d[1] = l;
             }
         }
+    }
     }
     __syncthreads();
 }
@@ -781,11 +784,12 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
     const int tiles = (it.key1 - it.key0 + G::TT - 1) / G::TT;
     const uint32_t base = lds_addr(lds);
     const auto unit_at = [&](int i) { return lds + (i % G::SHARED) * 2 * G::UNIT; };
-    const auto issue = [&](int i, const typename L::Pages &pg) {
+    const auto page_of = [&](int i) { return L::page(src, L::share_at(it.key0 + i * G::TT, wave)); };
+    const auto issue = [&](int i, int pg) {
         if (i < tiles) L::share(src, pg, it.key0 + i * G::TT, base + (i % G::SHARED) * 2 * G::UNIT, wave, lane);
     };
-    for (int i = 0; i < G::SHARED - 1; ++i) issue(i, L::pages(src, it.key0 + i * G::TT));
-    typename L::Pages next = L::pages(src, it.key0 + (G::SHARED - 1) * G::TT);
+    for (int i = 0; i < G::SHARED - 1; ++i) issue(i, page_of(i));
+    int next = page_of(G::SHARED - 1);
     w.load(a, it, h, mine, lane);  // (behind the first DMAs: one latency less; its loads wait for theirs)
     const int first = it.causal ? __builtin_amdgcn_readfirstlane(w.lim[0]) : it.key1;
     const int wave_last = it.causal ? w.last_limit() : it.key1;
@@ -803,7 +807,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
         lds_done();
         workgroup_barrier();
         issue(i + G::SHARED - 1, next);
-        next = L::pages(src, p0 + G::SHARED * G::TT);
+        next = page_of(i + G::SHARED);
         if (p0 + G::TT > it.key1) {  // (the last tile, for all waves)
             clear_tail<TYPE, DIM>(vu, it.key1 - p0, wave * 64 + lane, 256);
             lds_done();
@@ -861,15 +865,36 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
 }
 
 template <int TYPE, int DIM>
-__global__ __launch_bounds__(256, (Geo<TYPE, DIM>::PER_CU)) void attn_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(256, (Geo<TYPE, DIM>::PER_CU)) void attn_kernel(const AttnArgs args) {
     using G = Geo<TYPE, DIM>;
     extern __shared__ __align__(16) uint8_t lds[];
-    const PlanHeader *hd = reinterpret_cast<const PlanHeader *>(a.head);
+    const PlanHeader *hd = reinterpret_cast<const PlanHeader *>(args.head);
     // (constant memory: scalar loads)
     const auto *items = (const __attribute__((address_space(4))) AttnItem *)(uintptr_t)(hd + 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n_kv = a.kv.n_kv;
-    const long long all = a.work >= 0 ? a.work : (long long)hd->n_items * n_kv;
+    const long long all = args.work >= 0 ? args.work : (long long)hd->n_items * args.kv.n_kv;
     for (long long i = blockIdx.x; i < all; i += gridDim.x) {
+        // The arguments and the wave's number anew for each item: what the four
+        // ways below make of them would else be computed in front of this loop
+        // for all of them, and be moved in and out of vector registers (measured:
+        // 3 to 8 % of the many-row ways).
+        auto *ka = (const __attribute__((address_space(4))) AttnArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+        uint32_t w0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        asm volatile("" : "+s"(ka), "+s"(w0));
+        const int wave = (int)w0, lane = here(threadIdx.x & 63);
+        AttnArgs a;
+        a.q = ka->q;
+        a.out = ka->out;
+        a.head = ka->head;
+        a.part = ka->part;
+        a.kv.base = ka->kv.base;
+        a.kv.page_bytes = ka->kv.page_bytes;
+        a.kv.head_bytes = ka->kv.head_bytes;
+        a.kv.page_shift = ka->kv.page_shift;
+        a.kv.n_kv = ka->kv.n_kv;
+        a.scale = ka->scale;
+        a.group = ka->group;
+        a.part_cap = ka->part_cap;
+        const int n_kv = a.kv.n_kv, h = (int)i % n_kv;
         const auto &from = items[(int)i / n_kv];
         AttnItem it;
         it.row0 = from.row0;
@@ -879,7 +904,6 @@ __global__ __launch_bounds__(256, (Geo<TYPE, DIM>::PER_CU)) void attn_kernel(con
         it.page_at = from.page_at;
         it.causal = from.causal;
         it.part = from.part;
-        const int h = (int)i % n_kv, lane = here(threadIdx.x & 63);
         Source s;
         s.pages = (const __attribute__((address_space(4))) int32_t *)(uintptr_t)(a.head + it.page_at);
         s.base = a.kv.base + (size_t)h * a.kv.head_bytes;
@@ -888,7 +912,8 @@ __global__ __launch_bounds__(256, (Geo<TYPE, DIM>::PER_CU)) void attn_kernel(con
         s.v_off = (uint32_t)n_kv * a.kv.head_bytes;
         s.shift = a.kv.page_shift;
         s.last = (it.key1 - 1) >> a.kv.page_shift;
-        if (it.n_rows <= 16) attend_few<TYPE, DIM>(a, it, s, h, lds, wave, lane);
+        if (it.n_rows <= 16) attend_few<TYPE, DIM, 1>(a, it, s, h, lds, wave, lane);
+        else if (G::PAIR && it.n_rows <= 32) attend_few<TYPE, DIM, G::PAIR ? 2 : 1>(a, it, s, h, lds, wave, lane);
         else if (G::RT == 1 || it.n_rows <= 64)
             for (int r = 0; r < it.n_rows; r += 64) attend_many<TYPE, DIM, 1>(a, it, s, h, lds, r, wave, lane);
         else attend_many<TYPE, DIM, G::RT>(a, it, s, h, lds, 0, wave, lane);
@@ -972,10 +997,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 // Measured: 8 kv heads, 512 workgroups at once; keys of 4096 tokens a sequence
 // for few rows (bound by the loads, 5 to 6 TB/s), of one run of 131072 for more.
 RowCost attn_cost(int type, int dim) {
-    const int d = dim == 64 ? 0 : dim == 96 ? 1 : dim == 128 ? 2 : 3;  // (96: between its neighbours)
-    static const RowCost f32[4] = {{460, 970, 1540}, {660, 1350, 2180}, {860, 1740, 2820}, {1760, 4850, 9520}};
-    static const RowCost f16[4] = {{260, 320, 530}, {370, 450, 680}, {470, 590, 830}, {860, 1520, 2860}};
-    static const RowCost q80[4] = {{150, 590, 780}, {220, 740, 950}, {280, 880, 1130}, {660, 2680, 5240}};
+    const int d = dim == 64 ? 0 : dim == 96 ? 1 : dim == 128 ? 2 : 3;
+    static const RowCost f32[4] = {{{460, 540, 1000, 1580}}, {{666, 797, 1494, 2270}}, {{878, 1007, 1780, 2900}}, {{1765, 4750, 4760, 9390}}};
+    static const RowCost f16[4] = {{{237, 320, 320, 520}}, {{336, 470, 480, 730}}, {{474, 590, 595, 840}}, {{865, 1414, 1425, 2741}}};
+    static const RowCost q80[4] = {{{148, 267, 586, 774}}, {{230, 403, 878, 1100}}, {{286, 469, 920, 1160}}, {{648, 2609, 2624, 5137}}};
     return type == kTypeF32 ? f32[d] : type == kTypeF16 ? f16[d] : q80[d];
 }
 
@@ -1037,7 +1062,6 @@ extern "C" int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip
     a.kv = kv_view(kv, layer);
     a.scale = scale;
     a.group = b->n_heads / kv->n_kv;
-    a.page_tokens = kv->tables.page_tokens();
     // One workgroup an item and kv head; a captured call, whose plan may be
     // replaced before a replay, takes a fixed grid that walks whatever is there.
     const long long items = (long long)b->plan.items.size() * kv->n_kv;

@@ -48,9 +48,9 @@ struct PlanHeader {
 static_assert(sizeof(AttnItem) == 32 && sizeof(PlanToken) == 16 && sizeof(PlanHeader) == 64, "words of the device plan");
 
 // What a workgroup takes for one key, in tenths of a nanosecond with all others
-// at work, for at most 16, 64 and 128 rows.
+// at work, for at most 16, 32, 64 and 128 rows.
 struct RowCost {
-    int few, some, many;
+    int of[4];
 };
 struct PlanShape {
     int group;       // query heads of one kv head
@@ -58,11 +58,10 @@ struct PlanShape {
     RowCost cost;
     int part_cost;   // a row's partial result, written and read, in the same unit
     int workgroups;  // that run at once
-    int min_keys;    // no piece is cut shorter
+    int min_cost;    // a piece of fewer keys than this takes is not worth its start (of 64 to 256 keys)
 };
 
 struct AttnPlan {
-    static constexpr int kTileRows = 128;   // rows of one workgroup at most
     static constexpr int kKeyStep = 64;     // pieces are multiples of it
 
     std::vector<PlanToken> tokens;  // by token; order fields by plan order
@@ -85,6 +84,7 @@ struct AttnPlan {
         segs_.clear();
         parts = 0;
         writable = true;
+        weigh();
         nodes_.clear();
         for (int i = 0; i < n; ++i) {
             const KvTables::Seq &s = kv.seq(seqs[i]);
@@ -137,12 +137,26 @@ struct AttnPlan {
         return from;
     }
 
-    // Of one key for these rows.
-    long long cost(int rows) const {
-        const int rest = rows % kTileRows;
-        return (long long)(rows / kTileRows) * shape_.cost.many +
-               (rest == 0 ? 0 : rest <= 16 ? shape_.cost.few : rest <= 64 ? shape_.cost.some : shape_.cost.many);
+    // The cheapest cut of up to 8 units of 16 rows into workgroups of 1, 2, 4 and 8: its cost and its first piece, the
+    // larger of equals.
+    void weigh() {
+        best_[0] = 0;
+        for (int n = 1; n <= 8; ++n) {
+            step_[n] = 0;
+            for (int k = 3; k >= 0; --k) {
+                const int u = 1 << k, c = shape_.cost.of[k] + best_[n > u ? n - u : 0];
+                if (step_[n] == 0 || c < best_[n]) {
+                    best_[n] = c;
+                    step_[n] = u;
+                }
+            }
+        }
     }
+    // How many of `rows` rows the next workgroup takes.
+    int tile(int rows) const { return std::min(rows, 16 * step_[std::min(8, (rows + 15) / 16)]); }
+    int tile_cost(int rows) const { return shape_.cost.of[rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3]; }
+    // Of one key for these rows.
+    long long cost(int rows) const { return (long long)(rows / 128) * best_[8] + best_[(rows % 128 + 15) / 16]; }
 
     int list_pages(const KvTables::Seq &s, int from, int to) {
         // positions keep their own page index: pages[at + p / page_tokens]
@@ -199,13 +213,14 @@ struct AttnPlan {
         const long long share = (total + target - 1) / target;  // of one workgroup
         std::vector<int> count(rows, 0);
         for (const Segment &s : segs_) {
-            for (int r = 0; r < s.n_rows; r += kTileRows) {
-                const int nr = std::min(kTileRows, s.n_rows - r);
+            for (int r = 0, nr; r < s.n_rows; r += nr) {
+                nr = tile(s.n_rows - r);
                 int key1 = s.key1;
                 if (s.causal)  // the tile's last token sees no further than itself
                     key1 = std::min(key1, tokens[(s.row0 + r + nr - 1) / shape_.group].order_pos + 1);
                 const int keys = key1 - s.key0;
-                const long long piece = std::max<long long>(shape_.min_keys, share / cost(nr));
+                const int least = std::min(256, std::max(64, shape_.min_cost / tile_cost(nr)));
+                const long long piece = std::max<long long>(least, share / tile_cost(nr));
                 const int n = (int)((keys + piece / 2) / piece) > 1 ? (int)((keys + piece - 1) / piece) : 1;
                 const int step = ((keys + n - 1) / n + kKeyStep - 1) / kKeyStep * kKeyStep;
                 for (int k = 0; k < keys; k += step) {
@@ -217,7 +232,7 @@ struct AttnPlan {
         }
         // long pieces first: the short ones fill the end
         std::stable_sort(items.begin(), items.end(), [this](const AttnItem &a, const AttnItem &b) {
-            return cost(a.n_rows) * (a.key1 - a.key0) > cost(b.n_rows) * (b.key1 - b.key0);
+            return (long long)tile_cost(a.n_rows) * (a.key1 - a.key0) > (long long)tile_cost(b.n_rows) * (b.key1 - b.key0);
         });
         std::vector<int> start(rows + 1, 0);
         for (int r = 0; r < rows; ++r) {
@@ -247,6 +262,7 @@ struct AttnPlan {
     const KvTables *kv_ = nullptr;
     PlanShape shape_{};
     int pt_ = 0;
+    int best_[9] = {}, step_[9] = {};
     std::vector<Node> nodes_;
     std::vector<Segment> segs_;
 };

@@ -16,6 +16,12 @@
 
 namespace exq {
 
+// A piece of attention of less than 8 us costs more in its start and its
+// partial results than it gains.  Measured with 5, 8, 12 and 24 us: 4 tokens
+// each of 2 sequences behind 12499 f32 keys 17, 18, 18 and 25 us; 20 each of 8
+// behind 3000 Q8_0 keys 44, 34, 34 and 38; one f16 sequence of 700 11, 12, 13, 13.
+constexpr int kMinPieceCost = 80000;
+
 // Copies of pages, at most kMovesMax a launch, given as kernel arguments (no
 // transfer of a list in front of the kernel).
 constexpr int kMovesMax = 256;
@@ -436,10 +442,9 @@ int edgexpu_hip_batch_set(edgexpu_hip_batch *b, int n, const int *seqs, const in
     return guarded("batch_set", 0, [&] {
         b->set = false;
         const edgexpu_hip_kv *kv = b->kv;
-        static const int wgs = tuning_knob("EXQ_ATTN_WGS", 4), min_keys = tuning_knob("EXQ_ATTN_KEYS", 256);
         b->plan.build(kt, n, seqs, n_new,
                       {b->n_heads / kv->n_kv, kv->n_kv, attn_cost(kv->type, kv->dim), (kv->dim + 2) * 4 * 2,
-                       attn_workgroups(kv->type, kv->dim) * wgs / 4, min_keys});
+                       attn_workgroups(kv->type, kv->dim), kMinPieceCost});
         if (!upload(b, (hipStream_t)stream)) return 0;
         b->epoch = kt.epoch();
         b->set = true;

@@ -45,7 +45,7 @@ int host_pages(Host *h, int s, int *out) {
     return (int)p.size();
 }
 void host_plan(Host *h, int n, const int *s, const int *k, int group, int n_kv, const int *cost, int part_cost, int wgs) {
-    h->plan.build(h->kv, n, s, k, {group, n_kv, {cost[0], cost[1], cost[2]}, part_cost, wgs, 256});
+    h->plan.build(h->kv, n, s, k, {group, n_kv, {{cost[0], cost[1], cost[2], cost[3]}}, part_cost, wgs, 12000});
 }
 // 0 tokens (4 words each), 1 items (8), 2 pages, 3 join_rows, 4 join_at, 5 join_parts, 6 parts and writable
 int host_plan_get(Host *h, int what, int *out) {

@@ -223,7 +223,7 @@ def test_refusals_change_nothing(lib):
 # ------------------------------------------------------------------ the plan
 
 
-def plan(h, seqs, n_new, group, n_kv=2, cost=(47, 59, 83), part_cost=104, wgs=512):
+def plan(h, seqs, n_new, group, n_kv=2, cost=(47, 56, 59, 83), part_cost=104, wgs=512):
     h.L.host_plan(h.h, len(seqs), ints(seqs), ints(n_new), group, n_kv, ints(cost), part_cost, wgs)
     out = []
     for what, w in enumerate((4, 8, 1, 1, 1, 1, 2)):
@@ -288,7 +288,9 @@ def test_plan_of_a_tree(lib, seed):
     r.shuffle(seqs)
     seqs = seqs[: r.randint(1, len(seqs))]
     n_new = [min(len(h.want[s]), r.choice([0, 1, 1, 2, r.randint(0, 60)])) for s in seqs]
-    check_plan(h, seqs, n_new, r.choice([1, 3, 4, 7]), wgs=r.choice([8, 512, 4096]))
+    # (rows cheapest by the full tile, by 16 at a time, by 64)
+    cost = r.choice([(47, 56, 59, 83), (65, 260, 262, 514), (46, 54, 60, 158), (10, 10, 10, 10)])
+    check_plan(h, seqs, n_new, r.choice([1, 3, 4, 7, 40]), cost=cost, wgs=r.choice([8, 512, 4096]))
 
 
 def test_a_shared_run_is_read_once(lib):
