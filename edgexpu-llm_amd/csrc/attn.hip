@@ -776,11 +776,11 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
 // side by side.
 template <int TYPE, int DIM, int RT>
 __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &it, const Source &src, int h, uint8_t *lds,
-                                            int row_from, int wave, int lane) {
+                                            int wave, int lane) {
     using G = Geo<TYPE, DIM>;
     using L = Loader<TYPE, DIM>;
     Rows<TYPE, DIM, RT> w;
-    const int mine = row_from + wave * 16 * RT;  // (past the last row: computed from that row, not stored)
+    const int mine = wave * 16 * RT;  // (past the last row: computed from that row, not stored)
     const int tiles = (it.key1 - it.key0 + G::TT - 1) / G::TT;
     const uint32_t base = lds_addr(lds);
     const auto unit_at = [&](int i) { return lds + (i % G::SHARED) * 2 * G::UNIT; };
@@ -794,7 +794,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
     const int first = it.causal ? __builtin_amdgcn_readfirstlane(w.lim[0]) : it.key1;
     const int wave_last = it.causal ? w.last_limit() : it.key1;
     // (the workgroup's first row: the least limit of all waves)
-    const int all_first = it.causal ? min(it.key1, token_of(a, it, row_from)->order_pos + 1) : it.key1;
+    const int all_first = it.causal ? min(it.key1, token_of(a, it, 0)->order_pos + 1) : it.key1;
     wait_dma<0>();
     workgroup_barrier();
     uint8_t *wide = lds + G::SHARED * 2 * G::UNIT;  // Q8_0: f16 codes of the next tile's K, parts of this tile's V
@@ -914,9 +914,8 @@ __global__ __launch_bounds__(256, (Geo<TYPE, DIM>::PER_CU)) void attn_kernel(con
         s.last = (it.key1 - 1) >> a.kv.page_shift;
         if (it.n_rows <= 16) attend_few<TYPE, DIM, 1>(a, it, s, h, lds, wave, lane);
         else if (G::PAIR && it.n_rows <= 32) attend_few<TYPE, DIM, G::PAIR ? 2 : 1>(a, it, s, h, lds, wave, lane);
-        else if (G::RT == 1 || it.n_rows <= 64)
-            for (int r = 0; r < it.n_rows; r += 64) attend_many<TYPE, DIM, 1>(a, it, s, h, lds, r, wave, lane);
-        else attend_many<TYPE, DIM, G::RT>(a, it, s, h, lds, 0, wave, lane);
+        else if (G::RT == 1 || it.n_rows <= 64) attend_many<TYPE, DIM, 1>(a, it, s, h, lds, wave, lane);
+        else attend_many<TYPE, DIM, G::RT>(a, it, s, h, lds, wave, lane);
     }
 }
 
@@ -958,15 +957,16 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
             __syncthreads();
             const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
             const float c = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-            // a piece behind the row's last position has no weight (a NaN sum has)
-            const float f = mi == -INFINITY && li == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mi - mn);
+            // a piece behind the row's last position is left out; others count with any weight, zero too (NaN)
+            const bool out = mi == -INFINITY && li == 0.0f;
+            const float f = out ? -1.0f : __builtin_amdgcn_exp2f(mi - mn);
             weight[tid] = f;
             piece[tid] = ps;
             m = mn;
             l *= c;
             acc *= c;
             __syncthreads();
-            li = f == 0.0f ? 0.0f : f * li;
+            li = out ? 0.0f : f * li;
             li = wave_sum_f32(li);
             __syncthreads();
             if ((tid & 63) == 0) red[tid >> 6] = li;
@@ -975,7 +975,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
                 for (int p = grp; p < n; p += GROUPS) {
                     const float wp = weight[p];
                     const v4f v = *reinterpret_cast<const v4f *>(a.part + ((size_t)piece[p] * n_kv + h) * DIM + e);
-                    if (wp != 0.0f) acc += wp * v;
+                    if (!(wp < 0.0f)) acc += wp * v;
                 }
             }
             __syncthreads();
@@ -998,9 +998,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
 // for few rows (bound by the loads, 5 to 6 TB/s), of one run of 131072 for more.
 RowCost attn_cost(int type, int dim) {
     const int d = dim == 64 ? 0 : dim == 96 ? 1 : dim == 128 ? 2 : 3;
-    static const RowCost f32[4] = {{{460, 540, 1000, 1580}}, {{666, 797, 1494, 2270}}, {{878, 1007, 1780, 2900}}, {{1765, 4750, 4760, 9390}}};
-    static const RowCost f16[4] = {{{237, 320, 320, 520}}, {{336, 470, 480, 730}}, {{474, 590, 595, 840}}, {{865, 1414, 1425, 2741}}};
-    static const RowCost q80[4] = {{{148, 267, 586, 774}}, {{230, 403, 878, 1100}}, {{286, 469, 920, 1160}}, {{648, 2609, 2624, 5137}}};
+    static const RowCost f32[4] = {{{460, 540, 1000, 1580}}, {{666, 797, 1494, 2270}}, {{878, 1007, 1780, 2900}}, {{1765, 4750, 4760, 0}}};
+    static const RowCost f16[4] = {{{237, 320, 320, 520}}, {{336, 470, 480, 730}}, {{474, 590, 595, 840}}, {{865, 1414, 1425, 0}}};
+    static const RowCost q80[4] = {{{148, 267, 586, 774}}, {{230, 403, 878, 1100}}, {{286, 469, 920, 1160}}, {{648, 2609, 2624, 0}}};
     return type == kTypeF32 ? f32[d] : type == kTypeF16 ? f16[d] : q80[d];
 }
 
@@ -1012,12 +1012,20 @@ int per_cu(int type) {
 }
 
 template <int TYPE, int DIM>
-hipError_t launch_typed(const AttnArgs &a, unsigned grid, hipStream_t st) {
+hipError_t allow_lds() {
     constexpr int bytes = Geo<TYPE, DIM>::LDS_BYTES;
     static_assert(bytes <= 160 * 1024, "the rings fit the gfx950 LDS");
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void *>(attn_kernel<TYPE, DIM>),
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (set != hipSuccess) return set;
+    return hipFuncSetAttribute(reinterpret_cast<const void *>(attn_kernel<TYPE, DIM>),
+                               hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+template <int DIM>
+hipError_t allow_lds(int type) {
+    return type == kTypeF32 ? allow_lds<kTypeF32, DIM>() : type == kTypeF16 ? allow_lds<kTypeF16, DIM>() : allow_lds<kTypeQ8_0, DIM>();
+}
+
+template <int TYPE, int DIM>
+hipError_t launch_typed(const AttnArgs &a, unsigned grid, hipStream_t st) {
+    constexpr int bytes = Geo<TYPE, DIM>::LDS_BYTES;
     hipLaunchKernelGGL((attn_kernel<TYPE, DIM>), dim3(grid), dim3(256), bytes, st, a);
     return hipGetLastError();
 }
@@ -1035,6 +1043,10 @@ hipError_t launch_attention(const AttnArgs &a, int type, unsigned grid, unsigned
 
 }  // namespace
 
+hipError_t attn_prepare(int type, int dim) {
+    return dim == 64 ? allow_lds<64>(type) : dim == 96 ? allow_lds<96>(type) : dim == 128 ? allow_lds<128>(type) : allow_lds<256>(type);
+}
+
 int attn_workgroups(int type, int dim) {
     return 256 * (dim == 64 ? per_cu<64>(type) : dim == 96 ? per_cu<96>(type) : dim == 128 ? per_cu<128>(type) : per_cu<256>(type));
 }
@@ -1048,6 +1060,7 @@ extern "C" int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip
     if (!lib_ready("attention")) return 0;
     bool capturing = false;
     if (!batch_ready(b, layer, (hipStream_t)stream, "attention", &capturing)) return 0;
+    if (!capturing && b->plan.tokens.empty()) return 1;
     if (out == nullptr || q == nullptr || (((uintptr_t)out | (uintptr_t)q) & 15u) != 0) {
         lib_error(-2, "attention: null buffer, or q or out not 16-byte aligned");
         return 0;
@@ -1070,7 +1083,6 @@ extern "C" int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip
     a.joins = capturing ? -1 : joins;
     const unsigned grid = capturing ? 1024u : (unsigned)std::min<long long>(items, 1 << 20);
     const unsigned join_grid = capturing ? 1024u : (unsigned)std::min<long long>(joins, 1 << 20);
-    if (grid == 0) return 1;
     hipError_t e;
     switch (kv->dim) {
         case 64: e = launch_attention<64>(a, kv->type, grid, join_grid, (hipStream_t)stream); break;

@@ -49,7 +49,7 @@ struct PlanHeader {
 static_assert(sizeof(AttnItem) == 32 && sizeof(PlanToken) == 16 && sizeof(PlanHeader) == 64, "words of the device plan");
 
 // What a workgroup takes for one key, in tenths of a nanosecond with all others
-// at work, for at most 16, 32, 64 and 128 rows.
+// at work, for at most 16, 32, 64 and 128 rows (0: not that many at once).
 struct RowCost {
     int of[4];
 };
@@ -145,6 +145,7 @@ struct AttnPlan {
         for (int n = 1; n <= 8; ++n) {
             step_[n] = 0;
             for (int k = 3; k >= 0; --k) {
+                if (shape_.cost.of[k] == 0) continue;
                 const int u = 1 << k, c = shape_.cost.of[k] + best_[n > u ? n - u : 0];
                 if (step_[n] == 0 || c < best_[n]) {
                     best_[n] = c;

@@ -311,7 +311,7 @@ edgexpu_hip_batch *edgexpu_hip_batch_create(edgexpu_hip_kv *kv, int n_heads, int
                   max_seqs, max_tokens);
         return nullptr;
     }
-    if (!lib_ready("batch_create")) return nullptr;
+    if (!lib_ready("batch_create") || !lib_hip(attn_prepare(kv->type, kv->dim), "batch_create")) return nullptr;
     edgexpu_hip_batch *b =
         guarded("batch_create", (edgexpu_hip_batch *)nullptr, [] { return new edgexpu_hip_batch(); });
     if (b == nullptr) return nullptr;

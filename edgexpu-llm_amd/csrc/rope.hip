@@ -464,6 +464,7 @@ int edgexpu_hip_kv_append_dev(float *q_out, const float *q, long long ldq, const
     bool capturing = false;
     if (!batch_ready(b, layer, (hipStream_t)stream, "kv_append", &capturing)) return 0;
     const edgexpu_hip_kv *kv = b->kv;
+    if (!capturing && b->plan.tokens.empty()) return 1;
     if (q == nullptr || q_out == nullptr || k == nullptr || v == nullptr || ldq < (long long)b->n_heads * kv->dim ||
         ldk < (long long)kv->n_kv * kv->dim || ldv < (long long)kv->n_kv * kv->dim) {
         lib_error(-2, "kv_append: null buffer or short rows");

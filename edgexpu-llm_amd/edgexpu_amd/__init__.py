@@ -430,8 +430,9 @@ class KvCache:
         size = L.kv_pool_bytes(qtype, n_layers, n_kv_heads, head_dim, page_tokens, n_pages)
         if pool is None:
             pool = torch.empty(size, dtype=torch.uint8, device="cuda")
-        elif pool.dtype != torch.uint8 or pool.dim() != 1 or not pool.is_contiguous() or pool.numel() != size:
-            raise ValueError(f"pool must be a flat uint8 tensor of {size} bytes")
+        elif not pool.is_cuda or pool.dtype != torch.uint8 or pool.dim() != 1 or not pool.is_contiguous() or (
+                size and pool.numel() != size):
+            raise ValueError(f"pool must be a flat uint8 device tensor of {size} bytes")
         self.pool, self.n_kv_heads, self.head_dim = pool, n_kv_heads, head_dim
         h = L.kv_create(_ptr(pool) if size else None, qtype, n_layers, n_kv_heads, head_dim, page_tokens, n_pages,
                         max_seqs)
@@ -538,11 +539,25 @@ class Rope:
             _HIP.rope_destroy(self._h)
 
 
+def _f32(x) -> bool:
+    return x.is_cuda and x.element_size() == 4 and x.is_floating_point()
+
+
+def _dense(x, n: int, what: str):
+    if not _f32(x) or not x.is_contiguous() or x.numel() < n:
+        raise ValueError(f"{what} must be a dense float32 device tensor of at least {n} values")
+    return x
+
+
+def _weight(w, dim: int) -> int | None:
+    return None if w is None else _dense(w, dim, "the norm's weight").data_ptr()
+
+
 def _rows(x, n: int, what: str) -> int:
     """The distance of rows of n float32 values, which may be a slice of a wider buffer."""
     ld, one = x.stride() if x.dim() == 2 else (0, 0)
-    if one != 1 or x.shape[1] != n or x.element_size() != 4 or not x.is_floating_point():
-        raise ValueError(f"{what} must be float32 [tokens, {n}] with dense rows")
+    if one != 1 or x.shape[1] != n or not _f32(x):
+        raise ValueError(f"{what} must be a float32 device tensor [tokens, {n}] with dense rows")
     return ld if ld >= n else n if x.shape[0] < 2 else ld
 
 
@@ -553,18 +568,18 @@ def qk_norm_rope(q, k, n_heads: int, n_kv_heads: int, pos, rope: Rope | None = N
     (edgexpu_hip_qk_norm_rope_dev); rows may be slices of a wider buffer."""
     import torch
 
+    if n_heads <= 0 or q.dim() != 2 or q.shape[1] % n_heads:
+        raise ValueError(f"q must be [tokens, n_heads * head_dim] with {n_heads} heads")
     m, dim = q.shape[0], q.shape[1] // n_heads
     ldq, ldk = _rows(q, n_heads * dim, "q"), _rows(k, n_kv_heads * dim, "k")
-    if k.shape[0] != m or (pos is not None and (pos.numel() != m or pos.dtype != torch.int32)):
+    if k.shape[0] != m or (pos is not None and (pos.numel() != m or pos.dtype != torch.int32 or not pos.is_cuda)):
         raise ValueError("q, k and the int32 pos must have the same tokens")
-    if q_out is None:
-        q_out = torch.empty((m, n_heads * dim), dtype=torch.float32, device=q.device)
-    if k_out is None:
-        k_out = torch.empty((m, n_kv_heads * dim), dtype=torch.float32, device=q.device)
+    q_out = q.new_empty((m, n_heads * dim)) if q_out is None else _dense(q_out, m * n_heads * dim, "q_out")
+    k_out = q.new_empty((m, n_kv_heads * dim)) if k_out is None else _dense(k_out, m * n_kv_heads * dim, "k_out")
     L = hip()
-    L.check(L.qk_norm_rope_dev(_ptr(q_out), _ptr(k_out), _ptr(q), ldq, _ptr(k), ldk, m, n_heads, n_kv_heads, dim,
-                               _ptr(q_weight), _ptr(k_weight), eps, rope._h if rope else None, _ptr(pos), _stream()),
-            "qk_norm_rope")
+    L.check(L.qk_norm_rope_dev(q_out.data_ptr(), k_out.data_ptr(), q.data_ptr(), ldq, k.data_ptr(), ldk, m, n_heads,
+                               n_kv_heads, dim, _weight(q_weight, dim), _weight(k_weight, dim), eps,
+                               None if rope is None else rope._h, _ptr(pos), _stream()), "qk_norm_rope")
     return q_out, k_out
 
 
@@ -577,10 +592,10 @@ def kv_append(batch: KvBatch, layer: int, q, k, v, rope: Rope | None = None, q_w
     ldq, ldk, ldv = _rows(q, n, "q"), _rows(k, nk, "k"), _rows(v, nk, "v")
     if q.shape[0] < m or k.shape[0] < m or v.shape[0] < m:
         raise ValueError(f"q, k and v need the batch's {m} tokens")
-    if q_out is None:
-        q_out = q.new_empty((m, n))
+    q_out = q.new_empty((m, n)) if q_out is None else _dense(q_out, m * n, "q_out")
     if not _HIP.kv_append_dev(q_out.data_ptr(), q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, batch._h, layer,
-                              _ptr(q_weight), _ptr(k_weight), eps, None if rope is None else rope._h, _stream()):
+                              _weight(q_weight, c.head_dim), _weight(k_weight, c.head_dim), eps,
+                              None if rope is None else rope._h, _stream()):
         _HIP.check(0, "kv_append")
     return q_out
 
@@ -590,10 +605,8 @@ def attention(batch: KvBatch, layer: int, q, scale: float | None = None, out=Non
     (edgexpu_hip_attention_dev): q [tokens, n_heads * head_dim] float32; scale
     1/sqrt(head_dim) unless given."""
     m, n = batch.tokens(), batch.n_heads * batch.cache.head_dim
-    if q.element_size() != 4 or not q.is_floating_point() or not q.is_contiguous() or q.numel() < m * n:
-        raise ValueError(f"q must be dense float32 [tokens, {n}] with the batch's {m} tokens")
-    if out is None:
-        out = q.new_empty((m, n))
+    _dense(q, m * n, f"q [tokens, {n}]")
+    out = q.new_empty((m, n)) if out is None else _dense(out, m * n, "out")
     if scale is None:
         scale = batch.cache.head_dim ** -0.5
     if not _HIP.attention_dev(out.data_ptr(), q.data_ptr(), batch._h, layer, scale, _stream()):

@@ -352,7 +352,8 @@ int edgexpu_hip_gate_up_silu_dev(float *act, const float *x, const float *norm_w
  * too is copied before a sequence grows in it.  New pages are the free ones
  * with the lowest numbers, new sequences the lowest free numbers.  A call that
  * does not have the pages or sequences it needs is refused (error -6) and
- * changes nothing. */
+ * changes nothing; calls that copy pages (extend, compact, a fork with copies)
+ * are refused while `stream` is captured (error -7). */
 typedef struct edgexpu_hip_kv edgexpu_hip_kv;
 
 /* Bytes of such a pool; 0 (no error) for a shape that is not supported. */
@@ -404,7 +405,7 @@ int edgexpu_hip_kv_tables(const edgexpu_hip_kv *kv, int n, const int *seqs, int 
  * n_heads: query heads, a multiple of the cache's kv heads (query head h reads
  * kv head h / (n_heads / n_kv_heads)).
  * edgexpu_hip_batch_set copies the plan to the device on `stream`; it is
- * refused (error -7) while a stream of this thread is captured.  Its device
+ * refused (error -7) while that stream is captured.  Its device
  * buffers grow as plans need; a batch that a captured call has used keeps its
  * buffers, and a plan that outgrows them is refused (error -7): set the largest
  * one before the capture.  A captured step replays with whatever plan the last
@@ -451,8 +452,9 @@ int edgexpu_hip_kv_append_dev(float *q_out, const float *q, long long ldq, const
  * up to token t's own of its sequence, for the batch's tokens: q and out
  * [tokens][n_heads][head_dim] f32, dense, 16-byte aligned, out may be q.
  * Products of f16 and Q8_0 caches run on the matrix cores with q and the
- * weights as two f16 parts each (22 bits), sums in f32: results as those of 32
- * bits.  Contents of slots that a token does not see (behind the sequence's
+ * weights as two f16 parts each (22 bits; a weight below 2^-31 of its row's
+ * largest may be lost), sums in f32: results as those of 32 bits.  With f16 and
+ * Q8_0 a key or value that is not finite makes what it reaches NaN.  Contents of slots that a token does not see (behind the sequence's
  * end, or of later tokens of the step) have no influence, NaN and infinities
  * included. */
 int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip_batch *b, int layer, float scale, void *stream);

@@ -75,6 +75,7 @@ SINGLE = [  # (dim, kv, group, page, length, new)
     (96, 2, 2, 16, 47, 5), (256, 1, 8, 128, 127, 1), (128, 8, 4, 32, 1000, 1), (64, 1, 1, 64, 300, 300),
     (128, 1, 3, 16, 200, 77), (256, 2, 2, 64, 150, 33), (96, 1, 16, 256, 511, 2), (128, 1, 20, 64, 90, 2),
     (64, 3, 3, 64, 4099, 1), (128, 2, 1, 128, 2500, 17),
+    (64, 1, 1, 256, 140001, 1), (256, 1, 2, 16, 847, 315), (128, 1, 40, 32, 300, 1),
 ]
 
 
@@ -484,6 +485,48 @@ def test_captured_step_replays_later_plans(hipdev):
     E.attention(big, 0, qr)
 
 
+def test_no_tokens(hipdev):
+    rng = np.random.default_rng(4)
+    c = make(rng, E.F16, 2, 64, 16, 8, 3)
+    s = c.new()
+    c.extend([s], [20])
+    b = E.KvBatch(c, 4, 2, 8)
+    none = torch.empty((0, 256), device="cuda:0")
+    for ids, n_new in (([], []), ([s], [0])):
+        b.set(ids, n_new)
+        assert E.attention(b, 0, none).shape == (0, 256)
+        assert E.kv_append(b, 0, none, none[:, :128], none[:, :128]).shape == (0, 256)
+    e = c.new()
+    assert c.fork([e]) and c.length(e) == 0 and c.tables([e]).shape == (1, 0)
+    b.set([e, s], [0, 1])
+    check_attention(c, E.F16, 1, 8, 16, [e, s], [0, 1], 4, rng)
+
+
+def test_nan_reaches_its_rows_only(hipdev):
+    """A NaN key or query makes its own rows NaN through every split of the keys, and no others."""
+    rng = np.random.default_rng(14)
+    for qtype in (E.F16, E.F32, E.Q8_0):
+        c = make(rng, qtype, 1, 128, 64, 300, 3)
+        a, e = c.new(), c.new()
+        c.extend([a, e], [9000, 9000])
+        b = E.KvBatch(c, 2, 2, 2)
+        b.set([a, e], [1, 1])
+        q = dev(rng.standard_normal((2, 256)).astype(np.float32))
+        before = E.attention(b, 0, q).clone()
+        q2 = q.clone()
+        q2[1, 130] = float("nan")
+        got = E.attention(b, 0, q2)
+        assert torch.equal(got[0], before[0]) and torch.equal(got[1, :128], before[1, :128]) and got[1, 128:].isnan().all()
+        page = c.tables([a])[0][3]
+        raw = c.pool.view(300, 2, -1)
+        if qtype == E.Q8_0:
+            raw[page, 0, 64 * 128 + 10 * 8: 64 * 128 + 10 * 8 + 2] = dev(np.full(1, np.nan, np.float16).view(np.uint8))
+        else:
+            raw[page, 0].view(torch.float16 if qtype == E.F16 else torch.float32)[10 * 128 + 5] = float("nan")
+        got = E.attention(b, 0, q)
+        assert got[0].isnan().all() and torch.equal(got[1], before[1])
+
+
 def test_two_batches_on_two_streams(hipdev):
     rng = np.random.default_rng(21)
     c = make(rng, E.Q8_0, 4, 128, 64, 300, 8)
@@ -544,6 +587,15 @@ def test_refusals(hipdev):
         (lambda: E.kv_append(b, 0, q, k, k, E.Rope(128)), "128 values"),
     ]:
         with pytest.raises(E.HipError, match=what):
+            call()
+    for call in (lambda: E.attention(b, 0, q[:1]), lambda: E.attention(b, 0, q.half()), lambda: E.attention(b, 0, q.cpu()),
+                 lambda: E.attention(b, 0, q, out=q[:, :200]), lambda: E.kv_append(b, 0, q, k[:1], k),
+                 lambda: E.kv_append(b, 0, q, k, k, q_weight=k[0, :32]), lambda: E.kv_append(b, 0, q, k.double(), k),
+                 lambda: c.extend([s], [1, 2]), lambda: b.set([s], []), lambda: c.length(2),
+                 lambda: E.KvCache(E.F16, 1, 1, 64, 16, 4, 1, pool=q.view(torch.uint8).view(-1)),
+                 lambda: E.Rope(64, factors=[1.0] * 31), lambda: E.qk_norm_rope(q, k, 3, 2, None),
+                 lambda: E.qk_norm_rope(q, k, 4, 2, torch.zeros(7, dtype=torch.int32, device="cuda:0"))):
+        with pytest.raises(ValueError):
             call()
     # a batch set refused leaves the batch unset; a change of the cache makes it stale
     b.set([s], [2])
