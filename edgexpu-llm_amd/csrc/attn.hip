@@ -138,13 +138,17 @@ __device__ __forceinline__ uint32_t max_u16(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
 
-// High part and rest of eight values.
+// High part and rest of eight values.  The factor is one the compiler does not
+// know, so that x - hi is one v_fma_mix_f32 and not a conversion and a
+// subtraction.
 __device__ __forceinline__ void split8(const float (&x)[8], v8h &hi, v8h &lo) {
     typedef float v2f __attribute__((ext_vector_type(2)));
+    float minus = -1.0f;
+    asm("" : "+v"(minus));
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
         const h2 h = __builtin_convertvector((v2f{x[j], x[j + 1]}), h2);
-        const h2 l = __builtin_convertvector((v2f{fmaf((float)h[0], -1.0f, x[j]), fmaf((float)h[1], -1.0f, x[j + 1])}), h2);
+        const h2 l = __builtin_convertvector((v2f{fmaf((float)h[0], minus, x[j]), fmaf((float)h[1], minus, x[j + 1])}), h2);
         hi[j] = h[0];
         hi[j + 1] = h[1];
         lo[j] = l[0];
@@ -268,7 +272,7 @@ struct Rows {
     static constexpr int NQ = TYPE == kTypeF32 ? G::ND : G::NB;
     v8h qh[TYPE == kTypeF32 ? 1 : RT][TYPE == kTypeF32 ? 1 : G::NB], ql[TYPE == kTypeF32 ? 1 : RT][TYPE == kTypeF32 ? 1 : G::NB];
     v4f qf[TYPE == kTypeF32 ? RT : 1][TYPE == kTypeF32 ? G::ND : 1];
-    float rs[RT], m[RT], l[RT];  // score factor (positive); running maximum (of base-2 exponents), this lane's part of the sum
+    float top[RT], rs[RT], m[RT], l[RT];  // score factor (positive); running maximum (of base-2 exponents), this lane's part of the sum
     int lim[RT];                 // positions below are seen
     v4f acc[RT][G::ND];
     int ve;                      // Q8_0: acc is in units of 2^ve
@@ -392,18 +396,25 @@ struct Rows {
         for (int d = 0; d < G::ND; ++d) acc[t][d] *= c;
     }
 
+    // This lane's largest scores.
+    __device__ __forceinline__ void tops() {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            top[t] = -INFINITY;
+#pragma unroll
+            for (int hf = 0; hf < G::HALVES; ++hf)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top[t] = fmaxf(top[t], s[t][hf][r]);
+            top[t] *= rs[t];
+        }
+    }
+
     // The maximum is raised where scores exceed it by 8.
     __device__ __forceinline__ void raise() {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int hf = 0; hf < G::HALVES; ++hf)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][hf][r]);
-            top *= rs[t];
-            if (__builtin_amdgcn_ballot_w64(top > m[t] + 8.0f) != 0) {
-                const float mn = fmaxf(m[t], col_max(top));
+            if (__builtin_amdgcn_ballot_w64(top[t] > m[t] + 8.0f) != 0) {
+                const float mn = fmaxf(m[t], col_max(top[t]));
                 const float c = m[t] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[t] - mn);
                 m[t] = mn;
                 l[t] *= c;
@@ -704,6 +715,7 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
         issue(2 * (i + ahead) + 1, now);
         w.scores(ringp + (2 * i % G::RING) * G::UNIT, nullptr, lane);
         if (edge) w.mask(p0, lane);
+        w.tops();
         w.raise();
         w.weights();
         arrive(2 * i + 1);
@@ -799,6 +811,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
     workgroup_barrier();
     uint8_t *wide = lds + G::SHARED * 2 * G::UNIT;  // Q8_0: f16 codes of the next tile's K, parts of this tile's V
     w.scores(unit_at(0), nullptr, lane);
+    w.tops();
     for (int i = 0; i < tiles; ++i) {
         const int p0 = it.key0 + i * G::TT;
         uint8_t *vu = unit_at(i) + G::UNIT;
@@ -832,13 +845,17 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
             workgroup_barrier();
         }
         if (p0 >= wave_last) continue;  // behind all of this wave's rows
-        if (p0 + G::TT > first) w.mask(p0, lane);
+        if (p0 + G::TT > first) {
+            w.mask(p0, lane);
+            w.tops();
+        }
         w.raise();
         w.weights();
         // (behind the last tile: scores of whatever lies there, and not used)
         w.scores(unit_at(i + 1), TYPE == kTypeQ8_0 ? wide : nullptr, lane);
         if constexpr (TYPE == kTypeQ8_0) w.template values16<true>(wide + G::TILE16, wide + 2 * G::TILE16, lane);
         else w.values(vu, lane);
+        w.tops();
     }
     w.finish();
     const int c = lane & 15, g = lane >> 4;
