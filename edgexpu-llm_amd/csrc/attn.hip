@@ -11,7 +11,7 @@
 //                 weights it must supply, in an order of keys that the V
 //                 operand follows; no exchange between lanes.
 // K and V come into LDS by DMA (16-byte pieces of a row permuted so that the
-// reads below meet no bank twice); V is read transposed (ds_read_..._tr).
+// reads below spread over the banks); V is read transposed (ds_read_..._tr).
 //
 // Arithmetic.  F16 and Q8_0: q (after an exact power-of-two scaling of its row
 // that keeps both parts in range) and the weights as two f16 parts, high and
@@ -23,6 +23,17 @@
 // the f32 matrix instructions.  Weights are 2^(s - m + 7) with m at most 8
 // behind the true maximum: it is raised, and the sums rescaled, only when a
 // tile exceeds it by 2^8 (an exponent range the f16 parts have to spare).
+//
+// What bounds it, at head size 128 and 8 kv heads, measured:
+//   few rows (single tokens, no sharing): the loads.  f16 5.5 TB/s, Q8_0 4.9,
+//     f32 6.0 (a large copy: 5.1); 24 sequences of 200 to 12000 f16 keys 110 us;
+//   many rows (a shared run, a chunk of tokens): matrix and vector instructions
+//     together.  4 x 512 tokens behind 8192 f16 keys 490 us: 1.2 PFLOP/s of
+//     matrix instructions (two for each product; a loop of nothing but them on
+//     random operands reaches 1.75 on this card, a large library product 1.1);
+//     MFMA 57 % of the cycles, waves wait 27 % and contend for issue 30 %;
+//   short calls: a chain of loads (item -> page -> keys, item -> token -> query),
+//     the first tile and the join of the waves, 5 to 7 us.
 #include <hip/hip_runtime.h>
 
 #include "gemm_common.h"
@@ -84,7 +95,8 @@ struct Geo {
 // Piece permutation of row `row` of a tile: piece c lies at c ^ swz.  Chosen so
 // that 16 rows read at one piece (K), or 8 rows at two neighbouring pieces and
 // 16 rows at one (V, transposed reads of 16 and 8 bits), or 4 rows 4 apart at
-// 4 pieces (V, F32), fall on different banks of 64.
+// 4 pieces (V, F32), fall on different banks of 64 (a quarter of the LDS cycles
+// are conflicts all the same; LDS is busy a fifth of the time).
 template <int TYPE, int DIM, bool V>
 __device__ __forceinline__ int swz(int row) {
     if (TYPE == kTypeF32) {

@@ -1,7 +1,8 @@
 /*
  * edgexpu_hip.h -- C-ABI of libedgexpu_hip.so, the MI355X (gfx950) kernel set
  * for the GGUF quantized-weight matrix path (Q8_0 / Q4_K / Q6_K, and the
- * dispatcher's other formats Q4_0 / Q5_0 / Q5_K / F16 / F32).
+ * dispatcher's other formats Q4_0 / Q5_0 / Q5_K / F16 / F32) and for what a
+ * decoder layer does between its projections.
  *
  * Plain C types only (no HIP or torch types): device pointers are `void *` /
  * typed pointers into device memory, streams are `void *` holding a
@@ -324,10 +325,11 @@ int edgexpu_hip_gate_up_silu_dev(float *act, const float *x, const float *norm_w
 
 /* ---- between the projections: rotation, paged cache, attention ----
  * What a decoder layer does between its q/k/v and output projections
- * (per-head norms, RoPE, the key/value cache and attention over it:
- * src/native.c:2536-2571, src/cpu_kernel.c:659-760, src/kv_cache.c:22-127 of
- * the reference, where the cache is one sequence's f32 window), for a batch of
- * sequences on device-resident activations.  A step is
+ * (per-head norms, RoPE, the key/value cache and attention over it; the
+ * reference: between src/native.c:2532 and :2571, attention at :2545-2569, the
+ * ops among src/cpu_kernel.c:659-972, the cache, one sequence's f32 window, in
+ * src/kv_cache.c:22-127), for a batch of sequences on device-resident
+ * activations.  A step is
  *   edgexpu_hip_kv_extend (slots for the new tokens), edgexpu_hip_batch_set
  *   (what the step computes), then for each layer edgexpu_hip_kv_append_dev
  *   and edgexpu_hip_attention_dev.
@@ -423,7 +425,7 @@ int edgexpu_hip_batch_tokens(const edgexpu_hip_batch *b);
  * 256) turn in pairs by position * scale * base^(-2i / n_rot) / factors[i] (host
  * array of n_rot/2, NULL: ones), pair i being the values i and i + n_rot/2, or
  * with `interleaved` 2i and 2i + 1 (the reference's two RoPE forms,
- * src/cpu_kernel.c:659-760).  Angles are kept in 64 bits and reduced there, so
+ * among src/cpu_kernel.c:659-972).  Angles are kept in 64 bits and reduced there, so
  * far positions lose nothing.  NULL on error. */
 typedef struct edgexpu_hip_rope edgexpu_hip_rope;
 edgexpu_hip_rope *edgexpu_hip_rope_create(int n_rot, double base, double scale, const float *factors,
