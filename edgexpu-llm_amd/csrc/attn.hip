@@ -281,7 +281,6 @@ struct Loader {
 template <int TYPE, int DIM, int RT>
 struct Rows {
     using G = Geo<TYPE, DIM>;
-    static constexpr int NQ = TYPE == kTypeF32 ? G::ND : G::NB;
     v8h qh[TYPE == kTypeF32 ? 1 : RT][TYPE == kTypeF32 ? 1 : G::NB], ql[TYPE == kTypeF32 ? 1 : RT][TYPE == kTypeF32 ? 1 : G::NB];
     v4f qf[TYPE == kTypeF32 ? RT : 1][TYPE == kTypeF32 ? G::ND : 1];
     float top[RT], rs[RT], m[RT], l[RT];  // score factor (positive); running maximum (of base-2 exponents), this lane's part of the sum
@@ -303,7 +302,7 @@ struct Rows {
             if constexpr (TYPE == kTypeF32) {
 #pragma unroll
                 for (int c = 0; c < G::ND; ++c) qf[t][c] = sign * *reinterpret_cast<const v4f *>(q + c * 16 + g * 4);
-                rs[t] = scale;
+                rs[t] = fmaxf(scale, 1.17549435e-38f);
             } else {
                 float x[G::NB][8], top = 0.0f;
 #pragma unroll
@@ -482,11 +481,24 @@ struct Rows {
         }
     }
 
-    // Q8_0: the unit of acc is raised to 2^e where the largest scale `top` (of the wave's lanes together) exceeds it.
-    __device__ __forceinline__ void raise_unit(float top) {
+    // This lane's largest finite scale of the V unit at vu (the lanes together: the unit's).
+    static __device__ __forceinline__ float finite_top(const uint8_t *vu, int lane) {
+        const _Float16 *d = reinterpret_cast<const _Float16 *>(vu + G::TT * G::RB);
+        float top = 0.0f;
+        for (int k = lane; k < G::TT * G::NB; k += 64) {
+            const float x = fabsf((float)d[k]);
+            if (x < INFINITY) top = fmaxf(top, x);
+        }
+        return top;
+    }
+
+    // Q8_0: the unit of acc is raised to 2^e where the largest scale `top` (of the wave's lanes together) exceeds it, so
+    // that scales are at most 1 in it and weights times scale stay in f16's range.  A scale that is not finite makes its
+    // block's sums NaN in any unit, and has no say in the others'.
+    __device__ __forceinline__ void raise_unit(float top, const uint8_t *vu, int lane) {
         if (__builtin_amdgcn_ballot_w64(top > ldexpf(1.0f, ve)) == 0) return;
-        top = wave_max(top);
-        const int e = top < INFINITY ? __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top)) : 16;
+        if (__builtin_amdgcn_ballot_w64(top == INFINITY) != 0) top = finite_top(vu, lane);
+        const int e = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(wave_max(top)));
         if (e <= ve) return;
 #pragma unroll
         for (int t = 0; t < RT; ++t) rescale(ldexpf(1.0f, ve - e), t);
@@ -519,9 +531,7 @@ struct Rows {
                     sc[hf][i] = ds[hf * 8 * G::NB + i];
                     most = max_u16(most, sc[hf][i] & 0x7fff7fffu);
                 }
-            const float top = f16_bits_to_f32(max(most & 0xffffu, most >> 16));
-            // scales at most 1 in the units of acc: weights times scale stay in f16's range
-            raise_unit(top);
+            raise_unit(f16_bits_to_f32(min(max(most & 0xffffu, most >> 16), 0x7c00u)), vu, lane);
             const float f = ldexpf(1.0f, -ve);
             const int k = c16 >> 1, row = (k < 4 ? g * 4 + k : 16 + g * 4 + k - 4), sw = swz<TYPE, DIM, true>(row);
 #pragma unroll
@@ -756,40 +766,40 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
     const int tid = wave * 64 + lane;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-    __syncthreads();
+        __syncthreads();
 #pragma unroll
-    for (int d = 0; d < G::ND; ++d) *reinterpret_cast<v4f *>(mo + (wave * 16 + c) * DIM + d * 16 + g * 4) = w.acc[t][d];
-    if (g == 0) {
-        ml[2 * (wave * 16 + c)] = w.m[t];
-        ml[2 * (wave * 16 + c) + 1] = w.l[t];
-    }
-    __syncthreads();
-    for (int i = tid; i < min(16, it.n_rows - 16 * t) * (DIM / 4); i += 256) {
-        const int r = i / (DIM / 4), e = i % (DIM / 4) * 4;
-        float m = -INFINITY, l = 0.0f;
-#pragma unroll
-        for (int v = 0; v < 4; ++v) m = fmaxf(m, ml[2 * (v * 16 + r)]);
-        v4f o = {0, 0, 0, 0};
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const float mv = ml[2 * (v * 16 + r)];
-            if (mv == -INFINITY && ml[2 * (v * 16 + r) + 1] == 0.0f) continue;  // no key of this wave's is seen
-            const float f = __builtin_amdgcn_exp2f(mv - m);
-            l += f * ml[2 * (v * 16 + r) + 1];
-            o += f * *reinterpret_cast<const v4f *>(mo + (v * 16 + r) * DIM + e);
+        for (int d = 0; d < G::ND; ++d) *reinterpret_cast<v4f *>(mo + (wave * 16 + c) * DIM + d * 16 + g * 4) = w.acc[t][d];
+        if (g == 0) {
+            ml[2 * (wave * 16 + c)] = w.m[t];
+            ml[2 * (wave * 16 + c) + 1] = w.l[t];
         }
-        if (it.part < 0) {
-            *reinterpret_cast<v4f *>(a.out + row_at(a, it, h, 16 * t + r, DIM) + e) = o / l;
-        } else {
-            const size_t ps = (size_t)(it.part + 16 * t + r) * a.kv.n_kv + h;
-            *reinterpret_cast<v4f *>(a.part + ps * DIM + e) = o;
-            if (e == 0) {
-                float *d = a.part + a.part_cap * DIM + 2 * ps;
-                d[0] = m;
-                d[1] = l;
+        __syncthreads();
+        for (int i = tid; i < min(16, it.n_rows - 16 * t) * (DIM / 4); i += 256) {
+            const int r = i / (DIM / 4), e = i % (DIM / 4) * 4;
+            float m = -INFINITY, l = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) m = fmaxf(m, ml[2 * (v * 16 + r)]);
+            v4f o = {0, 0, 0, 0};
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float mv = ml[2 * (v * 16 + r)];
+                if (mv == -INFINITY && ml[2 * (v * 16 + r) + 1] == 0.0f) continue;  // no key of this wave's is seen
+                const float f = __builtin_amdgcn_exp2f(mv - m);
+                l += f * ml[2 * (v * 16 + r) + 1];
+                o += f * *reinterpret_cast<const v4f *>(mo + (v * 16 + r) * DIM + e);
+            }
+            if (it.part < 0) {
+                *reinterpret_cast<v4f *>(a.out + row_at(a, it, h, 16 * t + r, DIM) + e) = o / l;
+            } else {
+                const size_t ps = (size_t)(it.part + 16 * t + r) * a.kv.n_kv + h;
+                *reinterpret_cast<v4f *>(a.part + ps * DIM + e) = o;
+                if (e == 0) {
+                    float *d = a.part + a.part_cap * DIM + 2 * ps;
+                    d[0] = m;
+                    d[1] = l;
+                }
             }
         }
-    }
     }
     __syncthreads();
 }
@@ -851,7 +861,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
             float top = 0.0f;  // (every wave comes to the same unit)
             for (int k = lane; k < G::TT * G::NB; k += 64)
                 top = fmaxf(top, fabsf((float)reinterpret_cast<const _Float16 *>(vu + G::TT * G::RB)[k]));
-            w.raise_unit(top);
+            w.raise_unit(top, vu, lane);
             expand<DIM>(unit_at(i + 1), vu, wide, ldexpf(1.0f, -w.ve), wave * 64 + lane);
             lds_done();
             workgroup_barrier();
@@ -1090,8 +1100,8 @@ extern "C" int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip
     bool capturing = false;
     if (!batch_ready(b, layer, (hipStream_t)stream, "attention", &capturing)) return 0;
     if (!capturing && b->plan.tokens.empty()) return 1;
-    if (out == nullptr || q == nullptr || (((uintptr_t)out | (uintptr_t)q) & 15u) != 0) {
-        lib_error(-2, "attention: null buffer, or q or out not 16-byte aligned");
+    if (out == nullptr || q == nullptr || (((uintptr_t)out | (uintptr_t)q) & 15u) != 0 || !(fabsf(scale) < INFINITY)) {
+        lib_error(-2, "attention: null buffer, q or out not 16-byte aligned, or scale %g not finite", (double)scale);
         return 0;
     }
     const edgexpu_hip_kv *kv = b->kv;

@@ -349,7 +349,7 @@ bool rows_take(RopeArgs &a, int type, int m) {
     const auto least = [](long long x, long long y) { return x < y ? x : y; };
     const long long w = std::max(least((16384 + m - 1) / m, steps / 4), least((4096 + m - 1) / m, steps));
     a.waves = (int)std::max(w, 1LL);
-    return (long long)m * a.waves < INT_MAX;
+    return (long long)m * a.waves < INT_MAX - 4;
 }
 
 bool launch_rope(RopeArgs &a, int type, int m, hipStream_t st, const char *what) {
@@ -363,7 +363,7 @@ bool launch_rope(RopeArgs &a, int type, int m, hipStream_t st, const char *what)
     }
     const long long waves = (long long)m * (a.n_heads + a.n_kv * (type >= 0 ? 2 : 1));
     if (waves <= 0) return true;
-    if ((waves + 3) / 4 > INT_MAX) {
+    if (waves > INT_MAX) {
         lib_error(-2, "%s: %d tokens are too many", what, m);
         return false;
     }

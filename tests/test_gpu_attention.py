@@ -60,7 +60,7 @@ def check_attention(cache, qtype, layers, n_pages, page, seqs, n_new, heads, rng
     for s, m in zip(seqs, n_new):
         n = cache.length(s)
         k, v = P.values(vals, layer, [p for p in cache.tables([s])[0] if p >= 0], n)
-        want, tol = P.attend(q[at: at + m].reshape(m, heads, dim), k, v, n - m, scale or dim ** -0.5, qtype)
+        want, tol = P.attend(q[at: at + m].reshape(m, heads, dim), k, v, n - m, dim ** -0.5 if scale is None else scale, qtype)
         err = np.abs(got[at: at + m].reshape(m, heads, dim) - want)
         assert np.all(err <= tol), f"sequence of {n}, {m} new: {np.max(err / tol):.3g} times the tolerance"
         if m:
@@ -142,7 +142,7 @@ def test_extreme_scores_and_values(hipdev, qtype):
     rng = np.random.default_rng(11)
     dim, page, n = 128, 64, 700
     for std, qstd, scale in ((1.0, 60.0, 0.1), (2.0 ** -12, 1.0, 1.0), (200.0, 1e-3, 0.05), (1.0, 1e-30, 1e28), (1.0, 1e30, 1e-31),
-                             (1.0, 2.0, -0.3), (1.0, 0.0, 0.1)):
+                             (1.0, 2.0, -0.3), (1.0, 0.0, 0.1), (1.0, 1.0, 0.0), (1.0, 1.0, 1e-44)):
         c = make(rng, qtype, 1, dim, page, 12, 2, std=std)
         s = c.new()
         c.extend([s], [n])
@@ -527,6 +527,35 @@ def test_nan_reaches_its_rows_only(hipdev):
         assert got[0].isnan().all() and torch.equal(got[1], before[1])
 
 
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("bits", [0x7C00, 0xFC00, 0x7E00])
+def test_a_scale_that_is_not_finite_spoils_its_block_only(hipdev, dim, new, bits):
+    rng = np.random.default_rng(bits + dim + new)
+    kv, group, page, n = 1, 4, 64, 400
+    c = make(rng, E.Q8_0, kv, dim, page, 8, 2)
+    s = c.new()
+    c.extend([s], [n])
+    pages = c.tables([s])[0]
+    raw = c.pool.cpu().numpy().reshape(8, 2, -1)
+    scales = raw[..., page * dim:].view(np.uint16).reshape(8, 2, page, dim // 32)
+    scales[pages[0], 1, 5, 1] = bits
+    # the largest scale of all, next to it: the sums of its block are in range, and those of the others exact
+    scales[pages[0], 1, 4, 0] = np.float16(30.0).view(np.uint16)
+    c.pool.copy_(torch.from_numpy(raw.reshape(-1)))
+    scales[pages[0], 1, 5, 1] = 0
+    vals = P.decode(torch.from_numpy(raw.reshape(-1)), E.Q8_0, 1, 8, kv, page, dim)
+    q = rng.standard_normal((new, group * kv * dim)).astype(np.float32)
+    b = E.KvBatch(c, group * kv, 1, new)
+    b.set([s], [new])
+    got = E.attention(b, 0, dev(q)).cpu().numpy().reshape(new, group * kv, dim)
+    k, v = P.values(vals, 0, [p for p in pages if p >= 0], n)
+    want, tol = P.attend(q.reshape(new, group * kv, dim), k, v, n - new, dim ** -0.5, E.Q8_0)
+    assert not np.isfinite(got[..., 32:64]).any()
+    got[..., 32:64] = want[..., 32:64]
+    assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
+
+
 def test_two_batches_on_two_streams(hipdev):
     rng = np.random.default_rng(21)
     c = make(rng, E.Q8_0, 4, 128, 64, 300, 8)
@@ -613,6 +642,9 @@ def test_refusals(hipdev):
     L.clear_error()
     assert not L.attention_dev(q.data_ptr(), q.data_ptr() + 4, b._h, 0, 1.0, None)
     L.clear_error()
+    for scale in (float("nan"), float("inf")):
+        with pytest.raises(E.HipError, match="finite"):
+            E.attention(b, 0, q, scale)
     assert not L.kv_append_dev(q.data_ptr(), q.data_ptr(), 255, k.data_ptr(), 128, k.data_ptr(), 128, b._h, 0, None, None,
                                0.0, None, None)
     L.clear_error()
