@@ -1099,7 +1099,7 @@ extern "C" int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip
     if (!lib_ready("attention")) return 0;
     bool capturing = false;
     if (!batch_ready(b, layer, (hipStream_t)stream, "attention", &capturing)) return 0;
-    if (!capturing && b->plan.tokens.empty()) return 1;
+    if (b->plan.tokens.empty()) return 1;
     if (out == nullptr || q == nullptr || (((uintptr_t)out | (uintptr_t)q) & 15u) != 0 || !(fabsf(scale) < INFINITY)) {
         lib_error(-2, "attention: null buffer, q or out not 16-byte aligned, or scale %g not finite", (double)scale);
         return 0;

@@ -30,6 +30,8 @@ struct edgexpu_hip_batch {
     bool set = false;
     uint64_t epoch = 0;     // the tables' when the plan was made
     bool captured = false;  // a captured call holds the device pointers
+    int captured_tokens = INT32_MAX;  // the fewest that the buffers of a captured call hold
+    bool captured_append = false;     // a captured call writes to the plan's slots
     // device plan, 32-bit words: the tokens backwards (token t in the four
     // words before head - 4 * t), so that they and what follows are one copy;
     // from `head` on the header, the items, the pages, the joins

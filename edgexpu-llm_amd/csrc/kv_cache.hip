@@ -65,8 +65,9 @@ bool kv_shape_ok(uint32_t type, int n_layers, int n_kv, int dim, int page, int n
     if (dim != 64 && dim != 96 && dim != 128 && dim != 256) return false;
     if (page != 16 && page != 32 && page != 64 && page != 128 && page != 256) return false;
     // (grid limits of the copy kernel: 2 * n_kv and n_layers below 65536)
-    return n_layers > 0 && n_layers <= 4096 && n_kv > 0 && n_kv <= 4096 && n_pages > 0 &&
-           (long long)n_pages * page < INT_MAX;
+    if (n_layers <= 0 || n_layers > 4096 || n_kv <= 0 || n_kv > 4096 || n_pages <= 0 || (long long)n_pages * page >= INT_MAX)
+        return false;
+    return (double)n_layers * n_pages * 2 * n_kv * (double)head_page_bytes(type, dim, page) < 0x1p60;
 }
 
 const char *status_text(KvStatus s) {
@@ -144,7 +145,10 @@ bool batch_ready(edgexpu_hip_batch *b, int layer, hipStream_t st, const char *wh
         return false;
     }
     *capturing = is_capturing(st);
-    if (*capturing) b->captured = true;
+    if (*capturing) {
+        b->captured = true;
+        b->captured_tokens = std::min(b->captured_tokens, (int)b->plan.tokens.size());
+    }
     return true;
 }
 
@@ -442,12 +446,21 @@ int edgexpu_hip_batch_set(edgexpu_hip_batch *b, int n, const int *seqs, const in
         lib_error(-2, "batch_set: %lld tokens (at most %d)", tokens, b->max_tokens);
         return 0;
     }
+    if (tokens > b->captured_tokens) {
+        lib_error(-7, "batch_set: a plan of %lld tokens outgrows a captured call made for %d (set the largest plan before it)",
+                  tokens, b->captured_tokens);
+        return 0;
+    }
     return guarded("batch_set", 0, [&] {
         b->set = false;
         const edgexpu_hip_kv *kv = b->kv;
         b->plan.build(kt, n, seqs, n_new,
                       {b->n_heads / kv->n_kv, kv->n_kv, attn_cost(kv->type, kv->dim), (kv->dim + 2) * 4 * 2,
                        attn_workgroups(kv->type, kv->dim), kMinPieceCost});
+        if (b->captured_append && !b->plan.writable) {
+            lib_error(-2, "batch_set: a captured call appends, and a new token's page is held by another sequence too");
+            return 0;
+        }
         if (!upload(b, (hipStream_t)stream)) return 0;
         b->epoch = kt.epoch();
         b->set = true;

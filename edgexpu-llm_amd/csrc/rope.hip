@@ -466,7 +466,7 @@ int edgexpu_hip_kv_append_dev(float *q_out, const float *q, long long ldq, const
     bool capturing = false;
     if (!batch_ready(b, layer, (hipStream_t)stream, "kv_append", &capturing)) return 0;
     const edgexpu_hip_kv *kv = b->kv;
-    if (!capturing && b->plan.tokens.empty()) return 1;
+    if (b->plan.tokens.empty()) return 1;
     if (q == nullptr || q_out == nullptr || k == nullptr || v == nullptr || ldq < (long long)b->n_heads * kv->dim ||
         ldk < (long long)kv->n_kv * kv->dim || ldv < (long long)kv->n_kv * kv->dim) {
         lib_error(-2, "kv_append: null buffer or short rows");
@@ -498,9 +498,10 @@ int edgexpu_hip_kv_append_dev(float *q_out, const float *q, long long ldq, const
         a.n_rot = rope->n_rot;
         a.interleaved = rope->interleaved;
     }
-    // (a captured call covers any later plan of this batch; -1: as many tokens as the plan says)
-    const int m = capturing ? b->max_tokens : (int)b->plan.tokens.size();
+    // (a captured call covers any later plan, of fewer tokens; -1: as many as the plan says)
+    const int m = (int)b->plan.tokens.size();
     a.m = capturing ? -1 : m;
+    if (capturing) b->captured_append = true;
     return launch_rope(a, kv->type, m, (hipStream_t)stream, "kv_append") ? 1 : 0;
 }
 

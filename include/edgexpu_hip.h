@@ -347,7 +347,7 @@ int edgexpu_hip_gate_up_silu_dev(float *act, const float *x, const float *norm_w
  *     with codes and scales apart, so that codes start at 16-byte addresses).
  * The whole is [layer][page][K, V][kv head], edgexpu_hip_kv_pool_bytes bytes.
  * head_dim is 64, 96, 128 or 256; page_tokens 16, 32, 64, 128 or 256;
- * n_pages * page_tokens < 2^31.
+ * n_pages * page_tokens < 2^31, the pool less than 2^60 bytes.
  *
  * A sequence is a number below max_seqs with a length and a list of pages.
  * Sequences made by edgexpu_hip_kv_fork share pages; a page that others hold
@@ -409,10 +409,12 @@ int edgexpu_hip_kv_tables(const edgexpu_hip_kv *kv, int n, const int *seqs, int 
  * edgexpu_hip_batch_set copies the plan to the device on `stream`; it is
  * refused (error -7) while that stream is captured.  Its device
  * buffers grow as plans need; a batch that a captured call has used keeps its
- * buffers, and a plan that outgrows them is refused (error -7): set the largest
- * one before the capture.  A captured step replays with whatever plan the last
- * set has put there.  Calls of one batch share its workspace: on one stream, or
- * ordered by the caller. */
+ * buffers, and a plan that outgrows them, or has more tokens than the plan at
+ * the capture (the caller's buffers need hold no more), is refused (error -7):
+ * set the largest one before the capture.  A captured step replays with whatever
+ * plan the last set has put there; after a captured edgexpu_hip_kv_append_dev a
+ * plan is refused (error -2) where that call would be.  Calls of one batch share
+ * its workspace: on one stream, or ordered by the caller. */
 typedef struct edgexpu_hip_batch edgexpu_hip_batch;
 edgexpu_hip_batch *edgexpu_hip_batch_create(edgexpu_hip_kv *kv, int n_heads, int max_seqs, int max_tokens);
 /* Waits for the device, then frees. */
@@ -456,9 +458,10 @@ int edgexpu_hip_kv_append_dev(float *q_out, const float *q, long long ldq, const
  * Products of f16 and Q8_0 caches run on the matrix cores with q and the
  * weights as two f16 parts each (22 bits; a weight below 2^-31 of its row's
  * largest may be lost), sums in f32: results as those of 32 bits.  With f16 and
- * Q8_0 a key or value that is not finite makes what it reaches NaN.  Contents of slots that a token does not see (behind the sequence's
+ * Q8_0 a key or value that is not finite makes what it reaches NaN (a Q8_0 scale
+ * its block).  Contents of slots that a token does not see (behind the sequence's
  * end, or of later tokens of the step) have no influence, NaN and infinities
- * included. */
+ * included.  scale: finite (else error -2). */
 int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip_batch *b, int layer, float scale, void *stream);
 
 /* ---- host-pointer entry points (synchronous: inputs copied in, outputs

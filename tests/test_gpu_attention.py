@@ -485,6 +485,51 @@ def test_captured_step_replays_later_plans(hipdev):
     E.attention(big, 0, qr)
 
 
+def test_a_captured_step_bounds_later_plans(hipdev):
+    """More tokens than the captured call's buffers hold, and slots that a captured append may not write, are refused."""
+    rng = np.random.default_rng(20)
+    c = make(rng, E.F16, 1, 64, 16, 120, 6)
+    a, e = c.new(), c.new()
+    c.extend([a, e], [40, 50])
+    b = E.KvBatch(c, 1, 4, 64)
+    k = dev(rng.standard_normal((2, 64)).astype(np.float32))
+    q, qr, out = dev(rng.standard_normal((2, 64)).astype(np.float32)), torch.zeros((2, 64), device="cuda:0"), torch.zeros((2, 64), device="cuda:0")
+    b.set([a, e], [1, 1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        E.kv_append(b, 0, q, k, k, q_out=qr)
+        E.attention(b, 0, qr, out=out)
+    with pytest.raises(E.HipError, match="3 tokens outgrows"):
+        b.set([a, e], [2, 1])
+    assert b.tokens() == 2
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, E.attention(b, 0, q))
+    (f,) = c.fork([e])
+    with pytest.raises(E.HipError, match="appends"):
+        b.set([a, e], [1, 1])
+    c.extend([f], [1])
+    b.set([a, f], [1, 1])
+    before = c.pool.clone()
+    graph.replay()
+    torch.cuda.synchronize()
+    x = (c.pool != before).view(120, -1).any(1).nonzero().flatten().tolist()
+    assert set(x) <= {int(c.tables([a])[0].max()), int(c.tables([f])[0, 50 // 16])}
+    # read only: shared slots are no matter
+    r = E.KvBatch(c, 1, 4, 64)
+    r.set([a, f], [1, 1])
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        E.attention(r, 0, q, out=out)
+    c.fork([f])
+    r.set([a, f], [1, 1])
+    # as many tokens, but in pieces that need a workspace
+    g = c.new()
+    c.extend([g], [1000])
+    with pytest.raises(E.HipError, match="outgrows the workspace"):
+        r.set([g], [1])
+
+
 def test_no_tokens(hipdev):
     rng = np.random.default_rng(4)
     c = make(rng, E.F16, 2, 64, 16, 8, 3)

@@ -29,7 +29,8 @@ def test_pool_bytes(lib):
     assert n(E.F16, 1, 1, 64, 16, (2**31 - 1) // 16) == 2 * ((2**31 - 1) // 16) * 16 * 64 * 2
     for bad in [(E.Q4_K, 1, 1, 64, 16, 1), (30, 1, 1, 64, 16, 1), (E.F16, 0, 1, 64, 16, 1), (E.F16, 1, 0, 64, 16, 1),
                 (E.F16, 1, 1, 80, 16, 1), (E.F16, 1, 1, 512, 16, 1), (E.F16, 1, 1, 64, 8, 1), (E.F16, 1, 1, 64, 48, 1),
-                (E.F16, 1, 1, 64, 512, 1), (E.F16, 1, 1, 64, 16, 0), (E.F16, 1, 1, 64, 16, 2**27), (E.F16, -1, 1, 64, 16, 1)]:
+                (E.F16, 1, 1, 64, 512, 1), (E.F16, 1, 1, 64, 16, 0), (E.F16, 1, 1, 64, 16, 2**27), (E.F16, -1, 1, 64, 16, 1),
+                (E.F32, 4096, 4096, 256, 256, 2**31 // 256 - 1)]:
         assert n(*bad) == 0
     assert lib.last_error()[0] == 0
 
