@@ -52,6 +52,16 @@ __device__ __forceinline__ RopeToken rope_token(const RopeArgs &a, int t) {
     return {a.pos != nullptr ? a.pos[t] : 0, 0};
 }
 
+// A block's largest magnitude is the largest bit pattern: a NaN is above all, and
+// makes the scale NaN (edgexpu_hip_quantize_q8_0_dev leaves it out of the maximum,
+// and a cached NaN would be lost).  Else codes and scales are that quantizer's:
+// codes by 127 / max, out of range -128, the scale max / 127 rounded to f16.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ int q8_code(float v, float id) {
+    const float x = rintf(v * id);
+    return fabsf(x) <= 127.0f ? (int)x : -128;
+}
+
 // Any head size, pairing and alignment.  TYPE: the cache's, -1: k goes to k_out.
 // One wave a head of a token, in 64 bits; the row passes through LDS for its
 // partners.
@@ -124,13 +134,11 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
     for (int j = 0; j < 4; ++j) {
         const int e = lane + 64 * j;
         if (TYPE == kTypeQ8_0) {
-            float top = fabsf(y[j]);
-            top = row16_max(top);
-            top = fmaxf(top, shfl_xor_f(top, 16));
+            uint32_t most = row16_max_u32(magnitude(y[j]));
+            most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
             if (e >= a.dim) continue;
-            // as edgexpu_hip_quantize_q8_0_dev: codes by 127 / max, the scale max / 127 rounded to f16
-            const float id = top != 0.0f ? 127.0f / top : 0.0f;
-            reinterpret_cast<int8_t *>(base)[(size_t)off * a.dim + e] = (int8_t)(int)rintf(y[j] * id);
+            const float top = __uint_as_float(most), id = top != 0.0f ? 127.0f / top : 0.0f;
+            reinterpret_cast<int8_t *>(base)[(size_t)off * a.dim + e] = (int8_t)q8_code(y[j], id);
             if ((lane & 31) == 0)
                 reinterpret_cast<uint16_t *>(base + ((size_t)a.dim << a.kv.page_shift))[off * (a.dim / 32) + e / 32] =
                     (uint16_t)f32_to_f16_rne(top / 127.0f);
@@ -306,12 +314,12 @@ __global__ __launch_bounds__(256) void rope_rows_kernel(const RopeArgs a) {
                 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
                 if (some) *reinterpret_cast<v4h *>(base + ((size_t)off * a.dim + e) * 2) = __builtin_convertvector(out, v4h);
             } else {
-                // as edgexpu_hip_quantize_q8_0_dev: codes by 127 / max, the scale max / 127 rounded to f16; a block is 8 lanes
-                const float top = row8_max(fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
-                const float id = top != 0.0f ? 127.0f / top : 0.0f;
+                // (a block is 8 lanes)
+                const uint32_t most = max(max(magnitude(y[0]), magnitude(y[1])), max(magnitude(y[2]), magnitude(y[3])));
+                const float top = __uint_as_float(row8_max_u32(most)), id = top != 0.0f ? 127.0f / top : 0.0f;
                 uint32_t w = 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w |= ((uint32_t)(int)rintf(y[j] * id) & 0xffu) << (8 * j);
+                for (int j = 0; j < 4; ++j) w |= ((uint32_t)q8_code(y[j], id) & 0xffu) << (8 * j);
                 if (some) {
                     *reinterpret_cast<uint32_t *>(base + (size_t)off * a.dim + e) = w;
                     if ((l & 7) == 0)

@@ -447,8 +447,9 @@ int edgexpu_hip_qk_norm_rope_dev(float *q_out, float *k_out, const float *q, lon
 /* The same for the batch's tokens at their positions, with k (normed and
  * rotated) and v written to their slots of the cache in `layer` instead of
  * k_out.  Values are rounded once, to nearest, to the cache's type (f16: beyond
- * 65504 infinity; Q8_0 as edgexpu_hip_quantize_q8_0_dev).  Refused (error -2)
- * where a slot's page is held by another sequence too. */
+ * 65504 infinity; Q8_0 as edgexpu_hip_quantize_q8_0_dev, but a block with a NaN
+ * gets a NaN scale).  Refused (error -2) where a slot's page is held by another
+ * sequence too. */
 int edgexpu_hip_kv_append_dev(float *q_out, const float *q, long long ldq, const float *k, long long ldk,
                               const float *v, long long ldv, edgexpu_hip_batch *b, int layer, const float *q_weight,
                               const float *k_weight, float eps, const edgexpu_hip_rope *rope, void *stream);

@@ -329,6 +329,42 @@ def test_append_q8_0_codes_are_the_quantizers(hipdev):
             assert np.array_equal(codes, blocks[p][..., 2:]) and np.array_equal(d, blocks[p][..., :2])
 
 
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("norm", [False, True])
+def test_append_q8_0_of_values_at_the_limits(hipdev, offset, norm):
+    """Subnormal, infinite and huge values become the quantizer's blocks; a NaN's block has a NaN scale (not a finite
+    one, with which attention would not see it).  offset 1: rows that are not 16-byte aligned."""
+    rng = np.random.default_rng(21)
+    c = make(rng, E.Q8_0, 1, 128, 16, 2, 1)
+    s = c.new()
+    c.extend([s], [8])
+    b = E.KvBatch(c, 1, 1, 8)
+    b.set([s], [8])
+    x = rng.standard_normal((8, 128)).astype(np.float32)
+    x[0, :32] = 0.0
+    x[1, 5:32] = np.float32(1e-44)
+    x[1, :5] = np.float32(3e-37)
+    x[2] *= np.float32(1e-38)
+    x[3, 40], x[4, 41], x[5, 3] = np.inf, -np.inf, 3e38
+    x[6, 70], x[7, 0], x[7, 127] = np.nan, -np.nan, np.inf
+    wide = torch.zeros((8, 128 + offset), device="cuda:0")
+    v = wide[:, offset:]
+    v.copy_(dev(x))
+    E.kv_append(b, 0, v, v, v, k_weight=torch.ones(128, device="cuda:0") if norm else None)
+    raw = c.pool.cpu().numpy().reshape(2, 2, -1)[0]
+    blocks = E.quantize_q8_0(dev(x)).cpu().numpy().reshape(8, 4, 34)
+    for which in (0, 1):
+        codes = raw[which, : 16 * 128].reshape(16, 4, 32)[:8]
+        d = raw[which, 16 * 128:].copy().view(np.float16).reshape(16, 4)[:8]
+        if which == 0 and norm:  # one that is not finite reaches all of its head
+            assert np.isnan(d[[6, 7]]).all() and not np.isnan(d[:3]).any()
+            continue
+        nan = np.isnan(x).reshape(8, 4, 32).any(-1)
+        assert np.array_equal(np.isnan(d), nan)
+        assert np.array_equal(d[~nan].view(np.uint16), blocks[..., :2].copy().view(np.uint16).reshape(8, 4)[~nan])
+        assert np.array_equal(codes[~nan], blocks[..., 2:][~nan])
+
+
 # ------------------------------------------------------------------ pages
 
 
