@@ -336,7 +336,9 @@ int edgexpu_hip_gate_up_silu_dev(float *act, const float *x, const float *norm_w
  * All of these run on the device of edgexpu_hip_init and refuse (error -4) a
  * caller whose current device is another.  Work on one cache goes to one
  * stream, or to streams that the caller orders: the host tables change when a
- * call returns, the device work it queued runs later. */
+ * call returns, the device work it queued runs later.  A cache and its batches
+ * are used by one host thread at a time.  What a captured call was given (batch,
+ * rotation, weights, buffers) lives as long as its graph. */
 
 /* A paged cache of keys and values: n_layers x n_pages pages of page_tokens
  * tokens.  A layer's page holds K, then V; each holds, for every kv head, the
