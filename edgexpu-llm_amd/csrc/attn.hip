@@ -1,6 +1,6 @@
 // Attention of a step's tokens over the paged cache, by the plan of
 // attn_plan.h: out = sum_j p_j V_j / sum_j p_j, p_j = exp(scale q.K_j - m), one
-// pass over the keys with the running maximum m and sum.
+// pass over the keys with a running reference m and sum.
 //
 // Both products run on the matrix cores with the keys as the rows of the
 // first operand, so that a query row is one column, held by the four lanes
@@ -16,13 +16,21 @@
 // Arithmetic.  F16 and Q8_0: q (after an exact power-of-two scaling of its row
 // that keeps both parts in range) and the weights as two f16 parts, high and
 // rest, 22 bits together, against f16 values or the integer codes (exact in
-// f16); two products each, f32 sums: the error of f32 arithmetic, at twice the
-// matrix work, which stays under the time of the loads wherever few rows share
-// them.  A single f16 part would lose 2^-12 of every weight.  Q8_0 scales are
-// applied to the partial sums of a block (K) and to the weights (V).  F32:
-// the f32 matrix instructions.  Weights are 2^(s - m + 7) with m at most 8
-// behind the true maximum: it is raised, and the sums rescaled, only when a
-// tile exceeds it by 2^8 (an exponent range the f16 parts have to spare).
+// f16); two products each, f32 sums, at twice the matrix work, which stays under
+// the time of the loads wherever few rows share them.  A single f16 part would
+// lose 2^-11 of every weight.  Q8_0 scales are applied to the partial sums of a
+// block (K) and to the weights (V).  F32: the f32 matrix instructions.
+//
+// A part's finest step is 2^-24, so a weight below 2^-2 has fewer than 22 bits;
+// how many it has is a matter of the reference m in 2^(s - m + 10).  One that only
+// ever rises to the row's maximum leaves the keys behind a strong one (an
+// attention sink, whose value may well be next to zero) with few bits or none.  So
+// m follows the scores of the tile at hand: it moves to the tile's maximum, and
+// the row's sums are rescaled, where that is 2^5 above m or 2^13 below.  With t
+// the largest of a row's weights in a tile of 32 keys, a weight w there is off by
+// at most 2^-22 w, or 2^-22 t where that is more, and where t is the largest of
+// the row so far by 2^-35 t.  (Raised at 2^4: 64-key heads 4 % slower; lowered at
+// 2^10 and less: 3 to 5 %, tiles that no row has to move for are looked at.)
 //
 // What bounds it, at head size 128 and 8 kv heads, measured:
 //   few rows (single tokens, no sharing): the loads.  f16 5.5 TB/s, Q8_0 4.9,
@@ -48,6 +56,8 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
+// The window around a row's reference: base-2 exponents above and below it.
+constexpr float kUp = 5.0f, kDown = 13.0f;
 
 struct AttnArgs {
     const float *q;
@@ -283,7 +293,7 @@ struct Rows {
     using G = Geo<TYPE, DIM>;
     v8h qh[TYPE == kTypeF32 ? 1 : RT][TYPE == kTypeF32 ? 1 : G::NB], ql[TYPE == kTypeF32 ? 1 : RT][TYPE == kTypeF32 ? 1 : G::NB];
     v4f qf[TYPE == kTypeF32 ? RT : 1][TYPE == kTypeF32 ? G::ND : 1];
-    float top[RT], rs[RT], m[RT], l[RT];  // score factor (positive); running maximum (of base-2 exponents), this lane's part of the sum
+    float top[RT], rs[RT], m[RT], l[RT];  // score factor (positive); reference (a base-2 exponent), this lane's part of the sum
     int lim[RT];                 // positions below are seen
     v4f acc[RT][G::ND];
     int ve;                      // Q8_0: acc is in units of 2^ve
@@ -420,12 +430,18 @@ struct Rows {
         }
     }
 
-    // The maximum is raised where scores exceed it by 8.
-    __device__ __forceinline__ void raise() {
+    // A row's reference moves to the largest score of its tile where that is out of the window: by the row's own keys, no
+    // other row has a say.  It is lowered as long as the sums stay below 2^64 (weights of up to 2^15, values of 2^16).
+    __device__ __forceinline__ void follow() {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            if (__builtin_amdgcn_ballot_w64(top[t] > m[t] + 8.0f) != 0) {
-                const float mn = fmaxf(m[t], col_max(top[t]));
+            const float gap = top[t] - m[t];
+            const bool out = TYPE == kTypeF32 ? gap > kUp : fabsf(gap + (kDown - kUp) / 2) > (kDown + kUp) / 2;
+            if (__builtin_amdgcn_ballot_w64(out) != 0) {
+                const float row = col_max(top[t]);
+                const bool lower = TYPE != kTypeF32 && row < m[t] - kDown && row > -INFINITY &&
+                                   col_max(l[t]) * __builtin_amdgcn_exp2f(m[t] - row) < 0x1p64f;
+                const float mn = row > m[t] + kUp || lower ? row : m[t];
                 const float c = m[t] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[t] - mn);
                 m[t] = mn;
                 l[t] *= c;
@@ -438,7 +454,7 @@ struct Rows {
     __device__ __forceinline__ void weights() {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            const float off = m[t] == -INFINITY ? 0.0f : m[t] - 7.0f;
+            const float off = m[t] == -INFINITY ? 0.0f : m[t] - (TYPE == kTypeF32 ? 0.0f : 15.0f - kUp);
 #pragma unroll
             for (int hf = 0; hf < G::HALVES; ++hf)
 #pragma unroll
@@ -738,7 +754,7 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
         w.scores(ringp + (2 * i % G::RING) * G::UNIT, nullptr, lane);
         if (edge) w.mask(p0, lane);
         w.tops();
-        w.raise();
+        w.follow();
         w.weights();
         arrive(2 * i + 1);
         issue(2 * (i + ahead) + 2, then);
@@ -871,7 +887,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
             w.mask(p0, lane);
             w.tops();
         }
-        w.raise();
+        w.follow();
         w.weights();
         // (behind the last tile: scores of whatever lies there, and not used)
         w.scores(unit_at(i + 1), TYPE == kTypeQ8_0 ? wide : nullptr, lane);

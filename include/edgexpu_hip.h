@@ -459,8 +459,11 @@ int edgexpu_hip_kv_append_dev(float *q_out, const float *q, long long ldq, const
  * up to token t's own of its sequence, for the batch's tokens: q and out
  * [tokens][n_heads][head_dim] f32, dense, 16-byte aligned, out may be q.
  * Products of f16 and Q8_0 caches run on the matrix cores with q and the
- * weights as two f16 parts each (22 bits; a weight below 2^-31 of its row's
- * largest may be lost), sums in f32: results as those of 32 bits.  With f16 and
+ * weights as two f16 parts each, sums in f32.  Of q that is 22 bits, or 2^-39 of
+ * the row's largest value where that is more.  A weight w among 32 keys read
+ * together, the largest of their weights being t, is off by at most 2^-22 w, or
+ * 2^-22 t where that is more; where t is the row's largest so far, by 2^-22 w or
+ * 2^-35 t.  With f16 and
  * Q8_0 a key or value that is not finite makes what it reaches NaN (a Q8_0 scale
  * its block).  Contents of slots that a token does not see (behind the sequence's
  * end, or of later tokens of the step) have no influence, NaN and infinities

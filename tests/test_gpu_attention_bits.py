@@ -1,0 +1,168 @@
+"""How many bits attention keeps: few keys and queries with few nonzero values, so that what sums may lose is far below
+what one f16 part of a query or a weight would; rows whose heaviest key has a value of zero; Q8_0 scales far apart."""
+import numpy as np
+import pytest
+import torch
+
+import edgexpu_amd as E
+import kv_plain as P
+
+pytestmark = pytest.mark.gpu
+
+EPS = P.EPS32
+LOG2E = 1.4426950408889634
+TERMS = 4  # nonzero values of a query
+TILE = 32
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).to("cuda:0")
+
+
+def encode(x, qtype, page, scales=None):
+    """Pool bytes of values [2, heads, n, dim] in pages one after the other, and what they decode to.  Q8_0: x are the
+    codes, scales [2, heads, n, dim / 32]."""
+    two, kv, n, dim = x.shape
+    pages = -(-n // page)
+
+    def paged(a):  # [2, heads, n, ...] -> [pages, 2, heads, page, ...]
+        a = np.concatenate([a, np.zeros(a.shape[:2] + (pages * page - n,) + a.shape[3:], a.dtype)], 2)
+        return np.moveaxis(a.reshape((two, kv, pages, page) + a.shape[3:]), 2, 0)
+
+    if qtype != E.Q8_0:
+        t = x.astype(np.float16 if qtype == E.F16 else np.float32)
+        return torch.from_numpy(np.ascontiguousarray(paged(t)).reshape(-1).view(np.uint8).copy()), t.astype(np.float64)
+    d = scales.astype(np.float16)
+    codes = np.ascontiguousarray(paged(x.astype(np.int8))).reshape(pages, 2, kv, -1).view(np.uint8)
+    raw = np.concatenate([codes, np.ascontiguousarray(paged(d)).reshape(pages, 2, kv, -1).view(np.uint8)], -1)
+    with np.errstate(invalid="ignore"):
+        return torch.from_numpy(raw.reshape(-1).copy()), x.astype(np.float64) * np.repeat(d.astype(np.float64), 32, -1)
+
+
+def queries(rng, new, heads, dim, std=1.0):
+    """TERMS nonzero values a row, in channels spread over the head."""
+    q = np.zeros((new, heads, dim), np.float32)
+    at = np.arange(TERMS) * dim // TERMS
+    q[..., at] = rng.standard_normal((new, heads, TERMS)) * std
+    return q
+
+
+def run(pool, qtype, kv, dim, page, n, q, scale):
+    new, heads, _ = q.shape
+    c = E.KvCache(qtype, 1, kv, dim, page, -(-n // page), 1, pool=pool.cuda())
+    s = c.new()
+    c.extend([s], [n])
+    b = E.KvBatch(c, heads, 1, new)
+    b.set([s], [new])
+    return E.attention(b, 0, dev(q.reshape(new, -1)), scale).cpu().numpy().reshape(new, heads, dim)
+
+
+def expect(q, k, v, scale, qtype, terms=TERMS):
+    """(out, tolerance, weights) of q [new, heads, dim] at the last positions of k, v [kv heads, n, dim], all in 64 bits.
+
+    With B the largest sum of |scale q_i k_i| of a row in base-2 units (terms products) and eps = 2^-24, a weight is off
+    relatively by
+      ln2 eps ((2 terms + 16) B     products of q's two parts (4 eps of it lost), sums, a block's scale; terms 0: one
+                                    product, by a power of two, and nothing of it
+               + 2 B                the factor of the scores, rounded twice
+               + 2 (2 B + 32))      its exponent's argument, s - m and the reference's offset
+      + 4 eps                       exp2 and its two parts' 22 bits, 2 + 2
+      + 12 eps                      the joins of waves and pieces, a sum's rescaling
+      + 6 eps                       Q8_0: times a scale, and its value's parts (22 bits)
+    A weight passes through at most 64 + 4 n / 32 sums (32 products and two parts of a tile, then twice a tile and the
+    joins) in the numerator, 8 n / 32 + 32 in the denominator; a tile is 32 keys.  The division adds 3 eps.
+
+    The parts' finest step adds 2^-22 of the largest weight of its tile, 2^-35 of it where it is the largest so far."""
+    m, H, dim = q.shape
+    kv, n, _ = k.shape
+    out, tol, weights = np.zeros((m, H, dim)), np.zeros((m, H, dim)), []
+    for h in range(H):
+        kh, vh = k[h // (H // kv)], v[h // (H // kv)]
+        for t in range(m):
+            seen = n - m + t + 1
+            qt = q[t, h].astype(np.float64) * scale
+            s = kh[:seen] @ qt
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            out[t, h] = w @ vh[:seen]
+            B = float((np.abs(kh[:seen]) @ np.abs(qt)).max()) * LOG2E
+            rel = EPS * (np.log(2) * ((2 * terms + 18 if terms else 2) * B + 2 * (2 * B + 32)) + 16 + (6 if qtype == E.Q8_0 else 0))
+            tiles = -(-seen // TILE)
+            rel = 2 * rel + EPS * (64 + 4 * tiles + 8 * tiles + 32 + 3)
+            tol[t, h] = rel * (w @ np.abs(vh[:seen])) + 1e-30
+            if qtype != E.F32:
+                pad = np.zeros(tiles * TILE)
+                pad[:seen] = w
+                top = pad.reshape(tiles, TILE).max(1)
+                step = np.where(top >= np.maximum.accumulate(top), 2.0 ** -35, 2.0 ** -22) * top
+                tol[t, h] += np.repeat(step, TILE)[:seen] @ np.abs(vh[:seen])
+            weights.append(w)
+    return out, tol, weights
+
+
+# (dim, kv, group, new, n): rows of a workgroup 1, 8, 17 to 32, 33 to 64, 65 to 128; all keys in a tile or a few
+ROWS = [(64, 1, 1, 1, 5), (128, 2, 4, 2, 9), (96, 1, 5, 5, 12), (128, 1, 4, 8, 11), (64, 1, 6, 5, 7), (256, 1, 3, 2, 6), (64, 2, 8, 6, 9),
+        (128, 1, 6, 9, 13), (96, 1, 10, 6, 8), (256, 1, 8, 6, 10), (64, 1, 16, 7, 10), (128, 2, 16, 8, 12), (96, 1, 16, 8, 11), (256, 1, 16, 7, 9),
+        (128, 1, 12, 10, 45), (64, 1, 13, 8, 70)]
+PARTS = [E.F16]
+
+
+@pytest.mark.parametrize("qtype", PARTS)
+@pytest.mark.parametrize("case", ROWS)
+def test_both_parts_of_queries_and_weights(hipdev, qtype, case):
+    dim, kv, group, new, n = case
+    rng = np.random.default_rng(abs(hash(case)) % 2**31 + qtype)
+    heads, page = kv * group, 64
+    q = queries(rng, new, heads, dim)
+    if qtype == E.Q8_0:
+        x = rng.integers(-127, 128, (2, kv, n, dim))
+        pool, (k, v) = encode(x, qtype, page, rng.uniform(0.5, 2, (2, kv, n, dim // 32)) / 90)
+    else:
+        pool, (k, v) = encode(rng.standard_normal((2, kv, n, dim)), qtype, page)
+    got = run(pool, qtype, kv, dim, page, n, q, 1.0)
+    want, tol, weights = expect(q, k, v, 1.0, qtype)
+    err = np.abs(got - want)
+    assert np.all(err <= tol), np.max(err / tol)
+    # what one f16 part would give is outside: of the query, and of the weights
+    top = 2.0 ** np.ceil(np.log2(np.abs(q).max(-1, keepdims=True)))
+    once = expect((q / top).astype(np.float16).astype(np.float32) * top, k, v, 1.0, qtype)[0]
+    assert (np.abs(once - want) > tol).any()
+    if n > 1:
+        once = np.array([w.astype(np.float16).astype(np.float64) @ v[i % heads // group][: len(w)] for i, w in enumerate_rows(weights, new, heads)])
+        assert (np.abs(once.reshape(heads, new, dim).transpose(1, 0, 2) - want) > tol).any()
+
+
+def enumerate_rows(weights, new, heads):
+    """(head, weights of a row) in the order of expect: by head, then token; weights scaled to a largest of 1."""
+    for i, w in enumerate(weights):
+        yield i // new, w
+
+
+@pytest.mark.parametrize("qtype", PARTS)
+@pytest.mark.parametrize("dim,group,new,n,nats,at", [
+    (128, 1, 1, 64, 16.0, 0), (128, 4, 1, 150, 16.0, 100), (64, 2, 1, 80, 12.0, 0), (256, 1, 1, 100, 16.0, 40),
+    (96, 4, 8, 150, 16.0, 0), (128, 8, 16, 120, 16.0, 0), (64, 8, 16, 200, 9.0, 70), (96, 8, 10, 100, 30.0, 0),
+    (256, 8, 8, 100, 16.0, 0), (128, 8, 7, 130, 16.0, 64), (128, 2, 1, 300, 16.0, 0), (128, 8, 16, 150, 5.0, 0),
+    (128, 4, 1, 5000, 20.0, 4000), (64, 8, 16, 3000, 14.0, 0),
+])
+def test_a_heavy_key_of_no_value(hipdev, qtype, dim, group, new, n, nats, at):
+    """One key far above the rest, its value zero: the rest keep their bits."""
+    rng = np.random.default_rng(n + dim + int(nats))
+    page = 64
+    q = np.zeros((new, group, dim), np.float32)
+    q[..., 0] = 1.0
+    x = rng.standard_normal((2, 1, n, dim)) * 0.4
+    if qtype == E.Q8_0:
+        x = np.clip(np.rint(x * 60), -127, 127).astype(np.int64)
+        scales = np.full((2, 1, n, dim // 32), 1 / 64)
+        x[0, 0, at, 0], scales[0, 0, at, 0] = 64, nats / 64
+        x[1, 0, at] = 0
+        pool, (k, v) = encode(x, qtype, page, scales)
+    else:
+        x[0, 0, at, 0] = nats
+        x[1, 0, at] = 0.0
+        pool, (k, v) = encode(x, qtype, page)
+    got = run(pool, qtype, 1, dim, page, n, q, 1.0)
+    want, tol, _ = expect(q, k, v, 1.0, qtype, 0)
+    err = np.abs(got - want)
+    assert np.all(err <= tol), np.max(err / tol)
