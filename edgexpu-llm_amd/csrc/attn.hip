@@ -29,8 +29,16 @@
 // the row's sums are rescaled, where that is 2^5 above m or 2^13 below.  With t
 // the largest of a row's weights in a tile of 32 keys, a weight w there is off by
 // at most 2^-22 w, or 2^-22 t where that is more, and where t is the largest of
-// the row so far by 2^-35 t.  (Raised at 2^4: 64-key heads 4 % slower; lowered at
+// the row so far by 2^-34 t.  (Raised at 2^4: 64-key heads 4 % slower; lowered at
 // 2^10 and less: 3 to 5 %, tiles that no row has to move for are looked at.)
+//
+// Q8_0 values.  Few rows: the parts are of weight times scale, with a reference
+// for each row and block that follows in the same way, so a large scale costs
+// nothing but its own block, and only rows that give its key weight.  Many rows
+// share the values: those are code times scale in two f16 parts, the rest times
+// 2^11, which hold any f16 scale's values whole at 2^15 for the largest so far.
+// (Unscaled rests lost 2^-12 of a value 2^28 below it.  Single tokens as fast as
+// with one unit for a wave's scales; 17 to 32 rows and chunks 2 to 4 % slower.)
 //
 // What bounds it, at head size 128 and 8 kv heads, measured:
 //   few rows (single tokens, no sharing): the loads.  f16 5.5 TB/s, Q8_0 4.9,
@@ -58,6 +66,8 @@ typedef int v2i __attribute__((ext_vector_type(2)));
 constexpr float kLog2e = 1.4426950408889634f;
 // The window around a row's reference: base-2 exponents above and below it.
 constexpr float kUp = 5.0f, kDown = 13.0f;
+// What the rest of a Q8_0 value beside its high part is kept times (many rows).
+constexpr float kRest = 2048.0f;
 
 struct AttnArgs {
     const float *q;
@@ -154,12 +164,6 @@ __device__ __forceinline__ float wave_sum_f32(float v) {
     return col_sum(v);
 }
 
-// The larger of two pairs of unsigned 16-bit numbers (v_pk_max_u16).
-__device__ __forceinline__ uint32_t max_u16(uint32_t a, uint32_t b) {
-    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
-}
-
 // High part and rest of eight values.  The factor is one the compiler does not
 // know, so that x - hi is one v_fma_mix_f32 and not a conversion and a
 // subtraction.
@@ -171,6 +175,24 @@ __device__ __forceinline__ void split8(const float (&x)[8], v8h &hi, v8h &lo) {
     for (int j = 0; j < 8; j += 2) {
         const h2 h = __builtin_convertvector((v2f{x[j], x[j + 1]}), h2);
         const h2 l = __builtin_convertvector((v2f{fmaf((float)h[0], minus, x[j]), fmaf((float)h[1], minus, x[j + 1])}), h2);
+        hi[j] = h[0];
+        hi[j + 1] = h[1];
+        lo[j] = l[0];
+        lo[j + 1] = l[1];
+    }
+}
+
+// The same of eight small integers times f, the rest times kRest.
+__device__ __forceinline__ void split8(const v8h &q, float f, v8h &hi, v8h &lo) {
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    float minus = -kRest;
+    asm("" : "+v"(minus));
+    const auto times = [&q](int j, float by) { return fmaf((float)q[j], by, 0.0f); };  // (one v_fma_mix_f32)
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const h2 h = __builtin_convertvector((v2f{times(j, f), times(j + 1, f)}), h2);
+        const h2 l = __builtin_convertvector(
+            (v2f{fmaf((float)h[0], minus, times(j, f * kRest)), fmaf((float)h[1], minus, times(j + 1, f * kRest))}), h2);
         hi[j] = h[0];
         hi[j + 1] = h[1];
         lo[j] = l[0];
@@ -288,15 +310,19 @@ struct Loader {
 };
 
 // A wave's query rows: RT tiles of 16, row l % 16 of a tile on lane l.
-template <int TYPE, int DIM, int RT>
+template <int TYPE, int DIM, int RT, bool MANY>
 struct Rows {
     using G = Geo<TYPE, DIM>;
+    static constexpr bool BLOCKS = TYPE == kTypeQ8_0 && !MANY;         // the parts are of weight times scale, a block each
+    static constexpr bool FOLLOW = TYPE != kTypeF32 && !BLOCKS;        // the parts are of the weights
     v8h qh[TYPE == kTypeF32 ? 1 : RT][TYPE == kTypeF32 ? 1 : G::NB], ql[TYPE == kTypeF32 ? 1 : RT][TYPE == kTypeF32 ? 1 : G::NB];
     v4f qf[TYPE == kTypeF32 ? RT : 1][TYPE == kTypeF32 ? G::ND : 1];
     float top[RT], rs[RT], m[RT], l[RT];  // score factor (positive); reference (a base-2 exponent), this lane's part of the sum
     int lim[RT];                 // positions below are seen
     v4f acc[RT][G::ND];
-    int ve;                      // Q8_0: acc is in units of 2^ve
+    static constexpr int kMostUp = 64;            // (the first tile with a value that is not zero finds it out of the window)
+    float up[BLOCKS ? RT : 1][BLOCKS ? G::NB : 1];  // BLOCKS: acc of block b is times this power of two
+    int ve;                                         // Q8_0, many rows: acc is in units of 2^(ve - 8)
     float s[RT][G::HALVES][4], p[RT][G::HALVES][4];  // a tile's scores, its weights
 
     __device__ __forceinline__ void load(const AttnArgs &a, const AttnItem &it, int h, int row_from, int lane) {
@@ -342,6 +368,10 @@ struct Rows {
             l[t] = 0.0f;
 #pragma unroll
             for (int d = 0; d < G::ND; ++d) acc[t][d] = v4f{0, 0, 0, 0};
+            if constexpr (BLOCKS) {
+#pragma unroll
+                for (int b = 0; b < G::NB; ++b) up[t][b] = ldexpf(1.0f, kMostUp);
+            }
         }
         ve = -24;
     }
@@ -436,10 +466,10 @@ struct Rows {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             const float gap = top[t] - m[t];
-            const bool out = TYPE == kTypeF32 ? gap > kUp : fabsf(gap + (kDown - kUp) / 2) > (kDown + kUp) / 2;
+            const bool out = !FOLLOW ? gap > kUp : fabsf(gap + (kDown - kUp) / 2) > (kDown + kUp) / 2;
             if (__builtin_amdgcn_ballot_w64(out) != 0) {
                 const float row = col_max(top[t]);
-                const bool lower = TYPE != kTypeF32 && row < m[t] - kDown && row > -INFINITY &&
+                const bool lower = FOLLOW && row < m[t] - kDown && row > -INFINITY &&
                                    col_max(l[t]) * __builtin_amdgcn_exp2f(m[t] - row) < 0x1p64f;
                 const float mn = row > m[t] + kUp || lower ? row : m[t];
                 const float c = m[t] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[t] - mn);
@@ -465,15 +495,18 @@ struct Rows {
         }
     }
 
-    // acc += V^T P^T for f16 values in rows of DIM, or (PARTS) for their high parts at vu and the rests at vl.
+    // acc += V^T P^T for f16 values in rows of DIM, or (PARTS) for their high parts at vu and the rests, times kRest, at
+    // vl: those meet the weights / kRest, which loses no more of a weight than its own rest has lost.  The product of
+    // the two rests (2^-22 of a value) is left out.
     template <bool PARTS>
     __device__ __forceinline__ void values16(const uint8_t *vu, const uint8_t *vl, int lane) {
         const int g = lane >> 4, c16 = lane & 15;
-        v8h ph[RT], pl[RT];
+        v8h ph[RT], pl[RT], ps[RT];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             const float x[8] = {p[t][0][0], p[t][0][1], p[t][0][2], p[t][0][3], p[t][1][0], p[t][1][1], p[t][1][2], p[t][1][3]};
             split8(x, ph[t], pl[t]);
+            if (PARTS) ps[t] = ph[t] * (_Float16)(1.0f / kRest);
         }
         const int row = g * 4 + (c16 >> 2), sw = swz<kTypeF16, DIM, true>(row);  // the same for row + 16
         const auto read = [&](const uint8_t *from, int d) {
@@ -488,7 +521,7 @@ struct Rows {
             if (PARTS) {
                 const v8h rest = read(vl, d);
 #pragma unroll
-                for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(rest, ph[t], acc[t][d]);
+                for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(rest, ps[t], acc[t][d]);
             }
 #pragma unroll
             for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, pl[t], acc[t][d]);
@@ -508,9 +541,9 @@ struct Rows {
         return top;
     }
 
-    // Q8_0: the unit of acc is raised to 2^e where the largest scale `top` (of the wave's lanes together) exceeds it, so
-    // that scales are at most 1 in it and weights times scale stay in f16's range.  A scale that is not finite makes its
-    // block's sums NaN in any unit, and has no say in the others'.
+    // Q8_0, many rows: the unit of acc is raised to 2^(e - 8) where the largest scale `top` (of the wave's lanes together)
+    // exceeds 2^e, so that a value in it is below 2^15; its two parts (down to 2^-35) then hold it whole, whatever the
+    // other scales are.  A scale that is not finite makes its block's sums NaN in any unit, and has no say in the others'.
     __device__ __forceinline__ void raise_unit(float top, const uint8_t *vu, int lane) {
         if (__builtin_amdgcn_ballot_w64(top > ldexpf(1.0f, ve)) == 0) return;
         if (__builtin_amdgcn_ballot_w64(top == INFINITY) != 0) top = finite_top(vu, lane);
@@ -539,44 +572,73 @@ struct Rows {
         } else {
             // this lane's keys: 4 g + r of both halves; their blocks' scales, two to a word
             const uint32_t *ds = reinterpret_cast<const uint32_t *>(vu + G::TT * G::RB) + g * 2 * G::NB;
-            uint32_t sc[2][2 * G::NB], most = 0;
+            uint32_t sc[2][2 * G::NB];
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-                for (int i = 0; i < 2 * G::NB; ++i) {
-                    sc[hf][i] = ds[hf * 8 * G::NB + i];
-                    most = max_u16(most, sc[hf][i] & 0x7fff7fffu);
-                }
-            raise_unit(f16_bits_to_f32(min(max(most & 0xffffu, most >> 16), 0x7c00u)), vu, lane);
-            const float f = ldexpf(1.0f, -ve);
-            const int k = c16 >> 1, row = (k < 4 ? g * 4 + k : 16 + g * 4 + k - 4), sw = swz<TYPE, DIM, true>(row);
+                for (int i = 0; i < 2 * G::NB; ++i) sc[hf][i] = ds[hf * 8 * G::NB + i];
+            const int o = c16 >> 1, row = (o < 4 ? g * 4 + o : 16 + g * 4 + o - 4), sw = swz<TYPE, DIM, true>(row);
+            // Several blocks a branch: one for each would keep their products apart (5 to 13 % of the time), and all are
+            // too many registers with two tiles of rows.
+            constexpr int GROUP = RT == 1 ? G::NB : 2;
 #pragma unroll
-            for (int b = 0; b < G::NB; ++b) {
-                v8h ph[RT], pl[RT];
+            for (int b0 = 0; b0 < G::NB; b0 += GROUP) {
+                float x[GROUP][RT][8], big[GROUP][RT];
+                bool out = false;
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    float x[8];
+                for (int k = 0; k < GROUP && b0 + k < G::NB; ++k)
 #pragma unroll
-                    for (int hf = 0; hf < 2; ++hf)
+                    for (int t = 0; t < RT; ++t) {
+                        big[k][t] = 0.0f;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int i = r * G::NB + b;
-                            x[hf * 4 + r] = p[t][hf][r] * (f16_bits_to_f32(sc[hf][i / 2] >> (i % 2 * 16)) * f);
+                        for (int j = 0; j < 8; ++j) {
+                            const int i = j % 4 * G::NB + b0 + k;
+                            const float d = fmaf((float)__builtin_bit_cast(h2, sc[j / 4][i / 2])[i % 2], up[t][b0 + k], 0.0f);
+                            x[k][t][j] = p[t][j / 4][j % 4] * d;
+                            big[k][t] = fmaxf(big[k][t], fabsf(x[k][t][j]));
                         }
-                    split8(x, ph[t], pl[t]);
+                        out |= !in_window(big[k][t]);
+                    }
+                if (__builtin_amdgcn_ballot_w64(out) != 0) {
+#pragma unroll
+                    for (int k = 0; k < GROUP && b0 + k < G::NB; ++k)
+#pragma unroll
+                        for (int t = 0; t < RT; ++t) fit(t, b0 + k, col_max(big[k][t]), x[k][t]);
                 }
 #pragma unroll
-                for (int d = 2 * b; d < 2 * b + 2; ++d) {
-                    const uint8_t *at = vu + row * G::RB + ((d ^ sw) * 16) + (c16 & 1) * 8;
-                    const v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)at);
-                    const v8h v = bytes_h8((uint32_t)w[0], (uint32_t)w[1]);
+                for (int k = 0; k < GROUP && b0 + k < G::NB; ++k) {
+                    v8h ph[RT], pl[RT];
 #pragma unroll
-                    for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, pl[t], acc[t][d]);
+                    for (int t = 0; t < RT; ++t) split8(x[k][t], ph[t], pl[t]);
 #pragma unroll
-                    for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, ph[t], acc[t][d]);
+                    for (int d = 2 * (b0 + k); d < 2 * (b0 + k) + 2; ++d) {
+                        const uint8_t *at = vu + row * G::RB + ((d ^ sw) * 16) + (c16 & 1) * 8;
+                        const v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)at);
+                        const v8h v = bytes_h8((uint32_t)w[0], (uint32_t)w[1]);
+#pragma unroll
+                        for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, pl[t], acc[t][d]);
+#pragma unroll
+                        for (int t = 0; t < RT; ++t) acc[t][d] = mfma16(v, ph[t], acc[t][d]);
+                    }
                 }
             }
         }
+    }
+
+    // BLOCKS: whether a tile's largest weight times scale leaves its parts their bits, and the factor of block b that
+    // puts it, `big`, between 2^9 and 2^10 where not.  A row's own, from its own keys (one that is not finite makes the
+    // block NaN whatever the factor; zeros need none; sums stay below 2^102 n).
+    static __device__ __forceinline__ bool in_window(float v) { return v <= 32768.0f && v >= 0.125f; }
+    __device__ __forceinline__ void fit(int t, int b, float big, float (&x)[8]) {
+        if (in_window(big) || big == 0.0f || !(big < INFINITY)) return;
+        const int had = __builtin_amdgcn_frexp_expf(up[t][b]) - 1;
+        const int more = min(10 - __builtin_amdgcn_frexp_expf(big), kMostUp - had);
+        const float c = ldexpf(1.0f, more);
+#pragma unroll
+        for (int d = 2 * b; d < 2 * b + 2; ++d) acc[t][d] *= c;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= c;
+        up[t][b] *= c;
     }
 
     // The sums that a key's values marked in `odd` (NB words a key) belong to become NaN for the rows that see it.
@@ -610,7 +672,12 @@ struct Rows {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             l[t] = col_sum(l[t]);
-            if (TYPE == kTypeQ8_0) rescale(ldexpf(1.0f, ve), t);
+            if constexpr (BLOCKS) {
+#pragma unroll
+                for (int d = 0; d < G::ND; ++d) acc[t][d] *= 1.0f / up[t][d / 2];
+            } else if (TYPE == kTypeQ8_0) {
+                rescale(ldexpf(1.0f, ve - 8), t);
+            }
         }
     }
 };
@@ -681,7 +748,7 @@ __device__ __forceinline__ void mark_odd(uint8_t *vu, uint32_t *odd, int lane) {
 }
 
 // Q8_0, many rows: a tile's K codes and V values become f16 in LDS once for all
-// waves.  V: code * scale / unit (18 bits) as high part and rest.  Each wave
+// waves.  V: code * scale / unit (18 bits) as high part and rest times kRest.  Each wave
 // multiplying its own operands out took twice the vector instructions.
 template <int DIM>
 __device__ __forceinline__ void expand(const uint8_t *ku, const uint8_t *vu, uint8_t *to, float unit, int tid) {
@@ -702,11 +769,8 @@ __device__ __forceinline__ void expand(const uint8_t *ku, const uint8_t *vu, uin
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const v8h q = bytes_h8(vw[2 * j], vw[2 * j + 1]);
-            float x[8];
             v8h hi, lo;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (float)q[e] * f;
-            split8(x, hi, lo);
+            split8(q, f, hi, lo);
             *reinterpret_cast<v8h *>(o + G::TILE16 + (j ? o1 : o0)) = hi;
             *reinterpret_cast<v8h *>(o + 2 * G::TILE16 + (j ? o1 : o0)) = lo;
         }
@@ -720,7 +784,7 @@ __device__ __forceinline__ void attend_few(const AttnArgs &a, const AttnItem &it
                                            int wave, int lane) {
     using G = Geo<TYPE, DIM>;
     using L = Loader<TYPE, DIM>;
-    Rows<TYPE, DIM, RT> w;
+    Rows<TYPE, DIM, RT, false> w;
     const int tiles = (it.key1 - it.key0 + G::TT - 1) / G::TT;
     const int mine = (tiles - wave + 3) / 4, units = 2 * mine;
     const uint32_t ring = lds_addr(lds) + wave * G::RING * G::UNIT;
@@ -829,7 +893,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
                                             int wave, int lane) {
     using G = Geo<TYPE, DIM>;
     using L = Loader<TYPE, DIM>;
-    Rows<TYPE, DIM, RT> w;
+    Rows<TYPE, DIM, RT, true> w;
     const int mine = wave * 16 * RT;  // (past the last row: computed from that row, not stored)
     const int tiles = (it.key1 - it.key0 + G::TT - 1) / G::TT;
     const uint32_t base = lds_addr(lds);
@@ -878,7 +942,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
             for (int k = lane; k < G::TT * G::NB; k += 64)
                 top = fmaxf(top, fabsf((float)reinterpret_cast<const _Float16 *>(vu + G::TT * G::RB)[k]));
             w.raise_unit(top, vu, lane);
-            expand<DIM>(unit_at(i + 1), vu, wide, ldexpf(1.0f, -w.ve), wave * 64 + lane);
+            expand<DIM>(unit_at(i + 1), vu, wide, ldexpf(1.0f, 8 - w.ve), wave * 64 + lane);
             lds_done();
             workgroup_barrier();
         }

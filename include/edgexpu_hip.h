@@ -463,7 +463,9 @@ int edgexpu_hip_kv_append_dev(float *q_out, const float *q, long long ldq, const
  * the row's largest value where that is more.  A weight w among 32 keys read
  * together, the largest of their weights being t, is off by at most 2^-22 w, or
  * 2^-22 t where that is more; where t is the row's largest so far, by 2^-22 w or
- * 2^-35 t.  With f16 and
+ * 2^-34 t.  (Q8_0 with few rows: w times its value's scale, and t the largest of
+ * those of the block; a block's sums are off by 2^-22 of its largest value
+ * besides.)  With f16 and
  * Q8_0 a key or value that is not finite makes what it reaches NaN (a Q8_0 scale
  * its block).  Contents of slots that a token does not see (behind the sequence's
  * end, or of later tokens of the step) have no influence, NaN and infinities

@@ -57,7 +57,7 @@ def run(pool, qtype, kv, dim, page, n, q, scale):
     return E.attention(b, 0, dev(q.reshape(new, -1)), scale).cpu().numpy().reshape(new, heads, dim)
 
 
-def expect(q, k, v, scale, qtype, terms=TERMS):
+def expect(q, k, v, scale, qtype, terms=TERMS, scales=None):
     """(out, tolerance, weights) of q [new, heads, dim] at the last positions of k, v [kv heads, n, dim], all in 64 bits.
 
     With B the largest sum of |scale q_i k_i| of a row in base-2 units (terms products) and eps = 2^-24, a weight is off
@@ -72,7 +72,9 @@ def expect(q, k, v, scale, qtype, terms=TERMS):
     A weight passes through at most 64 + 4 n / 32 sums (32 products and two parts of a tile, then twice a tile and the
     joins) in the numerator, 8 n / 32 + 32 in the denominator; a tile is 32 keys.  The division adds 3 eps.
 
-    The parts' finest step adds 2^-22 of the largest weight of its tile, 2^-35 of it where it is the largest so far."""
+    The parts' finest step adds 2^-22 of the largest weight of its tile, 2^-34 of it where it is the largest so far With
+    Q8_0 it is that of weight times value scale for a block (single tokens and few; `scales` [kv heads, n, dim / 32]
+    where they differ), and 2^-22 of a block's largest value comes on top."""
     m, H, dim = q.shape
     kv, n, _ = k.shape
     out, tol, weights = np.zeros((m, H, dim)), np.zeros((m, H, dim)), []
@@ -94,8 +96,18 @@ def expect(q, k, v, scale, qtype, terms=TERMS):
                 pad = np.zeros(tiles * TILE)
                 pad[:seen] = w
                 top = pad.reshape(tiles, TILE).max(1)
-                step = np.where(top >= np.maximum.accumulate(top), 2.0 ** -35, 2.0 ** -22) * top
+                step = np.where(top >= np.maximum.accumulate(top), 2.0 ** -34, 2.0 ** -22) * top
                 tol[t, h] += np.repeat(step, TILE)[:seen] @ np.abs(vh[:seen])
+            if scales is not None:  # a code's part of what weight times scale is off by
+                x = np.zeros((tiles * TILE, dim // 32))
+                x[:seen] = w[:, None] * scales[h // (H // kv), :seen]
+                top = x.reshape(tiles, TILE, -1).max(1)
+                step = np.where(top >= np.maximum.accumulate(top, 0), 2.0 ** -34, 2.0 ** -22) * top
+                codes = np.abs(vh[:seen]) / np.repeat(np.maximum(scales[h // (H // kv), :seen], 1e-30), 32, -1)
+                tol[t, h] += (np.repeat(np.repeat(step, TILE, 0)[:seen], 32, -1) * codes).sum(0)
+            if qtype == E.Q8_0:
+                block = np.abs(vh[:seen]).reshape(seen, -1, 32).max(-1)
+                tol[t, h] += 2.0 ** -22 * np.repeat(w @ block, 32)
             weights.append(w)
     return out, tol, weights
 
@@ -104,7 +116,7 @@ def expect(q, k, v, scale, qtype, terms=TERMS):
 ROWS = [(64, 1, 1, 1, 5), (128, 2, 4, 2, 9), (96, 1, 5, 5, 12), (128, 1, 4, 8, 11), (64, 1, 6, 5, 7), (256, 1, 3, 2, 6), (64, 2, 8, 6, 9),
         (128, 1, 6, 9, 13), (96, 1, 10, 6, 8), (256, 1, 8, 6, 10), (64, 1, 16, 7, 10), (128, 2, 16, 8, 12), (96, 1, 16, 8, 11), (256, 1, 16, 7, 9),
         (128, 1, 12, 10, 45), (64, 1, 13, 8, 70)]
-PARTS = [E.F16]
+PARTS = [E.F16, E.Q8_0]
 
 
 @pytest.mark.parametrize("qtype", PARTS)
@@ -166,3 +178,56 @@ def test_a_heavy_key_of_no_value(hipdev, qtype, dim, group, new, n, nats, at):
     want, tol, _ = expect(q, k, v, 1.0, qtype, 0)
     err = np.abs(got - want)
     assert np.all(err <= tol), np.max(err / tol)
+
+
+def q8_cache(rng, n, dim, typical):
+    """Codes [K, V][1][n][dim] and scales, V's around `typical`."""
+    codes = rng.integers(-127, 128, (2, 1, n, dim))
+    scales = rng.uniform(0.5, 2, (2, 1, n, dim // 32))
+    scales[0] /= 90
+    scales[1] *= typical
+    return codes, scales
+
+
+# rows of a workgroup: 1, 4, 20, 40, 128; 128 twice
+FORMS = [(64, 1, 1), (96, 4, 1), (128, 4, 1), (256, 4, 2), (64, 4, 5), (128, 4, 5), (96, 8, 4), (128, 8, 5), (64, 8, 16), (96, 16, 8), (128, 16, 17),
+         (256, 8, 5)]
+
+
+@pytest.mark.parametrize("dim,group,new", FORMS)
+@pytest.mark.parametrize("typical,large", [(0.02, 512.0), (2e-4, 512.0), (2e-4, 8192.0), (2e-4, 65504.0), (6e-8, 1.0)])
+def test_a_large_value_scale_is_its_blocks_own(hipdev, dim, group, new, typical, large):
+    """One block of one key has a scale far above all others: the other blocks keep their bits."""
+    rng = np.random.default_rng(dim * new + int(large))
+    n, page = new + 60, 32
+    codes, scales = q8_cache(rng, n, dim, typical)
+    scales[1, 0, 5, 1] = large
+    pool, (k, v) = encode(codes, E.Q8_0, page, scales)
+    q = queries(rng, new, group, dim)
+    got = run(pool, E.Q8_0, 1, dim, page, n, q, 1.0)
+    want, tol, _ = expect(q, k, v, 1.0, E.Q8_0, scales=scales[1].astype(np.float16).astype(np.float64))
+    err = np.abs(got - want)
+    assert np.all(err <= tol), np.max(err / tol)
+
+
+@pytest.mark.parametrize("dim,group,new", [f for f in FORMS if f[2] > 3])
+@pytest.mark.parametrize("bad", [100.0, 65504.0, np.inf, np.nan])
+def test_value_scales_of_later_tokens_have_no_influence(hipdev, dim, group, new, bad):
+    """A scale of one of the step's later tokens, in one block or in all of them, leaves the rows before it as they are."""
+    rng = np.random.default_rng(dim + new)
+    n, page, at = new + 21, 16, new + 21 - 2
+    codes, scales = q8_cache(rng, n, dim, 1e-4)
+    q = queries(rng, new, group, dim)
+    pool, (k, v) = encode(codes, E.Q8_0, page, scales)
+    plain = run(pool, E.Q8_0, 1, dim, page, n, q, 1.0)
+    want, tol, _ = expect(q, k, v, 1.0, E.Q8_0, scales=scales[1].astype(np.float16).astype(np.float64))
+    assert np.all(np.abs(plain - want) <= tol)
+    rows = new - 2
+    for blocks in (slice(0, 1), slice(None)):
+        other = scales.copy()
+        other[1, 0, at, blocks] = bad
+        got = run(encode(codes, E.Q8_0, page, other)[0], E.Q8_0, 1, dim, page, n, q, 1.0)
+        err = np.abs(got - want)
+        assert np.all(err[:rows] <= tol[:rows]), np.max(err[:rows] / tol[:rows])
+        if bad == 100.0:  # (units are powers of two: not a bit of difference)
+            assert np.array_equal(got[:rows], plain[:rows])
