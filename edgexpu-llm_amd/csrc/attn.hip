@@ -667,7 +667,8 @@ struct Rows {
         return __builtin_amdgcn_readlane(v, 15);
     }
 
-    // acc in units of one, l the row's whole sum.
+    // acc in units of one, l the row's whole sum.  What is not finite becomes NaN: an infinite value gives infinity or NaN
+    // by the signs of the weights' rests, and NaN in a tile at the causal limit.
     __device__ __forceinline__ void finish() {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
@@ -678,6 +679,10 @@ struct Rows {
             } else if (TYPE == kTypeQ8_0) {
                 rescale(ldexpf(1.0f, ve - 8), t);
             }
+#pragma unroll
+            for (int d = 0; d < G::ND; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[t][d][j] = fmaf(acc[t][d][j], 0.0f, acc[t][d][j]);
         }
     }
 };

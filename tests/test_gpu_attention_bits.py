@@ -231,3 +231,46 @@ def test_value_scales_of_later_tokens_have_no_influence(hipdev, dim, group, new,
         assert np.all(err[:rows] <= tol[:rows]), np.max(err[:rows] / tol[:rows])
         if bad == 100.0:  # (units are powers of two: not a bit of difference)
             assert np.array_equal(got[:rows], plain[:rows])
+
+
+@pytest.mark.parametrize("qtype", [E.F16, E.Q8_0, E.F32])
+@pytest.mark.parametrize("dim,group,new", FORMS)
+@pytest.mark.parametrize("at", [3, 40, -1])
+def test_keys_and_values_that_are_not_finite(hipdev, qtype, dim, group, new, at):
+    """Wherever they lie and whatever the signs, a value makes itself (its block with Q8_0) NaN in the rows that see it; a
+    key makes them NaN, or with a score of minus infinity has no weight."""
+    rng = np.random.default_rng(dim + new + at)
+    n, page = new + 70, 32
+    at %= n
+    if qtype == E.Q8_0:
+        x, scales = q8_cache(rng, n, dim, 0.02)
+        x[x == 0] = 1
+    else:
+        x, scales = rng.standard_normal((2, 1, n, dim)), None
+    q = rng.standard_normal((new, group, dim)).astype(np.float32)
+    first = max(0, at - (n - new))  # the first row that sees it
+    pool, (k, v) = encode(x, qtype, page, scales)
+    plain = run(pool, qtype, 1, dim, page, n, q, dim ** -0.5)
+    assert np.isfinite(plain).all()
+    w = np.exp(np.einsum("thd,nd->thn", q.astype(np.float64), k[0]) * dim ** -0.5)
+    w[np.broadcast_to(np.arange(n) > np.arange(new)[:, None, None] + n - new, w.shape)] = 0.0
+    w[..., at] = 0.0
+    without = (w @ v[0]) / w.sum(-1, keepdims=True)
+    for bad in (np.inf, -np.inf, np.nan):
+        for which in (1, 0):
+            y, d = x.copy(), None if scales is None else scales.copy()
+            if qtype == E.Q8_0:
+                d[which, 0, at, 1] = bad
+            else:
+                y[which, 0, at, 37] = bad
+            got = run(encode(y, qtype, page, d)[0], qtype, 1, dim, page, n, q, dim ** -0.5)
+            assert np.array_equal(got[:first], plain[:first]), (bad, which)
+            if which == 1:
+                spoilt = slice(32, 64) if qtype == E.Q8_0 else slice(37, 38)
+                assert np.isnan(got[first:, :, spoilt]).all(), bad
+                rest = [e for e in range(dim) if not spoilt.start <= e < spoilt.stop]
+                assert np.array_equal(got[..., rest], plain[..., rest]), bad
+            else:
+                nan = np.isnan(got[first:]).any(-1)
+                assert np.isnan(got[first:][nan]).all() and (nan.all() or np.isinf(bad)), bad
+                assert np.allclose(got[first:][~nan], without[first:][~nan], rtol=0, atol=1e-4 * np.abs(v).max()), bad
