@@ -572,8 +572,10 @@ def qk_norm_rope(q, k, n_heads: int, n_kv_heads: int, pos, rope: Rope | None = N
         raise ValueError(f"q must be [tokens, n_heads * head_dim] with {n_heads} heads")
     m, dim = q.shape[0], q.shape[1] // n_heads
     ldq, ldk = _rows(q, n_heads * dim, "q"), _rows(k, n_kv_heads * dim, "k")
-    if k.shape[0] != m or (pos is not None and (pos.numel() != m or pos.dtype != torch.int32 or not pos.is_cuda)):
-        raise ValueError("q, k and the int32 pos must have the same tokens")
+    if k.shape[0] != m:
+        raise ValueError("q and k must have the same tokens")
+    if pos is not None and (pos.numel() != m or pos.dtype != torch.int32 or not pos.is_cuda or not pos.is_contiguous()):
+        raise ValueError(f"pos must be a dense int32 device tensor of {m} positions")
     q_out = q.new_empty((m, n_heads * dim)) if q_out is None else _dense(q_out, m * n_heads * dim, "q_out")
     k_out = q.new_empty((m, n_kv_heads * dim)) if k_out is None else _dense(k_out, m * n_kv_heads * dim, "k_out")
     L = hip()
