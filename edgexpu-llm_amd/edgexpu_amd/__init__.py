@@ -578,6 +578,8 @@ def qk_norm_rope(q, k, n_heads: int, n_kv_heads: int, pos, rope: Rope | None = N
         raise ValueError(f"pos must be a dense int32 device tensor of {m} positions")
     q_out = q.new_empty((m, n_heads * dim)) if q_out is None else _dense(q_out, m * n_heads * dim, "q_out")
     k_out = q.new_empty((m, n_kv_heads * dim)) if k_out is None else _dense(k_out, m * n_kv_heads * dim, "k_out")
+    if m == 0:
+        return q_out, k_out
     L = hip()
     L.check(L.qk_norm_rope_dev(q_out.data_ptr(), k_out.data_ptr(), q.data_ptr(), ldq, k.data_ptr(), ldk, m, n_heads,
                                n_kv_heads, dim, _weight(q_weight, dim), _weight(k_weight, dim), eps,

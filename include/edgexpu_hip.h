@@ -441,7 +441,8 @@ void edgexpu_hip_rope_destroy(edgexpu_hip_rope *r);
  * [m][n_kv_heads][head_dim] in one pass; token t stands at pos[t] >= 0 (device
  * int32).  Rows start ldq, ldk values apart (q, k and v may be slices of one
  * buffer); q_out and k_out are dense and may be q and k where those are dense
- * too.  head_dim even, at most 256.  k and k_out may be NULL with n_kv_heads 0. */
+ * too.  m at least 1; head_dim even, at most 256.  k and k_out may be NULL with
+ * n_kv_heads 0. */
 int edgexpu_hip_qk_norm_rope_dev(float *q_out, float *k_out, const float *q, long long ldq, const float *k,
                                  long long ldk, int m, int n_heads, int n_kv_heads, int head_dim,
                                  const float *q_weight, const float *k_weight, float eps,

@@ -53,3 +53,13 @@ def test_positions_are_dense(lib):
         with pytest.raises(ValueError):
             E.qk_norm_rope(q, k, 4, 2, bad)
     assert len(lib.calls) == n
+
+
+def test_rotation_of_no_tokens(lib):
+    """As kv_append and attention do; the library's entry points that take a token count have no call for none."""
+    q, k = on(torch.zeros(0, 256)), on(torch.zeros(0, 128))
+    qo, ko = E.qk_norm_rope(q, k, 4, 2, on(torch.zeros(0, dtype=torch.int32)))
+    assert qo.shape == (0, 256) and ko.shape == (0, 128) and not lib.calls
+    wide = on(torch.zeros(3, 1024))[:0]
+    qo, ko = E.qk_norm_rope(wide[:, :256], wide[:, 256:384], 4, 2, None, q_out=on(torch.zeros(0, 256)))
+    assert qo.shape == (0, 256) and ko.shape == (0, 128) and not lib.calls
