@@ -1189,6 +1189,7 @@ extern "C" int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip
         lib_error(-2, "attention: null buffer, q or out not 16-byte aligned, or scale %g not finite", (double)scale);
         return 0;
     }
+    if (capturing) batch_recorded(b);
     const edgexpu_hip_kv *kv = b->kv;
     AttnArgs a = {};
     a.q = q;

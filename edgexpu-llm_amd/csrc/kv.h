@@ -70,6 +70,8 @@ inline KvView kv_view(const edgexpu_hip_kv *kv, int layer) {
 
 // false (sticky error) unless the batch is set, fresh and `layer` exists; *capturing: the call is being recorded.
 bool batch_ready(edgexpu_hip_batch *b, int layer, hipStream_t st, const char *what, bool *capturing);
+// A call that nothing refuses any more is about to be recorded: the batch keeps the buffers that it holds.
+void batch_recorded(edgexpu_hip_batch *b);
 
 // attn.hip: what its kernel takes for a key, and how many of its workgroups run at once.
 RowCost attn_cost(int type, int dim);

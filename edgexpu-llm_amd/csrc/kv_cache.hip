@@ -145,11 +145,12 @@ bool batch_ready(edgexpu_hip_batch *b, int layer, hipStream_t st, const char *wh
         return false;
     }
     *capturing = is_capturing(st);
-    if (*capturing) {
-        b->captured = true;
-        b->captured_tokens = std::min(b->captured_tokens, (int)b->plan.tokens.size());
-    }
     return true;
+}
+
+void batch_recorded(edgexpu_hip_batch *b) {
+    b->captured = true;
+    b->captured_tokens = std::min(b->captured_tokens, (int)b->plan.tokens.size());
 }
 
 }  // namespace exq

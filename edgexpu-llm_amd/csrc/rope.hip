@@ -509,7 +509,10 @@ int edgexpu_hip_kv_append_dev(float *q_out, const float *q, long long ldq, const
     // (a captured call covers any later plan, of fewer tokens; -1: as many as the plan says)
     const int m = (int)b->plan.tokens.size();
     a.m = capturing ? -1 : m;
-    if (capturing) b->captured_append = true;
+    if (capturing) {
+        batch_recorded(b);
+        b->captured_append = true;
+    }
     return launch_rope(a, kv->type, m, (hipStream_t)stream, "kv_append") ? 1 : 0;
 }
 
