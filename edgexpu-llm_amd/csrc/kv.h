@@ -26,7 +26,7 @@ struct edgexpu_hip_kv {
 struct edgexpu_hip_batch {
     edgexpu_hip_kv *kv = nullptr;
     int n_heads = 0, max_seqs = 0, max_tokens = 0;
-    exq::AttnPlan plan;
+    exq::AttnPlan plan, made;  // made: of the set at hand, the plan once nothing refuses it
     bool set = false;
     uint64_t epoch = 0;     // the tables' when the plan was made
     bool captured = false;  // a captured call holds the device pointers

@@ -10,6 +10,7 @@
 #include <climits>
 #include <cstring>
 #include <new>
+#include <utility>
 
 #include "kv.h"
 #include "lib.h"
@@ -352,7 +353,7 @@ namespace {
 
 // Device memory of at least front + n * each bytes in *p, with room for half as
 // much again; *cap becomes the count that fits.  Refused, with nothing changed,
-// while a captured call holds the pointer.
+// while a captured call holds the pointer.  What it held goes: the batch is not set.
 bool grow(edgexpu_hip_batch *b, void **p, size_t front, size_t n, size_t each, size_t *cap, const char *what) {
     if (n <= *cap) return true;
     if (b->captured) {
@@ -360,6 +361,7 @@ bool grow(edgexpu_hip_batch *b, void **p, size_t front, size_t n, size_t each, s
                   what);
         return false;
     }
+    b->set = false;
     if (!lib_hip(hipDeviceSynchronize(), "batch_set: sync")) return false;
     if (*p) (void)hipFree(*p);
     *p = nullptr;
@@ -371,7 +373,7 @@ bool grow(edgexpu_hip_batch *b, void **p, size_t front, size_t n, size_t each, s
 }
 
 bool upload(edgexpu_hip_batch *b, hipStream_t st) {
-    AttnPlan &pl = b->plan;
+    const AttnPlan &pl = b->made;
     const size_t T = pl.tokens.size(), items_at = sizeof(PlanHeader) / 4, pages_at = items_at + 8 * pl.items.size(),
                  rows_at = pages_at + pl.pages.size(), joins_at = rows_at + pl.join_rows.size(),
                  parts_at = joins_at + pl.join_at.size(), words = parts_at + pl.join_parts.size();
@@ -419,6 +421,7 @@ bool upload(edgexpu_hip_batch *b, hipStream_t st) {
     put(rows_at, pl.join_rows);
     for (size_t i = 0; i < pl.join_at.size(); ++i) h[joins_at + i] = pl.join_at[i] + (int)parts_at;
     put(parts_at, pl.join_parts);
+    b->set = false;
     if (!lib_hip(hipMemcpyAsync(b->head() - 4 * T, b->stage[k], n * 4, hipMemcpyHostToDevice, st), "batch_set: copy"))
         return false;
     b->busy[k] = true;
@@ -453,16 +456,16 @@ int edgexpu_hip_batch_set(edgexpu_hip_batch *b, int n, const int *seqs, const in
         return 0;
     }
     return guarded("batch_set", 0, [&] {
-        b->set = false;
         const edgexpu_hip_kv *kv = b->kv;
-        b->plan.build(kt, n, seqs, n_new,
+        b->made.build(kt, n, seqs, n_new,
                       {b->n_heads / kv->n_kv, kv->n_kv, attn_cost(kv->type, kv->dim), (kv->dim + 2) * 4 * 2,
                        attn_workgroups(kv->type, kv->dim), kMinPieceCost});
-        if (b->captured_append && !b->plan.writable) {
+        if (b->captured_append && !b->made.writable) {
             lib_error(-2, "batch_set: a captured call appends, and a new token's page is held by another sequence too");
             return 0;
         }
         if (!upload(b, (hipStream_t)stream)) return 0;
+        std::swap(b->plan, b->made);
         b->epoch = kt.epoch();
         b->set = true;
         return 1;

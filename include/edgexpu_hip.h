@@ -416,7 +416,8 @@ int edgexpu_hip_kv_tables(const edgexpu_hip_kv *kv, int n, const int *seqs, int 
  * set the largest one before the capture.  A captured step replays with whatever
  * plan the last set has put there; after a captured edgexpu_hip_kv_append_dev a
  * plan is refused (error -2) where that call would be.  Calls of one batch share
- * its workspace: on one stream, or ordered by the caller. */
+ * its workspace: on one stream, or ordered by the caller.  A refused set (errors
+ * -2, -5, -7) leaves the batch as it was; one that the device fails, not set. */
 typedef struct edgexpu_hip_batch edgexpu_hip_batch;
 edgexpu_hip_batch *edgexpu_hip_batch_create(edgexpu_hip_kv *kv, int n_heads, int max_seqs, int max_tokens);
 /* Waits for the device, then frees. */

@@ -52,3 +52,41 @@ def test_a_refused_call_in_a_capture_holds_nothing(hipdev):
             calls()
         b.set([e], [4])  # more tokens, pieces that need a workspace
         assert b.tokens() == 4 and torch.isfinite(E.attention(b, 0, q)).all()
+
+
+def test_a_refused_set_leaves_the_batch_as_it_was(hipdev):
+    """Whatever refuses it: arguments, a captured call's tokens, plan buffer, workspace or slots."""
+    c, (a, e, g, h) = cache([40, 50, 2500, 6])
+    (f,) = c.fork([e])
+    q, k = rows(8, 64), rows(8, 64, 3)
+    qr, out = torch.zeros((8, 64), device="cuda:0"), torch.zeros((8, 64), device="cuda:0")
+    b = E.KvBatch(c, 1, 4, 8)
+    b.set([a, h], [2, 1])
+    want = E.attention(b, 0, q)[:3].clone()
+
+    def same():
+        assert b.tokens() == 3 and torch.equal(E.attention(b, 0, q)[:3], want)
+
+    for ids, n_new, what in (([a], [41], "41 new"), ([a], [9], "9 tokens"), ([a], [-1], "-1 new"), ([a, a], [1, 1], "twice"), ([9], [1], "not in use"),
+                             ([a, e, f, g, h], [1] * 5, "5 sequences")):
+        with pytest.raises(E.HipError, match=what):
+            b.set(ids, n_new)
+        same()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        E.kv_append(b, 0, q, k, k, q_out=qr)
+        E.attention(b, 0, qr, out=out)
+        with pytest.raises(E.HipError, match="captured"):
+            b.set([a], [1])
+    same()
+    for ids, n_new, what in (([a], [4], "4 tokens outgrows"), ([e], [1], "appends"), ([g], [1], "outgrows the workspace")):
+        with pytest.raises(E.HipError, match=what):
+            b.set(ids, n_new)
+        same()
+        for _ in range(2):  # and the graph replays the plan that is set
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out[:3], E.attention(b, 0, qr)[:3])
+        want = E.attention(b, 0, q)[:3].clone()  # (the replays have written its tokens' slots)
+    b.set([a], [1])
+    assert b.tokens() == 1
