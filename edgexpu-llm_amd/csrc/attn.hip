@@ -99,8 +99,11 @@ struct Geo {
     static constexpr int RING = UNIT * 16 <= 80 * 1024 ? 4 : 2;
     static constexpr int SHARED = 4;
     static constexpr int TILE16 = 32 * DIM * 2;  // a unit's values as f16
-    static constexpr int MANY = SHARED * 2 * UNIT + (SB ? 3 * TILE16 : 0);  // (Q8_0: codes of K, both parts of V)
-    static constexpr int RT = DIM == 256 ? 1 : 2;  // 16-row tiles of a wave, many rows
+    static constexpr int RT = DIM == 256 ? 1 : 2;  // 16-row tiles of a wave, many rows at most
+    // Many rows with one tile a wave: not for Q8_0 but at 128, where two workgroups of 32 (64, 96: 53 and 81 ns a key
+    // against 59 and 88) or four of 16 (256: 259 and 262) are faster.
+    static constexpr bool ONE = TYPE != kTypeQ8_0 || DIM == 128;
+    static constexpr int MANY = ONE || RT > 1 ? SHARED * 2 * UNIT + (SB ? 3 * TILE16 : 0) : 0;  // (Q8_0: codes of K, both parts of V)
     // 17 to 32 rows as few: with f16 no faster than the shared tiles (128: 56 and 57 ns a key), else near twice
     // (Q8_0 47 and 86, f32 101 and 169).
     static constexpr bool PAIR = RT == 2 && TYPE != kTypeF16;
@@ -579,8 +582,8 @@ struct Rows {
                 for (int i = 0; i < 2 * G::NB; ++i) sc[hf][i] = ds[hf * 8 * G::NB + i];
             const int o = c16 >> 1, row = (o < 4 ? g * 4 + o : 16 + g * 4 + o - 4), sw = swz<TYPE, DIM, true>(row);
             // Several blocks a branch: one for each would keep their products apart (5 to 13 % of the time), and all are
-            // too many registers with two tiles of rows.
-            constexpr int GROUP = RT == 1 ? G::NB : 2;
+            // too many registers with two tiles of rows or eight blocks.
+            constexpr int GROUP = RT == 1 && G::NB <= 4 ? G::NB : 2;
 #pragma unroll
             for (int b0 = 0; b0 < G::NB; b0 += GROUP) {
                 float x[GROUP][RT][8], big[GROUP][RT];
@@ -1038,8 +1041,11 @@ __global__ __launch_bounds__(256, (Geo<TYPE, DIM>::PER_CU)) void attn_kernel(con
         s.last = (it.key1 - 1) >> a.kv.page_shift;
         if (it.n_rows <= 16) attend_few<TYPE, DIM, 1>(a, it, s, h, lds, wave, lane);
         else if (G::PAIR && it.n_rows <= 32) attend_few<TYPE, DIM, G::PAIR ? 2 : 1>(a, it, s, h, lds, wave, lane);
-        else if (G::RT == 1 || it.n_rows <= 64) attend_many<TYPE, DIM, 1>(a, it, s, h, lds, wave, lane);
-        else attend_many<TYPE, DIM, G::RT>(a, it, s, h, lds, wave, lane);
+        else if (G::ONE && (G::RT == 1 || it.n_rows <= 64)) {
+            if constexpr (G::ONE) attend_many<TYPE, DIM, 1>(a, it, s, h, lds, wave, lane);
+        } else {
+            if constexpr (G::RT > 1) attend_many<TYPE, DIM, G::RT>(a, it, s, h, lds, wave, lane);
+        }
     }
 }
 
@@ -1116,16 +1122,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
         }
         __syncthreads();
     }
-}
-
-// Measured: 8 kv heads, 512 workgroups at once; keys of 4096 tokens a sequence
-// for few rows (bound by the loads, 5 to 6 TB/s), of one run of 131072 for more.
-RowCost attn_cost(int type, int dim) {
-    const int d = dim == 64 ? 0 : dim == 96 ? 1 : dim == 128 ? 2 : 3;
-    static const RowCost f32[4] = {{{460, 540, 1000, 1580}}, {{666, 797, 1494, 2270}}, {{878, 1007, 1780, 2900}}, {{1765, 4750, 4760, 0}}};
-    static const RowCost f16[4] = {{{237, 320, 320, 520}}, {{336, 470, 480, 730}}, {{474, 590, 595, 840}}, {{865, 1414, 1425, 0}}};
-    static const RowCost q80[4] = {{{148, 267, 586, 774}}, {{230, 403, 878, 1100}}, {{286, 469, 920, 1160}}, {{648, 2609, 2624, 0}}};
-    return type == kTypeF32 ? f32[d] : type == kTypeF16 ? f16[d] : q80[d];
 }
 
 namespace {

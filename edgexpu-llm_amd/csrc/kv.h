@@ -73,8 +73,7 @@ bool batch_ready(edgexpu_hip_batch *b, int layer, hipStream_t st, const char *wh
 // A call that nothing refuses any more is about to be recorded: the batch keeps the buffers that it holds.
 void batch_recorded(edgexpu_hip_batch *b);
 
-// attn.hip: what its kernel takes for a key, and how many of its workgroups run at once.
-RowCost attn_cost(int type, int dim);
+// attn.hip: how many of its kernel's workgroups run at once.
 int attn_workgroups(int type, int dim);
 // Allows the kernel the LDS it takes (once for a batch: nothing of it is left for a captured call).
 hipError_t attn_prepare(int type, int dim);
