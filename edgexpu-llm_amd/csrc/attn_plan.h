@@ -55,13 +55,14 @@ struct RowCost {
 };
 // Of csrc/attn.hip's kernel for a cache of f32 (type 0), f16 (1) or Q8_0 (8) and
 // heads of 64, 96, 128 or 256.  0: it has no form for as many (Geo::ONE, RT).
-// Measured: 8 kv heads, 512 workgroups at once; keys of 4096 tokens a sequence
-// for few rows (bound by the loads, 5 to 6 TB/s), of one run of 131072 for more.
+// Measured: 8 kv heads, 512 workgroups at once (f32 and f16 at 256: 256); keys of
+// 4096 tokens a sequence for few rows (bound by the loads, 5 to 6 TB/s), of one run
+// of 131072 for more, which no L2 holds: a chunk behind 8192 keys takes two thirds.
 inline RowCost attn_cost(int type, int dim) {
     const int d = dim == 64 ? 0 : dim == 96 ? 1 : dim == 128 ? 2 : 3;
-    static const RowCost f32[4] = {{{460, 540, 1000, 1580}}, {{666, 797, 1494, 2270}}, {{878, 1007, 1780, 2900}}, {{1765, 4750, 4760, 0}}};
-    static const RowCost f16[4] = {{{237, 320, 320, 520}}, {{336, 470, 480, 730}}, {{474, 590, 595, 840}}, {{865, 1414, 1425, 0}}};
-    static const RowCost q80[4] = {{{148, 267, 0, 774}}, {{230, 403, 0, 1100}}, {{286, 469, 920, 1160}}, {{648, 0, 0, 0}}};
+    static const RowCost f32[4] = {{{460, 540, 1000, 1580}}, {{666, 797, 1494, 2270}}, {{878, 1007, 1780, 2900}}, {{867, 2120, 2122, 0}}};
+    static const RowCost f16[4] = {{{237, 320, 320, 520}}, {{336, 470, 480, 730}}, {{474, 590, 595, 840}}, {{433, 648, 650, 0}}};
+    static const RowCost q80[4] = {{{148, 267, 0, 774}}, {{230, 403, 0, 1100}}, {{286, 469, 920, 1160}}, {{577, 0, 0, 0}}};
     return type == 0 ? f32[d] : type == 1 ? f16[d] : q80[d];
 }
 

@@ -457,9 +457,11 @@ int edgexpu_hip_batch_set(edgexpu_hip_batch *b, int n, const int *seqs, const in
     }
     return guarded("batch_set", 0, [&] {
         const edgexpu_hip_kv *kv = b->kv;
+        // (a partial result: its bytes twice, at a workgroup's part of 5.1 TB/s)
+        const int at_once = attn_workgroups(kv->type, kv->dim);
         b->made.build(kt, n, seqs, n_new,
-                      {b->n_heads / kv->n_kv, kv->n_kv, attn_cost(kv->type, kv->dim), (kv->dim + 2) * 4 * 2,
-                       attn_workgroups(kv->type, kv->dim), kMinPieceCost});
+                      {b->n_heads / kv->n_kv, kv->n_kv, attn_cost(kv->type, kv->dim), (kv->dim + 2) * 4 * 2 * at_once / 512,
+                       at_once, kMinPieceCost});
         if (b->captured_append && !b->made.writable) {
             lib_error(-2, "batch_set: a captured call appends, and a new token's page is held by another sequence too");
             return 0;
