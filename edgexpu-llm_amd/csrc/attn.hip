@@ -113,6 +113,8 @@ struct Geo {
     static constexpr int ODD_WORDS = TT * NB;
     static constexpr int LDS_BYTES = ODD + 4 * ODD_WORDS * 4;
     static constexpr int PER_CU = LDS_BYTES <= 80 * 1024 ? 2 : 1;  // workgroups that LDS leaves room for
+    // Registers for three where there is room for them (40 Q8_0 sequences behind 5000 tokens: 33 us with two, 28).
+    static constexpr int WAVES = DIM == 64 ? 3 : PER_CU;
 };
 
 // Piece permutation of row `row` of a tile: piece c lies at c ^ swz.  Chosen so
@@ -583,7 +585,7 @@ struct Rows {
             const int o = c16 >> 1, row = (o < 4 ? g * 4 + o : 16 + g * 4 + o - 4), sw = swz<TYPE, DIM, true>(row);
             // Several blocks a branch: one for each would keep their products apart (5 to 13 % of the time), and all are
             // too many registers with two tiles of rows or eight blocks.
-            constexpr int GROUP = RT == 1 && G::NB <= 4 ? G::NB : 2;
+            constexpr int GROUP = G::NB == 2 ? 2 / RT : RT == 1 && G::NB <= 4 ? G::NB : 2;
 #pragma unroll
             for (int b0 = 0; b0 < G::NB; b0 += GROUP) {
                 float x[GROUP][RT][8], big[GROUP][RT];
@@ -992,7 +994,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs &a, const AttnItem &i
 }
 
 template <int TYPE, int DIM>
-__global__ __launch_bounds__(256, (Geo<TYPE, DIM>::PER_CU)) void attn_kernel(const AttnArgs args) {
+__global__ __launch_bounds__(256, (Geo<TYPE, DIM>::WAVES)) void attn_kernel(const AttnArgs args) {
     using G = Geo<TYPE, DIM>;
     extern __shared__ __align__(16) uint8_t lds[];
     const PlanHeader *hd = reinterpret_cast<const PlanHeader *>(args.head);
