@@ -415,6 +415,26 @@ def _ints(v):
     return (C.c_int * len(v))(*v)
 
 
+_ENDED: list = []  # (entry point, handle) of objects that are gone while their handles are not
+
+
+def _end(destroy=None, handle=None):
+    """Ends a handle, and those that wait: while the current stream is captured, which the wait for the device would
+    break, and a cache's until its batches' have ended."""
+    import torch
+
+    if handle is not None:
+        _ENDED.append((destroy, handle))
+    if not _ENDED or (torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()):
+        return
+    todo = _ENDED[:]
+    del _ENDED[:]
+    for destroy, handle in todo:
+        if destroy(handle) == 0:
+            _HIP.clear_error()
+            _ENDED.append((destroy, handle))
+
+
 class KvCache:
     """A paged cache of keys and values (edgexpu_hip_kv_*): ``n_pages`` pages of
     ``page_tokens`` tokens in each of ``n_layers`` layers, values of type F32, F16
@@ -434,6 +454,7 @@ class KvCache:
                 size and pool.numel() != size):
             raise ValueError(f"pool must be a flat uint8 device tensor of {size} bytes")
         self.pool, self.n_kv_heads, self.head_dim = pool, n_kv_heads, head_dim
+        _end()
         h = L.kv_create(_ptr(pool) if size else None, qtype, n_layers, n_kv_heads, head_dim, page_tokens, n_pages,
                         max_seqs)
         L.check(bool(h), "kv_create")
@@ -441,7 +462,7 @@ class KvCache:
 
     def __del__(self, gone=sys.is_finalizing):
         if getattr(self, "_h", None) and not gone():
-            _HIP.kv_destroy(self._h)
+            _end(_HIP.kv_destroy, self._h)
 
     def new(self) -> int:
         """A new empty sequence."""
@@ -502,13 +523,14 @@ class KvBatch:
     def __init__(self, cache: KvCache, n_heads: int, max_seqs: int, max_tokens: int):
         self._h = None
         self.cache, self.n_heads = cache, n_heads
+        _end()
         h = _HIP.batch_create(cache._h, n_heads, max_seqs, max_tokens)
         _HIP.check(bool(h), "batch_create")
         self._h = h
 
     def __del__(self, gone=sys.is_finalizing):
         if getattr(self, "_h", None) and not gone():
-            _HIP.batch_destroy(self._h)
+            _end(_HIP.batch_destroy, self._h)
 
     def set(self, seqs, n_new):
         """The last n_new[i] tokens of seqs[i] are the step's."""
@@ -530,13 +552,14 @@ class Rope:
             if len(factors) != n_rot // 2:
                 raise ValueError(f"{len(factors)} factors for {n_rot // 2} pairs")
             factors = (C.c_float * len(factors))(*factors)
+        _end()
         h = L.rope_create(n_rot, base, scale, factors, int(interleaved))
         L.check(bool(h), "rope_create")
         self._h = h
 
     def __del__(self, gone=sys.is_finalizing):
         if getattr(self, "_h", None) and not gone():
-            _HIP.rope_destroy(self._h)
+            _end(_HIP.rope_destroy, self._h)
 
 
 def _f32(x) -> bool:

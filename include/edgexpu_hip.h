@@ -334,11 +334,15 @@ int edgexpu_hip_gate_up_silu_dev(float *act, const float *x, const float *norm_w
  *   (what the step computes), then for each layer edgexpu_hip_kv_append_dev
  *   and edgexpu_hip_attention_dev.
  * All of these run on the device of edgexpu_hip_init and refuse (error -4) a
- * caller whose current device is another.  Work on one cache goes to one
+ * caller whose current device is another (the _destroy calls, which return nothing,
+ * are made on it).  Work on one cache goes to one
  * stream, or to streams that the caller orders: the host tables change when a
  * call returns, the device work it queued runs later.  A cache and its batches
  * are used by one host thread at a time.  What a captured call was given (batch,
- * rotation, weights, buffers) lives as long as its graph. */
+ * rotation, weights, buffers) lives as long as its graph.  The calls that wait for
+ * the device or take memory (_create, _destroy, a edgexpu_hip_batch_set whose plan
+ * needs larger buffers) are not for a time in which any stream is captured: they
+ * break the capture. */
 
 /* A paged cache of keys and values: n_layers x n_pages pages of page_tokens
  * tokens.  A layer's page holds K, then V; each holds, for every kv head, the

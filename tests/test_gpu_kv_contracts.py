@@ -90,3 +90,26 @@ def test_a_refused_set_leaves_the_batch_as_it_was(hipdev):
         want = E.attention(b, 0, q)[:3].clone()  # (the replays have written its tokens' slots)
     b.set([a], [1])
     assert b.tokens() == 1
+
+
+def test_objects_that_go_during_a_capture(hipdev):
+    """A batch, a rotation and a cache collected while a step is captured: the capture stands, their handles end later."""
+    c, (a,) = cache([300])
+    old, (x,) = cache([10])
+    b, gone, rope = E.KvBatch(c, 1, 1, 1), E.KvBatch(old, 1, 1, 1), E.Rope(64)
+    b.set([a], [1])
+    gone.set([x], [1])
+    q, out = rows(1, 64), torch.zeros((1, 64), device="cuda:0")
+    want = E.attention(b, 0, q).clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        E.attention(b, 0, q, out=out)
+        del gone, rope, old
+    assert len(E._ENDED) == 3
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    E.Rope(64)
+    assert not E._ENDED

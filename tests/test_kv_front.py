@@ -63,3 +63,75 @@ def test_rotation_of_no_tokens(lib):
     wide = on(torch.zeros(3, 1024))[:0]
     qo, ko = E.qk_norm_rope(wide[:, :256], wide[:, 256:384], 4, 2, None, q_out=on(torch.zeros(0, 256)))
     assert qo.shape == (0, 256) and ko.shape == (0, 128) and not lib.calls
+
+
+class Ends(Notes):
+    """A cache with a live batch does not end."""
+
+    batches = 0
+    made = 0
+
+    def kv_pool_bytes(self, *args):
+        return 1024
+
+    def kv_create(self, *args):
+        self.made += 1
+        return self.made
+
+    def batch_create(self, *args):
+        self.batches += 1
+        self.made += 1
+        return self.made
+
+    def batch_destroy(self, h):
+        self.batches -= 1
+        self.calls.append(("batch_destroy", h))
+
+    def kv_destroy(self, h):
+        if self.batches:
+            return 0
+        self.calls.append(("kv_destroy", h))
+        return 1
+
+    def rope_create(self, *args):
+        self.made += 1
+        return self.made
+
+    def rope_destroy(self, h):
+        self.calls.append(("rope_destroy", h))
+
+
+def test_handles_end_outside_a_capture(monkeypatch):
+    """An object that goes while the stream is captured keeps its handle until an object is made or goes after it; a
+    cache that goes before its batch (in a cycle) ends after it."""
+    L = Ends()
+    monkeypatch.setattr(E, "hip", lambda: L)
+    monkeypatch.setattr(E, "_HIP", L)
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    capturing = False
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    pool = on(torch.zeros(1024, dtype=torch.uint8))
+
+    def ended():
+        return [c for c in L.calls if c[0].endswith("destroy")]
+
+    def cache():
+        return E.KvCache(E.F16, 1, 1, 64, 16, 4, 1, pool=pool)
+
+    c = cache()
+    b, r = E.KvBatch(c, 1, 1, 1), E.Rope(64)
+    capturing = True
+    del b, c, r
+    assert not ended()
+    capturing = False
+    c = cache()
+    assert ended() == [("batch_destroy", 2), ("kv_destroy", 1), ("rope_destroy", 3)]
+    del L.calls[:]
+    b = E.KvBatch(c, 1, 1, 1)
+    c.__del__()
+    c._h = None
+    assert not ended()
+    del b
+    assert ended() == [("batch_destroy", 5)]
+    E._end()
+    assert ended() == [("batch_destroy", 5), ("kv_destroy", 4)] and not E._ENDED
