@@ -466,7 +466,7 @@ struct Rows {
     }
 
     // A row's reference moves to the largest score of its tile where that is out of the window: by the row's own keys, no
-    // other row has a say.  It is lowered as long as the sums stay below 2^64 (weights of up to 2^15, values of 2^16).
+    // other row has a say.  It is lowered as long as the weights' sum stays below 2^96 (values: 2^16 at most).
     __device__ __forceinline__ void follow() {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
@@ -475,7 +475,7 @@ struct Rows {
             if (__builtin_amdgcn_ballot_w64(out) != 0) {
                 const float row = col_max(top[t]);
                 const bool lower = FOLLOW && row < m[t] - kDown && row > -INFINITY &&
-                                   col_max(l[t]) * __builtin_amdgcn_exp2f(m[t] - row) < 0x1p64f;
+                                   col_max(l[t]) * __builtin_amdgcn_exp2f(m[t] - row) < 0x1p96f;
                 const float mn = row > m[t] + kUp || lower ? row : m[t];
                 const float c = m[t] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[t] - mn);
                 m[t] = mn;

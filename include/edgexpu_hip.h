@@ -471,7 +471,7 @@ int edgexpu_hip_kv_append_dev(float *q_out, const float *q, long long ldq, const
  * 2^-22 t where that is more; where t is the row's largest so far, by 2^-22 w or
  * 2^-34 t.  (Q8_0 with few rows: w times its value's scale, and t the largest of
  * those of the block; a block's sums are off by 2^-22 of its largest value
- * besides.)  A value that is not finite makes itself (a Q8_0 scale its block) NaN
+ * besides.)  Weights below 2^-60 of the row's sum may be lost.  A value that is not finite makes itself (a Q8_0 scale its block) NaN
  * in the rows that see it, wherever it lies; a key that is not finite makes those
  * rows NaN, or has no weight where its score is minus infinity.  f32 sums of values
  * beyond 2^96 may overflow, and are NaN then.  Contents of slots that a token does not see (behind the sequence's
