@@ -403,11 +403,15 @@ edgexpu_hip_rope *edgexpu_hip_rope_create(int n_rot, double base, double scale, 
         lib_error(-2, "rope_create: n_rot=%d (even, 2..256), base=%g, scale=%g", n_rot, base, scale);
         return nullptr;
     }
-    if (!lib_ready("rope_create")) return nullptr;
     double turns[128];
-    for (int i = 0; i < n_rot / 2; ++i)
+    for (int i = 0; i < n_rot / 2; ++i) {
         turns[i] = scale * std::pow(base, -2.0 * i / n_rot) / (factors != nullptr ? (double)factors[i] : 1.0) /
                    6.283185307179586476925;
+        if (std::isfinite(turns[i] * INT_MAX)) continue;  // (any position's angle is a number)
+        lib_error(-2, "rope_create: pair %d turns by %g a position", i, turns[i]);
+        return nullptr;
+    }
+    if (!lib_ready("rope_create")) return nullptr;
     void *p = nullptr;
     if (!lib_hip(hipMalloc(&p, sizeof(turns)), "rope_create: hipMalloc")) return nullptr;
     edgexpu_hip_rope *r = new (std::nothrow) edgexpu_hip_rope();

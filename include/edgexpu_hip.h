@@ -435,7 +435,8 @@ int edgexpu_hip_batch_tokens(const edgexpu_hip_batch *b);
  * array of n_rot/2, NULL: ones), pair i being the values i and i + n_rot/2, or
  * with `interleaved` 2i and 2i + 1 (the reference's two RoPE forms,
  * among src/cpu_kernel.c:659-972).  Angles are kept in 64 bits and reduced there, so
- * far positions lose nothing.  NULL on error. */
+ * far positions lose nothing.  NULL on error (-2 also where an angle would be no
+ * number: a factor of zero). */
 typedef struct edgexpu_hip_rope edgexpu_hip_rope;
 edgexpu_hip_rope *edgexpu_hip_rope_create(int n_rot, double base, double scale, const float *factors,
                                           int interleaved);
