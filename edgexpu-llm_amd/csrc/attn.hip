@@ -29,8 +29,9 @@
 // the row's sums are rescaled, where that is 2^5 above m or 2^13 below.  With t
 // the largest of a row's weights in a tile of 32 keys, a weight w there is off by
 // at most 2^-22 w, or 2^-22 t where that is more, and where t is the largest of
-// the row so far by 2^-34 t.  (Raised at 2^4: 64-key heads 4 % slower; lowered at
-// 2^10 and less: 3 to 5 %, tiles that no row has to move for are looked at.)
+// the row so far by 2^-34 t.  (Raised at 2^4 instead of 2^6 chunks take 1 to 2 %
+// longer; lowered at 2^10 instead of 2^14 2 to 9 %, as tiles that no row has to
+// move for are looked at.)
 //
 // Q8_0 values.  Few rows: the parts are of weight times scale, with a reference
 // for each row and block that follows in the same way, so a large scale costs
@@ -47,7 +48,7 @@
 //     together.  4 x 512 tokens behind 8192 f16 keys 490 us: 1.2 PFLOP/s of
 //     matrix instructions (two for each product; a loop of nothing but them on
 //     random operands reaches 1.75 on this card, a large library product 1.1);
-//     MFMA 57 % of the cycles, waves wait 27 % and contend for issue 30 %;
+//     MFMA 55 % of the cycles, waves wait 23 % and contend for issue 36 %;
 //   short calls: a chain of loads (item -> page -> keys, item -> token -> query),
 //     the first tile and the join of the waves, 5 to 7 us.
 #include <hip/hip_runtime.h>
