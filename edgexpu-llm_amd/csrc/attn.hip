@@ -467,7 +467,8 @@ struct Rows {
     }
 
     // A row's reference moves to the largest score of its tile where that is out of the window: by the row's own keys, no
-    // other row has a say.  It is lowered as long as the weights' sum stays below 2^96 (values: 2^16 at most).
+    // other row has a say.  It is lowered as long as the weights' sum stays below 2^96 (values: 2^16 at most).  It is a
+    // whole number, so that the sums keep all their bits however often it moves.
     __device__ __forceinline__ void follow() {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
@@ -477,8 +478,9 @@ struct Rows {
                 const float row = col_max(top[t]);
                 const bool lower = FOLLOW && row < m[t] - kDown && row > -INFINITY &&
                                    col_max(l[t]) * __builtin_amdgcn_exp2f(m[t] - row) < 0x1p96f;
-                const float mn = row > m[t] + kUp || lower ? row : m[t];
-                const float c = m[t] == mn ? 1.0f : __builtin_amdgcn_exp2f(m[t] - mn);
+                const float mn = row > m[t] + kUp || lower ? rintf(row) : m[t];
+                // (-infinity, the first: zero)
+                const float c = m[t] == mn ? 1.0f : ldexpf(1.0f, (int)fmaxf(-200.0f, fminf(200.0f, m[t] - mn)));
                 m[t] = mn;
                 l[t] *= c;
                 rescale(c, t);
