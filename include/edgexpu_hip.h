@@ -418,7 +418,8 @@ int edgexpu_hip_kv_tables(const edgexpu_hip_kv *kv, int n, const int *seqs, int 
  * buffers, and a plan that outgrows them, or has more tokens than the plan at
  * the capture (the caller's buffers need hold no more), is refused (error -7):
  * set the largest one before the capture.  A captured step replays with whatever
- * plan the last set has put there; after a captured edgexpu_hip_kv_append_dev a
+ * plan the last set has put there (nothing refuses the replay of a stale one: set
+ * the batch after every change); after a captured edgexpu_hip_kv_append_dev a
  * plan is refused (error -2) where that call would be.  Calls of one batch share
  * its workspace: on one stream, or ordered by the caller.  A refused set (errors
  * -2, -5, -7) leaves the batch as it was; one that the device fails, not set. */

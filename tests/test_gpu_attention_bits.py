@@ -189,9 +189,9 @@ def q8_cache(rng, n, dim, typical):
     return codes, scales
 
 
-# rows of a workgroup: 1, 4, 20, 40, 128; 128 twice
-FORMS = [(64, 1, 1), (96, 4, 1), (128, 4, 1), (256, 4, 2), (64, 4, 5), (128, 4, 5), (96, 8, 4), (128, 8, 5), (64, 8, 16), (96, 16, 8), (128, 16, 17),
-         (256, 8, 5)]
+# rows of a workgroup: 1 to 10, 16, 20, 40, 128; 128 and more
+FORMS = [(128, 1, 6), (96, 2, 5), (256, 2, 4), (64, 1, 1), (96, 4, 1), (128, 4, 1), (256, 4, 2), (64, 4, 5), (128, 4, 5), (96, 8, 4),
+         (128, 8, 5), (64, 8, 16), (96, 16, 8), (128, 16, 17), (256, 8, 5)]
 
 
 @pytest.mark.parametrize("dim,group,new", FORMS)
