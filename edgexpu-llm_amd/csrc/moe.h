@@ -1,0 +1,37 @@
+// The routing of a step to experts, as its products see it.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "common.h"
+#include "edgexpu_hip.h"
+
+struct edgexpu_hip_moe {
+    int n_experts = 0, top_k = 0, max_tokens = 0, n_embd = 0, n_ff = 0;
+    int m = -1;  // tokens of the last routing (-1: none yet)
+    uint8_t *mem = nullptr;
+    int32_t *ids = nullptr;  // [max_tokens][top_k], -1: no expert
+    float *weights = nullptr;
+    uint8_t *xq = nullptr;  // quantized activations of the product at hand
+    float *part = nullptr;  // [max_tokens][top_k][n_embd]: a token's parts of the down product
+    size_t pairs() const { return (size_t)(m > 0 ? m : 0) * top_k; }
+};
+
+namespace exq {
+
+constexpr int kMoeMaxExperts = 512, kMoeMaxTopK = 32, kMoeMaxGroups = 64;
+
+struct RouteArgs {
+    const float *scores, *bias;
+    int32_t *ids, *ids_out;
+    float *weights, *weights_out;
+    int m, n_experts, top_k, sigmoid, n_groups, top_groups, group_best, normalise;
+    double scale;
+};
+
+hipError_t launch_moe_route(const RouteArgs &a, hipStream_t st);
+hipError_t launch_moe_assign(const int32_t *ids, const float *weights, int32_t *to_ids, float *to_weights, int pairs,
+                             int n_experts, hipStream_t st);
+
+}  // namespace exq

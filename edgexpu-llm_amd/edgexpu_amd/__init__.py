@@ -151,6 +151,17 @@ class HipLib:
                                    C.c_float, _vp, _vp])
         self.attention_dev = _sig(L, "edgexpu_hip_attention_dev", C.c_int,
                                   [_vp, _vp, _vp, C.c_int, C.c_float, _vp])
+        self.moe_create = _sig(L, "edgexpu_hip_moe_create", _vp, [C.c_int] * 5)
+        self.moe_destroy = _sig(L, "edgexpu_hip_moe_destroy", None, [_vp])
+        self.moe_tokens = _sig(L, "edgexpu_hip_moe_tokens", C.c_int, [_vp])
+        self.moe_route_dev = _sig(L, "edgexpu_hip_moe_route_dev", C.c_int,
+                                  [_vp, _vp, _vp, _vp, C.c_int, C.c_int, _vp, C.c_int, C.c_int, C.c_int, C.c_int,
+                                   C.c_double, _vp])
+        self.moe_assign_dev = _sig(L, "edgexpu_hip_moe_assign_dev", C.c_int, [_vp, _vp, _vp, C.c_int, _vp])
+        self.moe_gate_up_dev = _sig(L, "edgexpu_hip_moe_gate_up_dev", C.c_int,
+                                    [_vp, _vp, _vp, _vp, _vp, C.c_uint32, _vp, _vp, C.c_int, _vp])
+        self.moe_down_dev = _sig(L, "edgexpu_hip_moe_down_dev", C.c_int,
+                                 [_vp, _vp, _vp, _vp, C.c_uint32, _vp, _vp, _vp])
 
     def last_error(self) -> tuple[int, str]:
         buf = C.create_string_buffer(512)
@@ -638,6 +649,112 @@ def attention(batch: KvBatch, layer: int, q, scale: float | None = None, out=Non
         scale = batch.cache.head_dim ** -0.5
     if not _HIP.attention_dev(out.data_ptr(), q.data_ptr(), batch._h, layer, scale, _stream()):
         _HIP.check(0, "attention")
+    return out
+
+
+# ---------------------------------------------- a feed-forward of experts
+
+
+class MoePlan:
+    """The routing of a step's tokens to top_k of n_experts, and the workspaces of the
+    products that follow it (edgexpu_hip_moe_*)."""
+
+    def __init__(self, n_experts: int, top_k: int, max_tokens: int, n_embd: int, n_ff: int):
+        L = hip()
+        self._h = None
+        self.n_experts, self.top_k, self.n_embd, self.n_ff = n_experts, top_k, n_embd, n_ff
+        _end()
+        h = L.moe_create(n_experts, top_k, max_tokens, n_embd, n_ff)
+        L.check(bool(h), "moe_create")
+        self._h = h
+
+    def __del__(self, gone=sys.is_finalizing):
+        if getattr(self, "_h", None) and not gone():
+            _end(_HIP.moe_destroy, self._h)
+
+    def assign(self, ids, weights):
+        """The caller's own choices: int32 ids and float32 weights [tokens, top_k]."""
+        m = ids.shape[0]
+        _choices(ids, m, self.top_k, "ids", False)
+        _choices(weights, m, self.top_k, "weights", True)
+        _HIP.check(_HIP.moe_assign_dev(self._h, _ptr(ids), _ptr(weights), m, _stream()), "moe_assign")
+
+    def tokens(self) -> int:
+        return _HIP.moe_tokens(self._h)
+
+
+def _choices(t, m: int, k: int, what: str, floating: bool):
+    if not t.is_cuda or t.element_size() != 4 or t.is_floating_point() != floating or t.is_complex() or (
+            tuple(t.shape) != (m, k)) or not t.is_contiguous():
+        raise ValueError(f"{what} must be a dense {'float32' if floating else 'int32'} device tensor [{m}, {k}]")
+    return t
+
+
+def _expert_weights(w, qtype: int, n_experts: int, rows: int, n: int, what: str):
+    import torch
+
+    size = n_experts * rows * row_bytes(qtype, n)
+    if not w.is_cuda or w.dtype != torch.uint8 or not w.is_contiguous() or w.numel() != size:
+        raise ValueError(f"{what} must be a dense uint8 device tensor of {size} bytes ({n_experts} experts of {rows} rows)")
+    return w.data_ptr()
+
+
+def _expert_bias(b, n_experts: int, rows: int, what: str):
+    return None if b is None else _dense(b, n_experts * rows, what).data_ptr()
+
+
+def moe_route(plan: MoePlan, scores, score: str = "softmax", bias=None, n_groups: int = 1, top_groups: int = 1,
+              group_best: int = 1, normalise: bool = True, scale: float = 1.0, ids=None, weights=None):
+    """Chooses each token's experts by ``scores`` [tokens, n_experts] float32
+    (edgexpu_hip_moe_route_dev); returns ids int32 and weights float32
+    [tokens, top_k], -1 and 0 where no expert is left."""
+    import torch
+
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f"score must be softmax or sigmoid, not {score!r}")
+    if scores.dim() != 2 or scores.shape[1] != plan.n_experts:
+        raise ValueError(f"scores must be [tokens, {plan.n_experts}]")
+    m = scores.shape[0]
+    _dense(scores, m * plan.n_experts, "scores")
+    if bias is not None:
+        _dense(bias, plan.n_experts, "bias")
+    ids = scores.new_empty((m, plan.top_k), dtype=torch.int32) if ids is None else _choices(ids, m, plan.top_k, "ids", False)
+    weights = scores.new_empty((m, plan.top_k)) if weights is None else _choices(weights, m, plan.top_k, "weights", True)
+    _HIP.check(_HIP.moe_route_dev(plan._h, ids.data_ptr(), weights.data_ptr(), scores.data_ptr(), m,
+                                  int(score == "sigmoid"), _ptr(bias), n_groups, top_groups, group_best,
+                                  int(normalise), scale, _stream()), "moe_route")
+    return ids, weights
+
+
+def moe_gate_up(plan: MoePlan, w_gate, w_up, qtype: int, x, b_gate=None, b_up=None, activation: str = "silu", act=None):
+    """Gate and up of each token's experts with the activation between them
+    (edgexpu_hip_moe_gate_up_dev): x [tokens, n_embd] to act [tokens, top_k, n_ff].
+    Expert tensors are uint8, [n_experts][n_ff] rows of blocks."""
+    if activation not in ("silu", "gelu"):
+        raise ValueError(f"activation must be silu or gelu, not {activation!r}")
+    m, n, k, f = plan.tokens(), plan.n_embd, plan.top_k, plan.n_ff
+    _dense(x, m * n, f"x [tokens, {n}]")
+    wg = _expert_weights(w_gate, qtype, plan.n_experts, f, n, "w_gate")
+    wu = _expert_weights(w_up, qtype, plan.n_experts, f, n, "w_up")
+    act = x.new_empty((m, k, f)) if act is None else _dense(act, m * k * f, "act")
+    _HIP.check(_HIP.moe_gate_up_dev(act.data_ptr(), x.data_ptr(), plan._h, wg, wu, qtype,
+                                    _expert_bias(b_gate, plan.n_experts, f, "b_gate"),
+                                    _expert_bias(b_up, plan.n_experts, f, "b_up"), int(activation == "gelu"),
+                                    _stream()), "moe_gate_up")
+    return act
+
+
+def moe_down(plan: MoePlan, w_down, qtype: int, act, bias=None, residual=None, out=None):
+    """The weighted sum of each token's experts' down projections, and the residual
+    (edgexpu_hip_moe_down_dev): act [tokens, top_k, n_ff] to out [tokens, n_embd]."""
+    m, n, k, f = plan.tokens(), plan.n_embd, plan.top_k, plan.n_ff
+    _dense(act, m * k * f, f"act [tokens, {k}, {f}]")
+    w = _expert_weights(w_down, qtype, plan.n_experts, n, f, "w_down")
+    out = act.new_empty((m, n)) if out is None else _dense(out, m * n, "out")
+    if residual is not None:
+        _dense(residual, m * n, "residual")
+    _HIP.check(_HIP.moe_down_dev(out.data_ptr(), act.data_ptr(), plan._h, w, qtype,
+                                 _expert_bias(bias, plan.n_experts, n, "bias"), _ptr(residual), _stream()), "moe_down")
     return out
 
 

@@ -481,6 +481,78 @@ int edgexpu_hip_kv_append_dev(float *q_out, const float *q, long long ldq, const
  * included.  scale: finite (else error -2). */
 int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip_batch *b, int layer, float scale, void *stream);
 
+/* ---- a feed-forward of experts (no reference counterpart: its layers are dense) ----
+ * What takes the place of gate / up / down where a layer's tensors hold n_experts
+ * matrices each and a token goes through top_k of them.  A layer's step is
+ *   edgexpu_hip_moe_route_dev (each token's experts and their weights, from the
+ *   router's scores: a projection of the normed activations with n_experts rows),
+ *   edgexpu_hip_moe_gate_up_dev, edgexpu_hip_moe_down_dev.
+ * An expert tensor is [n_experts][rows][blocks] as GGUF holds it (ffn_gate_exps,
+ * ffn_up_exps: n_ff rows of n_embd; ffn_down_exps: n_embd rows of n_ff), type Q4_0,
+ * Q5_0, Q8_0, Q4_K, Q5_K or Q6_K (any other: error -3), at a 16-byte address;
+ * biases are [n_experts][rows] f32.  Products are those of
+ * edgexpu_hip_linear_quant_batch_dev: the activation quantized once to Q8_0 or Q8_K
+ * blocks, block integers exact, sums in f32 in an order that the call's sizes fix
+ * (the same call gives the same words).
+ * The plan holds the routing of the last edgexpu_hip_moe_route_dev or
+ * edgexpu_hip_moe_assign_dev and the workspaces of the products; all device memory
+ * is taken by _create, so every other call can be captured into a graph.  Work on one
+ * plan goes to one stream, or to streams that the caller orders, and is queued by one
+ * host thread at a time.  A captured product computes as many tokens as the routing
+ * had when it was captured: replay it after a routing of as many.  What a captured
+ * call was given lives as long as its graph.  All run on the device of
+ * edgexpu_hip_init (another current device: error -4). */
+typedef struct edgexpu_hip_moe edgexpu_hip_moe;
+/* n_experts at most 512; top_k at most n_experts and 32; n_embd and n_ff at most
+ * 2^20; max_tokens * top_k at most 2^22.  The device memory is about
+ * 5 max_tokens top_k n_embd + 1.2 (max_tokens + 16 n_experts) top_k max(n_embd, n_ff)
+ * bytes at most.  NULL on error. */
+edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens, int n_embd, int n_ff);
+/* Waits for the device, then frees. */
+void edgexpu_hip_moe_destroy(edgexpu_hip_moe *p);
+/* Tokens of the last routing; 0 before one. */
+int edgexpu_hip_moe_tokens(const edgexpu_hip_moe *p);
+
+/* Chooses top_k experts for each of m tokens (0 to max_tokens) by scores
+ * [m][n_experts], in 64 bits:
+ *   p = softmax(scores[t]) (EDGEXPU_HIP_MOE_SOFTMAX) or 1 / (1 + exp(-scores[t]))
+ *   c = p + bias (n_experts values, a bias for balance; NULL: c = p)
+ * A score that is not finite masks its expert, which has no share in the softmax and
+ * is not chosen, nor is one whose c is not finite.  With n_groups > 1 (at most 64,
+ * a divisor of n_experts) the experts are that many equal runs; a run ranks by the
+ * sum of its group_best (1 or 2) largest c, and those of the top_groups highest stay.
+ * The top_k largest c of what stays are chosen, in descending order; ties go to
+ * the lowest index, here and among runs.  A chosen expert's weight is p, with
+ * `normalise` divided by the sum of the chosen p (where that is not zero), times
+ * scale, rounded once.  Places left over get id -1 and weight 0.
+ * ids [m][top_k] int32 and weights [m][top_k] f32 (either may be NULL) receive
+ * copies of what the plan holds. */
+#define EDGEXPU_HIP_MOE_SOFTMAX 0
+#define EDGEXPU_HIP_MOE_SIGMOID 1
+int edgexpu_hip_moe_route_dev(edgexpu_hip_moe *p, int32_t *ids, float *weights, const float *scores, int m, int score,
+                              const float *bias, int n_groups, int top_groups, int group_best, int normalise,
+                              double scale, void *stream);
+/* The caller's own choices instead: ids and weights [m][top_k].  An id outside
+ * [0, n_experts) is no expert (as -1 above); a token may name an expert twice. */
+int edgexpu_hip_moe_assign_dev(edgexpu_hip_moe *p, const int32_t *ids, const float *weights, int m, void *stream);
+
+/* For the routing's m tokens and each of their experts e = ids[t][j]:
+ *   act[t][j] = f(b_gate[e] + W_gate[e] . q8(x[t])) * (b_up[e] + W_up[e] . q8(x[t]))
+ * x [m][n_embd], act [m][top_k][n_ff], 16-byte aligned, not overlapping; biases may
+ * be NULL (either alone too).  f(v): EDGEXPU_HIP_MOE_SILU v / (1 + exp(-v)),
+ * EDGEXPU_HIP_MOE_GELU v / (1 + exp(-2 sqrt(2 / pi) (v + 0.044715 v^3))), the tanh
+ * form.  A place without an expert is zeros.  n_embd a multiple of the type's block. */
+#define EDGEXPU_HIP_MOE_SILU 0
+#define EDGEXPU_HIP_MOE_GELU 1
+int edgexpu_hip_moe_gate_up_dev(float *act, const float *x, edgexpu_hip_moe *p, const void *w_gate, const void *w_up,
+                                uint32_t type, const float *b_gate, const float *b_up, int activation, void *stream);
+/* out[t] = [residual[t] +] sum_j weights[t][j] (bias[e] + W[e] . q8(act[t][j])) over
+ * the places with an expert, summed in order of j; out [m][n_embd], which may be
+ * residual and overlaps nothing else; act and out 16-byte aligned.  bias and residual
+ * may be NULL.  n_ff a multiple of the type's block. */
+int edgexpu_hip_moe_down_dev(float *out, const float *act, edgexpu_hip_moe *p, const void *w_down, uint32_t type,
+                             const float *bias, const float *residual, void *stream);
+
 /* ---- host-pointer entry points (synchronous: inputs copied in, outputs
  * copied out before return; the PCIe copies are part of the call) ---- */
 

@@ -1,0 +1,56 @@
+"""Arguments that the experts' entry points refuse before they touch a device."""
+import numpy as np
+import pytest
+
+import edgexpu_amd as E
+import moe_plain as P
+
+
+@pytest.fixture
+def lib():
+    L = E.HipLib()
+    L.clear_error()
+    yield L
+    L.clear_error()
+
+
+def refused(L, got, code, word):
+    assert not got
+    c, msg = L.last_error()
+    L.clear_error()
+    assert c == code and word in msg, (c, msg)
+
+
+@pytest.mark.parametrize("args", [
+    (0, 1, 1, 256, 256), (513, 1, 1, 256, 256), (8, 0, 1, 256, 256), (8, 9, 1, 256, 256), (64, 33, 1, 256, 256),
+    (8, 2, 0, 256, 256), (8, 2, 2**21 + 1, 256, 256), (8, 2, -1, 256, 256), (8, 2, 1, 0, 256), (8, 2, 1, 256, 0),
+    (8, 2, 1, 2**20 + 32, 256), (8, 2, 1, 256, 2**20 + 32), (2**31 - 1, 2, 1, 256, 256), (8, 2, 2**31 - 1, 256, 256)])
+def test_create(lib, args):
+    refused(lib, lib.moe_create(*args), -2, "moe_create")
+
+
+def test_null_plan(lib):
+    p = 0x1000  # (refused before anything reads it)
+    refused(lib, lib.moe_route_dev(None, p, p, p, 1, 0, None, 1, 1, 1, 1, 1.0, None), -2, "moe_route")
+    refused(lib, lib.moe_assign_dev(None, p, p, 1, None), -2, "moe_assign")
+    refused(lib, lib.moe_gate_up_dev(p, p, None, p, p, E.Q4_K, None, None, 0, None), -2, "moe_gate_up")
+    refused(lib, lib.moe_gate_up_dev(p, p, None, p, p, E.Q4_K, None, None, 2, None), -2, "activation 2")
+    refused(lib, lib.moe_down_dev(p, p, None, p, E.Q4_K, None, None, None), -2, "moe_down")
+    assert lib.moe_tokens(None) == 0
+    lib.moe_destroy(None)
+    assert lib.last_error()[0] == 0
+
+
+def test_the_plain_route():
+    """The plain form against counts by hand."""
+    s = np.array([[0.0, 1.0, 1.0, -np.inf], [np.nan, 2.0, np.inf, 2.0], [-np.inf] * 4, [5.0, 5.0, 5.0, 5.0]], np.float32)
+    ids, w = P.route(s, 3, normalise=False)
+    z = 1 + 2 * np.e
+    assert ids.tolist() == [[1, 2, 0], [1, 3, -1], [-1, -1, -1], [0, 1, 2]]
+    assert np.allclose(w, [[np.e / z, np.e / z, 1 / z], [0.5, 0.5, 0], [0, 0, 0], [0.25] * 3])
+    ids, w = P.route(s[:1], 2, score="sigmoid", bias=np.array([0, 0, -5, 9], np.float32), scale=2.0)
+    assert ids.tolist() == [[1, 0]] and abs(w.sum() - 2) < 1e-12
+    # the second run's two best sum to more than the first run's single best
+    s = np.array([[4.0, -9.0, 3.0, 2.9]], np.float32)
+    assert P.route(s, 1, "sigmoid", n_groups=2, top_groups=1, best=1)[0].tolist() == [[0]]
+    assert P.route(s, 1, "sigmoid", n_groups=2, top_groups=1, best=2)[0].tolist() == [[2]]
