@@ -7,20 +7,35 @@
 #include "common.h"
 #include "edgexpu_hip.h"
 
+namespace exq {
+
+constexpr int kMoeMaxExperts = 512, kMoeMaxTopK = 32, kMoeMaxGroups = 64;
+
+// A tile: `count` places from `start` of the sorted pairs, all of one expert.
+// Expert e's tiles begin at slot start_e / T + e (T places a tile): the next
+// expert's are then past them whatever the counts, so no expert needs to know the
+// others' tile counts.  Slots in between have count 0.
+struct MoeTile {
+    int expert, start, count, pad;
+};
+
+}  // namespace exq
+
 struct edgexpu_hip_moe {
     int n_experts = 0, top_k = 0, max_tokens = 0, n_embd = 0, n_ff = 0;
-    int m = -1;  // tokens of the last routing (-1: none yet)
+    int m = -1;     // tokens of the last routing (-1: none yet)
+    int tile = 0;   // places a tile of its sorted pairs; 0: not sorted
     uint8_t *mem = nullptr;
     int32_t *ids = nullptr;  // [max_tokens][top_k], -1: no expert
     float *weights = nullptr;
-    uint8_t *xq = nullptr;  // quantized activations of the product at hand
-    float *part = nullptr;  // [max_tokens][top_k][n_embd]: a token's parts of the down product
+    int32_t *order = nullptr;       // pairs (token * top_k + place) by expert, then by number
+    exq::MoeTile *tiles = nullptr;
+    uint8_t *pack = nullptr;        // quantized activations of the product at hand
+    float *part = nullptr;          // [max_tokens][top_k][n_embd]: a token's parts of the down product
     size_t pairs() const { return (size_t)(m > 0 ? m : 0) * top_k; }
 };
 
 namespace exq {
-
-constexpr int kMoeMaxExperts = 512, kMoeMaxTopK = 32, kMoeMaxGroups = 64;
 
 struct RouteArgs {
     const float *scores, *bias;
@@ -33,5 +48,9 @@ struct RouteArgs {
 hipError_t launch_moe_route(const RouteArgs &a, hipStream_t st);
 hipError_t launch_moe_assign(const int32_t *ids, const float *weights, int32_t *to_ids, float *to_weights, int pairs,
                              int n_experts, hipStream_t st);
+// Sorts the pairs by expert into tiles of T places; moe_slots(pairs, n_experts, T) slots are written.
+hipError_t launch_moe_sort(const int32_t *ids, int pairs, int n_experts, int T, int32_t *order, MoeTile *tiles,
+                           hipStream_t st);
+inline int moe_slots(long long pairs, int n_experts, int T) { return (int)(pairs / T) + n_experts; }
 
 }  // namespace exq

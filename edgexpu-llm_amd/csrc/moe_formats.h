@@ -1,0 +1,559 @@
+// Weight rows of each format as operands of the integer matrix cores, for the
+// products with routed experts, and the packed activation they meet.
+//
+// A step of every product is a group of 256 elements of 16 weight rows against
+// 16 tokens.  Operands of v_mfma_i32_16x16x64_i8: lane l supplies row l % 16 of A
+// (a weight row) and column l % 16 of B (a token), 16 bytes of group g = l / 16;
+// the 64 places of K may be any 64 elements as long as A and B agree.
+// Accumulator register r of lane l is C[4 g + r][l % 16] = C[row][token].
+//
+// K-quants: sum_j sc_j sum_i q_i x_i over the sub-blocks j of a group has to be
+// exact.  One product a sub-block, its sum times sc_j on the VALU, costs 8 (Q6_K:
+// 16, K = 32 holding two) multiply-adds for each of a lane's 4 sums, more
+// than the matrix cores' own time.  Here the scale goes into the operand instead:
+// sc is cut into digits of base 8, sc = s0 + 8 s1 (+ 64 s2), and q * s fits 8 bits,
+// so 4 products a digit sum a whole group and
+//   sum = S0 + 8 S1 (+ 64 S2)
+// costs one shift-add a digit.  q * s is one 16-bit packed product for four codes
+// (each byte's product stays below 256, so none carries into the next):
+//   Q4_K  15 * 7 = 105;  Q5_K  31 * 7 = 217, which is s8 - 128 with its top bit
+//   turned, and 128 (1 + 8) sum x is added back;  Q6_K has signed scales and codes
+//   of 6 bits, digits -3 .. 4 and the code less 32: -128 .. 124, even and odd codes
+//   apart.
+// The minima's sum, sum_j m_j sum_(i in j) x_i, is one product of f16 (integers
+// below 2^11, exact, as is the sum below 2^24) with the tokens' 16-element sums.
+//
+// Blocks of 32 with one f16 scale (Q8_0, Q4_0, Q5_0): v_mfma_i32_16x16x32_i8 a
+// block, then acc += S * (dw dx).
+//
+// Packed activation: a record of kMoeRec bytes for a token's group:
+//   K-quants  int8 codes[256] | f16 sums of 16 elements [16] | f32 dx | i32 sum of all
+//   others    int8 codes[256] | f32 dx[8] (a last group's missing blocks are zeros)
+// 304 bytes: 16-byte aligned, and 8 records apart by 48 (mod 128), so that 16 lanes
+// reading one place of 16 records from LDS meet no bank twice.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "common.h"
+#include "formats.h"
+#include "q8k.h"
+
+namespace exq {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kMoeRec = 304, kMoeBs = 256, kMoeDx = 288, kMoeSum = 292;
+
+__device__ __forceinline__ v4i mfma64(v4i a, v4i b, v4i c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ v4i mfma32(long a, long b) {
+    return __builtin_amdgcn_mfma_i32_16x16x32_i8(a, b, v4i{0, 0, 0, 0}, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mfma_f16(v4h a, v4h b) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+}
+__device__ __forceinline__ long two_words(uint32_t lo, uint32_t hi) {
+    return (long)((uint64_t)lo | ((uint64_t)hi << 32));
+}
+__device__ __forceinline__ uint32_t mul_u16x2(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, a) * __builtin_bit_cast(u16x2, b));
+}
+__device__ __forceinline__ uint32_t twice(uint32_t v) { return (v & 0xffffu) | (v << 16); }
+__device__ __forceinline__ v4i as_v4i(const uint4 &v) { return v4i{(int)v.x, (int)v.y, (int)v.z, (int)v.w}; }
+
+// ------------------------------------------------------------- activations
+
+// A token's group of a K-quant product as the operand (lane: token l % 16, group g).
+struct MoeXK {
+    v4i c[4];
+    v4h bs;
+    float dx;
+    int sum;
+};
+// ... of a product of 32-element blocks.
+struct MoeX0 {
+    long c[8];
+    float dx[8];
+};
+
+// 16 lanes of a DPP row quantize 256 elements and write their record.  Lane 4 j + q
+// holds elements 64 j + 8 q .. + 7 and 64 j + 32 + 8 q .. + 7 in xs.
+__device__ __forceinline__ void moe_pack_k(const float (&xs)[16], int r, uint8_t *rec) {
+    const int j = r >> 2, q = r & 3;
+    int qv[16];
+    const Q8KRow16 k = q8k_quantize_row16(xs, qv);
+    uint32_t w[4];
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = (uint32_t)(qv[4 * i] & 0xff) | ((uint32_t)(qv[4 * i + 1] & 0xff) << 8) |
+               ((uint32_t)(qv[4 * i + 2] & 0xff) << 16) | ((uint32_t)qv[4 * i + 3] << 24);
+        sum += (qv[4 * i] + qv[4 * i + 1]) + (qv[4 * i + 2] + qv[4 * i + 3]);
+    }
+    sum += (int)dpp_u32<kDppXor1>((uint32_t)sum);
+    sum += (int)dpp_u32<kDppXor2>((uint32_t)sum);
+    sum += (int)dpp_u32<kDppHalfMirror>((uint32_t)sum);
+    sum += (int)dpp_u32<kDppMirror>((uint32_t)sum);
+    *reinterpret_cast<uint2 *>(rec + 64 * j + 8 * q) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2 *>(rec + 64 * j + 32 + 8 * q) = make_uint2(w[2], w[3]);
+    if (q == 0) {
+        const v4h b = {(_Float16)(float)k.lo, (_Float16)(float)k.lo_next, (_Float16)(float)k.hi,
+                       (_Float16)(float)k.hi_next};
+        *reinterpret_cast<v4h *>(rec + kMoeBs + 8 * j) = b;
+    }
+    if (r == 0) {
+        *reinterpret_cast<float *>(rec + kMoeDx) = k.d;
+        *reinterpret_cast<int *>(rec + kMoeSum) = sum;
+    }
+}
+
+// 4 lanes quantize a block of 32 as quantize_q8_0_kernel does, lane g its elements
+// 8 g .. + 7, and write them to block b (0..7) of the record.
+__device__ __forceinline__ void moe_pack_0(const float (&a)[8], int b, int g, uint8_t *rec) {
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(a[i]));
+    amax = fmaxf(amax, __uint_as_float(dpp_u32<kDppXor1>(__float_as_uint(amax))));
+    amax = fmaxf(amax, __uint_as_float(dpp_u32<kDppXor2>(__float_as_uint(amax))));
+    const float id = amax != 0.0f ? 127.0f / amax : 0.0f;
+    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = rintf(a[i] * id);
+        const int k = (v >= -2147483648.0f && v < 2147483648.0f) ? (int)v : INT32_MIN;
+        const int c = k < -128 ? -128 : (k > 127 ? 127 : k);
+        w[i >> 2] |= (uint32_t)(c & 0xff) << (8 * (i & 3));
+    }
+    *reinterpret_cast<uint2 *>(rec + 32 * b + 8 * g) = make_uint2(w[0], w[1]);
+    if (g == 0) *reinterpret_cast<float *>(rec + kMoeBs + 4 * b) = f16_bits_to_f32(f32_to_f16_rne(amax / 127.0f));
+}
+
+__device__ __forceinline__ void load_f8(const float *p, float (&v)[16], int at) {
+    const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+    v[at] = a.x, v[at + 1] = a.y, v[at + 2] = a.z, v[at + 3] = a.w;
+    v[at + 4] = b.x, v[at + 5] = b.y, v[at + 6] = b.z, v[at + 7] = b.w;
+}
+
+// Part `part` of a row's packing: K-quants 16 lanes a group of 256, others 32 lanes
+// (4 a block).  x is the row, rec its first record, n its elements.
+template <bool K>
+__device__ __forceinline__ void moe_pack_part(const float *x, int n, int part, uint8_t *rec) {
+    if (K) {
+        const int sb = part >> 4, r = part & 15;
+        float xs[16];
+        const float *p = x + (size_t)sb * kQKK + 64 * (r >> 2) + 8 * (r & 3);
+        load_f8(p, xs, 0);
+        load_f8(p + 32, xs, 8);
+        moe_pack_k(xs, r, rec + (size_t)sb * kMoeRec);
+    } else {
+        const int blk = part >> 2, g = part & 3;
+        float v[16] = {0.0f};
+        if (blk * 32 < n) load_f8(x + (size_t)blk * 32 + 8 * g, v, 0);
+        const float a[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+        moe_pack_0(a, blk & 7, g, rec + (size_t)(blk >> 3) * kMoeRec);
+    }
+}
+__host__ __device__ constexpr int moe_groups(int n) { return (n + kQKK - 1) / kQKK; }
+template <bool K>
+__host__ __device__ constexpr int moe_pack_parts(int n) {
+    return moe_groups(n) * (K ? 16 : 32);
+}
+
+// ---------------------------------------------------------------- K-quants
+//
+// W: raw registers of a group of the lane's row; Op: the operand; chunk(s, g): which
+// 16 elements of the group lane group g holds in product s of 4.
+
+// The sum over the digits' products, as f32 for the block's scale.
+template <class F>
+__device__ __forceinline__ void moe_dot_k(float (&acc)[4], const typename F::Op &o, const MoeXK &x,
+                                          const float (&d)[4], const float (&nd)[4]) {
+    v4i s[F::kDigits];
+#pragma unroll
+    for (int k = 0; k < F::kDigits; ++k) s[k] = v4i{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < F::kDigits; ++k) s[k] = mfma64(o.a[k][i], x.c[i], s[k]);
+    v4f mn;
+    if (F::kMin) mn = mfma_f16(o.mn, x.bs);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        int t = s[F::kDigits - 1][r];
+#pragma unroll
+        for (int k = F::kDigits - 2; k >= 0; --k) t = (t << 3) + s[k][r];
+        if (F::kTurned) t += 1152 * x.sum;
+        float v = (float)t * d[r];
+        if (F::kMin) v = __builtin_fmaf(mn[r], nd[r], v);
+        acc[r] = __builtin_fmaf(v, x.dx, acc[r]);
+    }
+}
+
+template <class F>
+__device__ __forceinline__ void moe_load_xk(MoeXK &x, const uint8_t *rec, int g) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) x.c[s] = as_v4i(*reinterpret_cast<const uint4 *>(rec + 16 * F::chunk(s, g)));
+    x.bs = *reinterpret_cast<const v4h *>(rec + kMoeBs + 8 * g);
+    const uint2 e = *reinterpret_cast<const uint2 *>(rec + kMoeDx);
+    x.dx = __uint_as_float(e.x);
+    x.sum = (int)e.y;
+}
+
+// d and -dmin of the rows 4 g + r, which the lane's sums belong to, from the word
+// (d, dmin) that lane r16 of each group holds for its row.
+__device__ __forceinline__ void moe_row_scales(uint32_t own, int g, float (&d)[4], float (&nd)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const uint32_t v = (uint32_t)__shfl((int)own, 4 * g + r, 64);
+        d[r] = f16_bits_to_f32(v & 0xffffu);
+        nd[r] = -f16_bits_to_f32(v >> 16);
+    }
+}
+
+// The six-bit scales and minima of get_scale_min_k4 (src/gguf_quant.c:212-220), four a word.
+struct SixBits {
+    uint32_t s[2], m[2];
+};
+__device__ __forceinline__ SixBits six_bits(const uint4 &hd) {
+    SixBits b;
+    b.s[0] = hd.y & 0x3f3f3f3fu;
+    b.s[1] = (hd.w & 0x0f0f0f0fu) | ((hd.y >> 2) & 0x30303030u);
+    b.m[0] = hd.z & 0x3f3f3f3fu;
+    b.m[1] = ((hd.w >> 4) & 0x0f0f0f0fu) | ((hd.z >> 2) & 0x30303030u);
+    return b;
+}
+// Minima of lane group g's four 16-element sums.
+__device__ __forceinline__ v4h min_operand(const SixBits &b, int g) {
+    const uint32_t mm = ((g & 2) ? b.m[1] : b.m[0]) >> (16 * (g & 1));
+    const _Float16 x = (_Float16)(float)(mm & 0xffu), y = (_Float16)(float)((mm >> 8) & 0xffu);
+    return v4h{x, x, y, y};
+}
+
+struct MoeQ4K {
+    static constexpr bool kK = true, kMin = true, kTurned = false;
+    static constexpr int kType = kTypeQ4_K, kDigits = 2, kBytes = kBytesQ4_K;
+    struct W {
+        uint4 hd, q[2];
+    };
+    struct Op {
+        v4i a[2][4];
+        v4h mn;
+        uint32_t dm;
+    };
+    typedef MoeXK X;
+    __device__ static constexpr int chunk(int s, int g) { return 8 * (s >> 1) + 4 * (g >> 1) + 2 * (s & 1) + (g & 1); }
+    __device__ static __forceinline__ void load_w(W &w, const uint8_t *row, int u, int, int g) {
+        const uint8_t *p = row + (size_t)u * kBytes;
+        w.hd = *reinterpret_cast<const uint4 *>(p);
+        w.q[0] = *reinterpret_cast<const uint4 *>(p + 16 + 16 * g);
+        w.q[1] = *reinterpret_cast<const uint4 *>(p + 80 + 16 * g);
+    }
+    __device__ static __forceinline__ void decode(Op &o, const W &w, int g) {
+        const SixBits b = six_bits(w.hd);
+        o.mn = min_operand(b, g);
+        o.dm = w.hd.x;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t two = b.s[i] >> (16 * (g >> 1));  // the chunk's two scales
+            const uint32_t q[4] = {w.q[i].x, w.q[i].y, w.q[i].z, w.q[i].w};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t sc = (two >> (8 * h)) & 0xffu;
+                const uint32_t s0 = twice(sc & 7u), s1 = twice(sc >> 3);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const uint32_t c = (q[v] >> (4 * h)) & 0x0f0f0f0fu;
+                    o.a[0][2 * i + h][v] = (int)mul_u16x2(c, s0);
+                    o.a[1][2 * i + h][v] = (int)mul_u16x2(c, s1);
+                }
+            }
+        }
+    }
+};
+
+struct MoeQ5K {
+    static constexpr bool kK = true, kMin = true, kTurned = true;
+    static constexpr int kType = kTypeQ5_K, kDigits = 2, kBytes = kBytesQ5_K;
+    struct W {
+        uint4 hd, h, q[2];
+    };
+    typedef MoeQ4K::Op Op;
+    typedef MoeXK X;
+    __device__ static constexpr int chunk(int s, int g) { return MoeQ4K::chunk(s, g); }
+    __device__ static __forceinline__ void load_w(W &w, const uint8_t *row, int u, int, int g) {
+        const uint8_t *p = row + (size_t)u * kBytes;
+        w.hd = *reinterpret_cast<const uint4 *>(p);
+        w.h = *reinterpret_cast<const uint4 *>(p + 16 + 16 * (g & 1));
+        w.q[0] = *reinterpret_cast<const uint4 *>(p + 48 + 16 * g);
+        w.q[1] = *reinterpret_cast<const uint4 *>(p + 112 + 16 * g);
+    }
+    __device__ static __forceinline__ void decode(Op &o, const W &w, int g) {
+        const SixBits b = six_bits(w.hd);
+        o.mn = min_operand(b, g);
+        o.dm = w.hd.x;
+        const uint32_t fifth[4] = {w.h.x, w.h.y, w.h.z, w.h.w};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t two = b.s[i] >> (16 * (g >> 1));
+            const uint32_t q[4] = {w.q[i].x, w.q[i].y, w.q[i].z, w.q[i].w};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t sc = (two >> (8 * h)) & 0xffu;
+                const uint32_t s0 = twice(sc & 7u), s1 = twice(sc >> 3);
+                const int bit = 4 * i + 2 * (g >> 1) + h;  // of the 64-element chunk 2 i + g / 2, half h
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const uint32_t c = ((q[v] >> (4 * h)) & 0x0f0f0f0fu) | (((fifth[v] >> bit) & 0x01010101u) << 4);
+                    o.a[0][2 * i + h][v] = (int)(mul_u16x2(c, s0) ^ 0x80808080u);
+                    o.a[1][2 * i + h][v] = (int)(mul_u16x2(c, s1) ^ 0x80808080u);
+                }
+            }
+        }
+    }
+};
+
+// Blocks start at even addresses: words are read from the 4-byte address below and
+// joined by byte shifts (ldg16_a2).
+struct MoeQ6K {
+    static constexpr bool kK = true, kMin = false, kTurned = false;
+    static constexpr int kType = kTypeQ6_K, kDigits = 3, kBytes = kBytesQ6_K;
+    struct W {
+        uint4 l[2], h[2];
+        uint32_t sc;  // scales g, 4 + g, 8 + g, 12 + g
+        uint32_t d;
+    };
+    struct Op {
+        v4i a[3][4];
+        v4h mn;
+        uint32_t dm;
+    };
+    typedef MoeXK X;
+    __device__ static constexpr int chunk(int s, int g) { return 4 * s + g; }
+    __device__ static __forceinline__ void load_w(W &w, const uint8_t *row, int u, int, int g) {
+        const uint8_t *p = row + (size_t)u * kBytes;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            w.l[i] = ldg16_a2(p + 64 * i + 16 * g);
+            w.h[i] = ldg16_a2(p + 128 + 32 * i + 16 * (g & 1));
+        }
+        w.sc = (uint32_t)p[192 + g] | ((uint32_t)p[196 + g] << 8) | ((uint32_t)p[200 + g] << 16) |
+               ((uint32_t)p[204 + g] << 24);
+        w.d = *reinterpret_cast<const uint16_t *>(p + 208);
+    }
+    __device__ static __forceinline__ void decode(Op &o, const W &w, int g) {
+        o.dm = w.d;
+        o.mn = v4h{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t l[4] = {w.l[i].x, w.l[i].y, w.l[i].z, w.l[i].w};
+            const uint32_t hh[4] = {w.h[i].x, w.h[i].y, w.h[i].z, w.h[i].w};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int sc = (int)(int8_t)((w.sc >> (8 * (2 * i + h))) & 0xffu);
+                const int s0 = ((sc + 3) & 7) - 3, r1 = (sc - s0) >> 3, s1 = ((r1 + 3) & 7) - 3, s2 = (r1 - s1) >> 3;
+                const int dig[3] = {s0, s1, s2};
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    // this half's two high bits are bits 2 (g / 2) + 4 h of each byte
+                    const uint32_t top = (hh[v] >> (2 * (g >> 1) + 4 * h)) & 0x03030303u;
+                    const uint32_t c = ((l[v] >> (4 * h)) & 0x0f0f0f0fu) | (top << 4);
+                    const i16x2 even = __builtin_bit_cast(i16x2, c & 0x00ff00ffu) - (short)32;
+                    const i16x2 odd = __builtin_bit_cast(i16x2, (c >> 8) & 0x00ff00ffu) - (short)32;
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) {
+                        const short s = (short)dig[k];
+                        o.a[k][2 * i + h][v] = (int)__builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, odd * s),
+                                                                          __builtin_bit_cast(uint32_t, even * s),
+                                                                          0x06020400u);
+                    }
+                }
+            }
+        }
+    }
+};
+
+// ------------------------------------------------------- blocks of 32 elements
+//
+// A row of n blocks; those past the end of a last group are not read (their
+// codes and scales are zeros).
+
+// Scales of the rows 4 g + r for the group's 8 blocks, from the word (blocks g, g + 4)
+// that lane r16 of group g holds for its row.
+__device__ __forceinline__ void moe_block_scales(uint32_t own, int g, float (&d)[8][4]) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t v = (uint32_t)__shfl((int)own, 16 * b + 4 * g + r, 64);
+            d[b][r] = f16_bits_to_f32(v & 0xffffu);
+            d[b + 4][r] = f16_bits_to_f32(v >> 16);
+        }
+}
+
+struct MoeOp0 {
+    long a[8];
+    uint32_t dm;
+};
+
+__device__ __forceinline__ void moe_dot_0(float (&acc)[4], const MoeOp0 &o, const MoeX0 &x, const float (&d)[8][4]) {
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        const v4i s = mfma32(o.a[b], x.c[b]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf((float)s[r], d[b][r] * x.dx[b], acc[r]);
+    }
+}
+
+template <class F>
+__device__ __forceinline__ void moe_load_x0(MoeX0 &x, const uint8_t *rec, int g) {
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        const uint2 v = F::kQ80 ? *reinterpret_cast<const uint2 *>(rec + 32 * b + 8 * (((g & 1) << 1) | (g >> 1)))
+                                : make_uint2(*reinterpret_cast<const uint32_t *>(rec + 32 * b + 4 * g),
+                                             *reinterpret_cast<const uint32_t *>(rec + 32 * b + 16 + 4 * g));
+        x.c[b] = two_words(v.x, v.y);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float4 d = *reinterpret_cast<const float4 *>(rec + kMoeBs + 16 * i);
+        x.dx[4 * i] = d.x, x.dx[4 * i + 1] = d.y, x.dx[4 * i + 2] = d.z, x.dx[4 * i + 3] = d.w;
+    }
+}
+
+// Scales of blocks g and g + 4 of group u.
+template <int BYTES>
+__device__ __forceinline__ uint32_t load_scales(const uint8_t *row, int u, int n, int g) {
+    const int b0 = 8 * u + g, b1 = b0 + 4;
+    const uint32_t lo = b0 < n ? *reinterpret_cast<const uint16_t *>(row + (size_t)b0 * BYTES) : 0u;
+    const uint32_t hi = b1 < n ? *reinterpret_cast<const uint16_t *>(row + (size_t)b1 * BYTES) : 0u;
+    return lo | (hi << 16);
+}
+
+// Lane groups 0 and 1 read the halves of a pair's even block, 2 and 3 those of the
+// odd one; v_permlane32_swap then leaves group g with the 8-byte piece {0, 2, 1, 3}[g] of
+// either block.
+struct MoeQ80 {
+    static constexpr bool kK = false, kQ80 = true;
+    static constexpr int kType = kTypeQ8_0, kBytes = kBytesQ8_0;
+    struct W {
+        uint4 q[4];
+        uint32_t d;
+    };
+    typedef MoeOp0 Op;
+    typedef MoeX0 X;
+    __device__ static __forceinline__ void load_w(W &w, const uint8_t *row, int u, int n, int g) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int b = 8 * u + 2 * i + (g >> 1);
+            w.q[i] = ldg16_a2(row + (size_t)min(b, n - 1) * kBytes + 2 + 16 * (g & 1));
+        }
+        w.d = load_scales<kBytes>(row, u, n, g);
+    }
+    __device__ static __forceinline__ void decode(Op &o, const W &w, int) {
+        o.dm = w.d;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const auto x = __builtin_amdgcn_permlane32_swap(w.q[i].x, w.q[i].z, false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(w.q[i].y, w.q[i].w, false, false);
+            o.a[2 * i] = two_words((uint32_t)x[0], (uint32_t)y[0]);
+            o.a[2 * i + 1] = two_words((uint32_t)x[1], (uint32_t)y[1]);
+        }
+    }
+};
+
+// Lane group g holds elements 4 g .. + 3 and 16 + 4 g .. + 3 of a block: the low and
+// high nibbles of one word of its codes, less 8 (Q5_0, with their fifth bits, less 16).
+__device__ __forceinline__ uint32_t less_each(uint32_t c, uint32_t bias) {
+    // (a code is below 128: 0x80 + c - bias borrows nothing, and its top bit turned is the sign)
+    return ((c | 0x80808080u) - bias) ^ 0x80808080u;
+}
+struct MoeQ40 {
+    static constexpr bool kK = false, kQ80 = false;
+    static constexpr int kType = kTypeQ4_0, kBytes = kBytesQ4_0;
+    struct W {
+        uint32_t q[8], d;
+    };
+    typedef MoeOp0 Op;
+    typedef MoeX0 X;
+    __device__ static __forceinline__ void load_w(W &w, const uint8_t *row, int u, int n, int g) {
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+            const uint8_t *p = row + (size_t)min(8 * u + b, n - 1) * kBytes + 2 + 4 * g;
+            w.q[b] = (uint32_t)*reinterpret_cast<const uint16_t *>(p) |
+                     ((uint32_t)*reinterpret_cast<const uint16_t *>(p + 2) << 16);
+        }
+        w.d = load_scales<kBytes>(row, u, n, g);
+    }
+    __device__ static __forceinline__ void decode(Op &o, const W &w, int) {
+        o.dm = w.d;
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+            o.a[b] = two_words(less_each(w.q[b] & 0x0f0f0f0fu, 0x08080808u),
+                               less_each((w.q[b] >> 4) & 0x0f0f0f0fu, 0x08080808u));
+    }
+};
+
+struct MoeQ50 {
+    static constexpr bool kK = false, kQ80 = false;
+    static constexpr int kType = kTypeQ5_0, kBytes = kBytesQ5_0;
+    struct W {
+        uint32_t q[8], h[8], d;
+    };
+    typedef MoeOp0 Op;
+    typedef MoeX0 X;
+    __device__ static __forceinline__ void load_w(W &w, const uint8_t *row, int u, int n, int g) {
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+            const uint8_t *p = row + (size_t)min(8 * u + b, n - 1) * kBytes;
+            w.h[b] = (uint32_t)*reinterpret_cast<const uint16_t *>(p + 2) |
+                     ((uint32_t)*reinterpret_cast<const uint16_t *>(p + 4) << 16);
+            w.q[b] = (uint32_t)*reinterpret_cast<const uint16_t *>(p + 6 + 4 * g) |
+                     ((uint32_t)*reinterpret_cast<const uint16_t *>(p + 8 + 4 * g) << 16);
+        }
+        w.d = load_scales<kBytes>(row, u, n, g);
+    }
+    __device__ static __forceinline__ void decode(Op &o, const W &w, int g) {
+        o.dm = w.d;
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+            const uint32_t lo = (w.q[b] & 0x0f0f0f0fu) | spread4_bit4((w.h[b] >> (4 * g)) & 15u);
+            const uint32_t hi = ((w.q[b] >> 4) & 0x0f0f0f0fu) | spread4_bit4((w.h[b] >> (16 + 4 * g)) & 15u);
+            o.a[b] = two_words(less_each(lo, 0x10101010u), less_each(hi, 0x10101010u));
+        }
+    }
+};
+
+// ------------------------------------------------------------------ both kinds
+
+// The rows' scales of a lane's sums.
+template <class F, bool K = F::kK>
+struct MoeScales {
+    float d[4], nd[4];
+    __device__ __forceinline__ void from(const typename F::Op &o, int g) { moe_row_scales(o.dm, g, d, nd); }
+    __device__ __forceinline__ void dot(float (&acc)[4], const typename F::Op &o, const MoeXK &x) const {
+        moe_dot_k<F>(acc, o, x, d, nd);
+    }
+};
+template <class F>
+struct MoeScales<F, false> {
+    float d[8][4];
+    __device__ __forceinline__ void from(const typename F::Op &o, int g) { moe_block_scales(o.dm, g, d); }
+    __device__ __forceinline__ void dot(float (&acc)[4], const typename F::Op &o, const MoeX0 &x) const {
+        moe_dot_0(acc, o, x, d);
+    }
+};
+template <class F>
+__device__ __forceinline__ void moe_load_x(typename F::X &x, const uint8_t *rec, int g) {
+    if constexpr (F::kK)
+        moe_load_xk<F>(x, rec, g);
+    else
+        moe_load_x0<F>(x, rec, g);
+}
+
+}  // namespace exq

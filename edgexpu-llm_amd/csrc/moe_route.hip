@@ -173,6 +173,81 @@ __global__ __launch_bounds__(256) void moe_assign_kernel(const int32_t *__restri
     to_weights[i] = some ? weights[i] : 0.0f;
 }
 
+// Pairs by expert: a workgroup an expert counts the pairs of the experts before its
+// own, then writes its own pairs in ascending order (so the sort is stable and the
+// same every time) and its tiles.  Every workgroup reads all ids, 4 bytes a pair from
+// L2, and none waits for another.
+constexpr int kSortThreads = 512, kSortEach = 8;
+__global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t *__restrict__ ids, int pairs,
+                                                                int n_experts, int T, int slots,
+                                                                int32_t *__restrict__ order,
+                                                                MoeTile *__restrict__ tiles) {
+    __shared__ int sums[2][kSortThreads / 64];
+    const int e = (int)blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int less = 0, own = 0;
+    for (int i = tid; i < pairs; i += kSortThreads) {
+        const int v = ids[i];
+        less += v >= 0 && v < e ? 1 : 0;
+        own += v == e ? 1 : 0;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        less += __shfl_xor(less, off, 64);
+        own += __shfl_xor(own, off, 64);
+    }
+    if (lane == 0) {
+        sums[0][wave] = less;
+        sums[1][wave] = own;
+    }
+    __syncthreads();
+    less = own = 0;
+#pragma unroll
+    for (int w = 0; w < kSortThreads / 64; ++w) {
+        less += sums[0][w];
+        own += sums[1][w];
+    }
+    const int slot0 = less / T + e, slot1 = e + 1 < n_experts ? (less + own) / T + e + 1 : slots;
+    for (int s = slot0 + tid; s < slot1; s += kSortThreads) {
+        const int at = (s - slot0) * T;
+        tiles[s] = MoeTile{e, less + at, max(0, min(T, own - at)), 0};
+    }
+    int base = less;
+    for (int i0 = 0; i0 < pairs && base < less + own; i0 += kSortThreads * kSortEach) {
+        const int first = i0 + tid * kSortEach;
+        unsigned hit = 0u;
+#pragma unroll
+        for (int k = 0; k < kSortEach; ++k)
+            if (first + k < pairs && ids[first + k] == e) hit |= 1u << k;
+        const int mine = __popc(hit);
+        int before = mine;  // inclusive over the wave, then over the waves
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int o = __shfl_up(before, off, 64);
+            if (lane >= off) before += o;
+        }
+        __syncthreads();  // (the sums of the round before have been read)
+        if (lane == 63) sums[0][wave] = before;
+        __syncthreads();
+        int at = base + before - mine, total = 0;
+#pragma unroll
+        for (int w = 0; w < kSortThreads / 64; ++w) {
+            at += w < wave ? sums[0][w] : 0;
+            total += sums[0][w];
+        }
+#pragma unroll
+        for (int k = 0; k < kSortEach; ++k)
+            if ((hit >> k) & 1u) order[at++] = first + k;
+        base += total;
+    }
+}
+
+hipError_t launch_moe_sort(const int32_t *ids, int pairs, int n_experts, int T, int32_t *order, MoeTile *tiles,
+                           hipStream_t st) {
+    hipLaunchKernelGGL(moe_sort_kernel, dim3((unsigned)n_experts), dim3(kSortThreads), 0, st, ids, pairs, n_experts, T,
+                       moe_slots(pairs, n_experts, T), order, tiles);
+    return hipGetLastError();
+}
+
 hipError_t launch_moe_route(const RouteArgs &a, hipStream_t st) {
     const dim3 grid((unsigned)((a.m + kRouteWaves - 1) / kRouteWaves));
     hipLaunchKernelGGL(moe_route_kernel, grid, dim3(64 * kRouteWaves), 0, st, a);
