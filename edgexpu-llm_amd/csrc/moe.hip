@@ -169,14 +169,8 @@ __global__ __launch_bounds__(64 * kOneWaves) void moe_one_kernel(MoeArgs a) {
     }
 }
 
-// ------------------------------------------------------------------ few tokens an expert
+// ------------------------------------------------------------------ tiles of pairs
 //
-// A workgroup takes 16 rows (gate and up: of each; down: 32) for a tile of up to 16
-// TT pairs of one expert; its waves share the groups out, weights straight into
-// registers a group ahead, tokens' records from L2, and add their sums in LDS in wave
-// order.
-constexpr int kFewWaves = 8;
-
 // Rows o .. o + 3 of a pair.
 __device__ __forceinline__ void store_rows(float *out, int rows, size_t pair, int o, const float (&v)[4]) {
     float *p = out + pair * rows + o;
@@ -208,77 +202,167 @@ __device__ __forceinline__ void moe_finish(const MoeArgs &a, int e, size_t pair,
     store_rows(a.out, a.rows, pair, o, y);
 }
 
+// One LDS DMA: lane l's 16 bytes at src land at LDS address lds + 16 l.  Its wait is
+// wait_loads(): the compiler knows of neither, and its own waits for the weights
+// only ever wait for more.  (M0, which the compiler reserves, is put back.)
+__device__ __forceinline__ void dma16(uint32_t lds, const uint8_t *src) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %1\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, off\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "s"(lds), "v"(src)
+        : "memory");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_addr(const void *p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
+}
+
+// A workgroup of 4 waves takes a tile's pairs, up to T = 16 TT of one expert, against
+// 128 / KS weight rows: wave w rows 32 (w / KS) .. + 31 (gate and up: 16 of each),
+// part w % KS of the groups.  Weights go straight from memory into registers, each
+// row read by one wave, a group ahead of its products; the tokens' records, which all
+// waves read, come through LDS by DMA, CH groups of T tokens a buffer, two buffers.
+constexpr int kTileWaves = 4;
+__host__ __device__ constexpr int tile_chunk(int TT) { return TT == 1 ? 4 : TT == 2 ? 2 : 1; }
+__host__ __device__ constexpr int tile_lds(int TT) { return 2 * tile_chunk(TT) * 16 * TT * kMoeRec; }
+
 template <class F, bool PAIR, int TT>
-__global__ __launch_bounds__(64 * kFewWaves) void moe_few_kernel(MoeArgs a) {
-    __shared__ float4 red[kFewWaves][2 * TT][64];
-    const int n_row = (a.rows + (PAIR ? 15 : 31)) / (PAIR ? 16 : 32);
-    const int slot = (int)(blockIdx.x / (unsigned)n_row);
-    const MoeTile tile = a.tiles[slot];
-    if (tile.count == 0) return;
+__global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a, int ks_log, int slots, int sub_log, int n_rb) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ int s_pair[16 * TT];
+    constexpr int T = 16 * TT, CH = tile_chunk(TT), kBuf = CH * T * kMoeRec;
+    constexpr int kDma = kBuf / 1024, kEach = (kDma + kTileWaves - 1) / kTileWaves;
+    static_assert(kBuf % 1024 == 0, "whole DMAs");
+    // Workgroup b runs on chiplet b % 8: each chiplet takes a run of slots, a slot's row
+    // blocks one after the other, so that a tile's records and an expert's weights are
+    // read into one L2.
+    const int each8 = (slots + 7) / 8;
+    const int local = (int)(blockIdx.x >> 3);
+    const int slot = (int)(blockIdx.x & 7u) * each8 + local / n_rb;
+    if (slot >= slots) return;
+    MoeTile tile = a.tiles[slot >> sub_log];
+    const int skip = (slot & ((1 << sub_log) - 1)) * T;
+    tile.start += skip;
+    tile.count = min(tile.count - skip, T);
+    if (tile.count <= 0) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int g = lane >> 4, r16 = lane & 15;
-    const int row0 = (PAIR ? 16 : 32) * ((int)blockIdx.x - slot * n_row);
+    const int KS = 1 << ks_log, ks = wave & (KS - 1), rw = wave >> ks_log;
+    const int rb = local - local / n_rb * n_rb;
+    const int row0 = (PAIR ? 16 : 32) * (rb * (kTileWaves >> ks_log) + rw);
+    const int u0 = a.groups * ks >> ks_log, u1 = a.groups * (ks + 1) >> ks_log;
+    const int chs = CH >> ks_log;  // groups of a part in a buffer
+    const int n_chunk = (((a.groups + KS - 1) >> ks_log) + chs - 1) / chs;
+
+    if ((int)threadIdx.x < T) s_pair[threadIdx.x] = a.order[tile.start + min((int)threadIdx.x, tile.count - 1)];
+    __syncthreads();
+    // the DMAs' sources: 16-byte piece p of a buffer is piece p % 19 of record p / 19,
+    // token p / 19 % T's group p / 19 / T: group p / 19 / T / KS of part p / 19 / T % KS.  They
+    // are made anew for each buffer (rows from LDS): kept, they would be 20 registers
+    uint32_t from[kEach];  // token, and the piece's offset in its row
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int p = min(i * kTileWaves + wave, kDma - 1) * 64 + lane;
+        const int rec = p / (kMoeRec / 16), c = rec / T;
+        const int u = (a.groups * (c & (KS - 1)) >> ks_log) + (c >> ks_log);
+        from[i] = (uint32_t)(rec - c * T) | (uint32_t)(u * (kMoeRec / 16) + p - rec * (kMoeRec / 16)) << 8;
+    }
+    const size_t rec_row = (size_t)a.groups * kMoeRec;
+    const auto stage = [&](int chunk) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int d = i * kTileWaves + wave;
+            const unsigned pair = (unsigned)s_pair[from[i] & 255u];
+            const uint8_t *src = a.pack + (PAIR ? pair / (unsigned)a.top_k : pair) * rec_row +
+                                 ((from[i] >> 8) * 16u + (unsigned)(chunk * chs * kMoeRec));
+            if (d < kDma) dma16(lds_addr(lds) + (chunk & 1) * kBuf + 1024 * d, src);
+        }
+    };
     const uint8_t *wrow[2];
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt)
         wrow[rt] = a.w[PAIR ? rt : 0] + (size_t)tile.expert * a.expert_bytes +
                    (size_t)min(row0 + (PAIR ? 0 : 16 * rt) + r16, a.rows - 1) * a.row_bytes;
-    const uint8_t *rec[TT];
-#pragma unroll
-    for (int tt = 0; tt < TT; ++tt) {
-        const int pair = a.order[tile.start + min(16 * tt + r16, tile.count - 1)];
-        rec[tt] = a.pack + (size_t)(PAIR ? pair / a.top_k : pair) * a.groups * kMoeRec;
-    }
-    const int u0 = a.groups * wave / kFewWaves, u1 = a.groups * (wave + 1) / kFewWaves;
     float acc[2][TT][4] = {};
-    if (u0 < u1) {
-        typename F::W w[2];
+    typename F::W w[2];
+    stage(0);
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) F::load_w(w[rt], wrow[rt], u0, a.nblk, g);
-        for (int u = u0; u < u1; ++u) {
-            typename F::W next[2];
-            typename F::X x[TT];
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt) moe_load_x<F>(x[tt], rec[tt] + (size_t)u * kMoeRec, g);
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt) F::load_w(next[rt], wrow[rt], min(u + 1, u1 - 1), a.nblk, g);
-            __builtin_amdgcn_sched_barrier(0);
+    for (int rt = 0; rt < 2; ++rt) F::load_w(w[rt], wrow[rt], min(u0, a.groups - 1), a.nblk, g);
+    for (int i = 0; i < n_chunk; ++i) {
+        wait_loads();
+        __syncthreads();  // this buffer is whole, and the other one has been read
+        if (i + 1 < n_chunk) stage(i + 1);
+        const uint8_t *buf = lds + (i & 1) * kBuf + r16 * kMoeRec;
+        for (int c = 0; c < chs; ++c) {
+            const int u = u0 + i * chs + c;
+            if (u >= u1) break;
+            const uint8_t *rec = buf + ((c << ks_log) + ks) * (T * kMoeRec);
+            typename F::Op op[2];
+            MoeScales<F> s[2];
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt) {
-                typename F::Op op;
-                F::decode(op, w[rt], g);
-                MoeScales<F> s;
-                s.from(op, g);
+                F::decode(op[rt], w[rt], g);
+                s[rt].from(op[rt], g);
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
-                    if (16 * tt < tile.count) s.dot(acc[rt][tt], op, x[tt]);
-                w[rt] = next[rt];
+            for (int rt = 0; rt < 2; ++rt) F::load_w(w[rt], wrow[rt], min(u + 1, u1 - 1), a.nblk, g);
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) {
+                if (16 * tt >= tile.count) break;
+                typename F::X x;
+                moe_load_x<F>(x, rec + 16 * tt * kMoeRec, g);
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt) s[rt].dot(acc[rt][tt], op[rt], x);
+                // (these sums are made here: left to the compiler, all tiles' integer sums
+                // wait in registers for the end of the step)
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt)
+                    asm volatile("" : "+v"(acc[rt][tt][0]), "+v"(acc[rt][tt][1]), "+v"(acc[rt][tt][2]), "+v"(acc[rt][tt][3]));
             }
         }
     }
+    if (KS > 1) {
+        // the parts' sums, in their order, through LDS
+        float4 *red = reinterpret_cast<float4 *>(lds);
+        __syncthreads();
+        if (ks > 0)
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
+            for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
-            red[wave][rt * TT + tt][lane] = make_float4(acc[rt][tt][0], acc[rt][tt][1], acc[rt][tt][2], acc[rt][tt][3]);
-    __syncthreads();
-    const auto total = [&](int i, int l, float (&v)[4]) {
-        v[0] = v[1] = v[2] = v[3] = 0.0f;
+                for (int tt = 0; tt < TT; ++tt)
+                    red[((wave * 2 + rt) * TT + tt) * 64 + lane] =
+                        make_float4(acc[rt][tt][0], acc[rt][tt][1], acc[rt][tt][2], acc[rt][tt][3]);
+        __syncthreads();
+        if (ks > 0) return;
+        for (int k = 1; k < KS; ++k)
 #pragma unroll
-        for (int k = 0; k < kFewWaves; ++k) {
-            const float4 s = red[k][i][l];
-            v[0] += s.x, v[1] += s.y, v[2] += s.z, v[3] += s.w;
+            for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) {
+                    const float4 v = red[(((wave + k) * 2 + rt) * TT + tt) * 64 + lane];
+                    acc[rt][tt][0] += v.x, acc[rt][tt][1] += v.y, acc[rt][tt][2] += v.z, acc[rt][tt][3] += v.w;
+                }
+    }
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt) {
+        const int at = 16 * tt + r16;
+        if (at >= tile.count) continue;
+        const size_t pair = (size_t)a.order[tile.start + at];
+        if (PAIR) {
+            if (row0 + 4 * g < a.rows) moe_finish<true>(a, tile.expert, pair, row0 + 4 * g, acc[0][tt], acc[1][tt]);
+        } else {
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt)
+                if (row0 + 16 * rt + 4 * g < a.rows)
+                    moe_finish<false>(a, tile.expert, pair, row0 + 16 * rt + 4 * g, acc[rt][tt], acc[rt][tt]);
         }
-    };
-    for (int i = threadIdx.x; i < (PAIR ? 1 : 2) * TT * 64; i += 64 * kFewWaves) {
-        const int l = i & 63, ti = i >> 6, tt = ti % TT, rt = ti / TT;
-        const int at = 16 * tt + (l & 15), o = row0 + 16 * rt + 4 * (l >> 4);
-        if (at >= tile.count || o >= a.rows) continue;
-        float v[4], u[4] = {};
-        total(ti, l, v);
-        if (PAIR) total(TT + tt, l, u);
-        moe_finish<PAIR>(a, tile.expert, (size_t)a.order[tile.start + at], o, v, u);
     }
 }
 
@@ -333,7 +417,18 @@ bool moe_one(long long pairs) {
 int moe_tile(long long pairs, int n_experts) {
     static const int knob = tuning_knob("EXQ_MOE_TILE", 0);
     if (knob != 0) return knob;
-    return pairs <= 12LL * n_experts ? 16 : 32;
+    return pairs <= 12LL * n_experts ? 16 : pairs <= 24LL * n_experts ? 32 : pairs <= 48LL * n_experts ? 64 : 128;
+}
+
+template <class F, bool PAIR, int TT>
+void moe_tiles(const MoeArgs &a, int slots, int sub_log, int ks_log, hipStream_t st) {
+    slots <<= sub_log;
+    const int rows = (PAIR ? 16 : 32) * (kTileWaves >> ks_log);
+    const int n_rb = (a.rows + rows - 1) / rows;
+    // (a slot and 16 rows or more a workgroup: what the pairs' rows take in device memory keeps that below 2^31)
+    const dim3 grid((unsigned)((slots + 7) / 8) * 8u * (unsigned)n_rb);
+    hipLaunchKernelGGL((moe_tile_kernel<F, PAIR, TT>), grid, dim3(64 * kTileWaves), tile_lds(TT), st, a, ks_log, slots,
+                       sub_log, n_rb);
 }
 
 template <class F, bool PAIR>
@@ -361,20 +456,24 @@ bool moe_run(const edgexpu_hip_moe *p, MoeArgs &a, bool pair, hipStream_t st, co
     if (!lib_hip(hipGetLastError(), what)) return false;
     float *out = a.out;
     if (!pair) a.out = p->part;
-    const int each = pair ? 16 : 32;
-    // (a slot and 16 rows or more a workgroup: what the pairs' rows take in device memory keeps that below 2^31)
-    const dim3 grid((unsigned)((a.rows + each - 1) / each) * (unsigned)moe_slots(pairs, p->n_experts, p->tile));
-#define MOE_FEW(TT)                                                                                        \
-    if (pair)                                                                                              \
-        hipLaunchKernelGGL((moe_few_kernel<F, true, TT>), grid, dim3(64 * kFewWaves), 0, st, a);           \
-    else                                                                                                   \
-        hipLaunchKernelGGL((moe_few_kernel<F, false, TT>), grid, dim3(64 * kFewWaves), 0, st, a);
+    const int slots = moe_slots(pairs, p->n_experts, p->tile);
+    static const int ks_knob = tuning_knob("EXQ_MOE_KS", 0);
+    const int ks = std::min(ks_knob, p->tile == 16 ? 2 : p->tile == 32 ? 1 : 0);
+#define MOE_TILES(TT, SUB)                              \
+    if (pair)                                           \
+        moe_tiles<F, true, TT>(a, slots, SUB, ks, st);  \
+    else                                                \
+        moe_tiles<F, false, TT>(a, slots, SUB, ks, st);
     if (p->tile == 16) {
-        MOE_FEW(1)
+        MOE_TILES(1, 0)
+    } else if (p->tile == 32) {
+        MOE_TILES(2, 0)
+    } else if (p->tile == 64 || F::kMaxTT < 8) {
+        MOE_TILES(4, p->tile == 64 ? 0 : 1)
     } else {
-        MOE_FEW(2)
+        MOE_TILES(F::kMaxTT, 0)
     }
-#undef MOE_FEW
+#undef MOE_TILES
     if (!lib_hip(hipGetLastError(), what)) return false;
     if (pair) return true;
     const bool vec = (a.rows & 3) == 0;
@@ -411,6 +510,14 @@ bool moe_plan(edgexpu_hip_moe *p, int m, hipStream_t st, const char *what) {
     p->tile = tile;
     p->m = m;
     return true;
+}
+
+// LDS beyond 64 KiB is asked for once, when a plan is made: nothing of it is left for a captured call.
+hipError_t moe_prepare() {
+    const hipError_t e = hipFuncSetAttribute((const void *)moe_tile_kernel<MoeQ4K, true, 8>,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, tile_lds(8));
+    return e != hipSuccess ? e : hipFuncSetAttribute((const void *)moe_tile_kernel<MoeQ4K, false, 8>,
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, tile_lds(8));
 }
 
 // The checks that the products share.
@@ -486,7 +593,7 @@ edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens
                   n_experts, kMoeMaxTopK, kMoeMaxExperts, max_tokens, n_embd, n_ff);
         return nullptr;
     }
-    if (!lib_ready("moe_create")) return nullptr;
+    if (!lib_ready("moe_create") || !lib_hip(moe_prepare(), "moe_create")) return nullptr;
     edgexpu_hip_moe *p = new (std::nothrow) edgexpu_hip_moe();
     if (p == nullptr) {
         lib_error(-5, "moe_create: out of host memory");
@@ -500,7 +607,7 @@ edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens
     const size_t pairs = (size_t)max_tokens * top_k;
     const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const size_t sizes[6] = {4 * pairs, 4 * pairs, 4 * pairs, sizeof(MoeTile) * moe_slots(pairs, n_experts, 16),
-                             kMoeRec * std::max((size_t)moe_groups(n_embd) * max_tokens, (size_t)moe_groups(n_ff) * pairs),
+                             kMoeRec * (std::max((size_t)moe_groups(n_embd) * max_tokens, (size_t)moe_groups(n_ff) * pairs) + 8),
                              4 * pairs * n_embd};
     size_t total = 0, at[6];
     for (int i = 0; i < 6; ++i) {

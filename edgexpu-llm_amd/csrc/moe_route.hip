@@ -177,19 +177,42 @@ __global__ __launch_bounds__(256) void moe_assign_kernel(const int32_t *__restri
 // own, then writes its own pairs in ascending order (so the sort is stable and the
 // same every time) and its tiles.  Every workgroup reads all ids, 4 bytes a pair from
 // L2, and none waits for another.
-constexpr int kSortThreads = 512, kSortEach = 8;
+constexpr int kSortThreads = 1024, kSortEach = 8;  // (ids are read 8 a thread)
+struct Ids8 {
+    int v[kSortEach];
+};
+// Pairs first .. + 7, those past the last as no pair's id.
+__device__ __forceinline__ Ids8 load_ids(const int32_t *ids, int first, int pairs) {
+    Ids8 r;
+    const int4 *p = reinterpret_cast<const int4 *>(ids + first);
+    const int4 none = make_int4(-1, -1, -1, -1);
+    const int4 a = first < pairs ? p[0] : none, b = first + 4 < pairs ? p[1] : none;
+    const int v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) r.v[k] = first + k < pairs ? v[k] : -1;
+    return r;
+}
 __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t *__restrict__ ids, int pairs,
                                                                 int n_experts, int T, int slots,
                                                                 int32_t *__restrict__ order,
                                                                 MoeTile *__restrict__ tiles) {
-    __shared__ int sums[2][kSortThreads / 64];
+    constexpr int kWaves = kSortThreads / 64, kRound = kSortThreads * kSortEach, kKeep = 4;
+    __shared__ int sums[2][kWaves];
     const int e = (int)blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    Ids8 kept[kKeep];  // the first rounds' ids stay in registers for the second pass
     int less = 0, own = 0;
-    for (int i = tid; i < pairs; i += kSortThreads) {
-        const int v = ids[i];
-        less += v >= 0 && v < e ? 1 : 0;
-        own += v == e ? 1 : 0;
-    }
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) kept[i] = load_ids(ids, i * kRound + tid * kSortEach, pairs);
+    const auto count = [&](const Ids8 &c) {
+#pragma unroll
+        for (int k = 0; k < kSortEach; ++k) {
+            less += c.v[k] >= 0 && c.v[k] < e ? 1 : 0;
+            own += c.v[k] == e ? 1 : 0;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) count(kept[i]);
+    for (int i0 = kKeep * kRound; i0 < pairs; i0 += kRound) count(load_ids(ids, i0 + tid * kSortEach, pairs));
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
         less += __shfl_xor(less, off, 64);
@@ -202,7 +225,7 @@ __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t *_
     __syncthreads();
     less = own = 0;
 #pragma unroll
-    for (int w = 0; w < kSortThreads / 64; ++w) {
+    for (int w = 0; w < kWaves; ++w) {
         less += sums[0][w];
         own += sums[1][w];
     }
@@ -212,12 +235,12 @@ __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t *_
         tiles[s] = MoeTile{e, less + at, max(0, min(T, own - at)), 0};
     }
     int base = less;
-    for (int i0 = 0; i0 < pairs && base < less + own; i0 += kSortThreads * kSortEach) {
-        const int first = i0 + tid * kSortEach;
+    // (every thread runs the same rounds: base and own are the workgroup's)
+    const auto place = [&](const Ids8 &c, int first) {
         unsigned hit = 0u;
 #pragma unroll
         for (int k = 0; k < kSortEach; ++k)
-            if (first + k < pairs && ids[first + k] == e) hit |= 1u << k;
+            if (c.v[k] == e) hit |= 1u << k;
         const int mine = __popc(hit);
         int before = mine;  // inclusive over the wave, then over the waves
 #pragma unroll
@@ -230,7 +253,7 @@ __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t *_
         __syncthreads();
         int at = base + before - mine, total = 0;
 #pragma unroll
-        for (int w = 0; w < kSortThreads / 64; ++w) {
+        for (int w = 0; w < kWaves; ++w) {
             at += w < wave ? sums[0][w] : 0;
             total += sums[0][w];
         }
@@ -238,7 +261,12 @@ __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t *_
         for (int k = 0; k < kSortEach; ++k)
             if ((hit >> k) & 1u) order[at++] = first + k;
         base += total;
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i)
+        if (i * kRound < pairs && base < less + own) place(kept[i], i * kRound + tid * kSortEach);
+    for (int i0 = kKeep * kRound; i0 < pairs && base < less + own; i0 += kRound)
+        place(load_ids(ids, i0 + tid * kSortEach, pairs), i0 + tid * kSortEach);
 }
 
 hipError_t launch_moe_sort(const int32_t *ids, int pairs, int n_experts, int T, int32_t *order, MoeTile *tiles,
