@@ -217,26 +217,32 @@ __device__ __forceinline__ void dma16(uint32_t lds, const uint8_t *src) {
         : "s"(lds), "v"(src)
         : "memory");
 }
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // at most N loads or DMAs still on their way
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
 __device__ __forceinline__ uint32_t lds_addr(const void *p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
 }
 
-// A workgroup of 4 waves takes a tile's pairs, up to T = 16 TT of one expert, against
-// 128 / KS weight rows: wave w rows 32 (w / KS) .. + 31 (gate and up: 16 of each),
-// part w % KS of the groups.  Weights go straight from memory into registers, each
-// row read by one wave, a group ahead of its products; the tokens' records, which all
-// waves read, come through LDS by DMA, CH groups of T tokens a buffer, two buffers.
-constexpr int kTileWaves = 4;
+// A workgroup takes a tile's pairs, up to T = 16 TT of one expert, against its waves'
+// weight rows, RT tiles of 16 each: 4 waves of two tiles (gate and up: one of each), or
+// 8 of one (gate and up: every other wave) for formats whose decoded rows and scales
+// leave no registers for two.  With KS > 1, KS waves share a row tile's groups out.
+// Weights go straight from memory into registers, each row read by one wave, DEEP
+// groups ahead of their products; the tokens' records, which all waves read, come
+// through LDS by DMA, CH groups of T tokens a buffer, two buffers.
 __host__ __device__ constexpr int tile_chunk(int TT) { return TT == 1 ? 4 : TT == 2 ? 2 : 1; }
 __host__ __device__ constexpr int tile_lds(int TT) { return 2 * tile_chunk(TT) * 16 * TT * kMoeRec; }
+__host__ __device__ constexpr int tile_waves(int RT) { return RT == 2 ? 4 : 8; }
 
-template <class F, bool PAIR, int TT>
-__global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a, int ks_log, int slots, int sub_log, int n_rb) {
+template <class F, bool PAIR, int TT, int RT, int DEEP>
+__global__ __launch_bounds__(64 * tile_waves(RT), 2) void moe_tile_kernel(MoeArgs a, int ks_log, int slots, int n_rb) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ int s_pair[16 * TT];
-    constexpr int T = 16 * TT, CH = tile_chunk(TT), kBuf = CH * T * kMoeRec;
-    constexpr int kDma = kBuf / 1024, kEach = (kDma + kTileWaves - 1) / kTileWaves;
+    constexpr int kWaves = tile_waves(RT), T = 16 * TT, CH = tile_chunk(TT), kBuf = CH * T * kMoeRec;
+    constexpr int kDma = kBuf / 1024, kEach = (kDma + kWaves - 1) / kWaves;
+    constexpr bool kBoth = PAIR && RT == 2, kApart = PAIR && RT == 1;  // gate and up in one wave, or in two
     static_assert(kBuf % 1024 == 0, "whole DMAs");
     // Workgroup b runs on chiplet b % 8: each chiplet takes a run of slots, a slot's row
     // blocks one after the other, so that a tile's records and an expert's weights are
@@ -245,17 +251,16 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
     const int local = (int)(blockIdx.x >> 3);
     const int slot = (int)(blockIdx.x & 7u) * each8 + local / n_rb;
     if (slot >= slots) return;
-    MoeTile tile = a.tiles[slot >> sub_log];
-    const int skip = (slot & ((1 << sub_log) - 1)) * T;
-    tile.start += skip;
-    tile.count = min(tile.count - skip, T);
-    if (tile.count <= 0) return;
+    const MoeTile tile = a.tiles[slot];
+    if (tile.count == 0) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int g = lane >> 4, r16 = lane & 15;
-    const int KS = 1 << ks_log, ks = wave & (KS - 1), rw = wave >> ks_log;
+    const int KS = 1 << ks_log, ks = wave & (KS - 1), wr = wave >> ks_log;
     const int rb = local - local / n_rb * n_rb;
-    const int row0 = (PAIR ? 16 : 32) * (rb * (kTileWaves >> ks_log) + rw);
+    const int z = kApart ? wr & 1 : 0;
+    const int row0 = kApart ? 16 * (rb * (kWaves / 2 >> ks_log) + (wr >> 1))
+                            : 16 * (kBoth ? 1 : RT) * (rb * (kWaves >> ks_log) + wr);
     const int u0 = a.groups * ks >> ks_log, u1 = a.groups * (ks + 1) >> ks_log;
     const int chs = CH >> ks_log;  // groups of a part in a buffer
     const int n_chunk = (((a.groups + KS - 1) >> ks_log) + chs - 1) / chs;
@@ -268,7 +273,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
     uint32_t from[kEach];  // token, and the piece's offset in its row
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        const int p = min(i * kTileWaves + wave, kDma - 1) * 64 + lane;
+        const int p = min(i * kWaves + wave, kDma - 1) * 64 + lane;
         const int rec = p / (kMoeRec / 16), c = rec / T;
         const int u = (a.groups * (c & (KS - 1)) >> ks_log) + (c >> ks_log);
         from[i] = (uint32_t)(rec - c * T) | (uint32_t)(u * (kMoeRec / 16) + p - rec * (kMoeRec / 16)) << 8;
@@ -277,89 +282,121 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
     const auto stage = [&](int chunk) {
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int d = i * kTileWaves + wave;
+            const int d = i * kWaves + wave;
             const unsigned pair = (unsigned)s_pair[from[i] & 255u];
             const uint8_t *src = a.pack + (PAIR ? pair / (unsigned)a.top_k : pair) * rec_row +
                                  ((from[i] >> 8) * 16u + (unsigned)(chunk * chs * kMoeRec));
             if (d < kDma) dma16(lds_addr(lds) + (chunk & 1) * kBuf + 1024 * d, src);
         }
     };
-    const uint8_t *wrow[2];
+    const uint8_t *wrow[RT];
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
-        wrow[rt] = a.w[PAIR ? rt : 0] + (size_t)tile.expert * a.expert_bytes +
-                   (size_t)min(row0 + (PAIR ? 0 : 16 * rt) + r16, a.rows - 1) * a.row_bytes;
-    float acc[2][TT][4] = {};
-    typename F::W w[2];
+    for (int rt = 0; rt < RT; ++rt)
+        wrow[rt] = a.w[kBoth ? rt : z] + (size_t)tile.expert * a.expert_bytes +
+                   (size_t)min(row0 + (kBoth ? 0 : 16 * rt) + r16, a.rows - 1) * a.row_bytes;
+    float acc[RT][TT][4] = {};
+    typename F::W w[DEEP][RT];
+    const auto load = [&](typename F::W (&wv)[RT], int u) {
+        u = max(min(u, u1 - 1), 0);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) F::load_w(wv[rt], wrow[rt], u, a.nblk, g);
+    };
     stage(0);
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt) F::load_w(w[rt], wrow[rt], min(u0, a.groups - 1), a.nblk, g);
-    for (int i = 0; i < n_chunk; ++i) {
-        wait_loads();
-        __syncthreads();  // this buffer is whole, and the other one has been read
-        if (i + 1 < n_chunk) stage(i + 1);
-        const uint8_t *buf = lds + (i & 1) * kBuf + r16 * kMoeRec;
-        for (int c = 0; c < chs; ++c) {
-            const int u = u0 + i * chs + c;
-            if (u >= u1) break;
-            const uint8_t *rec = buf + ((c << ks_log) + ks) * (T * kMoeRec);
-            typename F::Op op[2];
-            MoeScales<F> s[2];
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
-                F::decode(op[rt], w[rt], g);
-                s[rt].from(op[rt], g);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt) F::load_w(w[rt], wrow[rt], min(u + 1, u1 - 1), a.nblk, g);
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt) {
-                if (16 * tt >= tile.count) break;
-                typename F::X x;
-                moe_load_x<F>(x, rec + 16 * tt * kMoeRec, g);
-#pragma unroll
-                for (int rt = 0; rt < 2; ++rt) s[rt].dot(acc[rt][tt], op[rt], x);
-                // (these sums are made here: left to the compiler, all tiles' integer sums
-                // wait in registers for the end of the step)
-#pragma unroll
-                for (int rt = 0; rt < 2; ++rt)
-                    asm volatile("" : "+v"(acc[rt][tt][0]), "+v"(acc[rt][tt][1]), "+v"(acc[rt][tt][2]), "+v"(acc[rt][tt][3]));
-            }
+    for (int k = 0; k < DEEP; ++k) load(w[k], u0 + k);
+    // One group.  Every step loads (its part's last group again past its end), so that the
+    // wait for a step's weights counts the same loads on every path.
+    const auto step = [&](int v, typename F::W (&wv)[RT]) {
+        if ((v & (chs - 1)) == 0) {
+            const int chunk = v / chs;
+            // a buffer's DMAs are older than the last step's loads, of which the 16-byte ones
+            // (Q4_K: 3 a row tile, the others more) are surely one instruction each
+            wait_loads<DEEP == 1 ? 0 : 3 * RT>();
+            __syncthreads();  // this buffer is whole, and the other one has been read
+            if (chunk + 1 < n_chunk) stage(chunk + 1);
         }
-    }
+        const int u = u0 + v;
+        const uint8_t *rec = lds + ((v / chs) & 1) * kBuf + (((v & (chs - 1)) << ks_log) + ks) * (T * kMoeRec) +
+                             r16 * kMoeRec;
+        typename F::Op op[RT];
+        MoeScales<F> s[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            F::decode(op[rt], wv[rt], g);
+            s[rt].from(op[rt], g);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load(wv, u + DEEP);
+        const int count = u < u1 ? tile.count : 0;
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+            if (16 * tt >= count) break;
+            typename F::X x;
+            moe_load_x<F>(x, rec + 16 * tt * kMoeRec, g);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) s[rt].dot(acc[rt][tt], op[rt], x);
+            // (these sums are made here: left to the compiler, all tiles' integer sums
+            // wait in registers for the end of the step)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+                asm volatile("" : "+v"(acc[rt][tt][0]), "+v"(acc[rt][tt][1]), "+v"(acc[rt][tt][2]), "+v"(acc[rt][tt][3]));
+        }
+    };
+    int v = 0;
+    for (; v + DEEP <= n_chunk * chs; v += DEEP)
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) step(v + k, w[k]);
+    if (DEEP == 2 && v < n_chunk * chs) step(v, w[0]);
+
+    float4 *red = reinterpret_cast<float4 *>(lds);
+    const auto give = [&]() {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt)
+                red[((wave * RT + rt) * TT + tt) * 64 + lane] =
+                    make_float4(acc[rt][tt][0], acc[rt][tt][1], acc[rt][tt][2], acc[rt][tt][3]);
+    };
     if (KS > 1) {
-        // the parts' sums, in their order, through LDS
-        float4 *red = reinterpret_cast<float4 *>(lds);
+        // the parts' sums, in their order
         __syncthreads();
-        if (ks > 0)
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
-#pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
-                    red[((wave * 2 + rt) * TT + tt) * 64 + lane] =
-                        make_float4(acc[rt][tt][0], acc[rt][tt][1], acc[rt][tt][2], acc[rt][tt][3]);
+        if (ks > 0) give();
         __syncthreads();
-        if (ks > 0) return;
-        for (int k = 1; k < KS; ++k)
+        if (ks == 0)
+            for (int k = 1; k < KS; ++k)
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
+                for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt) {
-                    const float4 v = red[(((wave + k) * 2 + rt) * TT + tt) * 64 + lane];
-                    acc[rt][tt][0] += v.x, acc[rt][tt][1] += v.y, acc[rt][tt][2] += v.z, acc[rt][tt][3] += v.w;
-                }
+                    for (int tt = 0; tt < TT; ++tt) {
+                        const float4 o = red[(((wave + k) * RT + rt) * TT + tt) * 64 + lane];
+                        acc[rt][tt][0] += o.x, acc[rt][tt][1] += o.y, acc[rt][tt][2] += o.z, acc[rt][tt][3] += o.w;
+                    }
     }
+    if (kApart) {
+        // up's sums to the wave that holds gate's
+        __syncthreads();
+        if (z == 1 && ks == 0) give();
+        __syncthreads();
+    }
+    if (z == 1 || ks > 0) return;
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
         const int at = 16 * tt + r16;
         if (at >= tile.count) continue;
-        const size_t pair = (size_t)a.order[tile.start + at];
+        const size_t pair = (size_t)s_pair[at];
         if (PAIR) {
-            if (row0 + 4 * g < a.rows) moe_finish<true>(a, tile.expert, pair, row0 + 4 * g, acc[0][tt], acc[1][tt]);
+            float up[4];
+            if (kBoth) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) up[r] = acc[RT - 1][tt][r];
+            } else {
+                const float4 o = red[((wave + KS) * TT + tt) * 64 + lane];
+                up[0] = o.x, up[1] = o.y, up[2] = o.z, up[3] = o.w;
+            }
+            if (row0 + 4 * g < a.rows) moe_finish<true>(a, tile.expert, pair, row0 + 4 * g, acc[0][tt], up);
         } else {
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
+            for (int rt = 0; rt < RT; ++rt)
                 if (row0 + 16 * rt + 4 * g < a.rows)
                     moe_finish<false>(a, tile.expert, pair, row0 + 16 * rt + 4 * g, acc[rt][tt], acc[rt][tt]);
         }
@@ -409,26 +446,41 @@ constexpr size_t kOneLds = 60 * 1024;
 
 // Whether a routing's products take a workgroup a token (gate and up: a pair) without sorting the pairs.
 bool moe_one(long long pairs) {
-    static const int most = tuning_knob("EXQ_MOE_ONE", 16);
+    const int most = tuning_knob("EXQ_MOE_ONE", 16);
     return pairs <= most;
 }
 
 // Places a tile of sorted pairs.
 int moe_tile(long long pairs, int n_experts) {
-    static const int knob = tuning_knob("EXQ_MOE_TILE", 0);
+    const int knob = tuning_knob("EXQ_MOE_TILE", 0);
     if (knob != 0) return knob;
     return pairs <= 12LL * n_experts ? 16 : pairs <= 24LL * n_experts ? 32 : pairs <= 48LL * n_experts ? 64 : 128;
 }
 
+// Row tiles a wave and groups of weights ahead, of a format's tiles of TT: as many as
+// leave no register in scratch memory.
+template <class F>
+constexpr int tile_rt(int TT) {
+    return F::kType == kTypeQ4_K || (F::kType == kTypeQ5_K && TT < 8) ? 2 : 1;
+}
+template <class F>
+constexpr int tile_deep(int TT) {
+    return tile_rt<F>(TT) == 2 && TT == (F::kType == kTypeQ4_K ? 8 : 4) ? 1 : 2;
+}
 template <class F, bool PAIR, int TT>
-void moe_tiles(const MoeArgs &a, int slots, int sub_log, int ks_log, hipStream_t st) {
-    slots <<= sub_log;
-    const int rows = (PAIR ? 16 : 32) * (kTileWaves >> ks_log);
+constexpr auto tile_kernel() {
+    return moe_tile_kernel<F, PAIR, TT, tile_rt<F>(TT), tile_deep<F>(TT)>;
+}
+
+template <class F, bool PAIR, int TT>
+void moe_tiles(const MoeArgs &a, int slots, int ks_log, hipStream_t st) {
+    constexpr int RT = tile_rt<F>(TT);
+    const int rows = (PAIR ? 8 : 16) * RT * (tile_waves(RT) >> ks_log);
     const int n_rb = (a.rows + rows - 1) / rows;
     // (a slot and 16 rows or more a workgroup: what the pairs' rows take in device memory keeps that below 2^31)
     const dim3 grid((unsigned)((slots + 7) / 8) * 8u * (unsigned)n_rb);
-    hipLaunchKernelGGL((moe_tile_kernel<F, PAIR, TT>), grid, dim3(64 * kTileWaves), tile_lds(TT), st, a, ks_log, slots,
-                       sub_log, n_rb);
+    hipLaunchKernelGGL((tile_kernel<F, PAIR, TT>()), grid, dim3(64 * tile_waves(RT)), tile_lds(TT), st, a, ks_log, slots,
+                       n_rb);
 }
 
 template <class F, bool PAIR>
@@ -457,21 +509,21 @@ bool moe_run(const edgexpu_hip_moe *p, MoeArgs &a, bool pair, hipStream_t st, co
     float *out = a.out;
     if (!pair) a.out = p->part;
     const int slots = moe_slots(pairs, p->n_experts, p->tile);
-    static const int ks_knob = tuning_knob("EXQ_MOE_KS", 0);
+    const int ks_knob = tuning_knob("EXQ_MOE_KS", 0);
     const int ks = std::min(ks_knob, p->tile == 16 ? 2 : p->tile == 32 ? 1 : 0);
-#define MOE_TILES(TT, SUB)                              \
-    if (pair)                                           \
-        moe_tiles<F, true, TT>(a, slots, SUB, ks, st);  \
-    else                                                \
-        moe_tiles<F, false, TT>(a, slots, SUB, ks, st);
+#define MOE_TILES(TT)                          \
+    if (pair)                                  \
+        moe_tiles<F, true, TT>(a, slots, ks, st);  \
+    else                                       \
+        moe_tiles<F, false, TT>(a, slots, ks, st);
     if (p->tile == 16) {
-        MOE_TILES(1, 0)
+        MOE_TILES(1)
     } else if (p->tile == 32) {
-        MOE_TILES(2, 0)
-    } else if (p->tile == 64 || F::kMaxTT < 8) {
-        MOE_TILES(4, p->tile == 64 ? 0 : 1)
+        MOE_TILES(2)
+    } else if (p->tile == 64) {
+        MOE_TILES(4)
     } else {
-        MOE_TILES(F::kMaxTT, 0)
+        MOE_TILES(8)
     }
 #undef MOE_TILES
     if (!lib_hip(hipGetLastError(), what)) return false;
@@ -513,11 +565,13 @@ bool moe_plan(edgexpu_hip_moe *p, int m, hipStream_t st, const char *what) {
 }
 
 // LDS beyond 64 KiB is asked for once, when a plan is made: nothing of it is left for a captured call.
-hipError_t moe_prepare() {
-    const hipError_t e = hipFuncSetAttribute((const void *)moe_tile_kernel<MoeQ4K, true, 8>,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, tile_lds(8));
-    return e != hipSuccess ? e : hipFuncSetAttribute((const void *)moe_tile_kernel<MoeQ4K, false, 8>,
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, tile_lds(8));
+template <class F>
+bool moe_prepare() {
+    const void *k[2] = {(const void *)tile_kernel<F, true, 8>(), (const void *)tile_kernel<F, false, 8>()};
+    for (const void *f : k)
+        if (!lib_hip(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, tile_lds(8)), "moe_create"))
+            return false;
+    return true;
 }
 
 // The checks that the products share.
@@ -593,7 +647,9 @@ edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens
                   n_experts, kMoeMaxTopK, kMoeMaxExperts, max_tokens, n_embd, n_ff);
         return nullptr;
     }
-    if (!lib_ready("moe_create") || !lib_hip(moe_prepare(), "moe_create")) return nullptr;
+    if (!lib_ready("moe_create") || !moe_prepare<MoeQ4K>() || !moe_prepare<MoeQ5K>() || !moe_prepare<MoeQ6K>() ||
+        !moe_prepare<MoeQ80>() || !moe_prepare<MoeQ40>() || !moe_prepare<MoeQ50>())
+        return nullptr;
     edgexpu_hip_moe *p = new (std::nothrow) edgexpu_hip_moe();
     if (p == nullptr) {
         lib_error(-5, "moe_create: out of host memory");

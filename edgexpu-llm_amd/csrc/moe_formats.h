@@ -237,7 +237,7 @@ __device__ __forceinline__ v4h min_operand(const SixBits &b, int g) {
 
 struct MoeQ4K {
     static constexpr bool kK = true, kMin = true, kTurned = false;
-    static constexpr int kType = kTypeQ4_K, kDigits = 2, kBytes = kBytesQ4_K, kMaxTT = 8;
+    static constexpr int kType = kTypeQ4_K, kDigits = 2, kBytes = kBytesQ4_K;
     struct W {
         uint4 hd, q[2];
     };
@@ -279,7 +279,7 @@ struct MoeQ4K {
 
 struct MoeQ5K {
     static constexpr bool kK = true, kMin = true, kTurned = true;
-    static constexpr int kType = kTypeQ5_K, kDigits = 2, kBytes = kBytesQ5_K, kMaxTT = 4;
+    static constexpr int kType = kTypeQ5_K, kDigits = 2, kBytes = kBytesQ5_K;
     struct W {
         uint4 hd, h, q[2];
     };
@@ -322,7 +322,7 @@ struct MoeQ5K {
 // joined by byte shifts (ldg16_a2).
 struct MoeQ6K {
     static constexpr bool kK = true, kMin = false, kTurned = false;
-    static constexpr int kType = kTypeQ6_K, kDigits = 3, kBytes = kBytesQ6_K, kMaxTT = 4;
+    static constexpr int kType = kTypeQ6_K, kDigits = 3, kBytes = kBytesQ6_K;
     struct W {
         uint4 l[2], h[2];
         uint32_t sc;  // scales g, 4 + g, 8 + g, 12 + g
@@ -440,7 +440,7 @@ __device__ __forceinline__ uint32_t load_scales(const uint8_t *row, int u, int n
 // either block.
 struct MoeQ80 {
     static constexpr bool kK = false, kQ80 = true;
-    static constexpr int kType = kTypeQ8_0, kBytes = kBytesQ8_0, kMaxTT = 4;
+    static constexpr int kType = kTypeQ8_0, kBytes = kBytesQ8_0;
     struct W {
         uint4 q[4];
         uint32_t d;
@@ -475,7 +475,7 @@ __device__ __forceinline__ uint32_t less_each(uint32_t c, uint32_t bias) {
 }
 struct MoeQ40 {
     static constexpr bool kK = false, kQ80 = false;
-    static constexpr int kType = kTypeQ4_0, kBytes = kBytesQ4_0, kMaxTT = 4;
+    static constexpr int kType = kTypeQ4_0, kBytes = kBytesQ4_0;
     struct W {
         uint32_t q[8], d;
     };
@@ -501,7 +501,7 @@ struct MoeQ40 {
 
 struct MoeQ50 {
     static constexpr bool kK = false, kQ80 = false;
-    static constexpr int kType = kTypeQ5_0, kBytes = kBytesQ5_0, kMaxTT = 4;
+    static constexpr int kType = kTypeQ5_0, kBytes = kBytesQ5_0;
     struct W {
         uint32_t q[8], h[8], d;
     };
