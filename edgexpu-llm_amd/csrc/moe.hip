@@ -225,178 +225,179 @@ __device__ __forceinline__ uint32_t lds_addr(const void *p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
 }
 
-// A workgroup takes a tile's pairs, up to T = 16 TT of one expert, against its waves'
-// weight rows, RT tiles of 16 each: 4 waves of two tiles (gate and up: one of each), or
-// 8 of one (gate and up: every other wave) for formats whose decoded rows and scales
-// leave no registers for two.  With KS > 1, KS waves share a row tile's groups out.
-// Weights go straight from memory into registers, each row read by one wave, DEEP
-// groups ahead of their products; the tokens' records, which all waves read, come
-// through LDS by DMA, CH groups of T tokens a buffer, two buffers.
+// A workgroup of 4 waves takes a tile's pairs, up to T = 16 TT of one expert, against a
+// block of weight rows: two tiles of 16 rows a wave (gate and up: one of each), or with
+// KS > 1 KS waves share two tiles' groups out.  Weights go straight from memory into
+// registers, each row read by one wave, DEEP groups ahead of their products; the tokens'
+// records, which all waves read, come through LDS by DMA, CH groups of T tokens a
+// buffer, two buffers.  BOTH: a step decodes both tiles, then reads each record once for
+// the two; otherwise one after the other, which halves the registers of the decoded rows.
 __host__ __device__ constexpr int tile_chunk(int TT) { return TT == 1 ? 4 : TT == 2 ? 2 : 1; }
 __host__ __device__ constexpr int tile_lds(int TT) { return 2 * tile_chunk(TT) * 16 * TT * kMoeRec; }
-__host__ __device__ constexpr int tile_waves(int RT) { return RT == 2 ? 4 : 8; }
+constexpr int kTileWaves = 4;
 
-template <class F, bool PAIR, int TT, int RT, int DEEP>
-__global__ __launch_bounds__(64 * tile_waves(RT), 2) void moe_tile_kernel(MoeArgs a, int ks_log, int slots, int n_rb) {
+// Sums made where they stand: left to the compiler, all tiles' integer sums wait in
+// registers for the end of a step.
+__device__ __forceinline__ void pin(float (&v)[4]) {
+    asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
+}
+
+template <class F, bool PAIR, int TT, bool BOTH, int DEEP>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a, int ks_log, int slots, int n_blk) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ int s_pair[16 * TT];
-    constexpr int kWaves = tile_waves(RT), T = 16 * TT, CH = tile_chunk(TT), kBuf = CH * T * kMoeRec;
-    constexpr int kDma = kBuf / 1024, kEach = (kDma + kWaves - 1) / kWaves;
-    constexpr bool kBoth = PAIR && RT == 2, kApart = PAIR && RT == 1;  // gate and up in one wave, or in two
+    constexpr int T = 16 * TT, CH = tile_chunk(TT), kBuf = CH * T * kMoeRec;
+    constexpr int kDma = kBuf / 1024, kEach = (kDma + kTileWaves - 1) / kTileWaves;
     static_assert(kBuf % 1024 == 0, "whole DMAs");
     // Workgroup b runs on chiplet b % 8: each chiplet takes a run of slots, a slot's row
-    // blocks one after the other, so that a tile's records and an expert's weights are
-    // read into one L2.
+    // blocks one after the other, so that a tile's records and an
+    // expert's weights are read into one L2.
     const int each8 = (slots + 7) / 8;
     const int local = (int)(blockIdx.x >> 3);
-    const int slot = (int)(blockIdx.x & 7u) * each8 + local / n_rb;
+    const int slot = (int)(blockIdx.x & 7u) * each8 + local / n_blk;
     if (slot >= slots) return;
     const MoeTile tile = a.tiles[slot];
     if (tile.count == 0) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int g = lane >> 4, r16 = lane & 15;
-    const int KS = 1 << ks_log, ks = wave & (KS - 1), wr = wave >> ks_log;
-    const int rb = local - local / n_rb * n_rb;
-    const int z = kApart ? wr & 1 : 0;
-    const int row0 = kApart ? 16 * (rb * (kWaves / 2 >> ks_log) + (wr >> 1))
-                            : 16 * (kBoth ? 1 : RT) * (rb * (kWaves >> ks_log) + wr);
+    const int KS = 1 << ks_log, ks = wave & (KS - 1);
+    constexpr int kRows = PAIR ? 16 : 32;
+    const int row0 = kRows * ((local - local / n_blk * n_blk) * (kTileWaves >> ks_log) + (wave >> ks_log));
     const int u0 = a.groups * ks >> ks_log, u1 = a.groups * (ks + 1) >> ks_log;
     const int chs = CH >> ks_log;  // groups of a part in a buffer
-    const int n_chunk = (((a.groups + KS - 1) >> ks_log) + chs - 1) / chs;
+    const int n_chunk = (((a.groups + KS - 1) >> ks_log) + chs - 1) / chs, n_step = n_chunk * chs;
 
     if ((int)threadIdx.x < T) s_pair[threadIdx.x] = a.order[tile.start + min((int)threadIdx.x, tile.count - 1)];
     __syncthreads();
-    // the DMAs' sources: 16-byte piece p of a buffer is piece p % 19 of record p / 19,
-    // token p / 19 % T's group p / 19 / T: group p / 19 / T / KS of part p / 19 / T % KS.  They
-    // are made anew for each buffer (rows from LDS): kept, they would be 20 registers
-    uint32_t from[kEach];  // token, and the piece's offset in its row
+    // The DMAs' sources, in units of 16 bytes: piece p of a buffer is piece p % 19 of record
+    // p / 19, token p / 19 % T's group p / 19 / T: group p / 19 / T / KS of part p / 19 / T % KS.
+    uint32_t from[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        const int p = min(i * kWaves + wave, kDma - 1) * 64 + lane;
+        const int p = min(i * kTileWaves + wave, kDma - 1) * 64 + lane;
         const int rec = p / (kMoeRec / 16), c = rec / T;
         const int u = (a.groups * (c & (KS - 1)) >> ks_log) + (c >> ks_log);
-        from[i] = (uint32_t)(rec - c * T) | (uint32_t)(u * (kMoeRec / 16) + p - rec * (kMoeRec / 16)) << 8;
+        const unsigned pair = (unsigned)s_pair[rec - c * T];
+        const unsigned row = PAIR ? pair / (unsigned)a.top_k : pair;
+        from[i] = (row * (unsigned)a.groups + u) * (kMoeRec / 16) + (p - rec * (kMoeRec / 16));
     }
-    const size_t rec_row = (size_t)a.groups * kMoeRec;
-    const auto stage = [&](int chunk) {
+    const auto stage = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int d = i * kWaves + wave;
-            const unsigned pair = (unsigned)s_pair[from[i] & 255u];
-            const uint8_t *src = a.pack + (PAIR ? pair / (unsigned)a.top_k : pair) * rec_row +
-                                 ((from[i] >> 8) * 16u + (unsigned)(chunk * chs * kMoeRec));
-            if (d < kDma) dma16(lds_addr(lds) + (chunk & 1) * kBuf + 1024 * d, src);
+            const int d = i * kTileWaves + wave;
+            if (d < kDma) dma16(lds_addr(lds) + buf * kBuf + 1024 * d, a.pack + ((size_t)from[i] << 4));
+            from[i] += (unsigned)chs * (kMoeRec / 16);
         }
     };
-    const uint8_t *wrow[RT];
+    const uint8_t *wrow[2];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-        wrow[rt] = a.w[kBoth ? rt : z] + (size_t)tile.expert * a.expert_bytes +
-                   (size_t)min(row0 + (kBoth ? 0 : 16 * rt) + r16, a.rows - 1) * a.row_bytes;
-    float acc[RT][TT][4] = {};
-    typename F::W w[DEEP][RT];
-    const auto load = [&](typename F::W (&wv)[RT], int u) {
-        u = max(min(u, u1 - 1), 0);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) F::load_w(wv[rt], wrow[rt], u, a.nblk, g);
-    };
+    for (int rt = 0; rt < 2; ++rt)
+        wrow[rt] = a.w[PAIR ? rt : 0] + (size_t)tile.expert * a.expert_bytes +
+                   (size_t)min(row0 + (PAIR ? 0 : 16 * rt) + r16, a.rows - 1) * a.row_bytes;
+    float acc[2][TT][4] = {};
+    typename F::W w[DEEP][2];
+    int next = u0;  // the next loads' group; past the end the last one again
+    const auto load = [&](typename F::W &wv, int rt) { F::load_w(wv, wrow[rt], max(min(next, u1 - 1), 0), a.nblk, g); };
     stage(0);
 #pragma unroll
-    for (int k = 0; k < DEEP; ++k) load(w[k], u0 + k);
-    // One group.  Every step loads (its part's last group again past its end), so that the
-    // wait for a step's weights counts the same loads on every path.
-    const auto step = [&](int v, typename F::W (&wv)[RT]) {
+    for (int k = 0; k < DEEP; ++k) {
+        load(w[k][0], 0);
+        load(w[k][1], 1);
+        ++next;
+    }
+    // Both row tiles against a buffer's group.  Every step loads, so that the wait for a
+    // step's weights counts the same loads on every path.
+    const auto step = [&](int v, typename F::W (&wv)[2]) {
         if ((v & (chs - 1)) == 0) {
-            const int chunk = v / chs;
             // a buffer's DMAs are older than the last step's loads, of which the 16-byte ones
             // (Q4_K: 3 a row tile, the others more) are surely one instruction each
-            wait_loads<DEEP == 1 ? 0 : 3 * RT>();
+            wait_loads<6>();
             __syncthreads();  // this buffer is whole, and the other one has been read
-            if (chunk + 1 < n_chunk) stage(chunk + 1);
+            if (v + chs < n_step) stage((v / chs + 1) & 1);
         }
-        const int u = u0 + v;
-        const uint8_t *rec = lds + ((v / chs) & 1) * kBuf + (((v & (chs - 1)) << ks_log) + ks) * (T * kMoeRec) +
-                             r16 * kMoeRec;
-        typename F::Op op[RT];
-        MoeScales<F> s[RT];
+        const uint8_t *rec = lds + ((v / chs) & 1) * kBuf + (((v & (chs - 1)) << ks_log) + ks) * (T * kMoeRec) + r16 * kMoeRec;
+        const int count = u0 + v < u1 ? tile.count : 0;
+        if constexpr (BOTH) {
+            typename F::Op op[2];
+            MoeScales<F> s[2];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            F::decode(op[rt], wv[rt], g);
-            s[rt].from(op[rt], g);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        load(wv, u + DEEP);
-        const int count = u < u1 ? tile.count : 0;
+            for (int rt = 0; rt < 2; ++rt) {
+                F::decode(op[rt], wv[rt], g);
+                s[rt].from(op[rt], g);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load(wv[0], 0);
+            load(wv[1], 1);
+            ++next;
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            if (16 * tt >= count) break;
-            typename F::X x;
-            moe_load_x<F>(x, rec + 16 * tt * kMoeRec, g);
+            for (int tt = 0; tt < TT; ++tt) {
+                if (16 * tt >= count) break;
+                typename F::X x;
+                moe_load_x<F>(x, rec + 16 * tt * kMoeRec, g);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) s[rt].dot(acc[rt][tt], op[rt], x);
-            // (these sums are made here: left to the compiler, all tiles' integer sums
-            // wait in registers for the end of the step)
+                for (int rt = 0; rt < 2; ++rt) s[rt].dot(acc[rt][tt], op[rt], x);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-                asm volatile("" : "+v"(acc[rt][tt][0]), "+v"(acc[rt][tt][1]), "+v"(acc[rt][tt][2]), "+v"(acc[rt][tt][3]));
+                for (int rt = 0; rt < 2; ++rt) pin(acc[rt][tt]);
+            }
+        } else {
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) {
+                typename F::Op op;
+                MoeScales<F> s;
+                F::decode(op, wv[rt], g);
+                s.from(op, g);
+                __builtin_amdgcn_sched_barrier(0);
+                load(wv[rt], rt);
+                if (rt == 1) ++next;
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) {
+                    if (16 * tt >= count) break;
+                    typename F::X x;
+                    moe_load_x<F>(x, rec + 16 * tt * kMoeRec, g);
+                    s.dot(acc[rt][tt], op, x);
+                    pin(acc[rt][tt]);
+                }
+            }
         }
     };
     int v = 0;
-    for (; v + DEEP <= n_chunk * chs; v += DEEP)
+    for (; v + DEEP <= n_step; v += DEEP)
 #pragma unroll
         for (int k = 0; k < DEEP; ++k) step(v + k, w[k]);
-    if (DEEP == 2 && v < n_chunk * chs) step(v, w[0]);
-
-    float4 *red = reinterpret_cast<float4 *>(lds);
-    const auto give = [&]() {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
-                red[((wave * RT + rt) * TT + tt) * 64 + lane] =
-                    make_float4(acc[rt][tt][0], acc[rt][tt][1], acc[rt][tt][2], acc[rt][tt][3]);
-    };
-    if (KS > 1) {
-        // the parts' sums, in their order
+    if (DEEP == 2 && v < n_step) step(v, w[0]);
+    if (KS > 1) {  // the parts' sums, in their order
+        float4 *red = reinterpret_cast<float4 *>(lds);
         __syncthreads();
-        if (ks > 0) give();
+        if (ks > 0)
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt)
+                    red[((wave * 2 + rt) * TT + tt) * 64 + lane] =
+                        make_float4(acc[rt][tt][0], acc[rt][tt][1], acc[rt][tt][2], acc[rt][tt][3]);
         __syncthreads();
-        if (ks == 0)
-            for (int k = 1; k < KS; ++k)
+        if (ks > 0) return;
+        for (int k = 1; k < KS; ++k)
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
+            for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
-                    for (int tt = 0; tt < TT; ++tt) {
-                        const float4 o = red[(((wave + k) * RT + rt) * TT + tt) * 64 + lane];
-                        acc[rt][tt][0] += o.x, acc[rt][tt][1] += o.y, acc[rt][tt][2] += o.z, acc[rt][tt][3] += o.w;
-                    }
+                for (int tt = 0; tt < TT; ++tt) {
+                    const float4 o = red[(((wave + k) * 2 + rt) * TT + tt) * 64 + lane];
+                    acc[rt][tt][0] += o.x, acc[rt][tt][1] += o.y, acc[rt][tt][2] += o.z, acc[rt][tt][3] += o.w;
+                }
     }
-    if (kApart) {
-        // up's sums to the wave that holds gate's
-        __syncthreads();
-        if (z == 1 && ks == 0) give();
-        __syncthreads();
-    }
-    if (z == 1 || ks > 0) return;
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
         const int at = 16 * tt + r16;
         if (at >= tile.count) continue;
         const size_t pair = (size_t)s_pair[at];
         if (PAIR) {
-            float up[4];
-            if (kBoth) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) up[r] = acc[RT - 1][tt][r];
-            } else {
-                const float4 o = red[((wave + KS) * TT + tt) * 64 + lane];
-                up[0] = o.x, up[1] = o.y, up[2] = o.z, up[3] = o.w;
-            }
-            if (row0 + 4 * g < a.rows) moe_finish<true>(a, tile.expert, pair, row0 + 4 * g, acc[0][tt], up);
+            if (row0 + 4 * g < a.rows)
+                moe_finish<true>(a, tile.expert, pair, row0 + 4 * g, acc[0][tt], acc[1][tt]);
         } else {
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
+            for (int rt = 0; rt < 2; ++rt)
                 if (row0 + 16 * rt + 4 * g < a.rows)
                     moe_finish<false>(a, tile.expert, pair, row0 + 16 * rt + 4 * g, acc[rt][tt], acc[rt][tt]);
         }
@@ -457,30 +458,29 @@ int moe_tile(long long pairs, int n_experts) {
     return pairs <= 12LL * n_experts ? 16 : pairs <= 24LL * n_experts ? 32 : pairs <= 48LL * n_experts ? 64 : 128;
 }
 
-// Row tiles a wave and groups of weights ahead, of a format's tiles of TT: as many as
+// Whether a format's tiles of TT decode two row tiles at once, and its groups of weights ahead: as many as
 // leave no register in scratch memory.
 template <class F>
-constexpr int tile_rt(int TT) {
-    return F::kType == kTypeQ4_K || (F::kType == kTypeQ5_K && TT < 8) ? 2 : 1;
+constexpr bool tile_both(int TT) {
+    return TT >= 4 && (F::kType == kTypeQ4_K || (F::kType == kTypeQ5_K && TT < 8));
 }
 template <class F>
 constexpr int tile_deep(int TT) {
-    return tile_rt<F>(TT) == 2 && TT == (F::kType == kTypeQ4_K ? 8 : 4) ? 1 : 2;
+    return TT <= 2 ? 2 : 1;
 }
 template <class F, bool PAIR, int TT>
 constexpr auto tile_kernel() {
-    return moe_tile_kernel<F, PAIR, TT, tile_rt<F>(TT), tile_deep<F>(TT)>;
+    return moe_tile_kernel<F, PAIR, TT, tile_both<F>(TT), tile_deep<F>(TT)>;
 }
 
 template <class F, bool PAIR, int TT>
 void moe_tiles(const MoeArgs &a, int slots, int ks_log, hipStream_t st) {
-    constexpr int RT = tile_rt<F>(TT);
-    const int rows = (PAIR ? 8 : 16) * RT * (tile_waves(RT) >> ks_log);
-    const int n_rb = (a.rows + rows - 1) / rows;
+    const int rows = (PAIR ? 16 : 32) * (kTileWaves >> ks_log);
+    const int n_blk = (a.rows + rows - 1) / rows;
     // (a slot and 16 rows or more a workgroup: what the pairs' rows take in device memory keeps that below 2^31)
-    const dim3 grid((unsigned)((slots + 7) / 8) * 8u * (unsigned)n_rb);
-    hipLaunchKernelGGL((tile_kernel<F, PAIR, TT>()), grid, dim3(64 * tile_waves(RT)), tile_lds(TT), st, a, ks_log, slots,
-                       n_rb);
+    const dim3 grid((unsigned)((slots + 7) / 8) * 8u * (unsigned)n_blk);
+    hipLaunchKernelGGL((tile_kernel<F, PAIR, TT>()), grid, dim3(64 * kTileWaves), tile_lds(TT), st, a, ks_log, slots,
+                       n_blk);
 }
 
 template <class F, bool PAIR>

@@ -170,28 +170,39 @@ __host__ __device__ constexpr int moe_pack_parts(int n) {
 // W: raw registers of a group of the lane's row; Op: the operand; chunk(s, g): which
 // 16 elements of the group lane group g holds in product s of 4.
 
-// The sum over the digits' products, as f32 for the block's scale.
+// A group's integer sums, a digit each, and the minima's.
 template <class F>
-__device__ __forceinline__ void moe_dot_k(float (&acc)[4], const typename F::Op &o, const MoeXK &x,
-                                          const float (&d)[4], const float (&nd)[4]) {
+struct MoeSums {
     v4i s[F::kDigits];
+    v4f mn;
+    float dx;
+    int sum;
+};
+template <class F>
+__device__ __forceinline__ void moe_mul_k(MoeSums<F> &m, const typename F::Op &o, const MoeXK &x) {
 #pragma unroll
-    for (int k = 0; k < F::kDigits; ++k) s[k] = v4i{0, 0, 0, 0};
+    for (int k = 0; k < F::kDigits; ++k) m.s[k] = v4i{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int k = 0; k < F::kDigits; ++k) s[k] = mfma64(o.a[k][i], x.c[i], s[k]);
-    v4f mn;
-    if (F::kMin) mn = mfma_f16(o.mn, x.bs);
+        for (int k = 0; k < F::kDigits; ++k) m.s[k] = mfma64(o.a[k][i], x.c[i], m.s[k]);
+    if (F::kMin) m.mn = mfma_f16(o.mn, x.bs);
+    m.dx = x.dx;
+    m.sum = x.sum;
+}
+// acc += dx * (sum * d - minima * dmin)
+template <class F>
+__device__ __forceinline__ void moe_add_k(float (&acc)[4], const MoeSums<F> &m, const float (&d)[4],
+                                          const float (&nd)[4]) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        int t = s[F::kDigits - 1][r];
+        int t = m.s[F::kDigits - 1][r];
 #pragma unroll
-        for (int k = F::kDigits - 2; k >= 0; --k) t = (t << 3) + s[k][r];
-        if (F::kTurned) t += 1152 * x.sum;
+        for (int k = F::kDigits - 2; k >= 0; --k) t = (t << 3) + m.s[k][r];
+        if (F::kTurned) t += 1152 * m.sum;
         float v = (float)t * d[r];
-        if (F::kMin) v = __builtin_fmaf(mn[r], nd[r], v);
-        acc[r] = __builtin_fmaf(v, x.dx, acc[r]);
+        if (F::kMin) v = __builtin_fmaf(m.mn[r], nd[r], v);
+        acc[r] = __builtin_fmaf(v, m.dx, acc[r]);
     }
 }
 
@@ -318,15 +329,30 @@ struct MoeQ5K {
     }
 };
 
-// Blocks start at even addresses: words are read from the 4-byte address below and
-// joined by byte shifts (ldg16_a2).
+// 16 bytes at an even address as the words from the 4-byte address below it (`sh` below) and the half word
+// that ends them; joined once they are needed.  One `sh` serves every piece of a block: wide loads at 2 mod 4
+// run several times slower (ldg16_a2).
+struct Even16 {
+    uint4 w;
+    uint32_t end;
+};
+__device__ __forceinline__ Even16 load_even(const uint8_t *below, uint32_t sh) {
+    return {*reinterpret_cast<const uint4 *>(below), *reinterpret_cast<const uint16_t *>(below + sh + 14)};
+}
+__device__ __forceinline__ void join_even(uint32_t (&v)[4], const Even16 &e, uint32_t sh) {
+    v[0] = __builtin_amdgcn_alignbyte(e.w.y, e.w.x, sh);
+    v[1] = __builtin_amdgcn_alignbyte(e.w.z, e.w.y, sh);
+    v[2] = __builtin_amdgcn_alignbyte(e.w.w, e.w.z, sh);
+    v[3] = __builtin_amdgcn_alignbyte(e.end, e.w.w, sh);
+}
+
 struct MoeQ6K {
     static constexpr bool kK = true, kMin = false, kTurned = false;
     static constexpr int kType = kTypeQ6_K, kDigits = 3, kBytes = kBytesQ6_K;
     struct W {
-        uint4 l[2], h[2];
-        uint32_t sc;  // scales g, 4 + g, 8 + g, 12 + g
-        uint32_t d;
+        Even16 l[2], h[2];
+        uint32_t sc[4];  // scales g, 4 + g, 8 + g, 12 + g
+        uint32_t d, sh;
     };
     struct Op {
         v4i a[3][4];
@@ -337,13 +363,15 @@ struct MoeQ6K {
     __device__ static constexpr int chunk(int s, int g) { return 4 * s + g; }
     __device__ static __forceinline__ void load_w(W &w, const uint8_t *row, int u, int, int g) {
         const uint8_t *p = row + (size_t)u * kBytes;
+        w.sh = (uint32_t)((uintptr_t)p & 3u);
+        const uint8_t *l = p - w.sh + 16 * g, *h = p - w.sh + 128 + 16 * (g & 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            w.l[i] = ldg16_a2(p + 64 * i + 16 * g);
-            w.h[i] = ldg16_a2(p + 128 + 32 * i + 16 * (g & 1));
+            w.l[i] = load_even(l + 64 * i, w.sh);
+            w.h[i] = load_even(h + 32 * i, w.sh);
         }
-        w.sc = (uint32_t)p[192 + g] | ((uint32_t)p[196 + g] << 8) | ((uint32_t)p[200 + g] << 16) |
-               ((uint32_t)p[204 + g] << 24);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.sc[i] = p[192 + g + 4 * i];
         w.d = *reinterpret_cast<const uint16_t *>(p + 208);
     }
     __device__ static __forceinline__ void decode(Op &o, const W &w, int g) {
@@ -351,11 +379,12 @@ struct MoeQ6K {
         o.mn = v4h{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint32_t l[4] = {w.l[i].x, w.l[i].y, w.l[i].z, w.l[i].w};
-            const uint32_t hh[4] = {w.h[i].x, w.h[i].y, w.h[i].z, w.h[i].w};
+            uint32_t l[4], hh[4];
+            join_even(l, w.l[i], w.sh);
+            join_even(hh, w.h[i], w.sh);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int sc = (int)(int8_t)((w.sc >> (8 * (2 * i + h))) & 0xffu);
+                const int sc = (int)(int8_t)w.sc[2 * i + h];
                 const int s0 = ((sc + 3) & 7) - 3, r1 = (sc - s0) >> 3, s1 = ((r1 + 3) & 7) - 3, s2 = (r1 - s1) >> 3;
                 const int dig[3] = {s0, s1, s2};
 #pragma unroll
@@ -537,7 +566,9 @@ struct MoeScales {
     float d[4], nd[4];
     __device__ __forceinline__ void from(const typename F::Op &o, int g) { moe_row_scales(o.dm, g, d, nd); }
     __device__ __forceinline__ void dot(float (&acc)[4], const typename F::Op &o, const MoeXK &x) const {
-        moe_dot_k<F>(acc, o, x, d, nd);
+        MoeSums<F> m;
+        moe_mul_k<F>(m, o, x);
+        moe_add_k<F>(acc, m, d, nd);
     }
 };
 template <class F>
