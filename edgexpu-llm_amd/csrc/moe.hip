@@ -324,6 +324,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt) {
                 F::decode(op[rt], wv[rt], g);
+                moe_hold_op(op[rt]);
                 s[rt].from(op[rt], g);
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -346,6 +347,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
                 typename F::Op op;
                 MoeScales<F> s;
                 F::decode(op, wv[rt], g);
+                moe_hold_op(op);
                 s.from(op, g);
                 __builtin_amdgcn_sched_barrier(0);
                 load(wv[rt], rt);

@@ -560,6 +560,24 @@ struct MoeQ50 {
 
 // ------------------------------------------------------------------ both kinds
 
+// The operand made where it stands, in its own registers: the raw registers are then free
+// for the next loads.  Left to the compiler the decoding moves down to the products, the loads
+// go to other registers, and the copies between the two wait for every load in flight.
+__device__ __forceinline__ void moe_hold(v4i (&a)[4]) {
+    asm volatile("" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]));
+}
+template <class Op>
+__device__ __forceinline__ void moe_hold_op(Op &o) {
+    if constexpr (sizeof(o.a) == sizeof(long[8])) {
+        asm volatile("" : "+v"(o.a[0]), "+v"(o.a[1]), "+v"(o.a[2]), "+v"(o.a[3]), "+v"(o.a[4]), "+v"(o.a[5]),
+                     "+v"(o.a[6]), "+v"(o.a[7]), "+v"(o.dm));
+    } else {
+#pragma unroll
+        for (auto &digit : o.a) moe_hold(digit);
+        asm volatile("" : "+v"(o.dm), "+v"(o.mn));
+    }
+}
+
 // The rows' scales of a lane's sums.
 template <class F, bool K = F::kK>
 struct MoeScales {
