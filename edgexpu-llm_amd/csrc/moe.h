@@ -11,12 +11,12 @@ namespace exq {
 
 constexpr int kMoeMaxExperts = 512, kMoeMaxTopK = 32, kMoeMaxGroups = 64;
 
-// A tile: `count` places from `start` of the sorted pairs, all of one expert.
-// Expert e's tiles begin at slot start_e / T + e (T places a tile): the next
-// expert's are then past them whatever the counts, so no expert needs to know the
-// others' tile counts.  Slots in between have count 0.
+// A tile of T places of the sorted pairs, all of one expert: the `index`-th of its
+// expert's, from `start`, with `rest` pairs from there to the expert's end (none: no tile).
+// Expert e's tiles begin at slot start_e / T + e: the next expert's are then past them
+// whatever the counts, so no expert needs to know the others' tile counts.
 struct MoeTile {
-    int expert, start, count, pad;
+    int expert, start, rest, index;
 };
 
 }  // namespace exq
@@ -24,7 +24,7 @@ struct MoeTile {
 struct edgexpu_hip_moe {
     int n_experts = 0, top_k = 0, max_tokens = 0, n_embd = 0, n_ff = 0;
     int m = -1;     // tokens of the last routing (-1: none yet)
-    int tile = 0;   // places a tile of its sorted pairs; 0: not sorted
+    int tile = 0;   // places a tile of its sorted pairs (32 or 64); 0: not sorted
     uint8_t *mem = nullptr;
     int32_t *ids = nullptr;  // [max_tokens][top_k], -1: no expert
     float *weights = nullptr;
@@ -48,7 +48,7 @@ struct RouteArgs {
 hipError_t launch_moe_route(const RouteArgs &a, hipStream_t st);
 hipError_t launch_moe_assign(const int32_t *ids, const float *weights, int32_t *to_ids, float *to_weights, int pairs,
                              int n_experts, hipStream_t st);
-// Sorts the pairs by expert into tiles of T places; moe_slots(pairs, n_experts, T) slots are written.
+// Sorts the pairs by expert into tiles of T places: moe_slots(pairs, n_experts, T) slots are written.
 hipError_t launch_moe_sort(const int32_t *ids, int pairs, int n_experts, int T, int32_t *order, MoeTile *tiles,
                            hipStream_t st);
 inline int moe_slots(long long pairs, int n_experts, int T) { return (int)(pairs / T) + n_experts; }

@@ -230,11 +230,14 @@ __device__ __forceinline__ uint32_t lds_addr(const void *p) {
 // KS > 1 KS waves share two tiles' groups out.  Weights go straight from memory into
 // registers, each row read by one wave, DEEP groups ahead of their products; the tokens'
 // records, which all waves read, come through LDS by DMA, CH groups of T tokens a
-// buffer, two buffers.  BOTH: a step decodes both tiles, then reads each record once for
-// the two; otherwise one after the other, which halves the registers of the decoded rows.
-__host__ __device__ constexpr int tile_chunk(int TT) { return TT == 1 ? 4 : TT == 2 ? 2 : 1; }
+// buffer, two buffers.  A step takes one of its row tiles after the other, so that
+// only one's decoded rows are in registers (both at once read each record once, but with a
+// third more registers and 2 waves a SIMD for 3: 512 tokens 109 us so, 103 one by one).
+__host__ __device__ constexpr int tile_chunk(int TT) { return TT == 2 ? 2 : 1; }
 __host__ __device__ constexpr int tile_lds(int TT) { return 2 * tile_chunk(TT) * 16 * TT * kMoeRec; }
 constexpr int kTileWaves = 4;
+// Groups of weights ahead: two where a step's products are too short to hide a load behind.
+constexpr int tile_deep(int TT) { return TT <= 2 ? 2 : 1; }
 
 // Sums made where they stand: left to the compiler, all tiles' integer sums wait in
 // registers for the end of a step.
@@ -242,8 +245,8 @@ __device__ __forceinline__ void pin(float (&v)[4]) {
     asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
 }
 
-template <class F, bool PAIR, int TT, bool BOTH, int DEEP>
-__global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a, int ks_log, int slots, int n_blk) {
+template <class F, bool PAIR, int TT, int DEEP>
+__global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a, int ks_log, int each, int slots, int n_blk) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ int s_pair[16 * TT];
     constexpr int T = 16 * TT, CH = tile_chunk(TT), kBuf = CH * T * kMoeRec;
@@ -257,7 +260,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
     const int slot = (int)(blockIdx.x & 7u) * each8 + local / n_blk;
     if (slot >= slots) return;
     const MoeTile tile = a.tiles[slot];
-    if (tile.count == 0) return;
+    if (tile.rest == 0 || tile.index % each != 0) return;  // (this kernel's tile is `each` of the sort's)
+    const int pairs = min(tile.rest, T);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int g = lane >> 4, r16 = lane & 15;
@@ -268,7 +272,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
     const int chs = CH >> ks_log;  // groups of a part in a buffer
     const int n_chunk = (((a.groups + KS - 1) >> ks_log) + chs - 1) / chs, n_step = n_chunk * chs;
 
-    if ((int)threadIdx.x < T) s_pair[threadIdx.x] = a.order[tile.start + min((int)threadIdx.x, tile.count - 1)];
+    if ((int)threadIdx.x < T) s_pair[threadIdx.x] = a.order[tile.start + min((int)threadIdx.x, pairs - 1)];
     __syncthreads();
     // The DMAs' sources, in units of 16 bytes: piece p of a buffer is piece p % 19 of record
     // p / 19, token p / 19 % T's group p / 19 / T: group p / 19 / T / KS of part p / 19 / T % KS.
@@ -317,49 +321,24 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
             if (v + chs < n_step) stage((v / chs + 1) & 1);
         }
         const uint8_t *rec = lds + ((v / chs) & 1) * kBuf + (((v & (chs - 1)) << ks_log) + ks) * (T * kMoeRec) + r16 * kMoeRec;
-        const int count = u0 + v < u1 ? tile.count : 0;
-        if constexpr (BOTH) {
-            typename F::Op op[2];
-            MoeScales<F> s[2];
+        const int count = u0 + v < u1 ? pairs : 0;
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
-                F::decode(op[rt], wv[rt], g);
-                moe_hold_op(op[rt]);
-                s[rt].from(op[rt], g);
-            }
+        for (int rt = 0; rt < 2; ++rt) {
+            typename F::Op op;
+            MoeScales<F> s;
+            F::decode(op, wv[rt], g);
+            moe_hold_op(op);
+            s.from(op, g);
             __builtin_amdgcn_sched_barrier(0);
-            load(wv[0], 0);
-            load(wv[1], 1);
-            ++next;
+            load(wv[rt], rt);
+            if (rt == 1) ++next;
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt) {
                 if (16 * tt >= count) break;
                 typename F::X x;
                 moe_load_x<F>(x, rec + 16 * tt * kMoeRec, g);
-#pragma unroll
-                for (int rt = 0; rt < 2; ++rt) s[rt].dot(acc[rt][tt], op[rt], x);
-#pragma unroll
-                for (int rt = 0; rt < 2; ++rt) pin(acc[rt][tt]);
-            }
-        } else {
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
-                typename F::Op op;
-                MoeScales<F> s;
-                F::decode(op, wv[rt], g);
-                moe_hold_op(op);
-                s.from(op, g);
-                __builtin_amdgcn_sched_barrier(0);
-                load(wv[rt], rt);
-                if (rt == 1) ++next;
-#pragma unroll
-                for (int tt = 0; tt < TT; ++tt) {
-                    if (16 * tt >= count) break;
-                    typename F::X x;
-                    moe_load_x<F>(x, rec + 16 * tt * kMoeRec, g);
-                    s.dot(acc[rt][tt], op, x);
-                    pin(acc[rt][tt]);
-                }
+                s.dot(acc[rt][tt], op, x);
+                pin(acc[rt][tt]);
             }
         }
     };
@@ -392,7 +371,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
 #pragma unroll
     for (int tt = 0; tt < TT; ++tt) {
         const int at = 16 * tt + r16;
-        if (at >= tile.count) continue;
+        if (at >= pairs) continue;
         const size_t pair = (size_t)s_pair[at];
         if (PAIR) {
             if (row0 + 4 * g < a.rows)
@@ -404,6 +383,11 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
                     moe_finish<false>(a, tile.expert, pair, row0 + 16 * rt + 4 * g, acc[rt][tt], acc[rt][tt]);
         }
     }
+}
+
+template <class F, bool PAIR, int TT>
+constexpr auto tile_kernel() {
+    return moe_tile_kernel<F, PAIR, TT, tile_deep(TT)>;
 }
 
 // ------------------------------------------------------------------ a token's parts
@@ -457,32 +441,17 @@ bool moe_one(long long pairs) {
 int moe_tile(long long pairs, int n_experts) {
     const int knob = tuning_knob("EXQ_MOE_TILE", 0);
     if (knob != 0) return knob;
-    return pairs <= 12LL * n_experts ? 16 : pairs <= 24LL * n_experts ? 32 : pairs <= 48LL * n_experts ? 64 : 128;
-}
-
-// Whether a format's tiles of TT decode two row tiles at once, and its groups of weights ahead: as many as
-// leave no register in scratch memory.
-template <class F>
-constexpr bool tile_both(int TT) {
-    return TT >= 4 && (F::kType == kTypeQ4_K || (F::kType == kTypeQ5_K && TT < 8));
-}
-template <class F>
-constexpr int tile_deep(int TT) {
-    return TT <= 2 ? 2 : 1;
-}
-template <class F, bool PAIR, int TT>
-constexpr auto tile_kernel() {
-    return moe_tile_kernel<F, PAIR, TT, tile_both<F>(TT), tile_deep<F>(TT)>;
+    return pairs <= 16LL * n_experts ? 32 : 64;
 }
 
 template <class F, bool PAIR, int TT>
-void moe_tiles(const MoeArgs &a, int slots, int ks_log, hipStream_t st) {
+void moe_tiles(const MoeArgs &a, int each, int slots, int ks_log, hipStream_t st) {
     const int rows = (PAIR ? 16 : 32) * (kTileWaves >> ks_log);
     const int n_blk = (a.rows + rows - 1) / rows;
     // (a slot and 16 rows or more a workgroup: what the pairs' rows take in device memory keeps that below 2^31)
     const dim3 grid((unsigned)((slots + 7) / 8) * 8u * (unsigned)n_blk);
-    hipLaunchKernelGGL((tile_kernel<F, PAIR, TT>()), grid, dim3(64 * kTileWaves), tile_lds(TT), st, a, ks_log, slots,
-                       n_blk);
+    hipLaunchKernelGGL((tile_kernel<F, PAIR, TT>()), grid, dim3(64 * kTileWaves), tile_lds(TT), st, a, ks_log, each,
+                       slots, n_blk);
 }
 
 template <class F, bool PAIR>
@@ -511,32 +480,34 @@ bool moe_run(const edgexpu_hip_moe *p, MoeArgs &a, bool pair, hipStream_t st, co
     float *out = a.out;
     if (!pair) a.out = p->part;
     const int slots = moe_slots(pairs, p->n_experts, p->tile);
-    const int ks_knob = tuning_knob("EXQ_MOE_KS", 0);
-    const int ks = std::min(ks_knob, p->tile == 16 ? 2 : p->tile == 32 ? 1 : 0);
-#define MOE_TILES(TT)                          \
-    if (pair)                                  \
-        moe_tiles<F, true, TT>(a, slots, ks, st);  \
-    else                                       \
-        moe_tiles<F, false, TT>(a, slots, ks, st);
-    if (p->tile == 16) {
-        MOE_TILES(1)
-    } else if (p->tile == 32) {
-        MOE_TILES(2)
-    } else if (p->tile == 64) {
-        MOE_TILES(4)
-    } else {
-        MOE_TILES(8)
+    // two waves share two row tiles' groups where the tiles are too few to fill the chip (12 tokens
+    // of 8 experts, 4096 rows of 14336: 256 workgroups 70 us, 512 so 62 us)
+    const long long blocks = (std::min<long long>(p->n_experts, pairs) + pairs / 32) * ((a.rows + 127) / 128);
+    const int ks_knob = tuning_knob("EXQ_MOE_KS", -1);
+    const int ks = p->tile != 32 ? 0 : ks_knob >= 0 ? ks_knob : !pair && blocks < 512 ? 1 : 0;
+    const bool wide = F::kWide && pairs > 48LL * p->n_experts;
+#define MOE_TILES(TT, EACH)                              \
+    if (pair)                                            \
+        moe_tiles<F, true, TT>(a, EACH, slots, ks, st);  \
+    else                                                 \
+        moe_tiles<F, false, TT>(a, EACH, slots, ks, st);
+    if (p->tile == 32) {
+        MOE_TILES(2, 1)
+    } else if (!wide) {
+        MOE_TILES(4, 1)
+    } else if constexpr (F::kWide) {
+        MOE_TILES(8, 2)
     }
 #undef MOE_TILES
     if (!lib_hip(hipGetLastError(), what)) return false;
     if (pair) return true;
     const bool vec = (a.rows & 3) == 0;
-    const unsigned blocks = (unsigned)(((size_t)p->m * (vec ? a.rows / 4 : a.rows) + 255) / 256);
+    const unsigned joins = (unsigned)(((size_t)p->m * (vec ? a.rows / 4 : a.rows) + 255) / 256);
     if (vec)
-        hipLaunchKernelGGL(moe_join_kernel<true>, dim3(blocks), dim3(256), 0, st, p->part, a.ids, a.residual, out, p->m,
+        hipLaunchKernelGGL(moe_join_kernel<true>, dim3(joins), dim3(256), 0, st, p->part, a.ids, a.residual, out, p->m,
                            p->top_k, a.rows);
     else
-        hipLaunchKernelGGL(moe_join_kernel<false>, dim3(blocks), dim3(256), 0, st, p->part, a.ids, a.residual, out,
+        hipLaunchKernelGGL(moe_join_kernel<false>, dim3(joins), dim3(256), 0, st, p->part, a.ids, a.residual, out,
                            p->m, p->top_k, a.rows);
     return lib_hip(hipGetLastError(), what);
 }
@@ -649,8 +620,8 @@ edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens
                   n_experts, kMoeMaxTopK, kMoeMaxExperts, max_tokens, n_embd, n_ff);
         return nullptr;
     }
-    if (!lib_ready("moe_create") || !moe_prepare<MoeQ4K>() || !moe_prepare<MoeQ5K>() || !moe_prepare<MoeQ6K>() ||
-        !moe_prepare<MoeQ80>() || !moe_prepare<MoeQ40>() || !moe_prepare<MoeQ50>())
+    if (!lib_ready("moe_create") || !moe_prepare<MoeQ6K>() || !moe_prepare<MoeQ80>() || !moe_prepare<MoeQ40>() ||
+        !moe_prepare<MoeQ50>())
         return nullptr;
     edgexpu_hip_moe *p = new (std::nothrow) edgexpu_hip_moe();
     if (p == nullptr) {
@@ -664,7 +635,7 @@ edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens
     p->n_ff = n_ff;
     const size_t pairs = (size_t)max_tokens * top_k;
     const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    const size_t sizes[6] = {4 * pairs, 4 * pairs, 4 * pairs, sizeof(MoeTile) * moe_slots(pairs, n_experts, 16),
+    const size_t sizes[6] = {4 * pairs, 4 * pairs, 4 * pairs, sizeof(MoeTile) * moe_slots(pairs, n_experts, 32),
                              kMoeRec * (std::max((size_t)moe_groups(n_embd) * max_tokens, (size_t)moe_groups(n_ff) * pairs) + 8),
                              4 * pairs * n_embd};
     size_t total = 0, at[6];

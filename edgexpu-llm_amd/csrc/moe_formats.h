@@ -64,7 +64,6 @@ __device__ __forceinline__ long two_words(uint32_t lo, uint32_t hi) {
 __device__ __forceinline__ uint32_t mul_u16x2(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, a) * __builtin_bit_cast(u16x2, b));
 }
-__device__ __forceinline__ uint32_t twice(uint32_t v) { return (v & 0xffffu) | (v << 16); }
 __device__ __forceinline__ v4i as_v4i(const uint4 &v) { return v4i{(int)v.x, (int)v.y, (int)v.z, (int)v.w}; }
 
 // ------------------------------------------------------------- activations
@@ -239,16 +238,39 @@ __device__ __forceinline__ SixBits six_bits(const uint4 &hd) {
     b.m[1] = ((hd.w >> 4) & 0x0f0f0f0fu) | ((hd.z >> 2) & 0x30303030u);
     return b;
 }
+// The digits of four scales at once, and one of them in both halves of a word: byte
+// 2 (g / 2) + h is the chunk's h-th scale for lane group g.
+struct Digits8 {
+    uint32_t lo[2], hi[2];
+};
+__device__ __forceinline__ Digits8 digits8(const SixBits &b) {
+    Digits8 d;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        d.lo[i] = b.s[i] & 0x07070707u;
+        d.hi[i] = (b.s[i] >> 3) & 0x07070707u;
+    }
+    return d;
+}
+__device__ __forceinline__ uint32_t both_halves(uint32_t bytes, int g, int h) {
+    return __builtin_amdgcn_perm(0u, bytes, 0x0c000c00u + 0x00010001u * (uint32_t)(2 * (g >> 1) + h));
+}
 // Minima of lane group g's four 16-element sums.
 __device__ __forceinline__ v4h min_operand(const SixBits &b, int g) {
-    const uint32_t mm = ((g & 2) ? b.m[1] : b.m[0]) >> (16 * (g & 1));
-    const _Float16 x = (_Float16)(float)(mm & 0xffu), y = (_Float16)(float)((mm >> 8) & 0xffu);
-    return v4h{x, x, y, y};
+    // a byte below 0x64 is the f16 1024 + m
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const uint32_t w = (g & 2) ? b.m[1] : b.m[0];
+    const uint32_t sel = 0x04000400u + 0x00010001u * (uint32_t)(2 * (g & 1));
+    const h2 k = {(_Float16)1024.0f, (_Float16)1024.0f};
+    const h2 x = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, sel)) - k;
+    const h2 y = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, sel + 0x00010001u)) - k;
+    return v4h{x[0], x[1], y[0], y[1]};
 }
 
 struct MoeQ4K {
     static constexpr bool kK = true, kMin = true, kTurned = false;
     static constexpr int kType = kTypeQ4_K, kDigits = 2, kBytes = kBytesQ4_K;
+    static constexpr bool kWide = false;
     struct W {
         uint4 hd, q[2];
     };
@@ -267,16 +289,15 @@ struct MoeQ4K {
     }
     __device__ static __forceinline__ void decode(Op &o, const W &w, int g) {
         const SixBits b = six_bits(w.hd);
+        const Digits8 dg = digits8(b);
         o.mn = min_operand(b, g);
         o.dm = w.hd.x;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint32_t two = b.s[i] >> (16 * (g >> 1));  // the chunk's two scales
             const uint32_t q[4] = {w.q[i].x, w.q[i].y, w.q[i].z, w.q[i].w};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t sc = (two >> (8 * h)) & 0xffu;
-                const uint32_t s0 = twice(sc & 7u), s1 = twice(sc >> 3);
+                const uint32_t s0 = both_halves(dg.lo[i], g, h), s1 = both_halves(dg.hi[i], g, h);
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
                     const uint32_t c = (q[v] >> (4 * h)) & 0x0f0f0f0fu;
@@ -291,6 +312,7 @@ struct MoeQ4K {
 struct MoeQ5K {
     static constexpr bool kK = true, kMin = true, kTurned = true;
     static constexpr int kType = kTypeQ5_K, kDigits = 2, kBytes = kBytesQ5_K;
+    static constexpr bool kWide = false;
     struct W {
         uint4 hd, h, q[2];
     };
@@ -306,17 +328,16 @@ struct MoeQ5K {
     }
     __device__ static __forceinline__ void decode(Op &o, const W &w, int g) {
         const SixBits b = six_bits(w.hd);
+        const Digits8 dg = digits8(b);
         o.mn = min_operand(b, g);
         o.dm = w.hd.x;
         const uint32_t fifth[4] = {w.h.x, w.h.y, w.h.z, w.h.w};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint32_t two = b.s[i] >> (16 * (g >> 1));
             const uint32_t q[4] = {w.q[i].x, w.q[i].y, w.q[i].z, w.q[i].w};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t sc = (two >> (8 * h)) & 0xffu;
-                const uint32_t s0 = twice(sc & 7u), s1 = twice(sc >> 3);
+                const uint32_t s0 = both_halves(dg.lo[i], g, h), s1 = both_halves(dg.hi[i], g, h);
                 const int bit = 4 * i + 2 * (g >> 1) + h;  // of the 64-element chunk 2 i + g / 2, half h
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
@@ -349,6 +370,7 @@ __device__ __forceinline__ void join_even(uint32_t (&v)[4], const Even16 &e, uin
 struct MoeQ6K {
     static constexpr bool kK = true, kMin = false, kTurned = false;
     static constexpr int kType = kTypeQ6_K, kDigits = 3, kBytes = kBytesQ6_K;
+    static constexpr bool kWide = true;
     struct W {
         Even16 l[2], h[2];
         uint32_t sc[4];  // scales g, 4 + g, 8 + g, 12 + g
@@ -470,6 +492,7 @@ __device__ __forceinline__ uint32_t load_scales(const uint8_t *row, int u, int n
 struct MoeQ80 {
     static constexpr bool kK = false, kQ80 = true;
     static constexpr int kType = kTypeQ8_0, kBytes = kBytesQ8_0;
+    static constexpr bool kWide = true;
     struct W {
         uint4 q[4];
         uint32_t d;
@@ -505,6 +528,7 @@ __device__ __forceinline__ uint32_t less_each(uint32_t c, uint32_t bias) {
 struct MoeQ40 {
     static constexpr bool kK = false, kQ80 = false;
     static constexpr int kType = kTypeQ4_0, kBytes = kBytesQ4_0;
+    static constexpr bool kWide = true;
     struct W {
         uint32_t q[8], d;
     };
@@ -531,6 +555,7 @@ struct MoeQ40 {
 struct MoeQ50 {
     static constexpr bool kK = false, kQ80 = false;
     static constexpr int kType = kTypeQ5_0, kBytes = kBytesQ5_0;
+    static constexpr bool kWide = true;
     struct W {
         uint32_t q[8], h[8], d;
     };

@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t *_
     const int slot0 = less / T + e, slot1 = e + 1 < n_experts ? (less + own) / T + e + 1 : slots;
     for (int s = slot0 + tid; s < slot1; s += kSortThreads) {
         const int at = (s - slot0) * T;
-        tiles[s] = MoeTile{e, less + at, max(0, min(T, own - at)), 0};
+        tiles[s] = MoeTile{e, less + at, max(0, own - at), s - slot0};
     }
     int base = less;
     // (every thread runs the same rounds: base and own are the workgroup's)
