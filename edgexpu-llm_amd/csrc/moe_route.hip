@@ -10,6 +10,7 @@
 //
 // One wave a token: lane l holds experts l, l + 64, ..., so a row is read in
 // whole lines.
+#include <algorithm>
 #include <cmath>
 
 #include "moe.h"
@@ -17,148 +18,192 @@
 namespace exq {
 
 constexpr int kRouteWaves = 4;
-constexpr int kRouteSlots = kMoeMaxExperts / 64;
 
-// A double's order as an unsigned integer's (minus infinity above zero; 0 is below every number).
+// A double's order as an unsigned integer's.  0 is below every number's key, and so is
+// every key whose high word is 0.
 __device__ __forceinline__ uint64_t order_key(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     return (b >> 63) ? ~b : b | 0x8000000000000000ull;
 }
-constexpr uint64_t kNoKey = 0;  // not to be chosen
 
-__device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int off) {
-    const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, off, 64);
-    const uint32_t hi = (uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), off, 64);
-    return (uint64_t)lo | ((uint64_t)hi << 32);
+// Reductions over the wave by DPP (row shifts, then row broadcasts: the total arrives in
+// lane 63): a step is a few cycles, where one through LDS is a hundred, and a token's
+// choices are one chain of them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or(uint32_t old, uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const uint64_t o = shfl_xor_u64(v, off);
-        v = o > v ? o : v;
-    }
-    return v;
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    v = max(v, dpp_or<0x111, 0xf>(v, v));
+    v = max(v, dpp_or<0x112, 0xf>(v, v));
+    v = max(v, dpp_or<0x114, 0xf>(v, v));
+    v = max(v, dpp_or<0x118, 0xf>(v, v));
+    v = max(v, dpp_or<0x142, 0xa>(v, v));
+    v = max(v, dpp_or<0x143, 0xc>(v, v));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-__device__ __forceinline__ int wave_min_i32(int v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = min(v, __shfl_xor(v, off, 64));
-    return v;
-}
-__device__ __forceinline__ double read_lane_f64(double v, int lane) {
+__device__ __forceinline__ double lane_f64(double v, int lane) {  // (lane: the same in the whole wave)
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)b, lane, 64);
-    const uint32_t hi = (uint32_t)__shfl((int)(uint32_t)(b >> 32), lane, 64);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {  // (lanes without a source add 0)
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = dpp_or<CTRL, ROWS>(0u, (uint32_t)b), hi = dpp_or<CTRL, ROWS>(0u, (uint32_t)(b >> 32));
+    return v + __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
+}
+__device__ __forceinline__ double wave_add_f64(double v) {
+    v = dpp_add<0x111, 0xf>(v);
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);
+    v = dpp_add<0x143, 0xc>(v);
+    return lane_f64(v, 63);
+}
+__device__ __forceinline__ double shfl_xor_f64(double v, int off) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)b, off, 64);
+    const uint32_t hi = (uint32_t)__shfl_xor((int)(uint32_t)(b >> 32), off, 64);
     return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
 }
 
+// S = ceil(n_experts / 64) experts a lane.
+template <int S>
 __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(RouteArgs a) {
-    __shared__ double cs[kRouteWaves][kMoeMaxExperts];
+    __shared__ double cs[kRouteWaves][64 * S];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     // (a wave past the last token repeats it and writes nothing: all reach the barrier)
-    const bool mine_t = (int)blockIdx.x * kRouteWaves + wave < a.m;
-    const int t = mine_t ? (int)blockIdx.x * kRouteWaves + wave : a.m - 1;
+    const bool own = (int)blockIdx.x * kRouteWaves + wave < a.m;
+    const int t = own ? (int)blockIdx.x * kRouteWaves + wave : a.m - 1;
     const float *s = a.scores + (size_t)t * a.n_experts;
-    double p[kRouteSlots];
-    bool live[kRouteSlots];
-    double top = -INFINITY;
+    float sc[S];
+    bool live[S];
+    uint32_t top = 0u;  // the largest live score's order
 #pragma unroll
-    for (int i = 0; i < kRouteSlots; ++i) {
+    for (int i = 0; i < S; ++i) {
         const int e = lane + 64 * i;
-        p[i] = e < a.n_experts ? (double)s[e] : INFINITY;
-        live[i] = fabs(p[i]) < INFINITY;
-        if (live[i]) top = fmax(top, p[i]);
+        sc[i] = e < a.n_experts ? s[e] : INFINITY;
+        live[i] = fabsf(sc[i]) < INFINITY;
+        const uint32_t b = __float_as_uint(sc[i]);
+        if (live[i]) top = max(top, (b >> 31) ? ~b : b | 0x80000000u);
     }
+    double p[S];
     if (a.sigmoid) {
 #pragma unroll
-        for (int i = 0; i < kRouteSlots; ++i) p[i] = live[i] ? 1.0 / (1.0 + exp(-p[i])) : 0.0;
+        for (int i = 0; i < S; ++i) p[i] = live[i] ? 1.0 / (1.0 + exp(-(double)sc[i])) : 0.0;
     } else {
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) {
-            const uint64_t o = shfl_xor_u64(__builtin_bit_cast(uint64_t, top), off);
-            top = fmax(top, __builtin_bit_cast(double, o));
-        }
+        top = wave_max_u32(top);
+        const double mx = (double)__uint_as_float((top >> 31) ? top & 0x7fffffffu : ~top);
         double sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kRouteSlots; ++i) {
-            p[i] = live[i] ? exp(p[i] - top) : 0.0;
+        for (int i = 0; i < S; ++i) {
+            p[i] = live[i] ? exp((double)sc[i] - mx) : 0.0;
             sum += p[i];
         }
-        sum = wave_sum_f64(sum);  // (0 only where no score is live)
+        const double inv = 1.0 / wave_add_f64(sum);  // (the sum is 0 only where no score is live)
 #pragma unroll
-        for (int i = 0; i < kRouteSlots; ++i) p[i] = live[i] ? p[i] / sum : 0.0;
+        for (int i = 0; i < S; ++i) p[i] = live[i] ? p[i] * inv : 0.0;
     }
-    uint64_t key[kRouteSlots];
+    uint32_t hi[S], lo[S];  // the choice's keys
 #pragma unroll
-    for (int i = 0; i < kRouteSlots; ++i) {
+    for (int i = 0; i < S; ++i) {
         const int e = lane + 64 * i;
         const double c = live[i] && a.bias != nullptr ? p[i] + (double)a.bias[e] : p[i];
-        key[i] = live[i] && fabs(c) < INFINITY ? order_key(c) : kNoKey;
-        if (a.n_groups > 1 && e < a.n_experts) cs[wave][e] = key[i] != kNoKey ? c : -INFINITY;
+        const bool open = live[i] && fabs(c) < INFINITY;
+        const uint64_t key = open ? order_key(c) : 0ull;
+        hi[i] = (uint32_t)(key >> 32);
+        lo[i] = (uint32_t)key;
+        if (a.n_groups > 1) cs[wave][e] = open ? c : -INFINITY;
     }
     if (a.n_groups > 1) {
-        // lane g ranks group g
         __syncthreads();
-        const int per = a.n_experts / a.n_groups;
+        // `width` lanes a group, each over its share of the group's values
+        const int per = a.n_experts / a.n_groups, log = 31 - __clz(64 / a.n_groups), width = 1 << log;
+        const int mine = lane >> log;
         double b0 = -INFINITY, b1 = -INFINITY;
-        if (lane < a.n_groups)
-            for (int i = 0; i < per; ++i) {
-                const double c = cs[wave][lane * per + i];
-                if (c > b0) {
-                    b1 = b0;
-                    b0 = c;
-                } else if (c > b1) {
-                    b1 = c;
-                }
-            }
+        const auto take = [&](double c) {
+            b1 = fmax(b1, fmin(b0, c));
+            b0 = fmax(b0, c);
+        };
+        if (mine < a.n_groups)
+            for (int i = lane & (width - 1); i < per; i += width) take(cs[wave][mine * per + i]);
+        for (int off = width >> 1; off > 0; off >>= 1) {
+            const double o0 = shfl_xor_f64(b0, off), o1 = shfl_xor_f64(b1, off);
+            take(o0);
+            take(o1);
+        }
         const double rank = a.group_best == 2 && b1 > -INFINITY ? b0 + b1 : b0;
         int ahead = 0;
         for (int g = 0; g < a.n_groups; ++g) {
-            const double o = read_lane_f64(rank, g);
-            ahead += o > rank || (o == rank && g < lane) ? 1 : 0;
+            const double o = lane_f64(rank, g << log);
+            ahead += o > rank || (o == rank && g < mine) ? 1 : 0;
         }
-        const unsigned long long stay = __ballot(lane < a.n_groups && ahead < a.top_groups);
+        const unsigned long long stay = __ballot(mine < a.n_groups && ahead < a.top_groups);
 #pragma unroll
-        for (int i = 0; i < kRouteSlots; ++i) {
+        for (int i = 0; i < S; ++i) {
             const int e = lane + 64 * i;
-            if (e < a.n_experts && !((stay >> (e / per)) & 1ull)) key[i] = kNoKey;
+            if (e < a.n_experts && !((stay >> ((e / per) << log)) & 1ull)) hi[i] = lo[i] = 0u;
         }
     }
-    // the choices, one after the other; lane j keeps the j-th
+    // The choices, one after the other; lane j keeps the j-th.  The largest high word
+    // mostly says which; where several have it, the largest low word among them, and
+    // of equals the first slot's first lane, the lowest number.
     int id = -1;
     double w = 0.0, total = 0.0;
     for (int j = 0; j < a.top_k; ++j) {
-        uint64_t best = kNoKey;
+        uint32_t best = hi[0];
 #pragma unroll
-        for (int i = 0; i < kRouteSlots; ++i) best = key[i] > best ? key[i] : best;
-        const uint64_t all = wave_max_u64(best);
-        if (all == kNoKey) break;  // (the same in every lane)
-        int mine = kMoeMaxExperts;
+        for (int i = 1; i < S; ++i) best = max(best, hi[i]);
+        const uint32_t H = wave_max_u32(best);
+        if (H == 0u) break;
+        unsigned long long has[S];
+        int n = 0;
 #pragma unroll
-        for (int i = kRouteSlots - 1; i >= 0; --i)
-            if (key[i] == all) mine = lane + 64 * i;
-        const int e = wave_min_i32(mine);
-        double pe = 0.0;
+        for (int i = 0; i < S; ++i) {
+            has[i] = __ballot(hi[i] == H);
+            n += __popcll(has[i]);
+        }
+        if (n > 1) {
+            uint32_t low = 0u;
 #pragma unroll
-        for (int i = 0; i < kRouteSlots; ++i)
-            if (lane + 64 * i == e) {
-                key[i] = kNoKey;
-                pe = p[i];
+            for (int i = 0; i < S; ++i)
+                if (hi[i] == H) low = max(low, lo[i]);
+            const uint32_t L = wave_max_u32(low);
+#pragma unroll
+            for (int i = 0; i < S; ++i) has[i] &= __ballot(lo[i] == L);
+        }
+        int slot = S - 1;
+        double ps = p[S - 1];
+        unsigned long long first = has[S - 1];
+#pragma unroll
+        for (int i = S - 2; i >= 0; --i)
+            if (has[i] != 0ull) {
+                slot = i;
+                ps = p[i];
+                first = has[i];
             }
-        pe = read_lane_f64(pe, e & 63);
+        const int at = __ffsll((long long)first) - 1;
+        const double pe = lane_f64(ps, at);
         total += pe;
         if (lane == j) {
-            id = e;
+            id = 64 * slot + at;
             w = pe;
         }
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+            if (slot == i && lane == at) hi[i] = lo[i] = 0u;
     }
-    if (mine_t && lane < a.top_k) {
+    if (own && lane < a.top_k) {
         if (a.normalise && total > 0.0) w /= total;
-        const float wf = (float)(w * a.scale);
+        const float wf = id >= 0 ? (float)(w * a.scale) : 0.0f;
         const size_t at = (size_t)t * a.top_k + lane;
         a.ids[at] = id;
-        a.weights[at] = id >= 0 ? wf : 0.0f;
+        a.weights[at] = wf;
         if (a.ids_out != nullptr) a.ids_out[at] = id;
-        if (a.weights_out != nullptr) a.weights_out[at] = id >= 0 ? wf : 0.0f;
+        if (a.weights_out != nullptr) a.weights_out[at] = wf;
     }
 }
 
@@ -177,108 +222,117 @@ __global__ __launch_bounds__(256) void moe_assign_kernel(const int32_t *__restri
 // own, then writes its own pairs in ascending order (so the sort is stable and the
 // same every time) and its tiles.  Every workgroup reads all ids, 4 bytes a pair from
 // L2, and none waits for another.
-constexpr int kSortThreads = 1024, kSortEach = 8;  // (ids are read 8 a thread)
-struct Ids8 {
-    int v[kSortEach];
-};
-// Pairs first .. + 7, those past the last as no pair's id.
-__device__ __forceinline__ Ids8 load_ids(const int32_t *ids, int first, int pairs) {
-    Ids8 r;
-    const int4 *p = reinterpret_cast<const int4 *>(ids + first);
-    const int4 none = make_int4(-1, -1, -1, -1);
-    const int4 a = first < pairs ? p[0] : none, b = first + 4 < pairs ? p[1] : none;
-    const int v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int k = 0; k < 8; ++k) r.v[k] = first + k < pairs ? v[k] : -1;
-    return r;
-}
+constexpr int kSortThreads = 1024, kSortMost = 32;  // ids a thread and round, read 4 at once
 __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t *__restrict__ ids, int pairs,
-                                                                int n_experts, int T, int slots,
+                                                                int n_experts, int T, int slots, int each,
                                                                 int32_t *__restrict__ order,
                                                                 MoeTile *__restrict__ tiles) {
-    constexpr int kWaves = kSortThreads / 64, kRound = kSortThreads * kSortEach, kKeep = 4;
+    constexpr int kWaves = kSortThreads / 64;
     __shared__ int sums[2][kWaves];
     const int e = (int)blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    Ids8 kept[kKeep];  // the first rounds' ids stay in registers for the second pass
-    int less = 0, own = 0;
+    const int round = each * kSortThreads;
+    // A thread's ids of a round from `first` on (each of them, those past the last as -1):
+    // which are this expert's, and how many are of those before it.
+    const auto read = [&](int first, int &less) {
+        int4 v[kSortMost / 4];
 #pragma unroll
-    for (int i = 0; i < kKeep; ++i) kept[i] = load_ids(ids, i * kRound + tid * kSortEach, pairs);
-    const auto count = [&](const Ids8 &c) {
+        for (int j = 0; j < kSortMost / 4; ++j)
+            v[j] = 4 * j < each && first + 4 * j < pairs ? *reinterpret_cast<const int4 *>(ids + first + 4 * j)
+                                                         : make_int4(-1, -1, -1, -1);
+        unsigned hit = 0u;
 #pragma unroll
-        for (int k = 0; k < kSortEach; ++k) {
-            less += c.v[k] >= 0 && c.v[k] < e ? 1 : 0;
-            own += c.v[k] == e ? 1 : 0;
+        for (int j = 0; j < kSortMost / 4; ++j) {
+            const int q[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int id = first + 4 * j + k < pairs ? q[k] : -1;
+                less += (unsigned)id < (unsigned)e ? 1 : 0;
+                hit |= id == e ? 1u << (4 * j + k) : 0u;
+            }
         }
+        return hit;
     };
+    int less = 0, own = 0;
+    const unsigned hit0 = read(tid * each, less);
+    own = __popc(hit0);
+    for (int i0 = round; i0 < pairs; i0 += round) own += __popc(read(i0 + tid * each, less));
+    int before = __popc(hit0);  // of the first round: inclusive over the wave
 #pragma unroll
-    for (int i = 0; i < kKeep; ++i) count(kept[i]);
-    for (int i0 = kKeep * kRound; i0 < pairs; i0 += kRound) count(load_ids(ids, i0 + tid * kSortEach, pairs));
+    for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(before, off, 64);
+        if (lane >= off) before += o;
+    }
+    __shared__ int first_sums[kWaves];
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
         less += __shfl_xor(less, off, 64);
         own += __shfl_xor(own, off, 64);
     }
-    if (lane == 0) {
+    if (lane == 63) {
         sums[0][wave] = less;
         sums[1][wave] = own;
+        first_sums[wave] = before;
     }
     __syncthreads();
     less = own = 0;
+    int at = before - __popc(hit0), total = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
         less += sums[0][w];
         own += sums[1][w];
+        at += w < wave ? first_sums[w] : 0;
+        total += first_sums[w];
     }
     const int slot0 = less / T + e, slot1 = e + 1 < n_experts ? (less + own) / T + e + 1 : slots;
     for (int s = slot0 + tid; s < slot1; s += kSortThreads) {
-        const int at = (s - slot0) * T;
-        tiles[s] = MoeTile{e, less + at, max(0, own - at), s - slot0};
+        const int from = (s - slot0) * T;
+        tiles[s] = MoeTile{e, less + from, max(0, own - from), s - slot0};
     }
-    int base = less;
-    // (every thread runs the same rounds: base and own are the workgroup's)
-    const auto place = [&](const Ids8 &c, int first) {
-        unsigned hit = 0u;
-#pragma unroll
-        for (int k = 0; k < kSortEach; ++k)
-            if (c.v[k] == e) hit |= 1u << k;
-        const int mine = __popc(hit);
-        int before = mine;  // inclusive over the wave, then over the waves
+    const auto place = [&](unsigned hit, int first, int to) {
+        while (hit != 0u) {
+            order[to++] = first + __ffs((int)hit) - 1;
+            hit &= hit - 1u;
+        }
+    };
+    place(hit0, tid * each, less + at);
+    int base = less + total;
+    for (int i0 = round; i0 < pairs && base < less + own; i0 += round) {  // (the same rounds in every thread)
+        int unused = 0;
+        const unsigned hit = read(i0 + tid * each, unused);
+        int upto = __popc(hit);
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
-            const int o = __shfl_up(before, off, 64);
-            if (lane >= off) before += o;
+            const int o = __shfl_up(upto, off, 64);
+            if (lane >= off) upto += o;
         }
         __syncthreads();  // (the sums of the round before have been read)
-        if (lane == 63) sums[0][wave] = before;
+        if (lane == 63) first_sums[wave] = upto;
         __syncthreads();
-        int at = base + before - mine, total = 0;
+        int to = base + upto - __popc(hit);
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            at += w < wave ? sums[0][w] : 0;
-            total += sums[0][w];
+            to += w < wave ? first_sums[w] : 0;
+            base += first_sums[w];
         }
-#pragma unroll
-        for (int k = 0; k < kSortEach; ++k)
-            if ((hit >> k) & 1u) order[at++] = first + k;
-        base += total;
-    };
-#pragma unroll
-    for (int i = 0; i < kKeep; ++i)
-        if (i * kRound < pairs && base < less + own) place(kept[i], i * kRound + tid * kSortEach);
-    for (int i0 = kKeep * kRound; i0 < pairs && base < less + own; i0 += kRound)
-        place(load_ids(ids, i0 + tid * kSortEach, pairs), i0 + tid * kSortEach);
+        place(hit, i0 + tid * each, to);
+    }
 }
 
 hipError_t launch_moe_sort(const int32_t *ids, int pairs, int n_experts, int T, int32_t *order, MoeTile *tiles,
                            hipStream_t st) {
+    const int each = std::min(kSortMost, (pairs + 4 * kSortThreads - 1) / (4 * kSortThreads) * 4);
     hipLaunchKernelGGL(moe_sort_kernel, dim3((unsigned)n_experts), dim3(kSortThreads), 0, st, ids, pairs, n_experts, T,
-                       moe_slots(pairs, n_experts, T), order, tiles);
+                       moe_slots(pairs, n_experts, T), each, order, tiles);
     return hipGetLastError();
 }
 
 hipError_t launch_moe_route(const RouteArgs &a, hipStream_t st) {
     const dim3 grid((unsigned)((a.m + kRouteWaves - 1) / kRouteWaves));
-    hipLaunchKernelGGL(moe_route_kernel, grid, dim3(64 * kRouteWaves), 0, st, a);
+    const auto k = a.n_experts <= 64    ? moe_route_kernel<1>
+                   : a.n_experts <= 128 ? moe_route_kernel<2>
+                   : a.n_experts <= 256 ? moe_route_kernel<4>
+                                        : moe_route_kernel<8>;
+    hipLaunchKernelGGL(k, grid, dim3(64 * kRouteWaves), 0, st, a);
     return hipGetLastError();
 }
 
