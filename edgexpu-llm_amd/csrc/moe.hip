@@ -64,106 +64,108 @@ __global__ __launch_bounds__(256) void moe_pack_kernel(MoeArgs a) {
 // launch (down).  Its waves share the groups out, and it quantizes the token's
 // rows itself: a launch less, and the first weights are on their way meanwhile.  All 16
 // columns of the products hold the same token.
-constexpr int kOneWaves = 8;
+constexpr int one_waves(bool) { return 8; }
 
 template <class F, bool PAIR>
-__global__ __launch_bounds__(64 * kOneWaves) void moe_one_kernel(MoeArgs a) {
+__global__ __launch_bounds__(64 * one_waves(PAIR), 4) void moe_one_kernel(MoeArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t recs[];
-    constexpr int RT = PAIR ? 2 : 1;
-    __shared__ float red[kOneWaves][RT][16];
-    __shared__ int s_expert[kMoeMaxTopK], s_place[kMoeMaxTopK], s_n;
+    // gate and up: half the waves each
+    constexpr int kOneWaves = one_waves(PAIR);
+    constexpr int kSets = PAIR ? 2 : 1, kShare = kOneWaves / kSets;
+    // groups whose weights are on their way at once: a wave of a single token mostly has no more
+    constexpr int kAhead = F::kK ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) float red[kOneWaves][16];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int g = lane >> 4, r16 = lane & 15;
     const int row0 = 16 * (int)blockIdx.x;
     const size_t pair0 = PAIR ? (size_t)blockIdx.y : (size_t)blockIdx.y * a.top_k;
 
-    // the experts that there are
-    int n_seg;
-    if (PAIR) {
-        const int e = a.ids[pair0];
-        if (threadIdx.x == 0) s_expert[0] = e;
-        n_seg = e >= 0 ? 1 : 0;
-        __syncthreads();
-    } else {
-        if (wave == 0) {
-            const int e = lane < a.top_k ? a.ids[pair0 + lane] : -1;
-            const unsigned long long some = __ballot(e >= 0);
-            const int at = __popcll(some & ((1ull << lane) - 1ull));
-            if (e >= 0) {
-                s_expert[at] = e;
-                s_place[at] = lane;
-            }
-            if (lane == 0) s_n = __popcll(some);
-        }
-        __syncthreads();
-        n_seg = s_n;
-    }
-    const int units = n_seg * a.groups;
-    const int u0 = units * wave / kOneWaves, u1 = units * (wave + 1) / kOneWaves;
-    const size_t row = (size_t)min(row0 + r16, a.rows - 1) * a.row_bytes;
-    const auto load = [&](typename F::W (&w)[RT], int u) {
-        const int seg = u / a.groups;
-        const size_t at = (size_t)s_expert[seg] * a.expert_bytes + row;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) F::load_w(w[rt], a.w[rt] + at, u - seg * a.groups, a.nblk, g);
+    // The token's rows need nothing from its experts: the first are read before them.
+    const int parts = moe_pack_parts<F::kK>(a.n), all = PAIR ? parts : a.top_k * parts;
+    const float *x = a.x + (PAIR ? pair0 / a.top_k : pair0) * a.n;
+    const auto read = [&](float (&v)[F::kK ? 16 : 8], int p) {
+        const int place = PAIR ? 0 : p / parts;
+        moe_read_part<F::kK>(v, x + (size_t)place * a.n, a.n, p - place * parts);
     };
-    typename F::W w[RT];
-    if (u0 < u1) load(w, u0);
-    // the token's rows
-    const int parts = moe_pack_parts<F::kK>(a.n);
-    for (int p = threadIdx.x; p < n_seg * parts; p += 64 * kOneWaves) {
-        const int seg = p / parts;
-        const size_t from = PAIR ? pair0 / a.top_k : pair0 + s_place[seg];
-        moe_pack_part<F::kK>(a.x + from * a.n, a.n, p - seg * parts, recs + (size_t)seg * a.groups * kMoeRec);
+    float first[F::kK ? 16 : 8];
+    if ((int)threadIdx.x < all) read(first, threadIdx.x);
+
+    // Lane j's expert, place and weight: the j-th that there is (every wave for itself).
+    const int own = PAIR ? 0 : lane;
+    int expert = own < (PAIR ? 1 : a.top_k) ? a.ids[pair0 + own] : -1, place = own, n_seg;
+    float weight = 1.0f;
+    if (PAIR) {
+        n_seg = expert >= 0 ? 1 : 0;
+    } else {
+        weight = lane < a.top_k ? a.weights[pair0 + lane] : 0.0f;
+        const unsigned long long some = __ballot(expert >= 0), below = (1ull << lane) - 1ull;
+        n_seg = __popcll(some);
+        const int at = 4 * (expert >= 0 ? __popcll(some & below) : n_seg + __popcll(~some & below));
+        expert = __builtin_amdgcn_ds_permute(at, expert);
+        place = __builtin_amdgcn_ds_permute(at, place);
+        weight = __int_as_float(__builtin_amdgcn_ds_permute(at, __float_as_int(weight)));
+    }
+    const auto nth = [](int v, int seg) { return PAIR ? v : __builtin_amdgcn_readlane(v, seg); };
+    const int units = n_seg * a.groups;
+    const int part = wave & (kShare - 1), u0 = units * part / kShare, u1 = units * (part + 1) / kShare;
+    const uint8_t *rows = a.w[wave / kShare] + (size_t)min(row0 + r16, a.rows - 1) * a.row_bytes;
+    const auto load = [&](typename F::W &w, int u) {
+        if (u >= u1) return;
+        const int seg = PAIR ? 0 : u / a.groups;
+        F::load_w(w, rows + (size_t)nth(expert, seg) * a.expert_bytes, u - seg * a.groups, a.nblk, g);
+    };
+    typename F::W w[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) load(w[k], u0 + k);
+    if ((int)threadIdx.x < all) moe_put_part<F::kK>(first, threadIdx.x, recs);
+    for (int p = threadIdx.x + 64 * kOneWaves; p < all; p += 64 * kOneWaves) {
+        read(first, p);
+        moe_put_part<F::kK>(first, p, recs);
     }
     __syncthreads();
-    float acc[RT][4] = {};
-    for (int u = u0; u < u1; ++u) {
-        typename F::W next[RT];
-        load(next, min(u + 1, u1 - 1));
-        typename F::X x;
-        moe_load_x<F>(x, recs + (size_t)u * kMoeRec, g);
-        // (down: each group's sum with its expert's weight at once.  A sum kept over an
-        // expert's groups needs a branch right behind the products, and the compiler, where a
-        // short block lies between, leaves out the wait that their results need)
-        const float f = PAIR ? 1.0f : a.weights[pair0 + s_place[u / a.groups]];
+    float acc[4] = {};
+    for (int base = u0; base < u1; base += kAhead)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
+        for (int k = 0; k < kAhead; ++k) {
+            const int u = base + k;
+            if (u >= u1) break;
+            const int seg = PAIR ? 0 : u / a.groups;
             typename F::Op op;
-            F::decode(op, w[rt], g);
+            F::decode(op, w[k], g);
+            moe_hold_op(op);
+            __builtin_amdgcn_sched_barrier(0);
+            load(w[k], u + kAhead);
+            typename F::X x;
+            moe_load_x<F>(x, recs + ((size_t)nth(place, seg) * a.groups + (u - seg * a.groups)) * kMoeRec, g);
             MoeScales<F> s;
             s.from(op, g);
-            float part[4] = {};
-            s.dot(PAIR ? acc[rt] : part, op, x);
+            // (down: each group's sum with its expert's weight at once.  A sum kept over an
+            // expert's groups needs a branch right behind the products, and the compiler, where a
+            // short block lies between, leaves out the wait that their results need)
+            const float f = __int_as_float(nth(__float_as_int(weight), seg));
+            float one[4] = {};
+            s.dot(PAIR ? acc : one, op, x);
             if (!PAIR)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[rt][r] = fmaf(f, part[r], acc[rt][r]);
-            w[rt] = next[rt];
+                for (int r = 0; r < 4; ++r) acc[r] = fmaf(f, one[r], acc[r]);
         }
-    }
-    if (r16 == 0)
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) red[wave][rt][4 * g + r] = acc[rt][r];
+    if (r16 == 0) *reinterpret_cast<float4 *>(&red[wave][4 * g]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
     __syncthreads();
     const int o = row0 + (int)threadIdx.x;
     if (threadIdx.x >= 16 || o >= a.rows) return;
-    float v[RT] = {};
+    float v[kSets] = {};
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int k = 0; k < kOneWaves; ++k) v[rt] += red[k][rt][threadIdx.x];
+    for (int k = 0; k < kOneWaves; ++k) v[k / kShare] += red[k][threadIdx.x];
     if (PAIR) {
-        const size_t b = (size_t)max(s_expert[0], 0) * a.rows + o;
+        const size_t b = (size_t)max(expert, 0) * a.rows + o;
         if (a.bias[0] != nullptr) v[0] += a.bias[0][b];
-        if (a.bias[1] != nullptr) v[RT - 1] += a.bias[1][b];
-        a.out[pair0 * a.rows + o] = n_seg == 0 ? 0.0f : moe_act(v[0], a.activation) * v[RT - 1];
+        if (a.bias[1] != nullptr) v[kSets - 1] += a.bias[1][b];
+        a.out[pair0 * a.rows + o] = n_seg == 0 ? 0.0f : moe_act(v[0], a.activation) * v[kSets - 1];
     } else {
         if (a.bias[0] != nullptr)
             for (int j = 0; j < n_seg; ++j)
-                v[0] = fmaf(a.weights[pair0 + s_place[j]], a.bias[0][(size_t)s_expert[j] * a.rows + o], v[0]);
+                v[0] = fmaf(__int_as_float(nth(__float_as_int(weight), j)), a.bias[0][(size_t)nth(expert, j) * a.rows + o], v[0]);
         const size_t at = (size_t)blockIdx.y * a.rows + o;
         a.out[at] = a.residual != nullptr ? a.residual[at] + v[0] : v[0];
     }
@@ -467,9 +469,9 @@ bool moe_run(const edgexpu_hip_moe *p, MoeArgs &a, bool pair, hipStream_t st, co
         const size_t lds = (size_t)(pair ? 1 : p->top_k) * a.groups * kMoeRec;
         const dim3 grid((unsigned)((a.rows + 15) / 16), (unsigned)(pair ? pairs : p->m));
         if (pair)
-            hipLaunchKernelGGL((moe_one_kernel<F, true>), grid, dim3(64 * kOneWaves), lds, st, a);
+            hipLaunchKernelGGL((moe_one_kernel<F, true>), grid, dim3(64 * one_waves(true)), lds, st, a);
         else
-            hipLaunchKernelGGL((moe_one_kernel<F, false>), grid, dim3(64 * kOneWaves), lds, st, a);
+            hipLaunchKernelGGL((moe_one_kernel<F, false>), grid, dim3(64 * one_waves(false)), lds, st, a);
         return lib_hip(hipGetLastError(), what);
     }
     if (pair)

@@ -133,30 +133,38 @@ __device__ __forceinline__ void moe_pack_0(const float (&a)[8], int b, int g, ui
     if (g == 0) *reinterpret_cast<float *>(rec + kMoeBs + 4 * b) = f16_bits_to_f32(f32_to_f16_rne(amax / 127.0f));
 }
 
-__device__ __forceinline__ void load_f8(const float *p, float (&v)[16], int at) {
+__device__ __forceinline__ void load_f8(const float *p, float *v) {
     const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-    v[at] = a.x, v[at + 1] = a.y, v[at + 2] = a.z, v[at + 3] = a.w;
-    v[at + 4] = b.x, v[at + 5] = b.y, v[at + 6] = b.z, v[at + 7] = b.w;
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
 // Part `part` of a row's packing: K-quants 16 lanes a group of 256, others 32 lanes
 // (4 a block).  x is the row, rec its first record, n its elements.
 template <bool K>
-__device__ __forceinline__ void moe_pack_part(const float *x, int n, int part, uint8_t *rec) {
+__device__ __forceinline__ void moe_read_part(float (&v)[K ? 16 : 8], const float *x, int n, int part) {
     if (K) {
-        const int sb = part >> 4, r = part & 15;
-        float xs[16];
-        const float *p = x + (size_t)sb * kQKK + 64 * (r >> 2) + 8 * (r & 3);
-        load_f8(p, xs, 0);
-        load_f8(p + 32, xs, 8);
-        moe_pack_k(xs, r, rec + (size_t)sb * kMoeRec);
+        const float *p = x + (size_t)(part >> 4) * kQKK + 64 * ((part & 15) >> 2) + 8 * (part & 3);
+        load_f8(p, v);
+        load_f8(p + 32, v + (K ? 8 : 0));
     } else {
-        const int blk = part >> 2, g = part & 3;
-        float v[16] = {0.0f};
-        if (blk * 32 < n) load_f8(x + (size_t)blk * 32 + 8 * g, v, 0);
-        const float a[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
-        moe_pack_0(a, blk & 7, g, rec + (size_t)(blk >> 3) * kMoeRec);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        if ((part >> 2) * 32 < n) load_f8(x + 8 * (size_t)part, v);
     }
+}
+template <bool K>
+__device__ __forceinline__ void moe_put_part(const float (&v)[K ? 16 : 8], int part, uint8_t *rec) {
+    if constexpr (K)
+        moe_pack_k(v, part & 15, rec + (size_t)(part >> 4) * kMoeRec);
+    else
+        moe_pack_0(v, (part >> 2) & 7, part & 3, rec + (size_t)(part >> 5) * kMoeRec);
+}
+template <bool K>
+__device__ __forceinline__ void moe_pack_part(const float *x, int n, int part, uint8_t *rec) {
+    float v[K ? 16 : 8];
+    moe_read_part<K>(v, x, n, part);
+    moe_put_part<K>(v, part, rec);
 }
 __host__ __device__ constexpr int moe_groups(int n) { return (n + kQKK - 1) / kQKK; }
 template <bool K>
@@ -350,21 +358,13 @@ struct MoeQ5K {
     }
 };
 
-// 16 bytes at an even address as the words from the 4-byte address below it (`sh` below) and the half word
-// that ends them; joined once they are needed.  One `sh` serves every piece of a block: wide loads at 2 mod 4
-// run several times slower (ldg16_a2).
-struct Even16 {
-    uint4 w;
-    uint32_t end;
-};
-__device__ __forceinline__ Even16 load_even(const uint8_t *below, uint32_t sh) {
-    return {*reinterpret_cast<const uint4 *>(below), *reinterpret_cast<const uint16_t *>(below + sh + 14)};
-}
-__device__ __forceinline__ void join_even(uint32_t (&v)[4], const Even16 &e, uint32_t sh) {
-    v[0] = __builtin_amdgcn_alignbyte(e.w.y, e.w.x, sh);
-    v[1] = __builtin_amdgcn_alignbyte(e.w.z, e.w.y, sh);
-    v[2] = __builtin_amdgcn_alignbyte(e.w.w, e.w.z, sh);
-    v[3] = __builtin_amdgcn_alignbyte(e.end, e.w.w, sh);
+// 16 bytes from byte sh = 0 or 2 of five words on.  Wide loads at 2 mod 4 run several times slower
+// (ldg16_a2), so that words are read from the 4-byte address below.
+__device__ __forceinline__ void join_even(uint32_t (&v)[4], const uint4 &w, uint32_t end, uint32_t sh) {
+    v[0] = __builtin_amdgcn_alignbyte(w.y, w.x, sh);
+    v[1] = __builtin_amdgcn_alignbyte(w.z, w.y, sh);
+    v[2] = __builtin_amdgcn_alignbyte(w.w, w.z, sh);
+    v[3] = __builtin_amdgcn_alignbyte(end, w.w, sh);
 }
 
 struct MoeQ6K {
@@ -372,9 +372,8 @@ struct MoeQ6K {
     static constexpr int kType = kTypeQ6_K, kDigits = 3, kBytes = kBytesQ6_K;
     static constexpr bool kWide = true;
     struct W {
-        Even16 l[2], h[2];
-        uint32_t sc[4];  // scales g, 4 + g, 8 + g, 12 + g
-        uint32_t d, sh;
+        uint4 l[2], h[2], sc;  // as words from the 4-byte address below; the scales are the same in all lane groups
+        uint32_t d, sh;        // the word that holds d
     };
     struct Op {
         v4i a[3][4];
@@ -386,28 +385,40 @@ struct MoeQ6K {
     __device__ static __forceinline__ void load_w(W &w, const uint8_t *row, int u, int, int g) {
         const uint8_t *p = row + (size_t)u * kBytes;
         w.sh = (uint32_t)((uintptr_t)p & 3u);
-        const uint8_t *l = p - w.sh + 16 * g, *h = p - w.sh + 128 + 16 * (g & 1);
+        p -= w.sh;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            w.l[i] = load_even(l + 64 * i, w.sh);
-            w.h[i] = load_even(h + 32 * i, w.sh);
+            w.l[i] = *reinterpret_cast<const uint4 *>(p + 64 * i + 16 * g);
+            w.h[i] = *reinterpret_cast<const uint4 *>(p + 128 + 32 * i + 16 * (g & 1));
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w.sc[i] = p[192 + g + 4 * i];
-        w.d = *reinterpret_cast<const uint16_t *>(p + 208);
+        w.sc = *reinterpret_cast<const uint4 *>(p + 192);
+        w.d = *reinterpret_cast<const uint32_t *>(p + 208);
     }
     __device__ static __forceinline__ void decode(Op &o, const W &w, int g) {
-        o.dm = w.d;
+        o.dm = w.d >> (8 * w.sh);
         o.mn = v4h{0, 0, 0, 0};
+        uint32_t sc[4];
+        join_even(sc, w.sc, w.d, w.sh);
+        // A piece's fifth word is the next piece's first: lane group g + 1's, or the next run's in group 0 (or,
+        // of two groups, in the even one), and behind the last the scales'.  Loads of two bytes for them cost
+        // a wave as much as whole ones.
+        const int lane = __lane_id(), next = ((lane + 16) & 63) << 2, other = (lane ^ 16) << 2;
+        const uint32_t end_l[2] = {
+            (uint32_t)__builtin_amdgcn_ds_bpermute(next, (int)(g == 0 ? w.l[1].x : w.l[0].x)),
+            (uint32_t)__builtin_amdgcn_ds_bpermute(next, (int)(g == 0 ? w.h[0].x : w.l[1].x))};
+        const uint32_t over = (uint32_t)__builtin_amdgcn_ds_bpermute(other, (int)w.h[1].x);
+        const uint32_t end_h[2] = {
+            (uint32_t)__builtin_amdgcn_ds_bpermute(other, (int)((g & 1) ? w.h[0].x : w.h[1].x)),
+            (g & 1) ? w.sc.x : over};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             uint32_t l[4], hh[4];
-            join_even(l, w.l[i], w.sh);
-            join_even(hh, w.h[i], w.sh);
+            join_even(l, w.l[i], end_l[i], w.sh);
+            join_even(hh, w.h[i], end_h[i], w.sh);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int sc = (int)(int8_t)w.sc[2 * i + h];
-                const int s0 = ((sc + 3) & 7) - 3, r1 = (sc - s0) >> 3, s1 = ((r1 + 3) & 7) - 3, s2 = (r1 - s1) >> 3;
+                const int q = (int)(int8_t)(sc[2 * i + h] >> (8 * g));  // scale 8 i + 4 h + g
+                const int s0 = ((q + 3) & 7) - 3, r1 = (q - s0) >> 3, s1 = ((r1 + 3) & 7) - 3, s2 = (r1 - s1) >> 3;
                 const int dig[3] = {s0, s1, s2};
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
