@@ -238,6 +238,10 @@ __device__ __forceinline__ uint32_t lds_addr(const void *p) {
 __host__ __device__ constexpr int tile_chunk(int TT) { return TT == 2 ? 2 : 1; }
 __host__ __device__ constexpr int tile_lds(int TT) { return 2 * tile_chunk(TT) * 16 * TT * kMoeRec; }
 constexpr int kTileWaves = 4;
+// Row blocks in a row on a chiplet: enough that they share a tile's records in its L2, few enough that every
+// chiplet has its part where slots are few or empty (16 tokens of 8 experts, 14336 rows of 4096: 124 us, with an eighth of the
+// slots a chiplet 219; 4096 tokens of 128 experts, 2560 rows of 768: 449 and 469, one by one 468).
+constexpr int kRun = 4;
 // Groups of weights ahead: two where a step's products are too short to hide a load behind.
 constexpr int tile_deep(int TT) { return TT <= 2 ? 2 : 1; }
 
@@ -254,12 +258,10 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
     constexpr int T = 16 * TT, CH = tile_chunk(TT), kBuf = CH * T * kMoeRec;
     constexpr int kDma = kBuf / 1024, kEach = (kDma + kTileWaves - 1) / kTileWaves;
     static_assert(kBuf % 1024 == 0, "whole DMAs");
-    // Workgroup b runs on chiplet b % 8: each chiplet takes a run of slots, a slot's row
-    // blocks one after the other, so that a tile's records and an
-    // expert's weights are read into one L2.
-    const int each8 = (slots + 7) / 8;
-    const int local = (int)(blockIdx.x >> 3);
-    const int slot = (int)(blockIdx.x & 7u) * each8 + local / n_blk;
+    // Workgroup b runs on chiplet b % 8: the row blocks of all slots, one slot after the other, go to
+    // the chiplets in runs of kRun.
+    const int turn = (int)(blockIdx.x >> 3), f = ((turn / kRun << 3) + (int)(blockIdx.x & 7u)) * kRun + turn % kRun;
+    const int slot = f / n_blk, blk = f - slot * n_blk;
     if (slot >= slots) return;
     const MoeTile tile = a.tiles[slot];
     if (tile.rest == 0 || tile.index % each != 0) return;  // (this kernel's tile is `each` of the sort's)
@@ -269,7 +271,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
     const int g = lane >> 4, r16 = lane & 15;
     const int KS = 1 << ks_log, ks = wave & (KS - 1);
     constexpr int kRows = PAIR ? 16 : 32;
-    const int row0 = kRows * ((local - local / n_blk * n_blk) * (kTileWaves >> ks_log) + (wave >> ks_log));
+    const int row0 = kRows * (blk * (kTileWaves >> ks_log) + (wave >> ks_log));
     const int u0 = a.groups * ks >> ks_log, u1 = a.groups * (ks + 1) >> ks_log;
     const int chs = CH >> ks_log;  // groups of a part in a buffer
     const int n_chunk = (((a.groups + KS - 1) >> ks_log) + chs - 1) / chs, n_step = n_chunk * chs;
@@ -451,7 +453,7 @@ void moe_tiles(const MoeArgs &a, int each, int slots, int ks_log, hipStream_t st
     const int rows = (PAIR ? 16 : 32) * (kTileWaves >> ks_log);
     const int n_blk = (a.rows + rows - 1) / rows;
     // (a slot and 16 rows or more a workgroup: what the pairs' rows take in device memory keeps that below 2^31)
-    const dim3 grid((unsigned)((slots + 7) / 8) * 8u * (unsigned)n_blk);
+    const dim3 grid((unsigned)((slots * n_blk + 8 * kRun - 1) / (8 * kRun)) * 8u * kRun);
     hipLaunchKernelGGL((tile_kernel<F, PAIR, TT>()), grid, dim3(64 * kTileWaves), tile_lds(TT), st, a, ks_log, each,
                        slots, n_blk);
 }
