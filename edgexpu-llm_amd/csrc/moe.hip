@@ -435,10 +435,14 @@ namespace {
 // LDS of a workgroup of one token that leaves room for two on a CU.
 constexpr size_t kOneLds = 60 * 1024;
 
-// Whether a routing's products take a workgroup a token (gate and up: a pair) without sorting the pairs.
-bool moe_one(long long pairs) {
-    const int most = tuning_knob("EXQ_MOE_ONE", 16);
-    return pairs <= most;
+// Whether a routing's products take a workgroup a token (gate and up: a pair) without sorting the pairs:
+// where few experts have two tokens, whose weights the tiles read once (us so and with tiles, without their
+// sort's 6: 128 experts of 768 x 2560, 48 pairs, gate and up 26 and 29, down 30 and 55; 96 pairs 46 and 39, 55 and 56; 8
+// of 14336 x 4096, 6 pairs 77 and 105, 8 pairs 120 and 95).
+bool moe_one(long long pairs, int n_experts) {
+    const int most = tuning_knob("EXQ_MOE_ONE", -1);
+    if (most >= 0) return pairs <= most;
+    return pairs <= std::max(8, n_experts / 2);
 }
 
 // Places a tile of sorted pairs.
@@ -532,7 +536,7 @@ bool moe_plan(edgexpu_hip_moe *p, int m, hipStream_t st, const char *what) {
     const long long pairs = (long long)m * p->top_k;
     const size_t one_lds = (size_t)std::max(moe_groups(p->n_embd), p->top_k * moe_groups(p->n_ff)) * kMoeRec;
     int tile = 0;
-    if (m > 0 && (!moe_one(pairs) || one_lds > kOneLds)) {
+    if (m > 0 && (!moe_one(pairs, p->n_experts) || one_lds > kOneLds)) {
         tile = moe_tile(pairs, p->n_experts);
         if (!lib_hip(launch_moe_sort(p->ids, (int)pairs, p->n_experts, tile, p->order, p->tiles, st), what)) return false;
     }
