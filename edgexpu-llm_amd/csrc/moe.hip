@@ -242,8 +242,11 @@ constexpr int kTileWaves = 4;
 // chiplet has its part where slots are few or empty (16 tokens of 8 experts, 14336 rows of 4096: 124 us, with an eighth of the
 // slots a chiplet 219; 4096 tokens of 128 experts, 2560 rows of 768: 449 and 469, one by one 468).
 constexpr int kRun = 4;
-// Groups of weights ahead: two where a step's products are too short to hide a load behind.
-constexpr int tile_deep(int TT) { return TT <= 2 ? 2 : 1; }
+// Groups of weights ahead: two where a step's products are too short to hide a load behind.  Not for
+// formats whose decoding is long: it is then what hides the load, and a second copy of it only costs
+// registers and instruction fetches (Q6_K, 64 tokens of 128 experts, 2560 rows of 768: 82 us with one, 89 with two).
+template <class F>
+constexpr int tile_deep(int TT) { return !F::kWide && TT <= 2 ? 2 : 1; }
 
 // Sums made where they stand: left to the compiler, all tiles' integer sums wait in
 // registers for the end of a step.
@@ -347,10 +350,11 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
         }
     };
     int v = 0;
-    for (; v + DEEP <= n_step; v += DEEP)
+    const int n_end = ks_log == 0 ? a.groups : n_step;  // (parts may differ by a group, and meet at the same barriers)
+    for (; v + DEEP <= n_end; v += DEEP)
 #pragma unroll
         for (int k = 0; k < DEEP; ++k) step(v + k, w[k]);
-    if (DEEP == 2 && v < n_step) step(v, w[0]);
+    if (DEEP == 2 && v < n_end) step(v, w[0]);
     if (KS > 1) {  // the parts' sums, in their order
         float4 *red = reinterpret_cast<float4 *>(lds);
         __syncthreads();
@@ -391,7 +395,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
 
 template <class F, bool PAIR, int TT>
 constexpr auto tile_kernel() {
-    return moe_tile_kernel<F, PAIR, TT, tile_deep(TT)>;
+    return moe_tile_kernel<F, PAIR, TT, tile_deep<F>(TT)>;
 }
 
 // ------------------------------------------------------------------ a token's parts
@@ -440,16 +444,13 @@ constexpr size_t kOneLds = 60 * 1024;
 // sort's 6: 128 experts of 768 x 2560, 48 pairs, gate and up 26 and 29, down 30 and 55; 96 pairs 46 and 39, 55 and 56; 8
 // of 14336 x 4096, 6 pairs 77 and 105, 8 pairs 120 and 95).
 bool moe_one(long long pairs, int n_experts) {
-    const int most = tuning_knob("EXQ_MOE_ONE", -1);
-    if (most >= 0) return pairs <= most;
     return pairs <= std::max(8, n_experts / 2);
 }
 
-// Places a tile of sorted pairs.
+// Places a tile of sorted pairs (us with 32 and 64, 128 experts of 768 x 2560: 8 pairs an expert, gate and up 64 and 71,
+// down Q6_K 79 and 90; 16 pairs 83 and 79, 100 and 94).
 int moe_tile(long long pairs, int n_experts) {
-    const int knob = tuning_knob("EXQ_MOE_TILE", 0);
-    if (knob != 0) return knob;
-    return pairs <= 16LL * n_experts ? 32 : 64;
+    return pairs < 16LL * n_experts ? 32 : 64;
 }
 
 template <class F, bool PAIR, int TT>
@@ -489,10 +490,12 @@ bool moe_run(const edgexpu_hip_moe *p, MoeArgs &a, bool pair, hipStream_t st, co
     if (!pair) a.out = p->part;
     const int slots = moe_slots(pairs, p->n_experts, p->tile);
     // two waves share two row tiles' groups where the tiles are too few to fill the chip (12 tokens
-    // of 8 experts, 4096 rows of 14336: 256 workgroups 70 us, 512 so 62 us)
+    // of 8 experts, 4096 rows of 14336: 256 workgroups 69 us, 512 so 63; where they are enough, 333 tokens of 64
+    // experts, 2560 rows of 1024, 75 us and 88 so)
     const long long blocks = (std::min<long long>(p->n_experts, pairs) + pairs / 32) * ((a.rows + 127) / 128);
-    const int ks_knob = tuning_knob("EXQ_MOE_KS", -1);
-    const int ks = p->tile != 32 ? 0 : ks_knob >= 0 ? ks_knob : !pair && blocks < 512 ? 1 : 0;
+    const int ks = p->tile == 32 && !pair && blocks < 512 ? 1 : 0;
+    // 128 pairs a workgroup where a decoded row is worth it (2048 tokens of 128 experts, 2560 rows of 768:
+    // Q6_K 354 us with 64, 292 with 128; Q5_K 204 and 211)
     const bool wide = F::kWide && pairs > 48LL * p->n_experts;
 #define MOE_TILES(TT, EACH)                              \
     if (pair)                                            \
@@ -628,6 +631,13 @@ edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens
                   n_experts, kMoeMaxTopK, kMoeMaxExperts, max_tokens, n_embd, n_ff);
         return nullptr;
     }
+    const size_t pairs = (size_t)max_tokens * top_k;
+    const size_t records = std::max((size_t)moe_groups(n_embd) * max_tokens, (size_t)moe_groups(n_ff) * pairs);
+    if (records > (size_t)1 << 27) {  // (their places are counted in 32 bits, 16 bytes a unit)
+        lib_error(-2, "moe_create: %d tokens of %d experts, rows of %d and %d: more than 2^27 groups of 256", max_tokens, top_k,
+                  n_embd, n_ff);
+        return nullptr;
+    }
     if (!lib_ready("moe_create") || !moe_prepare<MoeQ6K>() || !moe_prepare<MoeQ80>() || !moe_prepare<MoeQ40>() ||
         !moe_prepare<MoeQ50>())
         return nullptr;
@@ -641,10 +651,9 @@ edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens
     p->max_tokens = max_tokens;
     p->n_embd = n_embd;
     p->n_ff = n_ff;
-    const size_t pairs = (size_t)max_tokens * top_k;
     const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const size_t sizes[6] = {4 * pairs, 4 * pairs, 4 * pairs, sizeof(MoeTile) * moe_slots(pairs, n_experts, 32),
-                             kMoeRec * (std::max((size_t)moe_groups(n_embd) * max_tokens, (size_t)moe_groups(n_ff) * pairs) + 8),
+                             kMoeRec * (records + 8),
                              4 * pairs * n_embd};
     size_t total = 0, at[6];
     for (int i = 0; i < 6; ++i) {

@@ -213,6 +213,29 @@ def test_crowded_and_empty_experts(hipdev, qtype, m):
         check_down(qtype, 8, 2, m, 48, 512, ids=ids, inplace=True)
 
 
+# where the work is shared out otherwise: (experts, choices, tokens, n_embd, n_ff)
+SHARES = [(2, 2, 200, 768, 50), (3, 3, 150, 1280, 33),  # more than 128 pairs an expert
+          (8, 2, 100, 768, 70), (6, 2, 66, 512, 129),  # more than 16
+          (4, 2, 12, 1280, 96), (4, 2, 12, 256, 34), (8, 2, 9, 768, 47),  # few tiles
+          (64, 4, 8, 512, 40), (64, 4, 9, 512, 40), (8, 2, 4, 256, 31), (8, 2, 5, 256, 31)]  # from single tokens to tiles
+
+
+@pytest.mark.parametrize("size", SHARES, ids=str)
+@pytest.mark.parametrize("qtype", TYPES, ids=lambda t: E.TYPE_NAMES[t])
+def test_every_share_of_the_work(hipdev, qtype, size):
+    n, k, m, wide, narrow = size
+    check_gate_up(qtype, n, k, m, wide, narrow, seed=5)
+    check_down(qtype, n, k, m, narrow, wide, seed=6)  # (the products run over the same lengths)
+
+
+@pytest.mark.parametrize("n_ff", [12800, 14336])
+@pytest.mark.parametrize("qtype", [E.Q4_K, E.Q6_K, E.Q8_0], ids=lambda t: E.TYPE_NAMES[t])
+def test_one_token_of_long_rows(hipdev, qtype, n_ff):
+    """Four rows of 50 groups are quantized by one workgroup, of 56 are not."""
+    for none in (0.0, 0.5):
+        check_down(qtype, 5, 4, 1, 35, n_ff, seed=7, none=none)
+
+
 @pytest.mark.parametrize("qtype", TYPES, ids=lambda t: E.TYPE_NAMES[t])
 @pytest.mark.parametrize("m", [1, 6, 50])
 def test_zero_and_wide_activations(hipdev, qtype, m):

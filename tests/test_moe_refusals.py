@@ -29,6 +29,11 @@ def test_create(lib, args):
     refused(lib, lib.moe_create(*args), -2, "moe_create")
 
 
+@pytest.mark.parametrize("args", [(8, 2, 2**21, 256, 2**14), (8, 1, 2**22, 2**14, 256), (512, 32, 2**17, 256, 8449)])
+def test_create_beyond_the_counted_groups(lib, args):
+    refused(lib, lib.moe_create(*args), -2, "groups of 256")
+
+
 def test_null_plan(lib):
     p = 0x1000  # (refused before anything reads it)
     refused(lib, lib.moe_route_dev(None, p, p, p, 1, 0, None, 1, 1, 1, 1, 1.0, None), -2, "moe_route")
