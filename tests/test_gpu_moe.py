@@ -228,6 +228,25 @@ def test_every_share_of_the_work(hipdev, qtype, size):
     check_down(qtype, n, k, m, narrow, wide, seed=6)  # (the products run over the same lengths)
 
 
+@pytest.mark.parametrize("m", [1, 3, 40, 200])
+def test_an_expert_named_twice(hipdev, m):
+    """A token's places are summed one by one, whichever experts they name."""
+    rng = np.random.default_rng(m)
+    ids = rng.integers(-1, 3, (m, 4)).astype(np.int32)
+    ids[0] = 1
+    check_gate_up(E.Q5_K, 6, 4, m, 512, 40, seed=8, ids=ids)
+    check_down(E.Q6_K, 6, 4, m, 40, 512, seed=9, ids=ids)
+
+
+def test_more_pairs_than_one_round_of_the_sort(hipdev):
+    m, rng = 12000, np.random.default_rng(3)
+    ids = random_ids(rng, m, 5, 3, 0.2)
+    ids[:9000] = np.where(ids[:9000] == 4, -1, ids[:9000])  # (an expert whose pairs all come late)
+    ids[100:5000] = np.where(ids[100:5000] == 0, -1, ids[100:5000])
+    check_gate_up(E.Q8_0, 5, 3, m, 64, 8, seed=10, ids=ids)
+    check_down(E.Q4_0, 5, 3, m, 8, 64, seed=11, ids=ids)
+
+
 @pytest.mark.parametrize("n_ff", [12800, 14336])
 @pytest.mark.parametrize("qtype", [E.Q4_K, E.Q6_K, E.Q8_0], ids=lambda t: E.TYPE_NAMES[t])
 def test_one_token_of_long_rows(hipdev, qtype, n_ff):
