@@ -64,13 +64,16 @@ __global__ __launch_bounds__(256) void moe_pack_kernel(MoeArgs a) {
 // launch (down).  Its waves share the groups out, and it quantizes the token's
 // rows itself: a launch less, and the first weights are on their way meanwhile.  All 16
 // columns of the products hold the same token.
-constexpr int one_waves(bool) { return 8; }
+// What bounds it: for a token a chain (arguments 0.7 us, choice 0.9, weights 2, products, sums
+// 1.2): 8 of 128 experts of 768 x 2560, Q4_K, gate and up 7.4 us; down of 2560 x 768, Q6_K, 10.3, the decoding of three
+// groups a wave; for more pairs the memory: 3 tokens of 14336 x 4096 77 us, 4.0 TB/s.  At most
+// 128 registers, so that two workgroups fit a CU (162: gate and up 10.0 us); 16 waves, down 12.7.
+constexpr int kOneWaves = 8;
 
 template <class F, bool PAIR>
-__global__ __launch_bounds__(64 * one_waves(PAIR), 4) void moe_one_kernel(MoeArgs a) {
+__global__ __launch_bounds__(64 * kOneWaves, 4) void moe_one_kernel(MoeArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t recs[];
     // gate and up: half the waves each
-    constexpr int kOneWaves = one_waves(PAIR);
     constexpr int kSets = PAIR ? 2 : 1, kShare = kOneWaves / kSets;
     // groups whose weights are on their way at once: a wave of a single token mostly has no more
     constexpr int kAhead = F::kK ? 2 : 1;
@@ -235,6 +238,9 @@ __device__ __forceinline__ uint32_t lds_addr(const void *p) {
 // buffer, two buffers.  A step takes one of its row tiles after the other, so that
 // only one's decoded rows are in registers (both at once read each record once, but with a
 // third more registers and 2 waves a SIMD for 3: 512 tokens 109 us so, 103 one by one).
+// What bounds it: memory where tiles are few (12 tokens of 8 experts, 4096 rows of 14336, Q4_K, 59 us, 4.4 TB/s), else
+// vector instructions: to decode a row tile's group 110 (Q4_K) to 450 (Q6_K), and 20 for 16 pairs' scales
+// (4096 tokens of 128 experts, 768 rows of 2560 twice, Q4_K, 375 us, 690 TFLOP/s).
 __host__ __device__ constexpr int tile_chunk(int TT) { return TT == 2 ? 2 : 1; }
 __host__ __device__ constexpr int tile_lds(int TT) { return 2 * tile_chunk(TT) * 16 * TT * kMoeRec; }
 constexpr int kTileWaves = 4;
@@ -401,7 +407,7 @@ constexpr auto tile_kernel() {
 // ------------------------------------------------------------------ a token's parts
 
 // out[t] = [residual[t] +] the parts of its places with an expert, in their order; a
-// thread takes 4 rows (VEC) or one.
+// thread takes 4 rows (VEC) or one.  One pass over the parts: 4096 tokens of 8 x 2560, 80 us, 4.7 TB/s.
 template <bool VEC>
 __global__ __launch_bounds__(256) void moe_join_kernel(const float *__restrict__ part, const int32_t *__restrict__ ids,
                                                        const float *residual, float *out, int m, int top_k, int rows) {
@@ -476,9 +482,9 @@ bool moe_run(const edgexpu_hip_moe *p, MoeArgs &a, bool pair, hipStream_t st, co
         const size_t lds = (size_t)(pair ? 1 : p->top_k) * a.groups * kMoeRec;
         const dim3 grid((unsigned)((a.rows + 15) / 16), (unsigned)(pair ? pairs : p->m));
         if (pair)
-            hipLaunchKernelGGL((moe_one_kernel<F, true>), grid, dim3(64 * one_waves(true)), lds, st, a);
+            hipLaunchKernelGGL((moe_one_kernel<F, true>), grid, dim3(64 * kOneWaves), lds, st, a);
         else
-            hipLaunchKernelGGL((moe_one_kernel<F, false>), grid, dim3(64 * one_waves(false)), lds, st, a);
+            hipLaunchKernelGGL((moe_one_kernel<F, false>), grid, dim3(64 * kOneWaves), lds, st, a);
         return lib_hip(hipGetLastError(), what);
     }
     if (pair)

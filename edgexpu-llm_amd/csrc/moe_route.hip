@@ -30,16 +30,16 @@ __device__ __forceinline__ uint64_t order_key(double v) {
 // lane 63): a step is a few cycles, where one through LDS is a hundred, and a token's
 // choices are one chain of them.
 template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_or(uint32_t old, uint32_t v) {
+__device__ __forceinline__ uint32_t dpp_from(uint32_t old, uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROWS, 0xf, false);
 }
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-    v = max(v, dpp_or<0x111, 0xf>(v, v));
-    v = max(v, dpp_or<0x112, 0xf>(v, v));
-    v = max(v, dpp_or<0x114, 0xf>(v, v));
-    v = max(v, dpp_or<0x118, 0xf>(v, v));
-    v = max(v, dpp_or<0x142, 0xa>(v, v));
-    v = max(v, dpp_or<0x143, 0xc>(v, v));
+    v = max(v, dpp_from<0x111, 0xf>(v, v));
+    v = max(v, dpp_from<0x112, 0xf>(v, v));
+    v = max(v, dpp_from<0x114, 0xf>(v, v));
+    v = max(v, dpp_from<0x118, 0xf>(v, v));
+    v = max(v, dpp_from<0x142, 0xa>(v, v));
+    v = max(v, dpp_from<0x143, 0xc>(v, v));
     return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 __device__ __forceinline__ double lane_f64(double v, int lane) {  // (lane: the same in the whole wave)
@@ -51,7 +51,7 @@ __device__ __forceinline__ double lane_f64(double v, int lane) {  // (lane: the 
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp_add(double v) {  // (lanes without a source add 0)
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = dpp_or<CTRL, ROWS>(0u, (uint32_t)b), hi = dpp_or<CTRL, ROWS>(0u, (uint32_t)(b >> 32));
+    const uint32_t lo = dpp_from<CTRL, ROWS>(0u, (uint32_t)b), hi = dpp_from<CTRL, ROWS>(0u, (uint32_t)(b >> 32));
     return v + __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
 }
 __device__ __forceinline__ double wave_add_f64(double v) {
@@ -70,7 +70,8 @@ __device__ __forceinline__ double shfl_xor_f64(double v, int off) {
     return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
 }
 
-// S = ceil(n_experts / 64) experts a lane.
+// S = ceil(n_experts / 64) experts a lane.  Bound by the chain of a wave: 64-bit exponentials and one
+// choice after the other (1 token, 8 of 128, 4.1 us; 4096 tokens, 8 of 256 in groups, 12 us).
 template <int S>
 __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(RouteArgs a) {
     __shared__ double cs[kRouteWaves][64 * S];
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(256) void moe_assign_kernel(const int32_t *__restri
 // Pairs by expert: a workgroup an expert counts the pairs of the experts before its
 // own, then writes its own pairs in ascending order (so the sort is stable and the
 // same every time) and its tiles.  Every workgroup reads all ids, 4 bytes a pair from
-// L2, and none waits for another.
+// L2, and none waits for another (32768 pairs of 256 experts 9 us; a token's 5).
 constexpr int kSortThreads = 1024, kSortMost = 32;  // ids a thread and round, read 4 at once
 __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t *__restrict__ ids, int pairs,
                                                                 int n_experts, int T, int slots, int each,
