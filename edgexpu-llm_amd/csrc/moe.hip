@@ -18,11 +18,13 @@ __device__ __forceinline__ float gelu_f32(float v) {
     const float u = v * fmaf(0.044715f * v, v, 1.0f) * 1.5957691216057308f;
     return v / (1.0f + expf(-u));
 }
+constexpr float kNan = __builtin_nanf("");
 __device__ __forceinline__ float moe_act(float v, int activation) {
     return activation == EDGEXPU_HIP_MOE_GELU ? gelu_f32(v) : silu_f32(v);
 }
 
 struct MoeArgs {
+    const int32_t *routed;    // holds m, or the plan's routing is not of these tokens: NaN, and nothing of it is read
     const int32_t *ids;
     const float *weights;
     const int32_t *order;
@@ -42,19 +44,22 @@ struct MoeArgs {
 // ------------------------------------------------------------------ packing
 
 // Rows of x into records, 256 threads over a part of a row (blockIdx.y).  ACT: rows are
-// tokens, and the places of a token that have no expert get zeros in `out` by the way.
+// tokens, and the places of a token that have no expert get zeros in `out` by the way
+// (without a routing of these tokens all of them NaN).
 template <bool K, bool ACT>
 __global__ __launch_bounds__(256) void moe_pack_kernel(MoeArgs a) {
     const size_t row = blockIdx.x;
     const int part = (int)blockIdx.y * 256 + (int)threadIdx.x;
     if (part < moe_pack_parts<K>(a.n))
         moe_pack_part<K>(a.x + row * a.n, a.n, part, a.pack + row * a.groups * kMoeRec);
-    if (ACT && blockIdx.y == 0)
+    if (ACT && blockIdx.y == 0) {
+        const bool routed = *a.routed == a.m;
         for (int j = 0; j < a.top_k; ++j) {
             const size_t pair = row * a.top_k + j;
-            if (a.ids[pair] < 0)
-                for (int i = threadIdx.x; i < a.rows; i += 256) a.out[pair * a.rows + i] = 0.0f;
+            if (!routed || a.ids[pair] < 0)
+                for (int i = threadIdx.x; i < a.rows; i += 256) a.out[pair * a.rows + i] = routed ? 0.0f : kNan;
         }
+    }
 }
 
 // ------------------------------------------------------------------ one token
@@ -96,7 +101,9 @@ __global__ __launch_bounds__(64 * kOneWaves, 4) void moe_one_kernel(MoeArgs a) {
 
     // Lane j's expert, place and weight: the j-th that there is (every wave for itself).
     const int own = PAIR ? 0 : lane;
+    const bool routed = *a.routed == a.m;
     int expert = own < (PAIR ? 1 : a.top_k) ? a.ids[pair0 + own] : -1, place = own, n_seg;
+    if (!routed) expert = -1;
     float weight = 1.0f;
     if (PAIR) {
         n_seg = expert >= 0 ? 1 : 0;
@@ -164,13 +171,15 @@ __global__ __launch_bounds__(64 * kOneWaves, 4) void moe_one_kernel(MoeArgs a) {
         const size_t b = (size_t)max(expert, 0) * a.rows + o;
         if (a.bias[0] != nullptr) v[0] += a.bias[0][b];
         if (a.bias[1] != nullptr) v[kSets - 1] += a.bias[1][b];
-        a.out[pair0 * a.rows + o] = n_seg == 0 ? 0.0f : moe_act(v[0], a.activation) * v[kSets - 1];
+        const float y = n_seg == 0 ? 0.0f : moe_act(v[0], a.activation) * v[kSets - 1];
+        a.out[pair0 * a.rows + o] = routed ? y : kNan;
     } else {
         if (a.bias[0] != nullptr)
             for (int j = 0; j < n_seg; ++j)
                 v[0] = fmaf(__int_as_float(nth(__float_as_int(weight), j)), a.bias[0][(size_t)nth(expert, j) * a.rows + o], v[0]);
         const size_t at = (size_t)blockIdx.y * a.rows + o;
-        a.out[at] = a.residual != nullptr ? a.residual[at] + v[0] : v[0];
+        const float y = a.residual != nullptr ? a.residual[at] + v[0] : v[0];
+        a.out[at] = routed ? y : kNan;
     }
 }
 
@@ -273,6 +282,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void moe_tile_kernel(MoeArgs a,
     const int slot = f / n_blk, blk = f - slot * n_blk;
     if (slot >= slots) return;
     const MoeTile tile = a.tiles[slot];
+    if (*a.routed != a.m) return;  // (the tiles are another routing's)
     if (tile.rest == 0 || tile.index % each != 0) return;  // (this kernel's tile is `each` of the sort's)
     const int pairs = min(tile.rest, T);
     const int lane = threadIdx.x & 63;
@@ -410,14 +420,16 @@ constexpr auto tile_kernel() {
 // thread takes 4 rows (VEC) or one.  One pass over the parts: 4096 tokens of 8 x 2560, 80 us, 4.7 TB/s.
 template <bool VEC>
 __global__ __launch_bounds__(256) void moe_join_kernel(const float *__restrict__ part, const int32_t *__restrict__ ids,
-                                                       const float *residual, float *out, int m, int top_k, int rows) {
+                                                       const int32_t *__restrict__ routed, const float *residual,
+                                                       float *out, int m, int top_k, int rows) {
     const int each = VEC ? 4 : 1, per = rows / each;
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= (size_t)m * per) return;
     const size_t t = i / per;
     const int o = (int)(i - t * per) * each;
+    const bool whole = *routed == m;
     float s[4] = {};
-    for (int j = 0; j < top_k; ++j) {
+    for (int j = 0; whole && j < top_k; ++j) {
         const size_t pair = t * top_k + j;
         if (ids[pair] < 0) continue;
         const float *p = part + pair * rows + o;
@@ -432,6 +444,9 @@ __global__ __launch_bounds__(256) void moe_join_kernel(const float *__restrict__
     if (residual != nullptr)
 #pragma unroll
         for (int r = 0; r < each; ++r) s[r] = residual[at + r] + s[r];
+    if (!whole)
+#pragma unroll
+        for (int r = 0; r < each; ++r) s[r] = kNan;
     if (VEC)
         *reinterpret_cast<float4 *>(out + at) = make_float4(s[0], s[1], s[2], s[3]);
     else
@@ -521,11 +536,11 @@ bool moe_run(const edgexpu_hip_moe *p, MoeArgs &a, bool pair, hipStream_t st, co
     const bool vec = (a.rows & 3) == 0;
     const unsigned joins = (unsigned)(((size_t)p->m * (vec ? a.rows / 4 : a.rows) + 255) / 256);
     if (vec)
-        hipLaunchKernelGGL(moe_join_kernel<true>, dim3(joins), dim3(256), 0, st, p->part, a.ids, a.residual, out, p->m,
-                           p->top_k, a.rows);
+        hipLaunchKernelGGL(moe_join_kernel<true>, dim3(joins), dim3(256), 0, st, p->part, a.ids, a.routed, a.residual,
+                           out, p->m, p->top_k, a.rows);
     else
-        hipLaunchKernelGGL(moe_join_kernel<false>, dim3(joins), dim3(256), 0, st, p->part, a.ids, a.residual, out,
-                           p->m, p->top_k, a.rows);
+        hipLaunchKernelGGL(moe_join_kernel<false>, dim3(joins), dim3(256), 0, st, p->part, a.ids, a.routed, a.residual,
+                           out, p->m, p->top_k, a.rows);
     return lib_hip(hipGetLastError(), what);
 }
 
@@ -540,15 +555,20 @@ bool moe_product(const edgexpu_hip_moe *p, MoeArgs &a, uint32_t type, bool pair,
     }
 }
 
-// Sorts the pairs of a routing of m tokens where the products need it.
-bool moe_plan(edgexpu_hip_moe *p, int m, hipStream_t st, const char *what) {
+// Places a tile of the sorted pairs of a routing of m tokens; 0 where no product needs them sorted.
+int moe_sorted(const edgexpu_hip_moe *p, int m) {
     const long long pairs = (long long)m * p->top_k;
     const size_t one_lds = (size_t)std::max(moe_groups(p->n_embd), p->top_k * moe_groups(p->n_ff)) * kMoeRec;
-    int tile = 0;
-    if (m > 0 && (!moe_one(pairs, p->n_experts) || one_lds > kOneLds)) {
-        tile = moe_tile(pairs, p->n_experts);
-        if (!lib_hip(launch_moe_sort(p->ids, (int)pairs, p->n_experts, tile, p->order, p->tiles, st), what)) return false;
-    }
+    if (m == 0 || (moe_one(pairs, p->n_experts) && one_lds <= kOneLds)) return 0;
+    return moe_tile(pairs, p->n_experts);
+}
+
+// Sorts the pairs of a routing of m tokens where the products need it.
+bool moe_plan(edgexpu_hip_moe *p, int m, hipStream_t st, const char *what) {
+    const int tile = moe_sorted(p, m);
+    if (tile != 0 && !lib_hip(launch_moe_sort(p->ids, m * p->top_k, p->n_experts, tile, p->order, p->tiles, p->routed, m,
+                                              st), what))
+        return false;
     p->tile = tile;
     p->m = m;
     return true;
@@ -605,6 +625,7 @@ size_t block_bytes(uint32_t type) {
 
 MoeArgs moe_args(const edgexpu_hip_moe *p, uint32_t type, int rows, int n) {
     MoeArgs a = {};
+    a.routed = p->routed;
     a.ids = p->ids;
     a.weights = p->weights;
     a.order = p->order;
@@ -658,11 +679,10 @@ edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens
     p->n_embd = n_embd;
     p->n_ff = n_ff;
     const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    const size_t sizes[6] = {4 * pairs, 4 * pairs, 4 * pairs, sizeof(MoeTile) * moe_slots(pairs, n_experts, 32),
-                             kMoeRec * (records + 8),
-                             4 * pairs * n_embd};
-    size_t total = 0, at[6];
-    for (int i = 0; i < 6; ++i) {
+    const size_t sizes[7] = {4 * pairs, 4 * pairs, 4 * pairs, sizeof(MoeTile) * moe_slots(pairs, n_experts, 32),
+                             kMoeRec * (records + 8), 4 * pairs * n_embd, sizeof(int32_t)};
+    size_t total = 0, at[7];
+    for (int i = 0; i < 7; ++i) {
         at[i] = total;
         total += up(sizes[i]);
     }
@@ -676,6 +696,12 @@ edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens
     p->tiles = (MoeTile *)(p->mem + at[3]);
     p->pack = p->mem + at[4];
     p->part = (float *)(p->mem + at[5]);
+    p->routed = (int32_t *)(p->mem + at[6]);
+    if (!lib_hip(hipMemcpy(p->routed, &p->m, sizeof(p->m), hipMemcpyHostToDevice), "moe_create")) {
+        (void)hipFree(p->mem);
+        delete p;
+        return nullptr;
+    }
     return p;
 }
 
@@ -703,12 +729,20 @@ int edgexpu_hip_moe_route_dev(edgexpu_hip_moe *p, int32_t *ids, float *weights, 
         return 0;
     }
     if (!lib_ready("moe_route")) return 0;
-    if (m > 0) {
+    // (a sort, where one follows, writes the tokens)
+    const int now = moe_sorted(p, m) != 0 ? -1 : m;
+    if (m == 0) {
+        if (!lib_hip(launch_moe_assign(nullptr, nullptr, nullptr, nullptr, 0, p->n_experts, p->routed, 0,
+                                       (hipStream_t)stream), "moe_route"))
+            return 0;
+    } else {
         RouteArgs a = {};
         a.scores = scores;
         a.bias = bias;
         a.ids = p->ids;
         a.ids_out = ids;
+        a.routed = p->routed;
+        a.now = now;
         a.weights = p->weights;
         a.weights_out = weights;
         a.m = m;
@@ -732,8 +766,8 @@ int edgexpu_hip_moe_assign_dev(edgexpu_hip_moe *p, const int32_t *ids, const flo
         return 0;
     }
     if (!lib_ready("moe_assign")) return 0;
-    if (m > 0 && !lib_hip(launch_moe_assign(ids, weights, p->ids, p->weights, m * p->top_k, p->n_experts,
-                                            (hipStream_t)stream), "moe_assign"))
+    if (!lib_hip(launch_moe_assign(ids, weights, p->ids, p->weights, m * p->top_k, p->n_experts, p->routed,
+                                   moe_sorted(p, m) != 0 ? -1 : m, (hipStream_t)stream), "moe_assign"))
         return 0;
     return moe_plan(p, m, (hipStream_t)stream, "moe_assign") ? 1 : 0;
 }

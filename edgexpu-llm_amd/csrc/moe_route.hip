@@ -79,6 +79,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(RouteArgs a
     // (a wave past the last token repeats it and writes nothing: all reach the barrier)
     const bool own = (int)blockIdx.x * kRouteWaves + wave < a.m;
     const int t = own ? (int)blockIdx.x * kRouteWaves + wave : a.m - 1;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.routed = a.now;
     const float *s = a.scores + (size_t)t * a.n_experts;
     float sc[S];
     bool live[S];
@@ -210,8 +211,10 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(RouteArgs a
 
 __global__ __launch_bounds__(256) void moe_assign_kernel(const int32_t *__restrict__ ids,
                                                          const float *__restrict__ weights, int32_t *to_ids,
-                                                         float *to_weights, int pairs, int n_experts) {
+                                                         float *to_weights, int pairs, int n_experts,
+                                                         int32_t *routed, int now) {
     const int i = (int)(blockIdx.x * 256 + threadIdx.x);
+    if (i == 0) *routed = now;
     if (i >= pairs) return;
     const int e = ids[i];
     const bool some = e >= 0 && e < n_experts;
@@ -227,11 +230,12 @@ constexpr int kSortThreads = 1024, kSortMost = 32;  // ids a thread and round, r
 __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t *__restrict__ ids, int pairs,
                                                                 int n_experts, int T, int slots, int each,
                                                                 int32_t *__restrict__ order,
-                                                                MoeTile *__restrict__ tiles) {
+                                                                MoeTile *__restrict__ tiles, int32_t *routed, int m) {
     constexpr int kWaves = kSortThreads / 64;
     __shared__ int sums[2][kWaves];
     const int e = (int)blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int round = each * kSortThreads;
+    if (e == 0 && tid == 0) *routed = m;
     // A thread's ids of a round from `first` on (each of them, those past the last as -1):
     // which are this expert's, and how many are of those before it.
     const auto read = [&](int first, int &less) {
@@ -320,10 +324,10 @@ __global__ __launch_bounds__(kSortThreads) void moe_sort_kernel(const int32_t *_
 }
 
 hipError_t launch_moe_sort(const int32_t *ids, int pairs, int n_experts, int T, int32_t *order, MoeTile *tiles,
-                           hipStream_t st) {
+                           int32_t *routed, int m, hipStream_t st) {
     const int each = std::min(kSortMost, (pairs + 4 * kSortThreads - 1) / (4 * kSortThreads) * 4);
     hipLaunchKernelGGL(moe_sort_kernel, dim3((unsigned)n_experts), dim3(kSortThreads), 0, st, ids, pairs, n_experts, T,
-                       moe_slots(pairs, n_experts, T), each, order, tiles);
+                       moe_slots(pairs, n_experts, T), each, order, tiles, routed, m);
     return hipGetLastError();
 }
 
@@ -338,9 +342,9 @@ hipError_t launch_moe_route(const RouteArgs &a, hipStream_t st) {
 }
 
 hipError_t launch_moe_assign(const int32_t *ids, const float *weights, int32_t *to_ids, float *to_weights, int pairs,
-                             int n_experts, hipStream_t st) {
-    hipLaunchKernelGGL(moe_assign_kernel, dim3((unsigned)((pairs + 255) / 256)), dim3(256), 0, st, ids, weights, to_ids,
-                       to_weights, pairs, n_experts);
+                             int n_experts, int32_t *routed, int now, hipStream_t st) {
+    hipLaunchKernelGGL(moe_assign_kernel, dim3((unsigned)std::max(1, (pairs + 255) / 256)), dim3(256), 0, st, ids,
+                       weights, to_ids, to_weights, pairs, n_experts, routed, now);
     return hipGetLastError();
 }
 

@@ -657,7 +657,9 @@ def attention(batch: KvBatch, layer: int, q, scale: float | None = None, out=Non
 
 class MoePlan:
     """The routing of a step's tokens to top_k of n_experts, and the workspaces of the
-    products that follow it (edgexpu_hip_moe_*)."""
+    products that follow it (edgexpu_hip_moe_*).  A replayed graph's routing becomes the
+    plan's: eager products afterwards follow an eager routing (NaN otherwise), and the
+    plan lives as long as the graph."""
 
     def __init__(self, n_experts: int, top_k: int, max_tokens: int, n_embd: int, n_ff: int):
         L = hip()
@@ -680,6 +682,7 @@ class MoePlan:
         _HIP.check(_HIP.moe_assign_dev(self._h, _ptr(ids), _ptr(weights), m, _stream()), "moe_assign")
 
     def tokens(self) -> int:
+        """Tokens of the last routing that was queued or captured."""
         return _HIP.moe_tokens(self._h)
 
 

@@ -498,9 +498,12 @@ int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip_batch *b, 
  * edgexpu_hip_moe_assign_dev and the workspaces of the products; all device memory
  * is taken by _create, so every other call can be captured into a graph.  Work on one
  * plan goes to one stream, or to streams that the caller orders, and is queued by one
- * host thread at a time.  A captured product computes as many tokens as the routing
- * had when it was captured: replay it after a routing of as many.  What a captured
- * call was given lives as long as its graph.  All run on the device of
+ * host thread at a time.  A product computes as many tokens as the last routing
+ * that was queued, captured ones included; a captured product, as many as when it was
+ * captured.  Where the last routing that ran is of another number of tokens (or
+ * none ran), as after the replay of a captured one, every value that it gives is NaN,
+ * and nothing else is read or written: queue or replay a routing of as many before
+ * it.  What a captured call was given lives as long as its graph.  All run on the device of
  * edgexpu_hip_init (another current device: error -4). */
 typedef struct edgexpu_hip_moe edgexpu_hip_moe;
 /* n_experts at most 512; top_k at most n_experts and 32; n_embd and n_ff at most
@@ -510,7 +513,7 @@ typedef struct edgexpu_hip_moe edgexpu_hip_moe;
 edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens, int n_embd, int n_ff);
 /* Waits for the device, then frees. */
 void edgexpu_hip_moe_destroy(edgexpu_hip_moe *p);
-/* Tokens of the last routing; 0 before one. */
+/* Tokens of the last routing that was queued or captured; 0 before one. */
 int edgexpu_hip_moe_tokens(const edgexpu_hip_moe *p);
 
 /* Chooses top_k experts for each of m tokens (0 to max_tokens) by scores

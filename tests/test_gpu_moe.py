@@ -475,3 +475,79 @@ def test_the_python_front_refuses(hipdev):
                  lambda: E.moe_down(plan, w.cpu(), E.Q4_K, torch.zeros((4, 2, 256), device="cuda:0"))):
         with pytest.raises(ValueError):
             call()
+
+
+# ------------------------------------------------------------------ routings that are captured and replayed
+
+
+def capture(call):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    return graph
+
+
+def products_of(plan, layer, m):
+    """The plan's products as a caller makes them, into memory with something of its own before and behind it."""
+    k, n, f = layer.k, layer.n_embd, layer.n_ff
+    act, out = torch.full((m + 2, k, f), 7.5, device="cuda:0"), torch.full((m + 2, n), 7.5, device="cuda:0")
+    x, a, h = torch.ones((m, n), device="cuda:0"), torch.ones((m, k, f), device="cuda:0"), torch.ones((m, n), device="cuda:0")
+    E.moe_gate_up(plan, layer.dev["gate"], layer.dev["up"], layer.q, x, act=act[1:])
+    E.moe_down(plan, layer.dev["down"], layer.dq, a, residual=h, out=out[1:])
+    for t in (act, out):
+        assert bool((t[0] == 7.5).all()) and bool((t[m + 1:] == 7.5).all()), "memory beside the tokens was written"
+    return act[1:m + 1], out[1:m + 1]
+
+
+# (tokens of the routing that ran, tokens of the products): single tokens, sorted pairs, and between the two
+@pytest.mark.parametrize("ran,m", [(50, 20), (20, 50), (3, 50), (50, 2), (1, 2), (2, 1), (60, 40), (0, 20), (0, 1)])
+def test_a_replayed_routing_of_other_tokens(hipdev, ran, m):
+    """A product whose tokens are not those of the routing that ran last gives NaN and touches nothing else; with a routing
+    of its own it is right again."""
+    layer = Layer(E.Q4_K, E.Q6_K, 16, 4, 512, 256)
+    plan = E.MoePlan(16, 4, 64, 512, 256)
+    s, t = torch.randn((ran, 16), device="cuda:0"), torch.randn((m, 16), device="cuda:0")
+    E.moe_route(plan, t)
+    want = [v.clone() for v in products_of(plan, layer, m)]
+    assert all(bool(torch.isfinite(v).all()) for v in want)
+    graph = capture(lambda: E.moe_route(plan, s))
+    assert plan.tokens() == ran
+    E.moe_route(plan, t)
+    graph.replay()
+    for _ in range(2):
+        assert all(bool(torch.isnan(v).all()) for v in products_of(plan, layer, m))
+        E.moe_route(plan, t)
+        assert all(torch.equal(a, b) for a, b in zip(products_of(plan, layer, m), want))
+        graph.replay()
+
+
+@pytest.mark.parametrize("m", [1, 30])
+def test_a_captured_routing_that_never_ran(hipdev, m):
+    layer = Layer(E.Q4_K, E.Q6_K, 16, 4, 512, 256)
+    plan = E.MoePlan(16, 4, 64, 512, 256)
+    s = torch.randn((m, 16), device="cuda:0")
+    graph = capture(lambda: E.moe_route(plan, s))
+    assert all(bool(torch.isnan(v).all()) for v in products_of(plan, layer, m))
+    graph.replay()
+    got = [v.clone() for v in products_of(plan, layer, m)]
+    E.moe_route(plan, s)
+    assert all(torch.equal(a, b) and bool(torch.isfinite(a).all()) for a, b in zip(got, products_of(plan, layer, m)))
+
+
+def test_captured_products_after_a_routing_of_other_tokens(hipdev):
+    layer = Layer(E.Q8_0, E.Q8_0, 16, 4, 512, 256)
+    plan = E.MoePlan(16, 4, 64, 512, 256)
+    for m in (2, 30):
+        s, kept = torch.randn((m, 16), device="cuda:0"), []
+        E.moe_route(plan, s)
+        want = [v.clone() for v in products_of(plan, layer, m)]
+        x, a = torch.ones((m, 512), device="cuda:0"), torch.ones((m, 4, 256), device="cuda:0")
+        graph = capture(lambda: kept.extend([E.moe_gate_up(plan, layer.dev["gate"], layer.dev["up"], layer.q, x),
+                                             E.moe_down(plan, layer.dev["down"], layer.dq, a, residual=x)]))
+        for other in (31, 1, 0):
+            E.moe_route(plan, torch.randn((other, 16), device="cuda:0"))
+            graph.replay()
+            assert all(bool(torch.isnan(v).all()) for v in kept)
+            E.moe_route(plan, s)
+            graph.replay()
+            assert all(torch.equal(v, w) for v, w in zip(kept, want))
