@@ -373,7 +373,7 @@ struct MoeQ6K {
     static constexpr bool kWide = true;
     struct W {
         uint4 l[2], h[2], sc;  // as words from the 4-byte address below; the scales are the same in all lane groups
-        uint32_t d, sh;        // the word that holds d
+        uint32_t d, sh;        // the block's last word: two scales, then d
     };
     struct Op {
         v4i a[3][4];
@@ -384,6 +384,8 @@ struct MoeQ6K {
     __device__ static constexpr int chunk(int s, int g) { return 4 * s + g; }
     __device__ static __forceinline__ void load_w(W &w, const uint8_t *row, int u, int, int g) {
         const uint8_t *p = row + (size_t)u * kBytes;
+        // (where it begins: the aligned word that holds d may end behind the tensor)
+        __builtin_memcpy(&w.d, p + kBytes - 4, 4);
         w.sh = (uint32_t)((uintptr_t)p & 3u);
         p -= w.sh;
 #pragma unroll
@@ -392,13 +394,12 @@ struct MoeQ6K {
             w.h[i] = *reinterpret_cast<const uint4 *>(p + 128 + 32 * i + 16 * (g & 1));
         }
         w.sc = *reinterpret_cast<const uint4 *>(p + 192);
-        w.d = *reinterpret_cast<const uint32_t *>(p + 208);
     }
     __device__ static __forceinline__ void decode(Op &o, const W &w, int g) {
-        o.dm = w.d >> (8 * w.sh);
+        o.dm = w.d >> 16;
         o.mn = v4h{0, 0, 0, 0};
         uint32_t sc[4];
-        join_even(sc, w.sc, w.d, w.sh);
+        join_even(sc, w.sc, w.d, w.sh);  // (of the last word only where sh is 2: it begins at the fifth word then)
         // A piece's fifth word is the next piece's first: lane group g + 1's, or the next run's in group 0 (or,
         // of two groups, in the even one), and behind the last the scales'.  Loads of two bytes for them cost
         // a wave as much as whole ones.
