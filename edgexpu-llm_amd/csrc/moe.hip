@@ -455,17 +455,34 @@ __global__ __launch_bounds__(256) void moe_join_kernel(const float *__restrict__
 
 // ------------------------------------------------------------------ launches
 
-namespace {
-
 // LDS of a workgroup of one token that leaves room for two on a CU.
 constexpr size_t kOneLds = 60 * 1024;
 
-// Whether a routing's products take a workgroup a token (gate and up: a pair) without sorting the pairs:
-// where few experts have two tokens, whose weights the tiles read once (us so and with tiles, without their
-// sort's 6: 128 experts of 768 x 2560, 48 pairs, gate and up 26 and 29, down 30 and 55; 96 pairs 46 and 39, 55 and 56; 8
-// of 14336 x 4096, 6 pairs 77 and 105, 8 pairs 120 and 95).
-bool moe_one(long long pairs, int n_experts) {
-    return pairs <= std::max(8, n_experts / 2);
+// Whether a product takes a workgroup a token (gate and up: a pair) without sorting the pairs: where few experts
+// have two tokens, whose weights the tiles read once.  `weights`: an expert's elements in the product.  The tiles' launches
+// cost some 20 us, so that up to 8 pairs of smaller experts are faster without them; the larger an expert, the
+// fewer pairs (us so and with tiles, Q4_K, the weights from memory; their sort costs 5 besides:
+//   128 experts of 768 x 2560, gate and up: 64 pairs 32 and 30, 96 pairs 45 and 38; down (Q6_K): 35 and 38, 53 and 48
+//   gate and up, 14336 x 4096: 8 experts, 6 pairs 92 and 90, 8 pairs 119 and 90; 4 experts, 4 pairs 64 and 58, 6 pairs 88 and 58
+//   gate and up, 4096 x 4096: 8 experts, 8 pairs 39 and 39; 4 experts, 6 pairs 28 and 24, 8 pairs 37 and 26
+//   down, 4096 x 14336: 8 experts, 8 pairs 59 and 65; 4 experts, 6 pairs 46 and 46, 8 pairs 60 and 47).
+bool moe_takes_one(long long pairs, int n_experts, long long weights, size_t lds) {
+    const int half = n_experts / 2;
+    int most = std::max(8, half);
+    if (weights >= 1 << 26)
+        most = std::min(most, half + 2);
+    else if (weights >= 1 << 25)
+        most = std::min(most, half + 5);
+    return pairs <= most && lds <= kOneLds;
+}
+
+namespace {
+
+// A routing of m tokens in gate and up (`pair`), or in down, whose workgroups hold all of a token's rows.
+bool moe_one(const edgexpu_hip_moe *p, int m, bool pair) {
+    const size_t records = pair ? moe_groups(p->n_embd) : (size_t)p->top_k * moe_groups(p->n_ff);
+    return moe_takes_one((long long)m * p->top_k, p->n_experts, (pair ? 2LL : 1LL) * p->n_embd * p->n_ff,
+                         records * kMoeRec);
 }
 
 // Places a tile of sorted pairs (us with 32 and 64, 128 experts of 768 x 2560: 8 pairs an expert, gate and up 64 and 71,
@@ -493,7 +510,7 @@ void moe_pack(const MoeArgs &a, int rows, hipStream_t st) {
 template <class F>
 bool moe_run(const edgexpu_hip_moe *p, MoeArgs &a, bool pair, hipStream_t st, const char *what) {
     const long long pairs = (long long)p->pairs();
-    if (p->tile == 0) {
+    if (moe_one(p, p->m, pair)) {
         const size_t lds = (size_t)(pair ? 1 : p->top_k) * a.groups * kMoeRec;
         const dim3 grid((unsigned)((a.rows + 15) / 16), (unsigned)(pair ? pairs : p->m));
         if (pair)
@@ -557,10 +574,8 @@ bool moe_product(const edgexpu_hip_moe *p, MoeArgs &a, uint32_t type, bool pair,
 
 // Places a tile of the sorted pairs of a routing of m tokens; 0 where no product needs them sorted.
 int moe_sorted(const edgexpu_hip_moe *p, int m) {
-    const long long pairs = (long long)m * p->top_k;
-    const size_t one_lds = (size_t)std::max(moe_groups(p->n_embd), p->top_k * moe_groups(p->n_ff)) * kMoeRec;
-    if (m == 0 || (moe_one(pairs, p->n_experts) && one_lds <= kOneLds)) return 0;
-    return moe_tile(pairs, p->n_experts);
+    if (m == 0 || (moe_one(p, m, true) && moe_one(p, m, false))) return 0;
+    return moe_tile((long long)m * p->top_k, p->n_experts);
 }
 
 // Sorts the pairs of a routing of m tokens where the products need it.

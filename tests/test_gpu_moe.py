@@ -551,3 +551,37 @@ def test_captured_products_after_a_routing_of_other_tokens(hipdev):
             E.moe_route(plan, s)
             graph.replay()
             assert all(torch.equal(v, w) for v, w in zip(kept, want))
+
+
+# ------------------------------------------------------------------ products of one routing that share the work out differently
+
+
+def q4_k_of(shape, seed):
+    """Q4_K rows made on the device: random codes and scales, d and dmin of a trained projection's size."""
+    g = torch.Generator(device="cuda:0").manual_seed(seed)
+    w = torch.randint(0, 256, (*shape, 144), dtype=torch.uint8, device="cuda:0", generator=g)
+    w[..., :4] = (torch.rand((*shape, 2), device="cuda:0", generator=g) * 1e-4 + 1e-5).half().view(torch.uint8)
+    return w.view(*shape[:-1], -1)
+
+
+# (experts, choices, tokens, n_embd, n_ff): a token's rows too long for its workgroup in down alone, in gate and up alone;
+# matrices so large that tiles take gate and up from 8 pairs on, and down not yet; both; neither
+@pytest.mark.parametrize("size", [(5, 4, 1, 256, 14336), (5, 2, 1, 131072, 256), (8, 2, 4, 8192, 4096), (4, 2, 4, 8192, 4096),
+                                  (8, 2, 3, 8192, 4096), (4, 2, 3, 4096, 8192), (3, 1, 5, 4096, 14336)], ids=str)
+def test_products_that_share_the_work_out_differently(hipdev, size):
+    n, k, m, h, f = size
+    gate, up, down = (q4_k_of((n, r, c // 256), s) for r, c, s in ((f, h, 1), (f, h, 2), (h, f, 3)))
+    rng = np.random.default_rng(m)
+    ids, g = random_ids(rng, m, n, k, 0.1), rng.random((m, k)).astype(np.float32)
+    x, act, res = (rng.standard_normal(s).astype(np.float32) for s in ((m, h), (m, k, f), (m, h)))
+    plan = E.MoePlan(n, k, m, h, f)
+    for _ in range(2):
+        plan.assign(dev(ids), dev(g))
+        a = host(E.moe_gate_up(plan, gate, up, E.Q4_K, dev(x)))
+        o = host(E.moe_down(plan, down, E.Q4_K, dev(act), residual=dev(res)))
+    rows = sorted(rng.permutation(f)[:40].tolist() + [0, f - 1])
+    want, tol = P.gate_up(E.Q4_K, x, host(gate[:, rows]), host(up[:, rows]), ids)
+    assert np.all(np.abs(a[:, :, rows] - want) <= tol)
+    rows = sorted(rng.permutation(h)[:40].tolist() + [0, h - 1])
+    want, tol = P.down(E.Q4_K, act, host(down[:, rows]), ids, g, residual=res[:, rows])
+    assert np.all(np.abs(o[:, rows] - want) <= tol)
