@@ -261,7 +261,7 @@ constexpr int kRun = 4;
 // formats whose decoding is long: it is then what hides the load, and a second copy of it only costs
 // registers and instruction fetches (Q6_K, 64 tokens of 128 experts, 2560 rows of 768: 82 us with one, 89 with two).
 template <class F>
-constexpr int tile_deep(int TT) { return !F::kWide && TT <= 2 ? 2 : 1; }
+constexpr int tile_deep(int TT) { return !F::kLong && TT <= 2 ? 2 : 1; }
 
 // Sums made where they stand: left to the compiler, all tiles' integer sums wait in
 // registers for the end of a step.
@@ -476,6 +476,19 @@ bool moe_takes_one(long long pairs, int n_experts, long long weights, size_t lds
     return pairs <= most && lds <= kOneLds;
 }
 
+// Pairs an expert from which tiles hold 128 of them (0: none do), where a decoded row is worth it (us of gate, up and down
+// with 64 and 128, experts of 768 x 2560:
+//   Q6_K  50 pairs of each of 128 experts 394 and 369; of 32, 48 pairs 142 and 154, 64 pairs 151 and 143
+//   Q5_0  of 128, 64 pairs 781 and 772, 96 pairs 963 and 882; of 32, 64 pairs 253 and 296, 96 pairs 323 and 331
+//   Q8_0  of 128, 96 pairs 734 and 721, 128 pairs 886 and 792; of 32, 64 pairs 208 and 237, 192 pairs 346 and 328
+//   128 pairs: of 128, Q4_0 820 and 902; of 32, Q4_K 133 and 154, Q5_K 147 and 172).
+constexpr int wide_from(int type) {
+    return type == kTypeQ6_K ? 50 : type == kTypeQ5_0 ? 96 : type == kTypeQ8_0 ? 128 : 0;
+}
+bool moe_takes_wide(int type, long long pairs, int n_experts) {
+    return wide_from(type) > 0 && pairs >= (long long)wide_from(type) * n_experts;
+}
+
 namespace {
 
 // A routing of m tokens in gate and up (`pair`), or in down, whose workgroups hold all of a token's rows.
@@ -532,9 +545,7 @@ bool moe_run(const edgexpu_hip_moe *p, MoeArgs &a, bool pair, hipStream_t st, co
     // experts, 2560 rows of 1024, 75 us and 88 so)
     const long long blocks = (std::min<long long>(p->n_experts, pairs) + pairs / 32) * ((a.rows + 127) / 128);
     const int ks = p->tile == 32 && !pair && blocks < 512 ? 1 : 0;
-    // 128 pairs a workgroup where a decoded row is worth it (2048 tokens of 128 experts, 2560 rows of 768:
-    // Q6_K 354 us with 64, 292 with 128; Q5_K 204 and 211)
-    const bool wide = F::kWide && pairs > 48LL * p->n_experts;
+    const bool wide = moe_takes_wide(F::kType, pairs, p->n_experts);
 #define MOE_TILES(TT, EACH)                              \
     if (pair)                                            \
         moe_tiles<F, true, TT>(a, EACH, slots, ks, st);  \
@@ -544,7 +555,7 @@ bool moe_run(const edgexpu_hip_moe *p, MoeArgs &a, bool pair, hipStream_t st, co
         MOE_TILES(2, 1)
     } else if (!wide) {
         MOE_TILES(4, 1)
-    } else if constexpr (F::kWide) {
+    } else if constexpr (wide_from(F::kType) > 0) {
         MOE_TILES(8, 2)
     }
 #undef MOE_TILES
@@ -680,9 +691,7 @@ edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens
                   n_embd, n_ff);
         return nullptr;
     }
-    if (!lib_ready("moe_create") || !moe_prepare<MoeQ6K>() || !moe_prepare<MoeQ80>() || !moe_prepare<MoeQ40>() ||
-        !moe_prepare<MoeQ50>())
-        return nullptr;
+    if (!lib_ready("moe_create") || !moe_prepare<MoeQ6K>() || !moe_prepare<MoeQ80>() || !moe_prepare<MoeQ50>()) return nullptr;
     edgexpu_hip_moe *p = new (std::nothrow) edgexpu_hip_moe();
     if (p == nullptr) {
         lib_error(-5, "moe_create: out of host memory");

@@ -175,7 +175,7 @@ __host__ __device__ constexpr int moe_pack_parts(int n) {
 // ---------------------------------------------------------------- K-quants
 //
 // W: raw registers of a group of the lane's row; Op: the operand; chunk(s, g): which
-// 16 elements of the group lane group g holds in product s of 4.
+// 16 elements of the group lane group g holds in product s of 4; kLong: decode() is.
 
 // A group's integer sums, a digit each, and the minima's.
 template <class F>
@@ -278,7 +278,7 @@ __device__ __forceinline__ v4h min_operand(const SixBits &b, int g) {
 struct MoeQ4K {
     static constexpr bool kK = true, kMin = true, kTurned = false;
     static constexpr int kType = kTypeQ4_K, kDigits = 2, kBytes = kBytesQ4_K;
-    static constexpr bool kWide = false;
+    static constexpr bool kLong = false;
     struct W {
         uint4 hd, q[2];
     };
@@ -320,7 +320,7 @@ struct MoeQ4K {
 struct MoeQ5K {
     static constexpr bool kK = true, kMin = true, kTurned = true;
     static constexpr int kType = kTypeQ5_K, kDigits = 2, kBytes = kBytesQ5_K;
-    static constexpr bool kWide = false;
+    static constexpr bool kLong = false;
     struct W {
         uint4 hd, h, q[2];
     };
@@ -370,7 +370,7 @@ __device__ __forceinline__ void join_even(uint32_t (&v)[4], const uint4 &w, uint
 struct MoeQ6K {
     static constexpr bool kK = true, kMin = false, kTurned = false;
     static constexpr int kType = kTypeQ6_K, kDigits = 3, kBytes = kBytesQ6_K;
-    static constexpr bool kWide = true;
+    static constexpr bool kLong = true;
     struct W {
         uint4 l[2], h[2], sc;  // as words from the 4-byte address below; the scales are the same in all lane groups
         uint32_t d, sh;        // the block's last word: two scales, then d
@@ -504,7 +504,7 @@ __device__ __forceinline__ uint32_t load_scales(const uint8_t *row, int u, int n
 struct MoeQ80 {
     static constexpr bool kK = false, kQ80 = true;
     static constexpr int kType = kTypeQ8_0, kBytes = kBytesQ8_0;
-    static constexpr bool kWide = true;
+    static constexpr bool kLong = true;
     struct W {
         uint4 q[4];
         uint32_t d;
@@ -540,7 +540,7 @@ __device__ __forceinline__ uint32_t less_each(uint32_t c, uint32_t bias) {
 struct MoeQ40 {
     static constexpr bool kK = false, kQ80 = false;
     static constexpr int kType = kTypeQ4_0, kBytes = kBytesQ4_0;
-    static constexpr bool kWide = true;
+    static constexpr bool kLong = true;
     struct W {
         uint32_t q[8], d;
     };
@@ -567,7 +567,7 @@ struct MoeQ40 {
 struct MoeQ50 {
     static constexpr bool kK = false, kQ80 = false;
     static constexpr int kType = kTypeQ5_0, kBytes = kBytesQ5_0;
-    static constexpr bool kWide = true;
+    static constexpr bool kLong = true;
     struct W {
         uint32_t q[8], h[8], d;
     };

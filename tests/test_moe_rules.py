@@ -46,3 +46,29 @@ def test_the_line_bounds():
     assert one(256, 512, 1 << 30) and not one(257, 512, 1 << 10)
     assert one(8, 4, 1 << 20) and not one(9, 4, 1 << 20)
     assert one(1, 8, 1 << 20, 60 * 1024) and not one(1, 8, 1 << 20, 60 * 1024 + 1)
+
+
+# type, experts, pairs, measured us of gate, up and down with tiles of 64 and of 128 pairs
+TILES = [
+    (14, 32, 1536, 141.8, 153.9), (14, 32, 2048, 151.4, 142.5), (14, 32, 4096, 226.9, 198.9), (14, 128, 6400, 393.7, 368.8),
+    (14, 128, 8192, 443.2, 406.1), (14, 128, 32768, 1290.4, 1097.5), (14, 8, 1024, 377.7, 338.1),
+    (8, 32, 2048, 207.8, 236.6), (8, 32, 4096, 281.4, 289.2), (8, 32, 6144, 345.6, 327.9), (8, 32, 16384, 762.4, 660.5),
+    (8, 128, 6400, 499.4, 478.8), (8, 128, 12288, 734.0, 721.2), (8, 128, 16384, 886.3, 791.5), (8, 8, 768, 362.8, 459.4),
+    (8, 8, 1024, 534.8, 480.8), (8, 8, 1536, 664.2, 519.8),
+    (6, 32, 2048, 252.5, 296.4), (6, 32, 3072, 323.2, 331.1), (6, 32, 6144, 465.1, 436.7), (6, 128, 8192, 780.5, 772.1),
+    (6, 128, 12288, 962.5, 882.0), (6, 128, 32768, 2057.9, 1725.6), (6, 8, 768, 644.9, 578.7),
+    (2, 32, 4096, 273.8, 285.6), (2, 32, 16384, 692.8, 705.4), (2, 128, 8192, 512.1, 568.8), (2, 128, 16384, 820.3, 902.3),
+    (12, 32, 4096, 133.3, 154.0), (12, 32, 16384, 368.4, 373.4), (13, 32, 4096, 146.6, 172.3), (13, 32, 16384, 422.6, 406.0),
+]
+
+
+def wide(qt, pairs, experts):
+    f = E.hip().lib._ZN3exq14moe_takes_wideEixi
+    f.restype, f.argtypes = C.c_bool, [C.c_int, C.c_longlong, C.c_int]
+    return f(qt, pairs, experts)
+
+
+@pytest.mark.parametrize("qt,experts,pairs,narrow,broad", TILES)
+def test_the_tiles_are_the_faster_ones(qt, experts, pairs, narrow, broad):
+    """The tile that a type and a number of pairs take is within 10 % of the faster one."""
+    assert (broad if wide(qt, pairs, experts) else narrow) <= 1.1 * min(broad, narrow)
