@@ -423,37 +423,41 @@ __global__ __launch_bounds__(256) void moe_join_kernel(const float *__restrict__
                                                        const int32_t *__restrict__ routed, const float *residual,
                                                        float *out, int m, int top_k, int rows) {
     const int each = VEC ? 4 : 1, per = rows / each;
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (size_t)m * per) return;
-    const size_t t = i / per;
-    const int o = (int)(i - t * per) * each;
     const bool whole = *routed == m;
-    float s[4] = {};
-    for (int j = 0; whole && j < top_k; ++j) {
-        const size_t pair = t * top_k + j;
-        if (ids[pair] < 0) continue;
-        const float *p = part + pair * rows + o;
-        if (VEC) {
-            const float4 v = *reinterpret_cast<const float4 *>(p);
-            s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
-        } else {
-            s[0] += *p;
+    // (a turn, except where the rows are more than a launch's threads may be)
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < (size_t)m * per; i += (size_t)gridDim.x * 256) {
+        const size_t t = i / per;
+        const int o = (int)(i - t * per) * each;
+        float s[4] = {};
+        for (int j = 0; whole && j < top_k; ++j) {
+            const size_t pair = t * top_k + j;
+            if (ids[pair] < 0) continue;
+            const float *p = part + pair * rows + o;
+            if (VEC) {
+                const float4 v = *reinterpret_cast<const float4 *>(p);
+                s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+            } else {
+                s[0] += *p;
+            }
         }
+        const size_t at = t * rows + o;
+        if (residual != nullptr)
+#pragma unroll
+            for (int r = 0; r < each; ++r) s[r] = residual[at + r] + s[r];
+        if (!whole)
+#pragma unroll
+            for (int r = 0; r < each; ++r) s[r] = kNan;
+        if (VEC)
+            *reinterpret_cast<float4 *>(out + at) = make_float4(s[0], s[1], s[2], s[3]);
+        else
+            out[at] = s[0];
     }
-    const size_t at = t * rows + o;
-    if (residual != nullptr)
-#pragma unroll
-        for (int r = 0; r < each; ++r) s[r] = residual[at + r] + s[r];
-    if (!whole)
-#pragma unroll
-        for (int r = 0; r < each; ++r) s[r] = kNan;
-    if (VEC)
-        *reinterpret_cast<float4 *>(out + at) = make_float4(s[0], s[1], s[2], s[3]);
-    else
-        out[at] = s[0];
 }
 
 // ------------------------------------------------------------------ launches
+
+// Threads of a launch in x: 2^32 and more are taken modulo 2^32.
+constexpr size_t kLaunch = (size_t)1 << 31;
 
 // LDS of a workgroup of one token that leaves room for two on a CU.
 constexpr size_t kOneLds = 60 * 1024;
@@ -562,7 +566,7 @@ bool moe_run(const edgexpu_hip_moe *p, MoeArgs &a, bool pair, hipStream_t st, co
     if (!lib_hip(hipGetLastError(), what)) return false;
     if (pair) return true;
     const bool vec = (a.rows & 3) == 0;
-    const unsigned joins = (unsigned)(((size_t)p->m * (vec ? a.rows / 4 : a.rows) + 255) / 256);
+    const unsigned joins = (unsigned)std::min(((size_t)p->m * (vec ? a.rows / 4 : a.rows) + 255) / 256, kLaunch / 256);
     if (vec)
         hipLaunchKernelGGL(moe_join_kernel<true>, dim3(joins), dim3(256), 0, st, p->part, a.ids, a.routed, a.residual,
                            out, p->m, p->top_k, a.rows);

@@ -585,3 +585,21 @@ def test_products_that_share_the_work_out_differently(hipdev, size):
     rows = sorted(rng.permutation(h)[:40].tolist() + [0, h - 1])
     want, tol = P.down(E.Q4_K, act, host(down[:, rows]), ids, g, residual=res[:, rows])
     assert np.all(np.abs(o[:, rows] - want) <= tol)
+
+
+def test_more_rows_than_one_launch_has_threads(hipdev):
+    """Down of 2^22 tokens to rows of 1025: a row's part each makes more than 2^32."""
+    m, n, f, period = 1 << 22, 1025, 32, 64
+    rng = np.random.default_rng(1)
+    w = experts(E.Q8_0, 2, n, f, rng)
+    a = rng.standard_normal((period, 1, f)).astype(np.float32)
+    ids, g = (np.arange(period) % 3 - 1).astype(np.int32)[:, None], rng.random((period, 1)).astype(np.float32)
+    plan = E.MoePlan(2, 1, m, n, f)
+    plan.assign(dev(ids).repeat(m // period, 1), dev(g).repeat(m // period, 1))
+    out = E.moe_down(plan, dev(w), E.Q8_0, dev(a).repeat(m // period, 1, 1)).view(-1, period, n)
+    want, tol = P.down(E.Q8_0, a, w, ids, g)
+    assert np.all(np.abs(host(out[0]) - want) <= tol)
+    for i in range(0, m // period, 4096):
+        assert bool((out[i:i + 4096] == out[0]).all()), i
+    del plan, out
+    torch.cuda.empty_cache()
