@@ -456,8 +456,9 @@ __global__ __launch_bounds__(256) void moe_join_kernel(const float *__restrict__
 
 // ------------------------------------------------------------------ launches
 
-// Threads of a launch in x: 2^32 and more are taken modulo 2^32.
+// Threads of a launch in x, and workgroups of 256: 2^32 and more are taken modulo 2^32.
 constexpr size_t kLaunch = (size_t)1 << 31;
+constexpr long long kMoeBlocks = (1 << 24) - 32;
 
 // LDS of a workgroup of one token that leaves room for two on a CU.
 constexpr size_t kOneLds = 60 * 1024;
@@ -512,7 +513,8 @@ template <class F, bool PAIR, int TT>
 void moe_tiles(const MoeArgs &a, int each, int slots, int ks_log, hipStream_t st) {
     const int rows = (PAIR ? 16 : 32) * (kTileWaves >> ks_log);
     const int n_blk = (a.rows + rows - 1) / rows;
-    // (a slot and 16 rows or more a workgroup: what the pairs' rows take in device memory keeps that below 2^31)
+    // (at most kMoeBlocks, up to whole runs: _create's limit for gate and up; down's parts, 4 bytes each, are below 2^37 in
+    // the device's memory, which with 512 experts of 2^20 rows is 2^37 / (64 128) + 2^22 workgroups)
     const dim3 grid((unsigned)((slots * n_blk + 8 * kRun - 1) / (8 * kRun)) * 8u * kRun);
     hipLaunchKernelGGL((tile_kernel<F, PAIR, TT>()), grid, dim3(64 * kTileWaves), tile_lds(TT), st, a, ks_log, each,
                        slots, n_blk);
@@ -693,6 +695,12 @@ edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens
     if (records > (size_t)1 << 27) {  // (their places are counted in 32 bits, 16 bytes a unit)
         lib_error(-2, "moe_create: %d tokens of %d experts, rows of %d and %d: more than 2^27 groups of 256", max_tokens, top_k,
                   n_embd, n_ff);
+        return nullptr;
+    }
+    // (slots and row blocks of gate and up; at fewer pairs, where tiles hold 32, slots are at most 3 / 2 n_experts)
+    if (((long long)(pairs / 64) + n_experts) * ((n_ff + 63) / 64) > kMoeBlocks) {
+        lib_error(-2, "moe_create: %d tokens of %d of %d experts, rows of %d: too many workgroups for a launch", max_tokens,
+                  top_k, n_experts, n_ff);
         return nullptr;
     }
     if (!lib_ready("moe_create") || !moe_prepare<MoeQ6K>() || !moe_prepare<MoeQ80>() || !moe_prepare<MoeQ50>()) return nullptr;

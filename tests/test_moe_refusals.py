@@ -59,3 +59,9 @@ def test_the_plain_route():
     s = np.array([[4.0, -9.0, 3.0, 2.9]], np.float32)
     assert P.route(s, 1, "sigmoid", n_groups=2, top_groups=1, best=1)[0].tolist() == [[0]]
     assert P.route(s, 1, "sigmoid", n_groups=2, top_groups=1, best=2)[0].tolist() == [[2]]
+
+
+@pytest.mark.parametrize("args", [(512, 1, 2**15, 32, 2**20), (512, 8, 2**12, 32, 2**20)])
+def test_create_beyond_the_workgroups_of_a_launch(lib, args):
+    """2^24 workgroups of 256 threads are 2^32 threads, of which a launch would run none."""
+    refused(lib, lib.moe_create(*args), -2, "workgroups")
