@@ -65,3 +65,42 @@ def test_the_plain_route():
 def test_create_beyond_the_workgroups_of_a_launch(lib, args):
     """2^24 workgroups of 256 threads are 2^32 threads, of which a launch would run none."""
     refused(lib, lib.moe_create(*args), -2, "workgroups")
+
+
+@pytest.mark.parametrize("n,groups,top,best,k", [(9, 1, 1, 1, 4), (12, 4, 2, 1, 5), (12, 4, 2, 2, 7), (30, 6, 5, 2, 8), (8, 8, 3, 2, 2)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_the_plain_route_by_counting(n, groups, top, best, k, score):
+    """The plain form against another: an expert is chosen where fewer than k stand before it, of the runs that fewer
+    than `top` stand before, and its place is how many do."""
+    rng = np.random.default_rng(n + k)
+    m, per = 40, n // groups
+    s = rng.integers(-3, 4, (m, n)).astype(np.float32)  # (many equal scores)
+    s[rng.random((m, n)) < 0.2] = -np.inf
+    s[:3] = [[-np.inf], [1.0], [np.nan]]
+    bias = (rng.integers(-2, 3, n) / 4).astype(np.float32)
+    bias[n - 1] = np.inf
+    ids, w = P.route(s, k, score, bias, groups, top, best, normalise=False)
+    live = np.isfinite(s)
+    x = np.where(live, s, -1e30).astype(np.float64)
+    e = np.where(live, np.exp(np.minimum(x, 700)), 0)
+    p = e / (1 + e) if score == "sigmoid" else e / np.maximum(e.sum(1, keepdims=True), 1e-300)
+    c = np.where(live & np.isfinite(bias), p + np.where(np.isfinite(bias), bias, 0), -np.inf)
+    runs = np.sort(c.reshape(m, groups, per), 2)[:, :, ::-1][:, :, :best]
+    rank = np.where(np.isfinite(runs), runs, 0).sum(2) + np.where(np.isfinite(runs[:, :, 0]), 0, -np.inf)
+
+    def before(v):  # how many stand before each, by value and then by number
+        # (values that 64 bits hold apart by their last bits are equal here: the two forms round differently)
+        v = np.where(np.isfinite(v), np.round(v, 12), -np.inf)
+        i = np.arange(v.shape[1])
+        return ((v[:, None, :] > v[:, :, None]) | ((v[:, None, :] == v[:, :, None]) & (i[None, None, :] < i[None, :, None]))).sum(2)
+
+    stay = np.repeat(before(rank) < top, per, axis=1) if groups > 1 else np.ones((m, n), bool)
+    kept = np.where(stay, c, -np.inf)
+    place = np.where(np.isfinite(kept), before(kept), n)
+    for t in range(m):
+        want = np.full(k, -1)
+        for expert in range(n):
+            if place[t, expert] < k:
+                want[place[t, expert]] = expert
+        assert ids[t].tolist() == want.tolist(), t
+        assert np.allclose(w[t], np.where(want >= 0, p[t, want], 0), rtol=1e-12, atol=0)
