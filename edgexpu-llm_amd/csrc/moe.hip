@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void moe_pack_kernel(MoeArgs a) {
 // columns of the products hold the same token.
 // What bounds it: for a token a chain (arguments 0.7 us, choice 0.9, weights 2, products, sums
 // 1.2): 8 of 128 experts of 768 x 2560, Q4_K, gate and up 7.4 us; down of 2560 x 768, Q6_K, 10.3, the decoding of three
-// groups a wave; for more pairs the memory: 3 tokens of 14336 x 4096 77 us, 4.0 TB/s.  At most
+// groups a wave; for more pairs the memory: 3 tokens of 14336 x 4096 79 us, 3.9 TB/s.  At most
 // 128 registers, so that two workgroups fit a CU (162: gate and up 10.0 us); 16 waves, down 12.7.
 constexpr int kOneWaves = 8;
 
@@ -247,9 +247,11 @@ __device__ __forceinline__ uint32_t lds_addr(const void *p) {
 // buffer, two buffers.  A step takes one of its row tiles after the other, so that
 // only one's decoded rows are in registers (both at once read each record once, but with a
 // third more registers and 2 waves a SIMD for 3: 512 tokens 109 us so, 103 one by one).
-// What bounds it: memory where tiles are few (12 tokens of 8 experts, 4096 rows of 14336, Q4_K, 59 us, 4.4 TB/s), else
-// vector instructions: to decode a row tile's group 110 (Q4_K) to 450 (Q6_K), and 20 for 16 pairs' scales
-// (4096 tokens of 128 experts, 768 rows of 2560 twice, Q4_K, 375 us, 690 TFLOP/s).
+// What bounds it: memory where tiles are few (12 tokens of 8 experts, 4096 rows of 14336, Q4_K, 54 us, 4.7 TB/s); with
+// many pairs an expert vector instructions, to decode a row tile's group 110 (Q4_K) to 450 (Q6_K), and 20 for 16 pairs'
+// scales (4096 tokens of 128 experts, 768 rows of 2560 twice, Q4_K, 397 us, 650 TFLOP/s: they issue in 70 % of the
+// cycles); between the two how far loads and products overlap (512 tokens 100 us: bytes 61, vector instructions 44,
+// matrix products 18, waves wait 40 % of their time).
 __host__ __device__ constexpr int tile_chunk(int TT) { return TT == 2 ? 2 : 1; }
 __host__ __device__ constexpr int tile_lds(int TT) { return 2 * tile_chunk(TT) * 16 * TT * kMoeRec; }
 constexpr int kTileWaves = 4;
@@ -417,7 +419,7 @@ constexpr auto tile_kernel() {
 // ------------------------------------------------------------------ a token's parts
 
 // out[t] = [residual[t] +] the parts of its places with an expert, in their order; a
-// thread takes 4 rows (VEC) or one.  One pass over the parts: 4096 tokens of 8 x 2560, 80 us, 4.7 TB/s.
+// thread takes 4 rows (VEC) or one.  One pass over the parts: 4096 tokens of 8 x 2560, 81 us, 5.2 TB/s, part of them from the caches.
 template <bool VEC>
 __global__ __launch_bounds__(256) void moe_join_kernel(const float *__restrict__ part, const int32_t *__restrict__ ids,
                                                        const int32_t *__restrict__ routed, const float *residual,

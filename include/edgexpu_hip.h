@@ -492,8 +492,8 @@ int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip_batch *b, 
  * Q5_0, Q8_0, Q4_K, Q5_K or Q6_K (any other: error -3), at a 16-byte address;
  * biases are [n_experts][rows] f32.  Products are those of
  * edgexpu_hip_linear_quant_batch_dev: the activation quantized once to Q8_0 or Q8_K
- * blocks, block integers exact, sums in f32 in an order that the call's sizes fix
- * (the same call gives the same words).
+ * blocks, block integers exact, sums in f32 in an order that the call's sizes and
+ * the routing fix (the same call gives the same words).
  * The plan holds the routing of the last edgexpu_hip_moe_route_dev or
  * edgexpu_hip_moe_assign_dev and the workspaces of the products; all device memory
  * is taken by _create, so every other call can be captured into a graph.  Work on one
@@ -542,6 +542,7 @@ int edgexpu_hip_moe_assign_dev(edgexpu_hip_moe *p, const int32_t *ids, const flo
 
 /* For the routing's m tokens and each of their experts e = ids[t][j]:
  *   act[t][j] = f(b_gate[e] + W_gate[e] . q8(x[t])) * (b_up[e] + W_up[e] . q8(x[t]))
+ * Both tensors are of one type.
  * x [m][n_embd], act [m][top_k][n_ff], 16-byte aligned, not overlapping; biases may
  * be NULL (either alone too).  f(v): EDGEXPU_HIP_MOE_SILU v / (1 + exp(-v)),
  * EDGEXPU_HIP_MOE_GELU v / (1 + exp(-2 sqrt(2 / pi) (v + 0.044715 v^3))), the tanh
@@ -551,8 +552,8 @@ int edgexpu_hip_moe_assign_dev(edgexpu_hip_moe *p, const int32_t *ids, const flo
 int edgexpu_hip_moe_gate_up_dev(float *act, const float *x, edgexpu_hip_moe *p, const void *w_gate, const void *w_up,
                                 uint32_t type, const float *b_gate, const float *b_up, int activation, void *stream);
 /* out[t] = [residual[t] +] sum_j weights[t][j] (bias[e] + W[e] . q8(act[t][j])) over
- * the places with an expert, summed in order of j; out [m][n_embd], which may be
- * residual and overlaps nothing else; act and out 16-byte aligned.  bias and residual
+ * the places with an expert (few tokens: not in order of j, and the biases last); out
+ * [m][n_embd], which may be residual and overlaps nothing else; act and out 16-byte aligned.  bias and residual
  * may be NULL.  n_ff a multiple of the type's block. */
 int edgexpu_hip_moe_down_dev(float *out, const float *act, edgexpu_hip_moe *p, const void *w_down, uint32_t type,
                              const float *bias, const float *residual, void *stream);
