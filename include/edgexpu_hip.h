@@ -501,16 +501,16 @@ int edgexpu_hip_attention_dev(float *out, const float *q, edgexpu_hip_batch *b, 
  * host thread at a time.  A product computes as many tokens as the last routing
  * that was queued, captured ones included; a captured product, as many as when it was
  * captured.  Where the last routing that ran is of another number of tokens (or
- * none ran), as after the replay of a captured one, every value that it gives is NaN,
- * and nothing else is read or written: queue or replay a routing of as many before
+ * none ran), as after the replay of a captured one, every value of its own tokens' rows
+ * is NaN, and no other rows are written: queue or replay a routing of as many before
  * it.  What a captured call was given lives as long as its graph.  All run on the device of
  * edgexpu_hip_init (another current device: error -4). */
 typedef struct edgexpu_hip_moe edgexpu_hip_moe;
 /* n_experts at most 512; top_k at most n_experts and 32; n_embd and n_ff at most
- * 2^20; P = max_tokens * top_k at most 2^22; the larger of max_tokens ceil(n_embd / 256)
- * and P ceil(n_ff / 256) at most 2^27; (P / 64 + n_experts) ceil(n_ff / 64) at most
- * 2^24 - 32.  The device memory is 304 bytes times the latter
- * and 4 P n_embd bytes, besides 13 P.  NULL on error. */
+ * 2^20; P = max_tokens * top_k at most 2^22; (P / 64 + n_experts) ceil(n_ff / 64) at
+ * most 2^24 - 32; the larger of max_tokens ceil(n_embd / 256) and P ceil(n_ff / 256) at
+ * most 2^27.  The device memory is 304 bytes times the latter and 4 P n_embd bytes,
+ * besides 13 P.  NULL on error. */
 edgexpu_hip_moe *edgexpu_hip_moe_create(int n_experts, int top_k, int max_tokens, int n_embd, int n_ff);
 /* Waits for the device, then frees. */
 void edgexpu_hip_moe_destroy(edgexpu_hip_moe *p);

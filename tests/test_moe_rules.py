@@ -55,7 +55,7 @@ TILES = [
     (8, 32, 2048, 207.8, 236.6), (8, 32, 4096, 281.4, 289.2), (8, 32, 6144, 345.6, 327.9), (8, 32, 16384, 762.4, 660.5),
     (8, 128, 6400, 499.4, 478.8), (8, 128, 12288, 734.0, 721.2), (8, 128, 16384, 886.3, 791.5), (8, 8, 768, 362.8, 459.4),
     (8, 8, 1024, 534.8, 480.8), (8, 8, 1536, 664.2, 519.8),
-    (6, 32, 2048, 252.5, 296.4), (6, 32, 3072, 323.2, 331.1), (6, 32, 6144, 465.1, 436.7), (6, 128, 8192, 780.5, 772.1),
+    (6, 32, 2048, 252.5, 296.4), (6, 32, 6144, 465.1, 436.7), (6, 128, 8192, 780.5, 772.1),
     (6, 128, 12288, 962.5, 882.0), (6, 128, 32768, 2057.9, 1725.6), (6, 8, 768, 644.9, 578.7),
     (2, 32, 4096, 273.8, 285.6), (2, 32, 16384, 692.8, 705.4), (2, 128, 8192, 512.1, 568.8), (2, 128, 16384, 820.3, 902.3),
     (12, 32, 4096, 133.3, 154.0), (12, 32, 16384, 368.4, 373.4), (13, 32, 4096, 146.6, 172.3), (13, 32, 16384, 422.6, 406.0),
